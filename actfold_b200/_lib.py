@@ -43,6 +43,15 @@ SIGNATURES: dict[str, tuple] = {
         [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _f32,
          _vp, _vp],
     ),
+    "af_block_tables": (
+        _i32,
+        [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "af_tree_masks": (_i32, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "af_accept_tree": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "af_write_cache": (_i32, [_vp, _vp, _vp]),
+    "af_tree_attention": (_i32, [_vp, _vp, _vp]),
+    "af_tree_attention_workspace_bytes": (_i32, [_vp]),
 }
 
 _lib = None

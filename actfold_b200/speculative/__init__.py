@@ -7,7 +7,10 @@ from actfold_b200.speculative.acceptance_policy import (AcceptancePolicy, Greedy
 from actfold_b200.speculative.branch_tree import BranchNode, BranchTree
 from actfold_b200.speculative.folded_generation import FoldedGenerationResult, folded_generate
 from actfold_b200.speculative.verification_engine import ActFoldVerificationEngine, Branch, VerificationResult
+from actfold_b200.tree_kernels import (AcceptedPath, BlockTables, accept_tree, block_tables, tree_attention, tree_masks,
+                                       write_cache)
 
 __all__ = ["ActFoldVerificationEngine", "Branch", "VerificationResult", "BlockDecoder", "BlockDecodingConfig",
            "BlockDecodingResult", "SyntheticDraft", "AcceptancePolicy", "GreedyAcceptancePolicy",
-           "ThresholdAcceptancePolicy", "BranchNode", "BranchTree", "FoldedGenerationResult", "folded_generate"]
+           "ThresholdAcceptancePolicy", "BranchNode", "BranchTree", "FoldedGenerationResult", "folded_generate",
+           "AcceptedPath", "BlockTables", "accept_tree", "block_tables", "tree_attention", "tree_masks", "write_cache"]

@@ -434,6 +434,144 @@ int af_fold_promote(void* plan, int64_t child, const int64_t* child_tokens, cons
 int af_fold_set_timing(void* plan, int enabled);
 int af_fold_get_timing(void* plan, double* ms, int64_t* counts, int n_kinds, int64_t* launches_per_run);
 
+/* ------------------------------------------------------------------------
+ * Tree verification over a paged key/value cache.
+ *
+ * One step of speculative decoding for a batch of requests: every request has
+ * a cached prefix, kept in pages of a pool, and a tree of drafted tokens
+ * (nodes) that the target model evaluates at once. The branch tree and the
+ * acceptance of a branch are host objects in the reference
+ * (actfold/speculative/branch_tree.py:11-95,
+ * actfold/speculative/acceptance_policy.py:12-83), which verifies one branch
+ * per forward pass; paging and batching have no counterpart there.
+ *
+ * Nodes of all requests are packed: tree b holds nodes [starts[b],
+ * starts[b + 1]), a node's number within its tree is its local number, and a
+ * parent comes before its children. Rows behind the last tree are neither
+ * read nor written. Every size that changes from step to step is read on the
+ * device, so a captured step can be replayed. A bad device-side value (starts
+ * out of order, a parent behind its child, a page out of range) sets
+ * AF_STATUS_BOUNDS (4) in *status (nullable) and is skipped; what does not
+ * fit sets AF_STATUS_CAPACITY (2).
+ * ---------------------------------------------------------------------- */
+
+/*
+ * af_block_tables -- pages and slots for a step's new tokens.
+ *
+ * Request r holds the pages of its first held[r] tokens (held null: =
+ * lengths), keeps lengths[r] of them and gets grow[r] more. With page size S,
+ * it has ceil(held / S) entries in row r of tables (stride in elements) and
+ * needs ceil((lengths + grow) / S): missing pages are taken from the front of
+ * the ring free_pages[pool], pages no longer needed are appended to its end,
+ * both in the order of requests (returned pages are first handed out by a
+ * later call). The ring's free entries are [free_range[0], free_range[1]),
+ * counted without end and taken modulo pool; free_range_out (not free_range
+ * itself) receives the new range. Outputs: starts[batch + 1], the prefix sums
+ * of grow; totals[r] = lengths[r] + grow[r]; slots, for the i-th new token of
+ * request r page * S + offset of position lengths[r] + i, packed at starts[r]
+ * + i (slots_per_request 0) or at r * slots_per_request + i, -1 elsewhere.
+ * When the pages, a table row or the slots do not suffice nothing is taken or
+ * returned: starts is 0, totals = held, every slot -1, and AF_STATUS_CAPACITY
+ * is set.
+ */
+int af_block_tables(int32_t* tables, int64_t tables_stride, int64_t max_pages, const int32_t* held, const int32_t* lengths,
+                    const int32_t* grow, int64_t batch, int32_t* free_pages, int64_t pool, const int64_t* free_range,
+                    int64_t page_size, int64_t slot_capacity, int64_t slots_per_request, int32_t* starts, int32_t* totals,
+                    int64_t* slots, int64_t* free_range_out, uint32_t* status, void* stream);
+
+/*
+ * af_tree_masks -- ancestor bits and positions of drafted trees.
+ *
+ * parents[i]: local number of node i's parent, -1 for a node that follows the
+ * prefix. mask[i * words + j / 32] bit j % 32 = node j of the tree is i or an
+ * ancestor of i; positions[i] = base[b] + depth (base nullable = 0).
+ * A tree holds at most 32 * words nodes, words at most 512.
+ */
+int af_tree_masks(const int32_t* parents, const int32_t* starts, int64_t batch, int64_t total, int64_t words,
+                  const int32_t* base, int32_t* mask, int32_t* positions, uint32_t* status, void* stream);
+
+/*
+ * af_accept_tree -- the longest drafted path that the target model agrees with.
+ *
+ * A node is accepted when its token equals the target model's choice after
+ * its parent (targets[parent], root_targets[b] for a node that follows the
+ * prefix; root_targets null: such a node needs no agreement) and its parent is
+ * accepted. The deepest accepted node, of several the one with the smallest
+ * number, ends the path, of which the first `keep` nodes are kept:
+ * rows[b * keep + d] = packed number of the d-th node, -1 behind the last;
+ * counts[b] their number; next_tokens[b] = the target model's choice after the
+ * last one (root_targets[b], or -1, when there is none).
+ */
+int af_accept_tree(const int32_t* parents, const int64_t* tokens, const int64_t* targets, const int32_t* starts,
+                   int64_t batch, int64_t total, int64_t max_nodes, const int64_t* root_targets, int64_t keep,
+                   int32_t* rows, int32_t* counts, int64_t* next_tokens, uint32_t* status, void* stream);
+
+/*
+ * af_write_cache -- key and value rows into their slots of a paged cache.
+ *
+ * For every layer l and i < count with slots[i] >= 0 (and rows[i] >= 0):
+ * cache[l, slot / page_size, slot % page_size, h, :] = x[l, rows[i], h, :]
+ * (rows null: row i), for keys and for values. The innermost dimension
+ * (head_bytes) is contiguous; strides in bytes, in the order of the indexes.
+ * Live slots must differ from one another: of two rows for one slot an
+ * unspecified mixture is kept.
+ */
+typedef struct {
+  const void *k, *v;
+  int64_t k_strides[3], v_strides[3]; /* layer, row, head */
+  void *k_cache, *v_cache;
+  int64_t k_cache_strides[4], v_cache_strides[4]; /* layer, page, token, head */
+  const int64_t* slots;
+  const int32_t* rows;
+  int64_t n_rows, count, pages, page_size, layers, heads, head_bytes;
+} af_cache_rows;
+
+int af_write_cache(const af_cache_rows* w, uint32_t* status, void* stream);
+
+/*
+ * af_tree_attention -- drafted nodes over their cached prefix and their tree.
+ *
+ * out[i, h] = sum_j softmax_j(scale * q[i, h] . k_j) v_j over the lengths[b]
+ * cached keys of node i's request (positions in pages tables[b, p /
+ * page_size]) and the nodes j of its own tree with mask[i * words + j / 32]
+ * bit j % 32 set, whose keys and values are rows starts[b] + j of k and v
+ * (they are not in the cache yet). mask null: the nodes of a tree are a chain,
+ * node i sees the nodes up to itself. Query head h reads key/value head
+ * h / (n_heads / n_kv_heads). A row that sees no key is 0 (lse -inf). Keys and
+ * values that a row does not see have no influence on it, whatever they hold.
+ * dtype AF_DTYPE_F16 or AF_DTYPE_BF16, head_dim 64 or 128, page_size a
+ * multiple of 8, n_heads / n_kv_heads <= 64; every stride (bytes, in the
+ * order of the indexes) and address a multiple of 16, the innermost dimension
+ * contiguous. lse (nullable) [total, n_heads]: natural log of the sum of
+ * exponentials. workspace: af_tree_attention_workspace_bytes() bytes, not
+ * shared by calls that may run at once. Sums, maxima and the output rows are
+ * held in 32 bits; probabilities are rounded to dtype.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_strides[2], k_strides[2], v_strides[2]; /* node, head */
+  const void *k_cache, *v_cache;
+  int64_t k_cache_strides[3], v_cache_strides[3]; /* page, token, head */
+  int64_t pages, page_size;
+  const int32_t* tables;
+  int64_t tables_stride, max_pages; /* elements */
+  const int32_t *lengths, *starts;
+  const int32_t* mask;
+  int64_t mask_stride, words; /* elements */
+  int64_t batch, total, n_heads, n_kv_heads, head_dim, dtype;
+  double scale;
+  void* out;
+  int64_t out_strides[2]; /* node, head */
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+} af_tree_attention_args;
+
+int af_tree_attention(const af_tree_attention_args* a, uint32_t* status, void* stream);
+
+/* Bytes of scratch that af_tree_attention needs on the current device. */
+int af_tree_attention_workspace_bytes(int64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
