@@ -875,6 +875,25 @@ int make_tmap_bf16_heads(CUtensorMap* map, const void* base, uint64_t rows, uint
   return AF_OK;
 }
 
+int make_tmap_strided16(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims, const uint64_t* strides,
+                        const uint32_t* box) {
+  PFN_encodeTiled_t fn = encode_fn();
+  if (!fn) return fail(AF_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t gdim[5], gstride[4];
+  cuuint32_t bx[5], estr[5];
+  for (int i = 0; i < rank; ++i) {
+    gdim[i] = dims[i];
+    bx[i] = box[i];
+    estr[i] = 1;
+    if (i + 1 < rank) gstride[i] = strides[i];
+  }
+  CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void*>(base), gdim, gstride, bx,
+                  estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AF_ERR_ARG, "cuTensorMapEncodeTiled (strided) failed (" + std::to_string((int)r) + ")");
+  return AF_OK;
+}
+
 // Row capacities that are multiples of 512 (>= 1024) take 512-token tiles
 // where their (weight tile, token tile) CTAs fill at least two waves of one
 // CTA per SM: two 256-token MMAs per stage, staged and stored 256 tokens at a

@@ -310,5 +310,10 @@ int make_tmap_bf16_tiled(CUtensorMap* map, const void* base, uint64_t rows, uint
 // box 64 columns x 128 rows x 1 matrix, 128-byte swizzle; rows past `rows`
 // read as zeros.
 int make_tmap_bf16_heads(CUtensorMap* map, const void* base, uint64_t rows, uint64_t depth);
+// Map over a strided tensor of fp16 or bf16 values, dimensions innermost
+// first (strides of all but the innermost in bytes, multiples of 16), with the given
+// box (64 values wide), 128-byte swizzle; places outside read as zeros.
+int make_tmap_strided16(CUtensorMap* map, const void* base, bool bf16, int rank, const uint64_t* dims, const uint64_t* strides,
+                        const uint32_t* box);
 
 }  // namespace af

@@ -276,7 +276,7 @@ def _aligned(t: torch.Tensor) -> bool:
     if t.stride(-1) != 1 or t.data_ptr() & 15:
         return False
     unit = 16 // t.element_size()
-    return all(n == 1 or s % unit == 0 for n, s in zip(t.shape[:-1], t.stride()))
+    return all(n == 1 or (s > 0 and s % unit == 0) for n, s in zip(t.shape[:-1], t.stride()))
 
 
 def tree_attention(
