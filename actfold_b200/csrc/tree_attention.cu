@@ -4,7 +4,7 @@
 // group) of its tree attend to the cached prefix and to the visible nodes of
 // the tree. With few rows per head the work is one pass over the prefix's
 // keys and values, so the products are transposed: the 128 KEYS of a tile are
-// the M side of the tensor-core instruction and the rows (64 or 128 of them)
+// the M side of the tensor-core instruction and the rows (16 to 128 of them)
 // its N side,
 //   S^T [128 keys, rows] = K Q^T,       O^T [dim, rows] += V^T P^T,
 // so a tile with 7 rows costs the exponentials of 8 rows, not of 128.
@@ -16,14 +16,20 @@
 // share evenly whatever the lengths are; a row that several CTAs worked on is
 // joined by k_tree_attention_join from their partial sums.
 //
-// Warps 0-7 run the softmax (warp w: TMEM lanes 32 (w & 3).. = keys, columns
-// of half w >> 2), warp 8 loads (TMA), warp 9 issues the products. A column's
+// Warps 0-15 run the softmax: four groups of 128 threads (thread = key = TMEM
+// lane), of which 1, 2 or 4 share the columns of a tile; the others work on the
+// next tiles with maxima, sums and an O of their own (kPipes of them, joined at the
+// end of a row), which hides the latency of a tile's chain of load, product,
+// exponential, product. Warp 16 loads Q and K, warp 17 V (TMA; an issue takes
+// a warp some 80 cycles), warp 18 issues S, warp 19 issues O. A column's
 // reference maximum m is raised only when a score passes it by more than 2^8
 // (or at the row's first key): steady tiles take one comparison per score and one
 // barrier vote, no maximum across lanes. P then stays below 256, which bf16
 // and fp16 round with the same relative error. Sums and O are fp32. Every wait is
 // bounded; a timeout sets AF_STATUS_TIMEOUT.
 #include <cuda.h>
+
+#include <atomic>
 
 #include "tree.cuh"
 
@@ -33,8 +39,10 @@ namespace {
 
 constexpr int kKeys = 128;                  // keys per tile (MMA M)
 constexpr int kHalf = kKeys * 128;          // [128 rows][64 columns] of 16 bits, 128-byte swizzle
-constexpr int kSoft = 8;                    // softmax warps
-constexpr int kThreads = (kSoft + 2) * 32;
+constexpr int kSoft = 16;                   // softmax warps
+constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMmaS = kSoft + 2, kMmaO = kSoft + 3;
+constexpr int kThreads = (kSoft + 4) * 32;
+constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
 constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
 constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
 
@@ -42,18 +50,27 @@ constexpr float kRaise = 8.f;               // log2 headroom before a reference 
 // goes over its keys, which nobody needs once S is there.
 template <int N, int HD>
 struct Shape {
+  static constexpr int kCols = N < 32 ? N : 32;     // columns of a softmax thread
+  static constexpr int kGroups = N / kCols;         // groups of 128 threads per tile
+  static constexpr int kPipes = 4 / kGroups;        // tiles that are worked on at once
+  static constexpr int kS = N == 128 ? 2 : 4;       // S buffers in TMEM
+  static constexpr int kTmem = (kS + 2 * kPipes) * N <= 256 ? 256 : 512;  // S, then O [2 segments][kPipes]
   static constexpr int kHalves = HD / 64;
-  static constexpr int kPBytes = (N / 64) * kHalf;  // [128 keys][64 rows] blocks
+  static constexpr int kPitch = N < 64 ? 2 * N : 128;         // bytes of a key's row of P^T (blocks of 64 rows where there are more)
+  static constexpr int kPBytes = (N < 64 ? 1 : N / 64) * kKeys * kPitch;
   static constexpr int kKBytes = kHalves * kHalf > kPBytes ? kHalves * kHalf : kPBytes;
   static constexpr int kStage = kKBytes + kHalves * kHalf;
-  static constexpr int kStages = (192 * 1024) / kStage;
+  // At most kPipes + kS, so that a tile with its S there has all products of O behind it but those of the last kPipes + kS - 1
+  // tiles: a wait for the pipe's last one is then never two phases ahead.
+  static constexpr int kStages = (192 * 1024) / kStage < kPipes + kS ? (192 * 1024) / kStage : kPipes + kS;
   static constexpr int kQBytes = kHalves * N * 128;
   static constexpr int kQ = kQBytes <= 16384 ? 2 : 1;         // Q buffers
   static constexpr int kOffQ = kStages * kStage;
-  static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [N] reference maxima
-  static constexpr int kOffRed = kOffM + N * 4;               // [4][N] per-warp maxima or sums; row 0: factors, row sums
-  static constexpr int kOffBar = kOffRed + 4 * N * 4;
-  static constexpr int kBytes = kOffBar + 384;
+  static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
+  static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
+  static constexpr int kOffBar = kOffRed + kPipes * 4 * N * 4;
+  static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4;
+  static constexpr int kBytes = kOffBar + kBars * 8 + 32 + kThreads / 32 * 8;
 };
 
 struct Params {
@@ -94,6 +111,21 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   return r;
 }
 
+// a / b of positive numbers, mostly small ones.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
+// The list of tiles cut into one share per CTA: the first `more` shares have each + 1.
+struct Shares {
+  int64_t each, more;
+  __device__ __forceinline__ int64_t begin(int64_t i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int64_t owner(int64_t t) const {
+    const int64_t big = more * (each + 1);
+    return t < big ? quotient(t, each + 1) : more + quotient(t - big, each);
+  }
+};
+
 // The tiles [k0, k1) of one row tile that a CTA works on.
 struct Segment {
   Request r;
@@ -103,24 +135,34 @@ struct Segment {
 };
 
 struct Walk {
-  int64_t t, end, before;  // next tile, last one, tiles of the requests before b
+  int64_t t, end, before;  // next tile, end of the share, tiles of the requests before b
   int b;
+  // A row of up to kWhole tiles belongs to the CTA whose share it begins in.
   __device__ __forceinline__ bool next(const Params& p, Segment& s) {
-    if (t >= end) return false;
-    s.r = request(p, b);
-    while (t >= before + s.r.tiles(p.kv_heads)) {
-      before += s.r.tiles(p.kv_heads);
-      s.r = request(p, ++b);
+    while (true) {
+      if (t >= end) return false;
+      s.r = request(p, b);
+      while (t >= before + s.r.tiles(p.kv_heads)) {
+        before += s.r.tiles(p.kv_heads);
+        s.r = request(p, ++b);
+      }
+      const int64_t rel = t - before;
+      const int64_t row = quotient(rel, s.r.kt);
+      s.k0 = (int)(rel - row * s.r.kt);
+      s.row_end = before + (row + 1) * s.r.kt;
+      if (s.r.kt <= kWhole) {
+        t = s.row_end;
+        if (s.k0 > 0) continue;
+        s.k1 = s.r.kt;
+      } else {
+        s.k1 = (int)min((int64_t)s.r.kt, s.k0 + (end - t));
+        t += s.k1 - s.k0;
+      }
+      const int64_t head = quotient(row, s.r.qt);
+      s.kvh = (int)head;
+      s.qt = (int)(row - head * s.r.qt);
+      return true;
     }
-    const int64_t rel = t - before;
-    const int64_t row = rel / s.r.kt;
-    s.k0 = (int)(rel - row * s.r.kt);
-    s.k1 = (int)min((int64_t)s.r.kt, s.k0 + (end - t));
-    s.qt = (int)(row % s.r.qt);
-    s.kvh = (int)(row / s.r.qt);
-    s.row_end = before + (row + 1) * s.r.kt;
-    t += s.k1 - s.k0;
-    return true;
   }
 };
 
@@ -132,6 +174,19 @@ struct Started {
 
 // Workspace: Started[ctas], then per CTA two partial rows (0: begun by an
 // earlier CTA, 1: begun here) of [N][HD] fp32 sums and [N] (maximum, sum) pairs.
+// P^T [128 keys][N rows] in shared memory: rows of kPitch bytes whose 16-byte
+// pieces are swizzled over as many bytes (32, 64 or 128), N >= 64 as blocks of 64.
+template <int N>
+__device__ __forceinline__ uint64_t p_desc(uint32_t at) {
+  constexpr uint64_t pitch = N < 64 ? 2 * N : 128, swizzle = N == 16 ? 6 : N == 32 ? 4 : 2;
+  return (uint64_t)((at & 0x3ffffu) >> 4) | (uint64_t)(kHalf >> 4) << 16 | (8 * pitch >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
+}
+template <int N>
+__device__ __forceinline__ uint32_t p_piece(int key, int col) {  // byte offset of columns col .. col + 7 (a multiple of 8)
+  constexpr int pieces = N < 64 ? N / 8 : 8, shift = N == 16 ? 2 : N == 32 ? 1 : 0;
+  return col / 64 * kHalf + key * (16 * pieces) + 16 * ((col / 8 % pieces) ^ ((key >> shift) % pieces));
+}
+
 template <int N, int HD>
 struct Scratch {
   char* base;
@@ -162,10 +217,52 @@ __device__ __forceinline__ uint16_t to_bits(float x) {
   return (uint16_t)pack2<DT>(x, 0.f);
 }
 
+__device__ __forceinline__ bool elect_one() {
+  int r;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
   return e;
+}
+
+// Pairs of fp32 values in one register pair (two results per instruction).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* failed) {
+  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, failed);
+}
+
+// Lane i's 32 bits become bit i of every lane's word.
+__device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
+#pragma unroll
+  for (uint32_t k = 16, m = 0x0000ffffu; k > 0; k >>= 1, m ^= m << k) {
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, k);
+    x = lane & k ? ((y >> k) & m) | (x & ~m) : (x & m) | ((y & m) << k);
+  }
+  return x;
 }
 
 template <int THREADS>
@@ -182,16 +279,36 @@ __device__ __forceinline__ bool vote_any(int bar, bool mine) {
   return r != 0;
 }
 
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+// C consecutive columns of the thread's TMEM lane. Load and wait are one
+// statement: nothing that reads the registers can be placed between them.
+template <int C>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
+  if constexpr (C == 8) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+  } else if constexpr (C == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+  } else {
+    static_assert(C == 32, "columns");
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                   "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+  }
+}
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
@@ -201,31 +318,111 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// 32 values per lane reduced across the warp: lane j returns the result of
-// values j. Each step halves the values that a lane keeps (31 exchanges, where
-// a reduction per value takes 160).
-template <typename Op>
+// C values per lane (16 or 32) reduced across the warp: lane x returns the
+// result of value x * C / 32. Each step halves the values that a lane keeps
+// (C - 1 exchanges and one more where C is 16; a reduction per value takes 5 C).
+template <int C, typename Op>
 __device__ __forceinline__ float transpose_reduce(float* v, int lane, Op op) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int o = 16, n = C / 2; n > 0; o >>= 1, n >>= 1) {
     const bool up = (lane & o) != 0;
 #pragma unroll
-    for (int i = 0; i < o; ++i) {
-      const float give = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+    for (int i = 0; i < n; ++i) {
+      const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
       v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
     }
   }
-  return v[0];
+  return C == 32 ? v[0] : op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
 }
 
 // Bits of the warp's 32 keys (nodes j0, j0 + 1, ... of the tree) that node i
 // sees; a bit outside the tree means nothing.
-__device__ __forceinline__ uint32_t seen_bits(const Params& p, const Segment& s, int i, int j0) {
+__device__ __forceinline__ uint32_t seen_bits(const Params& p, int s0, int i, int j0) {
   if (!p.mask) return i < j0 ? 0u : i - j0 >= 31 ? 0xffffffffu : (2u << (i - j0)) - 1u;
-  const uint32_t* row = p.mask + (int64_t)(s.r.s0 + i) * p.mask_ld;
+  const uint32_t* row = p.mask + (int64_t)(s0 + i) * p.mask_ld;
   const int w = j0 >> 5;  // j0 may be negative: rounds down
   const uint32_t lo = w >= 0 && w < p.words ? row[w] : 0u, hi = w + 1 >= 0 && w + 1 < p.words ? row[w + 1] : 0u;
   return __funnelshift_r(lo, hi, j0 & 31);
+}
+
+// The values of dim d that are not finite among nodes [x0, x1) that node i sees, added up.
+template <int DT>
+__device__ __noinline__ float set_aside_sum(const Params& p, int s0, int kvh, int i, int x0, int x1, int d) {
+  float sum = 0.f;
+  for (int x = x0; x < x1; ++x) {
+    const float y = load_scalar<DT>(p.v_rows + (int64_t)(s0 + x) * p.v_n + kvh * p.v_h, d);
+    if (!isfinite(y) && (seen_bits(p, s0, i, x) & 1u)) sum += y;
+  }
+  return sum;
+}
+
+// Loads of one operand by a warp: K (with the Q of each segment) or V.
+template <int N, int HD, bool VALUES>
+__device__ __forceinline__ bool load_tiles(const Params& p, Walk walk, uint32_t base, uint32_t full, uint32_t empty, uint32_t q_full,
+                                           uint32_t q_empty, volatile int* failed) {
+  using S = Shape<N, HD>;
+  const int lane = threadIdx.x & 31;
+  const CUtensorMap* cache = VALUES ? &p.vc : &p.kc;
+  const CUtensorMap* tree_rows = VALUES ? &p.v : &p.k;
+  // Lane (box, half) loads rows [box * R, (box + 1) * R) of each tile; the page is fetched a tile ahead.
+  const int box = lane / S::kHalves, half = lane % S::kHalves, row = box * p.box;
+  const bool in_use = row < kKeys;
+  int j = 0, seg = 0;
+  bool ok = true;
+  Segment s;
+  while (ok && walk.next(p, s)) {
+    if constexpr (!VALUES) {
+      const int qb = seg % S::kQ, use = seg / S::kQ;
+      if (use > 0) ok = __all_sync(0xffffffffu, wait_for(q_empty + 8 * qb, (use - 1) & 1, failed));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(q_full + 8 * qb, S::kHalves * p.nt * p.group * 128);
+        for (int h = 0; h < S::kHalves; ++h)
+          tma_load_3d(base + S::kOffQ + qb * S::kQBytes + h * N * 128, &p.q, q_full + 8 * qb, 64 * h, s.kvh * p.group, s.r.s0 + s.qt * p.nt);
+      }
+      __syncwarp();
+      ++seg;
+    }
+    const int* table = p.tables + (int64_t)walk.b * p.tables_ld;
+    auto page_of = [&](int kt) {
+      const int key = kt * kKeys + row;
+      return in_use && kt < s.k1 && key < s.r.len ? table[key / p.page] : 0;
+    };
+    int page = page_of(s.k0);
+    for (int kt = s.k0; kt < s.k1; ++kt, ++j) {
+      const int key = kt * kKeys + row, node = key - s.r.pad;
+      const bool cached = in_use && key < s.r.len, tree = in_use && node >= 0 && node < s.r.n;
+      if (cached && (page < 0 || page >= p.pages)) {
+        if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+        page = p.pages;  // out of range: the box reads as zeros
+      }
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, cached || tree)) * p.box * 128;
+      const int off = cached ? key % p.page : 0;
+      const int stage = j % S::kStages, round = j / S::kStages;
+      if (round > 0) ok = __all_sync(0xffffffffu, wait_for(empty + 8 * stage, (round - 1) & 1, failed));
+      if (!ok) break;
+      const uint32_t bar = full + 8 * stage;
+      if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+      __syncwarp();
+      const uint32_t dst = base + stage * S::kStage + (VALUES ? S::kKBytes : 0) + half * kHalf + row * 128;
+      if (cached) tma_load_4d(dst, cache, bar, 64 * half, s.kvh, off, page);
+      else if (tree) tma_load_3d(dst, tree_rows, bar, 64 * half, s.kvh, s.r.s0 + node);
+      page = page_of(kt + 1);
+    }
+  }
+  if (!ok) {
+    *failed = 1;
+    if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+  }
+  __syncwarp();
+  if (*failed && lane == 0) {
+    // Copies still in flight land before the CTA's shared memory is given up (bounded).
+    volatile int no_abort = 0;
+    for (int i = max(0, j - S::kStages); i < j; ++i) mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
+    if (!VALUES)
+      for (int i = max(0, seg - S::kQ); i < seg; ++i) mbar_wait(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
+  }
+  return ok;
 }
 
 template <int DT, int N, int HD>
@@ -235,19 +432,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_u32(gb), sQ = base + S::kOffQ;
-  auto sK = [&](int stage) { return base + stage * S::kStage; };
-  auto sV = [&](int stage) { return base + stage * S::kStage + S::kKBytes; };
-  // K full, V full, stage empty [stages]; then pairs: Q full, Q empty, S full, P full, O of a tile done, O full, O empty
-  const uint32_t k_full = base + S::kOffBar, v_full = k_full + 8 * S::kStages, empty = v_full + 8 * S::kStages,
-                 q_full = empty + 8 * S::kStages, q_empty = q_full + 16, s_full = q_empty + 16, p_full = s_full + 16,
-                 done = p_full + 16, o_full = done + 16, o_empty = o_full + 16;
-  static_assert(24 * S::kStages + 7 * 16 <= 256, "barriers");
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffBar + 256);
-  volatile int* failed = reinterpret_cast<volatile int*>(gb + S::kOffBar + 260);
-  int* found_b = reinterpret_cast<int*>(gb + S::kOffBar + 264);
-  int64_t* found = reinterpret_cast<int64_t*>(gb + S::kOffBar + 272);  // tiles before request found_b
-  int64_t* scan = reinterpret_cast<int64_t*>(gb + S::kOffBar + 280);   // sums of the warps
-  static_assert(280 + 8 * kThreads / 32 <= 384, "scan");
+  const uint32_t k_full = base + S::kOffBar, v_full = k_full + 8 * S::kStages, empty = v_full + 8 * S::kStages, q_full = empty + 8 * S::kStages,
+                 q_empty = q_full + 16, s_full = q_empty + 16, p_full = s_full + 8 * S::kS, done = p_full + 8 * S::kS, o_full = done + 8 * S::kS,
+                 o_empty = o_full + 16;
+  uint8_t* misc = gb + S::kOffBar + 8 * S::kBars;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
+  volatile int* failed = reinterpret_cast<volatile int*>(misc + 4);
+  int* found_b = reinterpret_cast<int*>(misc + 8);
+  int64_t* found = reinterpret_cast<int64_t*>(misc + 16);  // tiles before request found_b
+  int64_t* scan = reinterpret_cast<int64_t*>(misc + 32);   // sums of the warps
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -255,19 +448,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       mbar_init(v_full + 8 * i, 1);
       mbar_init(empty + 8 * i, 1);
     }
+    for (int i = 0; i < S::kS; ++i) {
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4 * S::kGroups);
+      mbar_init(done + 8 * i, 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + 8 * i, 1);
       mbar_init(q_empty + 8 * i, 1);
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, kSoft);
-      mbar_init(done + 8 * i, 1);
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, kSoft);
     }
     *failed = 0;
     fence_barrier_init();
   }
-  if (warp == kSoft) tmem_alloc(smem_u32(tmem_slot), 4 * N);
+  if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
 
   // This CTA's share [t0, t1) of the list of tiles, and the request it begins with.
   const int per = (p.batch + kThreads - 1) / kThreads, b_lo = min(p.batch, tid * per), b_hi = min(p.batch, b_lo + per);
@@ -288,13 +483,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   __syncthreads();
   tc_fence_after();
   int64_t all = 0, at = upto - mine;
-#pragma unroll
+#pragma unroll 4
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) at += scan[w];
     all += scan[w];
   }
-  const int64_t ctas = min((int64_t)gridDim.x, all);
-  const int64_t t0 = blockIdx.x < ctas ? all * blockIdx.x / ctas : 0, t1 = blockIdx.x < ctas ? all * (blockIdx.x + 1) / ctas : 0;
+  Shares shares;
+  shares.each = quotient(all, gridDim.x);
+  shares.more = all - shares.each * gridDim.x;
+  const int64_t t0 = shares.begin(blockIdx.x), t1 = shares.begin(blockIdx.x + 1);
   if (t0 < t1 && at <= t0 && t0 < at + mine) {
     for (int b = b_lo; b < b_hi; ++b) {
       const int64_t w = request(p, b).tiles(p.kv_heads);
@@ -315,297 +512,237 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   walk.b = t0 < t1 ? *found_b : 0;
   walk.before = t0 < t1 ? *found : 0;
   Segment s;
+  constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
+  auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
 
-  if (warp == kSoft) {
-    // ---------------- loads: Q of a segment, then K and V of its tiles into the stages ----------------
-    const int boxes = kKeys / p.box;
-    int j = 0, seg = 0;
+  if (warp == kLoadK) {
+    load_tiles<N, HD, false>(p, walk, base, k_full, empty, q_full, q_empty, failed);
+  } else if (warp == kLoadV) {
+    load_tiles<N, HD, true>(p, walk, base, v_full, empty, q_full, q_empty, failed);
+  } else if (warp == kMmaS) {
+    // ---------------- S^T of every tile ----------------
+    // The whole warp keeps the books, one lane issues: descriptors stay in uniform registers.
+    constexpr uint32_t id_s = idesc_bf16(kKeys, N) ^ kind;
+    const uint64_t d_k = sw128_desc(base), d_q = sw128_desc(sQ);
     bool ok = true;
+    int j = 0, seg = 0, stage = 0, stage_phase = 0;
     while (ok && walk.next(p, s)) {
-      const int qb = seg % S::kQ, use = seg / S::kQ;
-      if (use > 0) ok = mbar_wait(q_empty + 8 * qb, (use - 1) & 1, failed);
-      if (!ok) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(q_full + 8 * qb, S::kHalves * p.nt * p.group * 128);
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_load_3d(sQ + qb * S::kQBytes + h * N * 128, &p.q, q_full + 8 * qb, 64 * h, s.kvh * p.group, s.r.s0 + s.qt * p.nt);
-      }
-      ++seg;
-      // Lane (box, half) loads rows [box * R, (box + 1) * R) of each tile; the page is fetched a tile ahead.
-      const int box = lane / S::kHalves, half = lane % S::kHalves, row = box * p.box;
-      const int* table = p.tables + (int64_t)walk.b * p.tables_ld;
-      auto page_of = [&](int kt) {
-        const int key = kt * kKeys + row;
-        return box < boxes && kt < s.k1 && key < s.r.len ? table[key / p.page] : 0;
-      };
-      int page = page_of(s.k0);
-      for (int kt = s.k0; kt < s.k1; ++kt, ++j) {
-        const int key = kt * kKeys + row;
-        const int node = key - s.r.pad;
-        const bool cached = box < boxes && key < s.r.len, tree = box < boxes && node >= 0 && node < s.r.n;
-        if (cached && (page < 0 || page >= p.pages)) {
-          if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-          page = p.pages;  // out of range: the box reads as zeros
-        }
-        const unsigned who = __ballot_sync(0xffffffffu, cached || tree);
-        const uint32_t bytes = __popc(who) * p.box * 128;
-        const int off = cached ? key % p.page : 0;
-        const int stage = j % S::kStages, round = j / S::kStages;
-        if (round > 0) ok = mbar_wait(empty + 8 * stage, (round - 1) & 1, failed);
-        ok = __all_sync(0xffffffffu, ok);
+      const int qb = seg % S::kQ;
+      ok = agreed(wait_for(q_full + 8 * qb, (seg / S::kQ) & 1, failed));
+      const uint64_t b = d_q + (uint32_t)qb * (S::kQBytes >> 4);
+      for (int kt = s.k0; ok && kt < s.k1; ++kt, ++j) {
+        const int sb = j % S::kS;
+        ok = agreed(wait_for(k_full + 8 * stage, stage_phase, failed));
+        if (ok && j >= S::kS) ok = agreed(wait_for(p_full + 8 * sb, (j / S::kS - 1) & 1, failed));  // S buffer sb is read
         if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(k_full + 8 * stage, bytes);
-          mbar_arrive_expect_tx(v_full + 8 * stage, bytes);
+        tc_fence_after();
+        const uint64_t a = d_k + (uint32_t)stage * (S::kStage >> 4);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            tc_mma_bf16(tmem + sb * N, a + (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3), b + (kk >> 2) * (N * 8) + 2 * (kk & 3), id_s, kk ? 1u : 0u);
+          tc_commit(s_full + 8 * sb);
+          if (kt + 1 == s.k1) tc_commit(q_empty + 8 * qb);
         }
         __syncwarp();
-        const uint32_t at = half * kHalf + row * 128;
-        if (cached) {
-          tma_load_4d(sK(stage) + at, &p.kc, k_full + 8 * stage, 64 * half, s.kvh, off, page);
-          tma_load_4d(sV(stage) + at, &p.vc, v_full + 8 * stage, 64 * half, s.kvh, off, page);
-        } else if (tree) {
-          tma_load_3d(sK(stage) + at, &p.k, k_full + 8 * stage, 64 * half, s.kvh, s.r.s0 + node);
-          tma_load_3d(sV(stage) + at, &p.v, v_full + 8 * stage, 64 * half, s.kvh, s.r.s0 + node);
+        if (++stage == S::kStages) {
+          stage = 0;
+          stage_phase ^= 1;
         }
-        page = page_of(kt + 1);
       }
+      ++seg;
     }
     if (!ok) {
       *failed = 1;
       if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
     }
-    __syncwarp();
-    if (*failed && lane == 0) {
-      // Copies still in flight land before the CTA's shared memory is given up (bounded).
-      volatile int no_abort = 0;
-      for (int i = max(0, j - S::kStages); i < j; ++i) {
-        mbar_wait(k_full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
-        mbar_wait(v_full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
-      }
-      for (int i = max(0, seg - S::kQ); i < seg; ++i) mbar_wait(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
-    }
-  } else if (warp == kSoft + 1 && lane == 0) {
-    // ---------------- products: S_j, then O += V P of tile j - 1 ----------------
-    constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // formats: bf16 = 1, f16 = 0
-    constexpr uint32_t id_s = idesc_bf16(kKeys, N) ^ kind;
+  } else if (warp == kMmaO) {
+    // ---------------- O^T += V^T P^T of every tile, into its pipe's O ----------------
     constexpr uint32_t id_o = (idesc_bf16(128, N) ^ kind) | (1u << 15) | (1u << 16);  // A and B MN-major
+    const uint64_t d_v = sw128_desc_mn(base + S::kKBytes, kHalf, 1024), d_p = p_desc<N>(base);
     bool ok = true;
-    int j = 0, seg = 0;
-    // State of tile j - 1 for its second product.
-    int last_seg = 0;
-    bool last_first = false, last_last = false;
-    auto second = [&](int i) {
-      const int pb = i & 1, stage = i % S::kStages, ob = last_seg & 1;
-      ok = mbar_wait(p_full + 8 * pb, (i >> 1) & 1, failed) && mbar_wait(v_full + 8 * stage, (i / S::kStages) & 1, failed);
-      if (ok && last_first && last_seg >= 2) ok = mbar_wait(o_empty + 8 * ob, ((last_seg >> 1) - 1) & 1, failed);
-      if (!ok) return;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < kKeys / 16; ++kk) {
-        const uint64_t a = sw128_desc_mn(sV(stage) + kk * 2048, kHalf, 1024);
-        const uint64_t b = sw128_desc_mn(sK(stage) + kk * 2048, kHalf, 1024);
-        tc_mma_bf16(tmem + 2 * N + ob * N, a, b, id_o, last_first && kk == 0 ? 0u : 1u);
-      }
-      tc_commit(empty + 8 * stage);
-      tc_commit(done + 8 * pb);
-      if (last_last) tc_commit(o_full + 8 * ob);
-    };
+    int j = 0, seg = 0, stage = 0, stage_phase = 0;
     while (ok && walk.next(p, s)) {
-      const int qb = seg % S::kQ;
+      const int ob = seg & 1;
+      if (seg >= 2) ok = agreed(wait_for(o_empty + 8 * ob, ((seg >> 1) - 1) & 1, failed));
       for (int kt = s.k0; ok && kt < s.k1; ++kt, ++j) {
-        const int sb = j & 1, stage = j % S::kStages;
-        // With one Q buffer the next rows arrive after the last S of these ones: do what is left first.
-        const bool early = S::kQ == 1 && kt == s.k0 && j > 0;
-        if (early) second(j - 1);
-        if (ok && kt == s.k0) ok = mbar_wait(q_full + 8 * qb, (seg / S::kQ) & 1, failed);
-        ok = ok && mbar_wait(k_full + 8 * stage, (j / S::kStages) & 1, failed);
-        // S buffer sb is read: P of tile j - 2 was waited for by its second product.
+        const int sb = j % S::kS, pipe = j % S::kPipes;
+        ok = agreed(wait_for(v_full + 8 * stage, stage_phase, failed)) && agreed(wait_for(p_full + 8 * sb, (j / S::kS) & 1, failed));
         if (!ok) break;
         tc_fence_after();
+        const uint64_t a = d_v + (uint32_t)stage * (S::kStage >> 4), b = d_p + (uint32_t)stage * (S::kStage >> 4);
+        const uint32_t o = tmem + (S::kS + ob * S::kPipes + pipe) * N;
+        const uint32_t add = kt - s.k0 < S::kPipes ? 0u : 1u;
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk) {
-          const uint64_t a = sw128_desc(sK(stage) + (kk >> 2) * kHalf) + 2 * (kk & 3);
-          const uint64_t b = sw128_desc(sQ + qb * S::kQBytes + (kk >> 2) * N * 128) + 2 * (kk & 3);
-          tc_mma_bf16(tmem + sb * N, a, b, id_s, kk ? 1u : 0u);
+          for (int kk = 0; kk < kKeys / 16; ++kk) tc_mma_bf16(o, a + kk * 128, b + kk * S::kPitch, id_o, kk ? 1u : add);
+          tc_commit(empty + 8 * stage);
+          tc_commit(done + 8 * sb);
+          if (kt + 1 == s.k1) tc_commit(o_full + 8 * ob);
         }
-        tc_commit(s_full + 8 * sb);
-        if (kt + 1 == s.k1) tc_commit(q_empty + 8 * qb);
-        if (j > 0 && !early) second(j - 1);
-        last_seg = seg;
-        last_first = kt == s.k0;
-        last_last = kt + 1 == s.k1;
+        __syncwarp();
+        if (++stage == S::kStages) {
+          stage = 0;
+          stage_phase ^= 1;
+        }
       }
       ++seg;
     }
-    if (ok && j > 0) second(j - 1);
     if (!ok) {
       *failed = 1;
-      if (p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+      if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
     }
-  } else if (warp < kSoft) {
-    // ---------------- softmax: key 32 * quad + lane, columns c0 .. c0 + C - 1 ----------------
-    constexpr int C = N / 2, G32 = C / 32;
-    const int quad = warp & 3, wg = warp >> 2, r = 32 * quad + lane, c0 = wg * C, wg_tid = tid - 128 * wg;
+  } else {
+    // ---------------- softmax: key 32 * quad + lane, columns c0 .. c0 + C - 1 of its pipe's tiles ----------------
+    constexpr int C = S::kCols, kTeam = 128;
+    const int quad = warp & 3, wg = warp >> 2, pipe = wg / S::kGroups, r = 32 * quad + lane, c0 = wg % S::kGroups * C;
+    const int team = 1 + wg, team_tid = tid - kTeam * wg;  // barrier of the threads with the same columns
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
-    float* m_ref = reinterpret_cast<float*>(gb + S::kOffM) + c0;
-    float* red = reinterpret_cast<float*>(gb + S::kOffRed) + c0;  // red[w * N + column]
-    float* factor = red;
+    float* m_all = reinterpret_cast<float*>(gb + S::kOffM);
+    float* red_all = reinterpret_cast<float*>(gb + S::kOffRed);
+    float* fac = m_all;
+    float* m_neg = m_all + pipe * N + c0;        // -(reference maximum) of the thread's columns
+    float* red = red_all + pipe * 4 * N + c0;    // red[quad * N + column]; row 0: factors of the old O
+    const int red_at = quad * N + lane * C / 32;
+    const uint64_t scale2 = pair(p.scale, p.scale);
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (!mbar_wait(bar, parity, failed)) *failed = 1;
+      if (!wait_for(bar, parity, failed)) *failed = 1;
     };
-    int j = 0, seg = 0;
+    int j0 = 0, seg = 0;  // tiles before this segment
     bool wrote_start = false;
     while (walk.next(p, s)) {
-      const int nodes = min(p.nt, s.r.n - s.qt * p.nt), cols = nodes * p.group;
-      const int live = min(C, max(0, cols - c0));  // columns of this half that are rows
-      float l[C];
+      const int cols = min(p.nt, s.r.n - s.qt * p.nt) * p.group;
+      const int live = min(C, max(0, cols - c0));  // columns of this thread that are rows
+      uint64_t l[C / 2];                           // this key's part of the sums
 #pragma unroll
-      for (int i = 0; i < C; ++i) l[i] = 0.f;
-      if (wg_tid < C) m_ref[wg_tid] = kUnset;
-      bool sick = false;  // a visible value that is not finite was set aside
-      named_bar_sync(1 + wg, 128);
-      for (int kt = s.k0; kt < s.k1; ++kt, ++j) {
-        const int sb = j & 1, stage = j % S::kStages, key0 = kt * kKeys, key = key0 + r;
+      for (int i = 0; i < C / 2; ++i) l[i] = 0ull;
+      if (team_tid < C) m_neg[team_tid] = -kUnset;
+      bool sick = false, begun = false;  // a drafted value that is not finite was set aside; this pipe's O holds something
+      named_bar_sync(team, kTeam);
+      const int tiles = s.k1 - s.k0;
+      for (int i0 = (pipe + S::kPipes - j0 % S::kPipes) % S::kPipes; i0 < tiles; i0 += S::kPipes) {
+        const int j = j0 + i0, sb = j % S::kS, stage = j % S::kStages;
+        const int key0 = (s.k0 + i0) * kKeys, key = key0 + r, node = key - s.r.pad;
         const bool masked = key0 + kKeys > s.r.len;
-        uint32_t vis[G32];
-        if (masked) {
-          const int node = key - s.r.pad, j0 = key0 + 32 * quad - s.r.pad;
-          const bool in_prefix = key < s.r.len, in_tree = node >= 0 && node < s.r.n;
-#pragma unroll
-          for (int g = 0; g < G32; ++g) {
-            const int c = c0 + 32 * g + lane;
-            const uint32_t bits = c < cols ? seen_bits(p, s, s.qt * p.nt + c / p.group, j0) : 0u;
-            uint32_t v = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v |= ((__shfl_sync(0xffffffffu, bits, i) >> lane) & 1u) << i;
-            vis[g] = in_prefix ? 0xffffffffu : in_tree ? v : 0u;
-          }
-        }
-        wait(s_full + 8 * sb, (j >> 1) & 1);
+        const bool in_prefix = key < s.r.len, in_tree = node >= 0 && node < s.r.n;
+        const uint32_t stage_at = base + stage * S::kStage;
+        // S of this tile also says that its stage was loaded, so the wait for its V below is at most one phase ahead.
+        wait(s_full + 8 * sb, (j / S::kS) & 1);
         tc_fence_after();
-        uint32_t x[C];
-        auto load_scores = [&]() {
-#pragma unroll
-          for (int g = 0; g < G32; ++g)
-            if (32 * g < live) tmem_ld32_nowait(lanes + sb * N + c0 + 32 * g, x + 32 * g);
-          tmem_wait_ld();
-        };
-        load_scores();
-        // x = score - reference maximum (in log2 units); hidden scores -inf.
-        float top = -INFINITY;
-        auto shift = [&]() {
-#pragma unroll
-          for (int q8 = 0; q8 < C / 8; ++q8) {
-            if (8 * q8 < live) {
-              const float4 m0 = *reinterpret_cast<const float4*>(m_ref + 8 * q8), m1 = *reinterpret_cast<const float4*>(m_ref + 8 * q8 + 4);
-              const float mm[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int c = 8 * q8 + i;
-                float y = fmaf(__uint_as_float(x[c]), p.scale, -mm[i]);
-                if (masked) y = (vis[c >> 5] >> (c & 31)) & 1u ? y : -INFINITY;
-                top = fmaxf(top, y);
-                x[c] = __float_as_uint(y);
-              }
-            }
-          }
-        };
-        shift();
-        if (vote_any<128>(1 + wg, top > kRaise)) {
-          // New maxima of the columns that need one, from the scores themselves.
-          load_scores();
-#pragma unroll
-          for (int g = 0; g < G32; ++g) {
-            if (32 * g < live) {
-              float y[32];
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                y[i] = __uint_as_float(x[32 * g + i]) * p.scale;
-                if (masked) y[i] = (vis[g] >> i) & 1u ? y[i] : -INFINITY;
-              }
-              red[quad * N + 32 * g + lane] = transpose_reduce(y, lane, [](float a, float b) { return fmaxf(a, b); });
-            }
-          }
-          named_bar_sync(1 + wg, 128);
-          if (wg_tid < live) {
-            const float t = fmaxf(fmaxf(red[wg_tid], red[N + wg_tid]), fmaxf(red[2 * N + wg_tid], red[3 * N + wg_tid]));
-            const float old = m_ref[wg_tid];
-            const bool raise = old == kUnset ? t > kUnset : t > old + kRaise;
-            factor[wg_tid] = raise ? (old == kUnset ? 0.f : exp2f(old - t)) : 1.f;
-            if (raise) m_ref[wg_tid] = t;
-          }
-          named_bar_sync(1 + wg, 128);
-          if (kt > s.k0) {
-            // O of the tiles before this one is complete once the product of tile j - 1 is.
-            wait(done + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);
-            tc_fence_after();
-#pragma unroll
-            for (int g = 0; g < G32; ++g) {
-              if (32 * g < live) {
-                uint32_t o[32];
-                const uint32_t addr = lanes + 2 * N + (seg & 1) * N + c0 + 32 * g;
-                tmem_ld32_nowait(addr, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                  const float f = 32 * g + i < live ? factor[32 * g + i] : 1.f;
-                  o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  l[32 * g + i] *= f;
-                }
-                tmem_store32(addr, o);
-              }
-            }
-          }
-          load_scores();
-          shift();
-        }
+        uint32_t vis = 0xffffffffu;  // bit i: column c0 + i sees this key
         if (masked) {
+          const int c = c0 + lane;
+          vis = transpose_bits(lane < C && c < cols ? seen_bits(p, s.r.s0, s.qt * p.nt + c / p.group, node - lane) : 0u, lane);
+          vis = in_prefix ? 0xffffffffu : in_tree ? vis : 0u;
           // Rows of V without a key are whatever lay there: cleared. A drafted value that is not finite would reach
           // every column as 0 * inf: it is cleared too, and added at the end to the columns that see it.
-          const int node = key - s.r.pad;
-          const bool in_prefix = key < s.r.len, in_tree = node >= 0 && node < s.r.n;
           wait(v_full + 8 * stage, (j / S::kStages) & 1);
-          if (wg < S::kHalves) {
-            const uint32_t row = sV(stage) + wg * kHalf + r * 128;
-            if (!in_prefix && !in_tree) {
-#pragma unroll
-              for (int c = 0; c < 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + 16 * (c ^ (r & 7))), "r"(0) : "memory");
-            } else if (in_tree) {
-              constexpr uint32_t e = DT == AF_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll
-              for (int c = 0; c < 8; ++c) {
-                const uint32_t where = row + 16 * (c ^ (r & 7));
-                uint32_t w[4];
+          if (!in_prefix) {
+            constexpr uint32_t e = DT == AF_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll 1
+            for (int c16 = c0 / C; c16 < 8 * S::kHalves; c16 += S::kGroups) {
+              const uint32_t where = stage_at + S::kKBytes + (c16 >> 3) * kHalf + r * 128 + 16 * ((c16 & 7) ^ (r & 7));
+              uint32_t w[4] = {0u, 0u, 0u, 0u};
+              bool bad = !in_tree;
+              if (in_tree) {
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(where) : "memory");
-                bool bad = false;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   const bool lo = (w[i] & e) == e, hi = ((w[i] >> 16) & e) == e;
                   w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
                   bad |= lo || hi;
                 }
-                if (bad) {
-                  sick = true;
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(where), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
-                }
+                sick |= bad;
               }
+              if (bad)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(where), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
             }
           }
         }
+        uint32_t x[C];
+        // x = score - reference maximum (in log2 units); hidden scores -inf.
+        float top = -INFINITY;
+        auto shift = [&]() {
+          tmem_load<C>(lanes + sb * N + c0, x);
+#pragma unroll
+          for (int q8 = 0; q8 < C / 8; ++q8) {
+            if (8 * q8 < live) {
+#pragma unroll
+              for (int q = 8 * q8; q < 8 * q8 + 8; q += 4) {
+                const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(m_neg + q);
+                const float2 y0 = unpair(fma2(pair(__uint_as_float(x[q]), __uint_as_float(x[q + 1])), scale2, m.x));
+                const float2 y1 = unpair(fma2(pair(__uint_as_float(x[q + 2]), __uint_as_float(x[q + 3])), scale2, m.y));
+                x[q] = __float_as_uint(y0.x);
+                x[q + 1] = __float_as_uint(y0.y);
+                x[q + 2] = __float_as_uint(y1.x);
+                x[q + 3] = __float_as_uint(y1.y);
+                top = fmaxf(top, fmaxf(y0.x, y0.y));
+                top = fmaxf(top, fmaxf(y1.x, y1.y));
+              }
+            }
+          }
+          if (masked) {
+            top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+              if (!((vis >> i) & 1u)) x[i] = 0xff800000u;
+              if (i < live) top = fmaxf(top, __uint_as_float(x[i]));
+            }
+          }
+        };
+        shift();
+        if (vote_any<kTeam>(team, top > kRaise)) {
+          // New maxima of the columns that need one, from the scores themselves.
+          tmem_load<C>(lanes + sb * N + c0, x);
+          float y[C];
+#pragma unroll
+          for (int i = 0; i < C; ++i) y[i] = (vis >> i) & 1u ? __uint_as_float(x[i]) * p.scale : -INFINITY;
+          red[red_at] = transpose_reduce<C>(y, lane, [](float a, float b) { return fmaxf(a, b); });
+          named_bar_sync(team, kTeam);
+          if (team_tid < C) {
+            const float t = fmaxf(fmaxf(red[team_tid], red[N + team_tid]), fmaxf(red[2 * N + team_tid], red[3 * N + team_tid]));
+            const float old = -m_neg[team_tid];
+            const bool raise = old == kUnset ? t > kUnset : t > old + kRaise;
+            red[team_tid] = raise ? (old == kUnset ? 0.f : exp2f(old - t)) : 1.f;
+            if (raise) m_neg[team_tid] = -t;
+          }
+          named_bar_sync(team, kTeam);
+          if (begun) {
+            // O of the pipe's tiles before this one is complete once the last one's product is.
+            const int jb = j - S::kPipes;
+            wait(done + 8 * (jb % S::kS), (jb / S::kS) & 1);
+            tc_fence_after();
+#pragma unroll
+            for (int q8 = 0; q8 < C / 8; ++q8) {
+              if (8 * q8 < live) {
+                uint32_t o[8];
+                const uint32_t addr = lanes + (S::kS + (seg & 1) * S::kPipes + pipe) * N + c0 + 8 * q8;
+                tmem_load<8>(addr, o);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = *reinterpret_cast<const float2*>(red + 8 * q8 + 2 * i);
+                  o[2 * i] = __float_as_uint(__uint_as_float(o[2 * i]) * f.x);
+                  o[2 * i + 1] = __float_as_uint(__uint_as_float(o[2 * i + 1]) * f.y);
+                  l[4 * q8 + i] = fma2(l[4 * q8 + i], pair(f.x, f.y), 0ull);
+                }
+                tmem_store8(addr, o);
+              }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+          shift();
+        }
+        begun = true;
         // P^T row of this key: 16-byte pieces of 8 columns.
-        const uint32_t prow = sK(stage) + (N == 128 ? wg * kHalf : 0) + r * 128;
 #pragma unroll
         for (int q8 = 0; q8 < C / 8; ++q8) {
           if (8 * q8 < live) {
             float e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              e[i] = ex2(__uint_as_float(x[8 * q8 + i]));
-              l[8 * q8 + i] += e[i];
-            }
-            const int piece = (N == 128 ? 0 : 4 * wg) + q8;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(prow + 16 * (piece ^ (r & 7))), "r"(pack2<DT>(e[0], e[1])),
+            for (int i = 0; i < 8; ++i) e[i] = ex2(__uint_as_float(x[8 * q8 + i]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[4 * q8 + i] = add2(l[4 * q8 + i], pair(e[2 * i], e[2 * i + 1]));
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_at + p_piece<N>(r, c0 + 8 * q8)), "r"(pack2<DT>(e[0], e[1])),
                          "r"(pack2<DT>(e[2], e[3])), "r"(pack2<DT>(e[4], e[5])), "r"(pack2<DT>(e[6], e[7]))
                          : "memory");
           }
@@ -615,53 +752,77 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * sb);
       }
-      // ---- the segment's rows: O^T lane = dim, column = row ----
-      named_bar_sync(1 + wg, 128);  // the last factors are read
-#pragma unroll
-      for (int g = 0; g < G32; ++g)
-        if (32 * g < live) red[quad * N + 32 * g + lane] = transpose_reduce(l + 32 * g, lane, [](float a, float b) { return a + b; });
-      wait(o_full + 8 * (seg & 1), (seg >> 1) & 1);
-      tc_fence_after();
-      named_bar_sync(1 + wg, 128);
-      if (wg_tid < live) factor[wg_tid] = (red[wg_tid] + red[N + wg_tid]) + (red[2 * N + wg_tid] + red[3 * N + wg_tid]);
-      const bool set_aside = vote_any<256>(3, sick);  // (and the sums are there)
+      // ---- the segment's rows: the pipes' sums and O joined; O^T lane = dim, column = row ----
       const bool whole = s.whole();
       const int which = s.k0 == 0 ? 1 : 0;
-      float* part = scratch.sums(blockIdx.x, which) + (int64_t)c0 * HD;
-      int node = c0 / p.group, head = c0 % p.group;
       const int64_t first = s.r.s0 + (int64_t)s.qt * p.nt;
-      // The values of dim r that are not finite among the segment's nodes that node i sees.
-      auto aside = [&](int i) {
-        float sum = 0.f;
-        for (int x = max(0, s.k0 * kKeys - s.r.pad); x < min(s.r.n, s.k1 * kKeys - s.r.pad); ++x) {
-          const float y = load_scalar<DT>(p.v_rows + (int64_t)(s.r.s0 + x) * p.v_n + s.kvh * p.v_h, r);
-          if (!isfinite(y) && (seen_bits(p, s, i, x) & 1u)) sum += y;
+      named_bar_sync(team, kTeam);  // the last factors are read
+      {
+        float y[C];
+#pragma unroll
+        for (int i = 0; i < C / 2; ++i) {
+          const float2 v = unpair(l[i]);
+          y[2 * i] = v.x;
+          y[2 * i + 1] = v.y;
         }
-        return sum;
-      };
+        const float sum = transpose_reduce<C>(y, lane, [](float a, float b) { return a + b; });
+        red[red_at] = sum;
+      }
+      const bool set_aside = vote_any<kSoft * 32>(5, sick);  // (and the sums are there)
+      if (tid < cols) {
+        float m = kUnset, sum = 0.f, f[S::kPipes];
 #pragma unroll
-      for (int g = 0; g < G32; ++g) {
-        if (32 * g < live) {
-          uint32_t o[32];
-          tmem_ld32_nowait(lanes + 2 * N + (seg & 1) * N + c0 + 32 * g, o);
-          tmem_wait_ld();
+        for (int q = 0; q < S::kPipes; ++q) m = fmaxf(m, -m_all[q * N + tid]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int c = 32 * g + i;
-            if (c < live && r < HD) {
-              float y = __uint_as_float(o[i]);
-              if (set_aside) y += aside(s.qt * p.nt + node);
-              if (whole) {
-                const float sum = factor[c];
-                y = sum == 0.f ? 0.f : y / sum;
-                *reinterpret_cast<uint16_t*>(p.out + (first + node) * p.out_n + (s.kvh * p.group + head) * p.out_h + 2 * r) = to_bits<DT>(y);
-              } else {
-                part[(int64_t)c * HD + r] = y;
-              }
-              if (++head == p.group) {
-                head = 0;
-                ++node;
-              }
+        for (int q = 0; q < S::kPipes; ++q) {
+          const float* lq = red_all + q * 4 * N + tid;
+          f[q] = -m_all[q * N + tid] == m ? 1.f : exp2f(-m_all[q * N + tid] - m);
+          sum += f[q] * ((lq[0] + lq[N]) + (lq[2 * N] + lq[3 * N]));
+        }
+        const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int q = 0; q < S::kPipes; ++q) fac[q * N + tid] = f[q] * inv;
+        if (!whole) scratch.stats(blockIdx.x, which)[tid] = make_float2(m, sum);
+        else if (p.lse)
+          p.lse[(first + tid / p.group) * p.heads + s.kvh * p.group + tid % p.group] =
+              sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+      }
+      wait(o_full + 8 * (seg & 1), (seg >> 1) & 1);
+      tc_fence_after();
+      named_bar_sync(5, kSoft * 32);
+      constexpr int kOut = N >= 32 ? N / 4 : 8;  // columns that a group of 128 threads writes
+      const int o0 = wg * kOut, o1 = min(cols, o0 + kOut);
+      if (32 * quad < HD && o0 < o1) {
+        float* part = scratch.sums(blockIdx.x, which) + r;
+        int i = o0 / p.group, head = o0 % p.group;
+        char* out = p.out + (first + i) * p.out_n + (s.kvh * p.group + head) * p.out_h + 2 * r;
+        const int64_t wrap = p.out_n - (p.group - 1) * p.out_h;  // from a node's last head to the next node's first
+#pragma unroll 1
+        for (int c8 = o0; c8 < o1; c8 += 8) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = 0.f;
+#pragma unroll
+          for (int q = 0; q < S::kPipes; ++q) {
+            // A pipe without a tile of this segment has an O of anything.
+            if ((q + S::kPipes - j0 % S::kPipes) % S::kPipes < tiles) {
+              uint32_t o[8];
+              tmem_load<8>(lanes + (S::kS + (seg & 1) * S::kPipes + q) * N + c8, o);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = fmaf(__uint_as_float(o[e]), fac[q * N + c8 + e], y[e]);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (c8 + e < o1) {
+              if (set_aside)
+                y[e] += set_aside_sum<DT>(p, s.r.s0, s.kvh, s.qt * p.nt + i, max(0, s.k0 * kKeys - s.r.pad), min(s.r.n, s.k1 * kKeys - s.r.pad), r);
+              if (whole) *reinterpret_cast<uint16_t*>(out) = to_bits<DT>(y[e]);
+              else part[(c8 + e) * HD] = y[e];
+              const bool next = ++head == p.group;
+              out += next ? wrap : p.out_h;
+              head = next ? 0 : head;
+              i += next;
             }
           }
         }
@@ -669,23 +830,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty + 8 * (seg & 1));
-      if (wg_tid < live) {
-        const float m = m_ref[wg_tid], sum = factor[wg_tid];
-        if (!whole) {
-          scratch.stats(blockIdx.x, which)[c0 + wg_tid] = make_float2(m, sum);
-        } else if (p.lse) {
-          const int c = c0 + wg_tid;
-          p.lse[(first + c / p.group) * p.heads + s.kvh * p.group + c % p.group] =
-              sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
-        }
-      }
+      named_bar_sync(5, kSoft * 32);  // the factors lie where the next maxima go
       if (!whole && s.k0 == 0) {
         wrote_start = true;
-        if (tid == 0) {
-          const int64_t last = (s.row_end * ctas - 1) / all;  // the CTA with the row's last tile
-          *scratch.started(blockIdx.x) = Started{(int)last, (int)first, cols, s.kvh};
-        }
+        if (tid == 0) *scratch.started(blockIdx.x) = Started{(int)shares.owner(s.row_end - 1), (int)first, cols, s.kvh};
       }
+      j0 += tiles;
       ++seg;
     }
     if (!wrote_start && tid == 0) scratch.started(blockIdx.x)->last = 0;
@@ -695,9 +845,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
-  if (warp == kSoft) {
+  if (warp == kMmaS) {
     tc_fence_after();
-    tmem_dealloc(tmem, 4 * N);
+    tmem_dealloc(tmem, S::kTmem);
   }
 }
 
@@ -812,20 +962,31 @@ template <int DT, int N, int HD>
 int launch(const Params& p, cudaStream_t s) {
   using S = Shape<N, HD>;
   static_assert(S::kBytes <= 232448, "shared memory");
-  const cudaError_t attr = cudaFuncSetAttribute(k_tree_attention<DT, N, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-  if (attr != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: ") + cudaGetErrorString(attr));
+  static std::atomic<uint64_t> allowed{0};  // a bit per device whose copy of the kernel may use this much shared memory
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(k_tree_attention<DT, N, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
+    if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: ") + cudaGetErrorString(e));
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int ctas = sm_count();
   cudaError_t e = launch_ex(k_tree_attention<DT, N, HD>, dim3(ctas), dim3(kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
-  if (e == cudaSuccess && p.capacity + p.total > kKeys)  // else every row is one tile
+  if (e == cudaSuccess && p.capacity + p.total > kWhole * kKeys)  // else no row is shared
     e = launch_ex(k_tree_attention_join<DT, N, HD>, dim3(ctas, kJoinBlocks), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: launch: ") + cudaGetErrorString(e));
   return check_launch("af_tree_attention");
 }
 
+template <int DT, int HD>
+int launch_rows(const Params& p, int n, cudaStream_t s) {
+  return n == 16 ? launch<DT, 16, HD>(p, s) : n == 32 ? launch<DT, 32, HD>(p, s) : n == 64 ? launch<DT, 64, HD>(p, s) : launch<DT, 128, HD>(p, s);
+}
+
 template <int DT>
 int launch_shape(const Params& p, int n, int64_t head_dim, cudaStream_t s) {
-  if (head_dim == 128) return n == 64 ? launch<DT, 64, 128>(p, s) : launch<DT, 128, 128>(p, s);
-  return n == 64 ? launch<DT, 64, 64>(p, s) : launch<DT, 128, 64>(p, s);
+  return head_dim == 128 ? launch_rows<DT, 128>(p, n, s) : launch_rows<DT, 64>(p, n, s);
 }
 
 }  // namespace
@@ -847,8 +1008,9 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   Params p;
   memset(&p, 0, sizeof(p));
   const int group = (int)(a.n_heads / a.n_kv_heads);
-  // Columns of a tile: 64 when the average tree fits, else 128 (the keys are read once per row tile).
-  const int n = ceil_div(a.total, a.batch) * group <= 64 ? 64 : 128;
+  // Columns of a tile: the fewest that the average tree fits (the keys are read once per row tile).
+  const int64_t rows = ceil_div(a.total, a.batch) * group;
+  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
   p.nt = n / group;
   const uint64_t hd = (uint64_t)a.head_dim, kvh = (uint64_t)a.n_kv_heads;

@@ -54,32 +54,37 @@ class AcceptedPath(NamedTuple):
     next_tokens: torch.Tensor  # [trees] int64: the target model's choice after the path
 
 
-def _call(what: str, device: torch.device, fn, *args) -> None:
-    if device.index == torch.cuda.current_device():
-        st = fn(*args, _lib.stream_ptr(device))
+# These calls are short, so what the host does per call counts: plain
+# comparisons, no helper objects, and the stream's handle without a Stream object.
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _launch(what: str, index: int, fn, *args) -> None:
+    if index == _current_device():
+        st = fn(*args, _current_stream(index))
     else:
-        with torch.cuda.device(device):
-            st = fn(*args, _lib.stream_ptr(device))
+        with torch.cuda.device(index):
+            st = fn(*args, _current_stream(index))
     if st:
         _lib.check(st, what)
 
 
-def _vector(what: str, name: str, t: torch.Tensor, dtype: torch.dtype, n: int | None = None) -> torch.Tensor:
-    if t.dim() != 1 or t.dtype is not dtype or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{what}: {name} must be a {dtype} vector{'' if n is None else f' of {n}'}, got {t.dtype} {tuple(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _on_device(what: str, *tensors: torch.Tensor | None) -> torch.device:
-    dev = tensors[0].device
+def _same_device(what: str, *tensors: torch.Tensor | None) -> int:
+    """The index of the CUDA device that every given tensor is on."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            _lib.require_cuda(t, what=what)
-        if t.device != dev:
-            raise ValueError(f"{what}: tensors are on {dev} and {t.device}")
-    return dev
+        if t is not None and (index < 0 or t.get_device() != index):
+            _lib.require_cuda(*tensors, what=what)
+            raise ValueError(f"{what}: tensors are on {tensors[0].device} and {t.device}")
+    return index
+
+
+def _vectors(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
+    """Refuse what is not a vector of ``dtype``."""
+    for name, t in tensors.items():
+        if t is not None and (t.dtype is not dtype or t.dim() != 1):
+            raise ValueError(f"{what}: {name} must be a {dtype} vector, got {t.dtype} {tuple(t.shape)}")
 
 
 def _status(status: DeviceStatus | None) -> int | None:
@@ -112,32 +117,33 @@ def block_tables(
     not fit leave everything as it was, with empty ``starts`` and -1 slots, and
     set the capacity bit of ``status``.
     """
-    if tables.dim() != 2 or tables.dtype is not _I32 or (tables.shape[1] > 1 and tables.stride(1) != 1) or \
-            (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]):
-        raise ValueError(f"block_tables: tables must be int32 [requests, max_pages] with contiguous rows, got {tables.dtype} {tuple(tables.shape)}")
+    if tables.dim() != 2 or tables.dtype is not _I32:
+        raise ValueError(f"block_tables: tables must be int32 [requests, max_pages], got {tables.dtype} {tuple(tables.shape)}")
     n, most = tables.shape
-    lengths = _vector("block_tables", "lengths", lengths, _I32, n)
-    grow = _vector("block_tables", "grow", grow, _I32, n)
-    if held is not None:
-        held = _vector("block_tables", "held", held, _I32, n)
-    if free_pages.dim() != 1 or free_pages.dtype is not _I32 or not free_pages.is_contiguous():
-        raise ValueError("block_tables: free_pages must be a contiguous int32 vector")
-    free_range = _vector("block_tables", "free_range", free_range, _I64, 2)
+    row, inner = tables.stride()
+    if (inner != 1 and most > 1) or (row < most and n > 1):
+        raise ValueError("block_tables: the rows of tables must be contiguous and must not overlap")
+    _vectors("block_tables", _I32, lengths=lengths, grow=grow, held=held, free_pages=free_pages)
+    if lengths.shape[0] != n or grow.shape[0] != n or (held is not None and held.shape[0] != n):
+        raise ValueError(f"block_tables: lengths, grow and held must have one entry for each of {n} requests")
+    if not free_pages.is_contiguous():
+        raise ValueError("block_tables: free_pages must be contiguous")
+    if free_range.dtype is not _I64 or free_range.shape != (2,):
+        raise ValueError(f"block_tables: free_range must be two int64 numbers, got {free_range.dtype} {tuple(free_range.shape)}")
     if page_size <= 0 or slot_capacity < 0:
-        raise ValueError(f"block_tables: page_size {page_size} and slot_capacity {slot_capacity} must be positive")
-    dev = _on_device("block_tables", tables, lengths, grow, free_pages, free_range, held)
-    small = torch.empty(2 * n + 1, dtype=_I32, device=dev)
-    slots = torch.empty((n, slot_capacity) if padded else slot_capacity, dtype=_I64, device=dev)
-    out = torch.empty(2, dtype=_I64, device=dev)
+        raise ValueError(f"block_tables: page_size {page_size} must be positive and slot_capacity {slot_capacity} not negative")
+    index = _same_device("block_tables", tables, lengths, grow, free_pages, free_range, held)
+    lengths, grow, free_range = lengths.contiguous(), grow.contiguous(), free_range.contiguous()
+    if held is not None:
+        held = held.contiguous()
+    starts, totals, out = lengths.new_empty(n + 1), lengths.new_empty(n), free_range.new_empty(2)
+    slots = free_range.new_empty((n, slot_capacity) if padded else slot_capacity)
     if n == 0:
-        out.copy_(free_range)
-        return BlockTables(small.zero_(), small[1:], slots.fill_(-1), out)
-    at = small.data_ptr()
-    _call("block_tables", dev, _lib.load().af_block_tables, tables.data_ptr(), tables.stride(0) if n > 1 else most, most,
-          None if held is None else held.data_ptr(), lengths.data_ptr(), grow.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0],
-          free_range.data_ptr(), page_size, n * slot_capacity if padded else slot_capacity, slot_capacity if padded else 0,
-          at, at + 4 * (n + 1), slots.data_ptr(), out.data_ptr(), _status(status))
-    starts, totals = small.split((n + 1, n))
+        return BlockTables(starts.zero_(), totals, slots.fill_(-1), out.copy_(free_range))
+    _launch("block_tables", index, _lib.load().af_block_tables, tables.data_ptr(), row if n > 1 else most, most,
+            None if held is None else held.data_ptr(), lengths.data_ptr(), grow.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0],
+            free_range.data_ptr(), page_size, n * slot_capacity if padded else slot_capacity, slot_capacity if padded else 0,
+            starts.data_ptr(), totals.data_ptr(), slots.data_ptr(), out.data_ptr(), _status(status))
     return BlockTables(starts, totals, slots, out)
 
 
@@ -156,18 +162,19 @@ def tree_masks(
     base[b] + depth`` (``base`` = the prefix lengths). A tree may hold up to
     ``32 * words`` nodes. Rows behind ``starts[-1]`` are not written.
     """
-    parents = _vector("tree_masks", "parents", parents, _I32)
-    starts = _vector("tree_masks", "starts", starts, _I32)
+    _vectors("tree_masks", _I32, parents=parents, starts=starts, base=base)
     batch, total = starts.shape[0] - 1, parents.shape[0]
     if batch < 0 or words <= 0:
         raise ValueError(f"tree_masks: starts needs one entry more than there are trees, words {words} must be positive")
+    if base is not None and base.shape[0] != batch:
+        raise ValueError(f"tree_masks: base must have one entry for each of {batch} trees")
+    index = _same_device("tree_masks", parents, starts, base)
+    parents, starts = parents.contiguous(), starts.contiguous()
     if base is not None:
-        base = _vector("tree_masks", "base", base, _I32, batch)
-    dev = _on_device("tree_masks", parents, starts, base)
-    mask = torch.empty((total, words), dtype=_I32, device=dev)
-    positions = torch.empty(total, dtype=_I32, device=dev)
-    _call("tree_masks", dev, _lib.load().af_tree_masks, parents.data_ptr(), starts.data_ptr(), batch, total, words,
-          None if base is None else base.data_ptr(), mask.data_ptr(), positions.data_ptr(), _status(status))
+        base = base.contiguous()
+    mask, positions = parents.new_empty((total, words)), parents.new_empty(total)
+    _launch("tree_masks", index, _lib.load().af_tree_masks, parents.data_ptr(), starts.data_ptr(), batch, total, words,
+            None if base is None else base.data_ptr(), mask.data_ptr(), positions.data_ptr(), _status(status))
     return mask, positions
 
 
@@ -193,29 +200,29 @@ def accept_tree(
     (after the prefix when there is none, -1 when that is not given).
     ``max_nodes``: nodes of the largest tree, when known (at most 16384).
     """
-    parents = _vector("accept_tree", "parents", parents, _I32)
-    total = parents.shape[0]
-    tokens = _vector("accept_tree", "tokens", tokens, _I64, total)
-    targets = _vector("accept_tree", "targets", targets, _I64, total)
-    starts = _vector("accept_tree", "starts", starts, _I32)
-    batch = starts.shape[0] - 1
+    _vectors("accept_tree", _I32, parents=parents, starts=starts)
+    _vectors("accept_tree", _I64, tokens=tokens, targets=targets, root_targets=root_targets)
+    batch, total = starts.shape[0] - 1, parents.shape[0]
+    if tokens.shape[0] != total or targets.shape[0] != total:
+        raise ValueError(f"accept_tree: tokens and targets must have one entry for each of {total} nodes")
     if batch < 0 or keep <= 0:
         raise ValueError(f"accept_tree: starts needs one entry more than there are trees, keep {keep} must be positive")
+    if root_targets is not None and root_targets.shape[0] != batch:
+        raise ValueError(f"accept_tree: root_targets must have one entry for each of {batch} trees")
+    index = _same_device("accept_tree", parents, tokens, targets, starts, root_targets)
+    parents, tokens, targets, starts = parents.contiguous(), tokens.contiguous(), targets.contiguous(), starts.contiguous()
     if root_targets is not None:
-        root_targets = _vector("accept_tree", "root_targets", root_targets, _I64, batch)
-    dev = _on_device("accept_tree", parents, tokens, targets, starts, root_targets)
-    rows = torch.empty((batch, keep), dtype=_I32, device=dev)
-    counts = torch.empty(batch, dtype=_I32, device=dev)
-    following = torch.empty(batch, dtype=_I64, device=dev)
-    _call("accept_tree", dev, _lib.load().af_accept_tree, parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), starts.data_ptr(),
-          batch, total, 16384 if max_nodes is None else max_nodes, None if root_targets is None else root_targets.data_ptr(), keep,
-          rows.data_ptr(), counts.data_ptr(), following.data_ptr(), _status(status))
+        root_targets = root_targets.contiguous()
+    rows, counts, following = parents.new_empty((batch, keep)), parents.new_empty(batch), tokens.new_empty(batch)
+    _launch("accept_tree", index, _lib.load().af_accept_tree, parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), starts.data_ptr(),
+            batch, total, 16384 if max_nodes is None else max_nodes, None if root_targets is None else root_targets.data_ptr(), keep,
+            rows.data_ptr(), counts.data_ptr(), following.data_ptr(), _status(status))
     return AcceptedPath(rows, counts, following)
 
 
-def _strides(t: torch.Tensor, scale: int) -> list[int]:
-    """Strides in bytes, 0 for a dimension of one entry (torch leaves any value there)."""
-    return [0 if n == 1 else s * scale for n, s in zip(t.shape[:-1], t.stride())]
+def _bytes(t: torch.Tensor, size: int) -> list[int]:
+    """Strides of all dimensions but the innermost in bytes, 0 for a dimension of one entry (torch leaves any value there)."""
+    return [x * size if n > 1 else 0 for x, n in zip(t.stride()[:-1], t.shape)]
 
 
 def write_cache(
@@ -236,47 +243,59 @@ def write_cache(
     may have any shape, the same one. Any dtype, the caches' own; any strides but the
     innermost. Live slots must differ from one another.
     """
-    if k.shape != v.shape or k_cache.shape != v_cache.shape or k.dim() not in (3, 4) or k_cache.dim() != k.dim() + 1:
+    shape, cache = k.shape, k_cache.shape
+    if v.shape != shape or v_cache.shape != cache or len(shape) not in (3, 4) or len(cache) != len(shape) + 1:
         raise ValueError(f"write_cache: k, v {tuple(k.shape)}, {tuple(v.shape)} do not match caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    if k.dim() == 3:
-        k, v, k_cache, v_cache = k[None], v[None], k_cache[None], v_cache[None]
-    layers, n, heads, dim = k.shape
-    pages, page_size = k_cache.shape[1:3]
-    if k_cache.shape[0] != layers or k_cache.shape[3:] != k.shape[2:]:
-        raise ValueError(f"write_cache: rows {tuple(k.shape)} do not match caches {tuple(k_cache.shape)}")
-    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+    if len(shape) == 3:
+        return write_cache(k[None], v[None], k_cache[None], v_cache[None], slots, rows, status)
+    layers, n, heads, dim = shape
+    if cache[0] != layers or cache[3] != heads or cache[4] != dim:
+        raise ValueError(f"write_cache: rows {tuple(shape)} do not match caches {tuple(cache)}")
+    dtype = k.dtype
+    if v.dtype is not dtype or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError(f"write_cache: rows {k.dtype}, {v.dtype} and caches {k_cache.dtype}, {v_cache.dtype} differ in dtype")
     if slots.dtype is not _I64 or (rows is not None and (rows.dtype is not _I32 or rows.shape != slots.shape)):
         raise ValueError("write_cache: slots must be int64, rows int32 of the same shape")
-    if rows is None and slots.numel() > n:
-        raise ValueError(f"write_cache: {slots.numel()} slots for {n} rows")
-    if page_size == 0:
+    count = slots.numel()
+    if rows is None and count > n:
+        raise ValueError(f"write_cache: {count} slots for {n} rows")
+    if cache[2] == 0:
         raise ValueError("write_cache: page_size must be positive")
-    if dim > 1 and (k_cache.stride(-1) != 1 or v_cache.stride(-1) != 1):
-        raise ValueError("write_cache: the innermost dimension of the caches must be contiguous")
     for c in (k_cache, v_cache):
-        if any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape)):
+        st = c.stride()
+        if dim > 1 and st[4] != 1:
+            raise ValueError("write_cache: the innermost dimension of the caches must be contiguous")
+        if 0 in st and any(x == 0 and m > 1 for x, m in zip(st, cache)):
             raise ValueError("write_cache: the caches have entries that share memory")
-    if dim > 1 and k.stride(-1) != 1:
+    index = _same_device("write_cache", k, v, k_cache, v_cache, slots, rows)
+    if dim > 1 and k.stride(3) != 1:
         k = k.contiguous()
-    if dim > 1 and v.stride(-1) != 1:
+    if dim > 1 and v.stride(3) != 1:
         v = v.contiguous()
     slots = slots.contiguous()
-    rows = None if rows is None else rows.contiguous()
-    dev = _on_device("write_cache", k, v, k_cache, v_cache, slots, rows)
-    es = k.element_size()
-    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *_strides(k, es), *_strides(v, es), k_cache.data_ptr(), v_cache.data_ptr(),
-                      *_strides(k_cache, es), *_strides(v_cache, es), slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n,
-                      slots.numel(), pages, page_size, layers, heads, dim * es)
-    _call("write_cache", dev, _lib.load().af_write_cache, args, _status(status))
+    if rows is not None:
+        rows = rows.contiguous()
+    size = k.element_size()
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *_bytes(k, size), *_bytes(v, size), k_cache.data_ptr(), v_cache.data_ptr(),
+                      *_bytes(k_cache, size), *_bytes(v_cache, size), slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n,
+                      count, cache[1], cache[2], layers, heads, dim * size)
+    _launch("write_cache", index, _lib.load().af_write_cache, args, _status(status))
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Innermost dimension contiguous, address and strides multiples of 16 bytes."""
-    if t.stride(-1) != 1 or t.data_ptr() & 15:
-        return False
-    unit = 16 // t.element_size()
-    return all(n == 1 or (s > 0 and s % unit == 0) for n, s in zip(t.shape[:-1], t.stride()))
+def _grid(t: torch.Tensor) -> list[int] | None:
+    """Strides in bytes of a 16-bit tensor (0 for a dimension of one entry), or None where its address or a stride is
+    not a multiple of 16 bytes, the innermost dimension is not contiguous or entries share memory."""
+    *outer, inner = t.stride()
+    if inner != 1 or t.data_ptr() & 15:
+        return None
+    out = []
+    for x, n in zip(outer, t.shape):
+        if n == 1:
+            x = 0
+        elif x <= 0 or x & 7:
+            return None
+        out.append(2 * x)
+    return out
 
 
 def tree_attention(
@@ -309,62 +328,77 @@ def tree_attention(
     -0.5. A row that sees nothing is 0. ``lse`` [nodes, heads] float32 receives the
     natural log of each row's sum of exponentials. Rows of ``out`` behind ``starts[-1]`` are not written.
     """
-    if q.dim() != 3 or k.dim() != 3 or k_cache.dim() != 4 or k.shape != v.shape or k_cache.shape != v_cache.shape:
+    qs, ks, cs = q.shape, k.shape, k_cache.shape
+    if len(qs) != 3 or len(ks) != 3 or len(cs) != 4 or v.shape != ks or v_cache.shape != cs:
         raise ValueError(f"tree_attention: bad shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, caches "
                          f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    total, heads, dim = q.shape
-    kv_heads = k.shape[1]
-    pages, page_size = k_cache.shape[:2]
-    if k.shape[0] != total or k.shape[2] != dim or k_cache.shape[2] != kv_heads or k_cache.shape[3] != dim:
-        raise ValueError(f"tree_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and caches {tuple(k_cache.shape)} do not match")
-    if q.dtype not in (torch.float16, torch.bfloat16) or not (q.dtype == k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+    total, heads, dim = qs
+    if ks[0] != total or ks[2] != dim or cs[2] != ks[1] or cs[3] != dim:
+        raise ValueError(f"tree_attention: q {tuple(qs)}, k {tuple(ks)} and caches {tuple(cs)} do not match")
+    dtype = q.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k.dtype is not dtype or v.dtype is not dtype \
+            or k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError(f"tree_attention: q, k, v and caches must all be fp16 or all bf16, got {q.dtype}, {k.dtype}, {v.dtype}, "
                          f"{k_cache.dtype}, {v_cache.dtype}")
     if tables.dim() != 2 or tables.dtype is not _I32:
         raise ValueError(f"tree_attention: tables must be int32 [requests, max_pages], got {tables.dtype} {tuple(tables.shape)}")
     batch, most = tables.shape
-    if most > 1 and tables.stride(1) != 1:
-        tables = tables.contiguous()
-    lengths = _vector("tree_attention", "lengths", lengths, _I32, batch)
-    starts = _vector("tree_attention", "starts", starts, _I32, batch + 1)
-    words = 0
+    _vectors("tree_attention", _I32, lengths=lengths, starts=starts)
+    if lengths.shape[0] != batch or starts.shape[0] != batch + 1:
+        raise ValueError(f"tree_attention: {batch} requests need as many lengths and one entry of starts more")
+    index = q.get_device()
+    mask_at = mask_row = words = 0
     if mask is not None:
         if mask.dim() != 2 or mask.dtype is not _I32 or mask.shape[0] != total or mask.shape[1] == 0:
             raise ValueError(f"tree_attention: mask must be int32 [{total}, words], got {mask.dtype} {tuple(mask.shape)}")
         words = mask.shape[1]
-        if (words > 1 and mask.stride(1) != 1) or (total > 1 and mask.stride(0) < words):
+        mask_row, inner = mask.stride()
+        if (words > 1 and inner != 1) or mask_row < words:
             mask = mask.contiguous()
-    if out is not None and (out.shape != q.shape or out.dtype is not q.dtype or not _aligned(out)):
-        raise ValueError("tree_attention: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
+            mask_row = words
+        mask_at = mask.data_ptr()
+    k_grid, v_grid = _grid(k_cache), _grid(v_cache)
+    if k_grid is None or v_grid is None:
+        raise ValueError("tree_attention: the caches' innermost dimension must be contiguous, their other strides multiples of 16 bytes")
+    out_grid = None
+    if out is not None:
+        if out.shape != qs or out.dtype is not dtype or (out_grid := _grid(out)) is None:
+            raise ValueError("tree_attention: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
     if lse is not None and (lse.shape != (total, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
         raise ValueError(f"tree_attention: lse must be contiguous float32 [{total}, {heads}]")
-    if not (_aligned(k_cache) and _aligned(v_cache)):
-        raise ValueError("tree_attention: the caches' innermost dimension must be contiguous, their other strides multiples of 16 bytes")
-    dev = _on_device("tree_attention", q, k, v, k_cache, v_cache, tables, lengths, starts, mask, out, lse)
-    q, k, v = (t if _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    _same_device("tree_attention", q, k, v, k_cache, v_cache, tables, lengths, starts, mask, out, lse)
+    if most > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lengths, starts = lengths.contiguous(), starts.contiguous()
+    if (q_grid := _grid(q)) is None:
+        q = q.clone(memory_format=torch.contiguous_format)
+        q_grid = _grid(q)
+    if (kr_grid := _grid(k)) is None:
+        k = k.clone(memory_format=torch.contiguous_format)
+        kr_grid = _grid(k)
+    if (vr_grid := _grid(v)) is None:
+        v = v.clone(memory_format=torch.contiguous_format)
+        vr_grid = _grid(v)
     if out is None:
-        out = torch.empty((total, heads, dim), dtype=q.dtype, device=dev)
-    lib = _lib.load()
-    size = _workspace_bytes(dev)
-    workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+        out = q.new_empty(qs)
+        out_grid = (2 * heads * dim, 2 * dim)
+    size = _scratch.get(index) or _workspace_bytes(index)
+    workspace = lengths.new_empty(size >> 2)
     args = _ATTENTION.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, 2), *_strides(k, 2), *_strides(v, 2), k_cache.data_ptr(), v_cache.data_ptr(),
-        *_strides(k_cache, 2), *_strides(v_cache, 2), pages, page_size, tables.data_ptr(), tables.stride(0) if batch > 1 else most, most,
-        lengths.data_ptr(), starts.data_ptr(), 0 if mask is None else mask.data_ptr(), words if total == 1 or mask is None else mask.stride(0), words,
-        batch, total, heads, kv_heads, dim, _lib.DTYPE[q.dtype], dim ** -0.5 if scale is None else float(scale),
-        out.data_ptr(), *_strides(out, 2), 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size)
-    _call("tree_attention", dev, lib.af_tree_attention, args, _status(status))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q_grid, *kr_grid, *vr_grid, k_cache.data_ptr(), v_cache.data_ptr(), *k_grid, *v_grid,
+        cs[0], cs[1], tables.data_ptr(), tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(), starts.data_ptr(),
+        mask_at, mask_row if total > 1 else words, words, batch, total, heads, ks[1], dim, _lib.DTYPE[dtype],
+        dim ** -0.5 if scale is None else scale, out.data_ptr(), *out_grid, 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size)
+    _launch("tree_attention", index, _lib.load().af_tree_attention, args, _status(status))
     return out
 
 
-_scratch: dict[torch.device, int] = {}
+_scratch: dict[int, int] = {}  # bytes of scratch per device
 
 
-def _workspace_bytes(device: torch.device) -> int:
-    size = _scratch.get(device)
-    if size is None:
-        n = C.c_int64()
-        with torch.cuda.device(device):
-            _lib.check(_lib.load().af_tree_attention_workspace_bytes(C.byref(n)), "tree_attention")
-        size = _scratch[device] = n.value
-    return size
+def _workspace_bytes(index: int) -> int:
+    n = C.c_int64()
+    with torch.cuda.device(index):
+        _lib.check(_lib.load().af_tree_attention_workspace_bytes(C.byref(n)), "tree_attention")
+    _scratch[index] = (n.value + 15) & ~15
+    return _scratch[index]
