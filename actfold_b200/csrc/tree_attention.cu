@@ -21,7 +21,7 @@
 // next tiles with maxima, sums and an O of their own (kPipes of them, joined at the
 // end of a row), which hides the latency of a tile's chain of load, product,
 // exponential, product. Warp 16 loads Q and K, warp 17 V (TMA; an issue takes
-// a warp some 80 cycles), warp 18 issues S, warp 19 issues O. A column's
+// some 60 cycles), warp 18 issues S, warp 19 plans the CTA's work and issues O. A column's
 // reference maximum m is raised only when a score passes it by more than 2^8
 // (or at the row's first key): steady tiles take one comparison per score and one
 // barrier vote, no maximum across lanes. P then stays below 256, which bf16
@@ -42,6 +42,7 @@ constexpr int kHalf = kKeys * 128;          // [128 rows][64 columns] of 16 bits
 constexpr int kSoft = 16;                   // softmax warps
 constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMmaS = kSoft + 2, kMmaO = kSoft + 3;
 constexpr int kThreads = (kSoft + 4) * 32;
+constexpr int kPlans = 4;                   // segments planned in shared memory, up to two ahead of the products of O
 constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
 constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
 constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
@@ -69,8 +70,9 @@ struct Shape {
   static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
   static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
   static constexpr int kOffBar = kOffRed + kPipes * 4 * N * 4;
-  static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4;
-  static constexpr int kBytes = kOffBar + kBars * 8 + 32 + kThreads / 32 * 8;
+  static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4 + kPlans;
+  static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
+  static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
 };
 
 struct Params {
@@ -95,7 +97,7 @@ struct Params {
 struct Request {
   int s0, n, len, pad, kt, qt;
   bool bad;
-  __device__ __forceinline__ int64_t tiles(int kv_heads) const { return (int64_t)kt * qt * kv_heads; }
+  __device__ __forceinline__ int tiles(int kv_heads) const { return kt * qt * kv_heads; }  // (of all requests below 2^31: checked by the host)
 };
 
 __device__ __forceinline__ Request request(const Params& p, int b) {
@@ -105,66 +107,70 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.bad = s0 < 0 || s1 < s0 || s1 > p.total || r.len < 0 || r.len > p.capacity || (p.mask && s1 - s0 > 32 * (int64_t)p.words);
   r.s0 = s0;
   r.n = r.bad ? 0 : s1 - s0;
-  r.pad = (r.len + p.box - 1) / p.box * p.box;
-  r.kt = r.n ? (int)(((int64_t)r.pad + r.n + kKeys - 1) / kKeys) : 0;
-  r.qt = (r.n + p.nt - 1) / p.nt;
+  r.pad = (r.len + p.box - 1) & -p.box;
+  r.kt = r.n ? (r.pad + r.n + kKeys - 1) / kKeys : 0;
+  r.qt = r.n <= p.nt ? 1 : (r.n + p.nt - 1) / p.nt;
   return r;
-}
-
-// a / b of positive numbers, mostly small ones.
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
-  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
 // The list of tiles cut into one share per CTA: the first `more` shares have each + 1.
 struct Shares {
-  int64_t each, more;
-  __device__ __forceinline__ int64_t begin(int64_t i) const { return each * i + min(i, more); }
-  __device__ __forceinline__ int64_t owner(int64_t t) const {
-    const int64_t big = more * (each + 1);
-    return t < big ? quotient(t, each + 1) : more + quotient(t - big, each);
+  int each, more;
+  __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int owner(int t) const {
+    const int big = more * (each + 1);
+    return t < big ? t / (each + 1) : more + (t - big) / each;
   }
 };
 
-// The tiles [k0, k1) of one row tile that a CTA works on.
-struct Segment {
-  Request r;
-  int kvh, qt, k0, k1;
-  int64_t row_end;  // list index behind the row tile's last tile
-  __device__ __forceinline__ bool whole() const { return k0 == 0 && k1 == r.kt; }
+// The tiles [k0, k1) of one row tile that a CTA works on, as one warp plans
+// it and the others read it (k1 = 0: the share is done).
+struct __align__(16) Segment {
+  int s0, n, len, pad;       // the request's nodes, cached keys, and where the tree's keys begin
+  int b, kvh, node0, k0;     // request, head, first node of the row tile
+  int k1, whole, row_end;    // all tiles of the row?; list index behind its last one
+  int last;                  // the CTA with the row's last tile, where this one begins a row that others go on with
 };
-
 struct Walk {
-  int64_t t, end, before;  // next tile, end of the share, tiles of the requests before b
+  int t, end, before;  // next tile, end of the share, tiles of the requests before b
   int b;
-  // A row of up to kWhole tiles belongs to the CTA whose share it begins in.
-  __device__ __forceinline__ bool next(const Params& p, Segment& s) {
-    while (true) {
-      if (t >= end) return false;
-      s.r = request(p, b);
-      while (t >= before + s.r.tiles(p.kv_heads)) {
-        before += s.r.tiles(p.kv_heads);
-        s.r = request(p, ++b);
-      }
-      const int64_t rel = t - before;
-      const int64_t row = quotient(rel, s.r.kt);
-      s.k0 = (int)(rel - row * s.r.kt);
-      s.row_end = before + (row + 1) * s.r.kt;
-      if (s.r.kt <= kWhole) {
-        t = s.row_end;
-        if (s.k0 > 0) continue;
-        s.k1 = s.r.kt;
-      } else {
-        s.k1 = (int)min((int64_t)s.r.kt, s.k0 + (end - t));
-        t += s.k1 - s.k0;
-      }
-      const int64_t head = quotient(row, s.r.qt);
-      s.kvh = (int)head;
-      s.qt = (int)(row - head * s.r.qt);
-      return true;
-    }
-  }
 };
+
+// The share's next segment. A row of up to kWhole tiles belongs to the CTA
+// whose share it begins in.
+__device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& s) {
+#pragma unroll 1
+  while (w.t < w.end) {
+    Request r = request(p, w.b);
+#pragma unroll 1
+    while (w.t >= w.before + r.tiles(p.kv_heads)) {
+      w.before += r.tiles(p.kv_heads);
+      r = request(p, ++w.b);
+    }
+    const int rel = w.t - w.before, row = rel / r.kt;
+    s.k0 = rel - row * r.kt;
+    s.row_end = w.before + (row + 1) * r.kt;
+    s.kvh = r.qt == 1 ? row : row / r.qt;
+    s.node0 = (row - s.kvh * r.qt) * p.nt;
+    s.s0 = r.s0;
+    s.n = r.n;
+    s.len = r.len;
+    s.pad = r.pad;
+    s.b = w.b;
+    if (r.kt <= kWhole) {
+      w.t = s.row_end;
+      if (s.k0 > 0) continue;
+      s.k1 = r.kt;
+    } else {
+      s.k1 = min(r.kt, s.k0 + (w.end - w.t));
+      w.t += s.k1 - s.k0;
+    }
+    s.whole = s.k0 == 0 && s.k1 == r.kt;
+    return true;
+  }
+  s.k1 = 0;
+  return false;
+}
 
 // What CTA c left for k_tree_attention_join: it began a row tile that CTAs
 // c + 1 .. last went on with (last = 0: it did not).
@@ -251,8 +257,12 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Bounded wait for a phase: some seconds of attempts (each of which may itself sleep a little).
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* failed) {
-  return mbar_try_wait(bar, parity) || mbar_wait(bar, parity, failed);
+#pragma unroll 1
+  for (int n = 0; !mbar_try_wait(bar, parity); ++n)
+    if (n > (1 << 24) || *failed) return false;
+  return true;
 }
 
 // Lane i's 32 bits become bit i of every lane's word.
@@ -305,6 +315,40 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
                  : "memory");
   }
 }
+// W columns (4 or 8) of each of P blocks of N columns.
+template <int P, int N, int W>
+__device__ __forceinline__ void tmem_load_rows(uint32_t taddr, uint32_t* r) {
+#define AF_LD4(a, b) "tcgen05.ld.sync.aligned.32x32b.x4.b32 {" a "}, [" b "];\n\t"
+#define AF_LD8(a, b) "tcgen05.ld.sync.aligned.32x32b.x8.b32 {" a "}, [" b "];\n\t"
+  if constexpr (P == 1) {
+    tmem_load<8>(taddr, r);
+  } else if constexpr (P == 2) {
+    asm volatile(AF_LD8("%0,%1,%2,%3,%4,%5,%6,%7", "%16") AF_LD8("%8,%9,%10,%11,%12,%13,%14,%15", "%17") "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr), "r"(taddr + N)
+                 : "memory");
+  } else if constexpr (W == 4) {
+    asm volatile(AF_LD4("%0,%1,%2,%3", "%16") AF_LD4("%4,%5,%6,%7", "%17") AF_LD4("%8,%9,%10,%11", "%18")
+                     AF_LD4("%12,%13,%14,%15", "%19") "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr), "r"(taddr + N), "r"(taddr + 2 * N), "r"(taddr + 3 * N)
+                 : "memory");
+  } else {
+    asm volatile(AF_LD8("%0,%1,%2,%3,%4,%5,%6,%7", "%32") AF_LD8("%8,%9,%10,%11,%12,%13,%14,%15", "%33")
+                     AF_LD8("%16,%17,%18,%19,%20,%21,%22,%23", "%34") AF_LD8("%24,%25,%26,%27,%28,%29,%30,%31", "%35")
+                         "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+                   "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+                   "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr), "r"(taddr + N), "r"(taddr + 2 * N), "r"(taddr + 3 * N)
+                 : "memory");
+  }
+#undef AF_LD4
+#undef AF_LD8
+}
 __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -349,6 +393,7 @@ __device__ __forceinline__ uint32_t seen_bits(const Params& p, int s0, int i, in
 template <int DT>
 __device__ __noinline__ float set_aside_sum(const Params& p, int s0, int kvh, int i, int x0, int x1, int d) {
   float sum = 0.f;
+#pragma unroll 1
   for (int x = x0; x < x1; ++x) {
     const float y = load_scalar<DT>(p.v_rows + (int64_t)(s0 + x) * p.v_n + kvh * p.v_h, d);
     if (!isfinite(y) && (seen_bits(p, s0, i, x) & 1u)) sum += y;
@@ -357,57 +402,80 @@ __device__ __noinline__ float set_aside_sum(const Params& p, int s0, int kvh, in
 }
 
 // Loads of one operand by a warp: K (with the Q of each segment) or V.
-template <int N, int HD, bool VALUES>
-__device__ __forceinline__ bool load_tiles(const Params& p, Walk walk, uint32_t base, uint32_t full, uint32_t empty, uint32_t q_full,
+template <int N, int HD, bool VALUES, typename Planned>
+__device__ __forceinline__ void load_tiles(const Params& p, Planned planned, uint32_t base, uint32_t full, uint32_t empty, uint32_t q_full,
                                            uint32_t q_empty, volatile int* failed) {
   using S = Shape<N, HD>;
   const int lane = threadIdx.x & 31;
   const CUtensorMap* cache = VALUES ? &p.vc : &p.kc;
   const CUtensorMap* tree_rows = VALUES ? &p.v : &p.k;
-  // Lane (box, half) loads rows [box * R, (box + 1) * R) of each tile; the page is fetched a tile ahead.
-  const int box = lane / S::kHalves, half = lane % S::kHalves, row = box * p.box;
-  const bool in_use = row < kKeys;
+  if (lane < (VALUES ? 2 : 3)) tma_prefetch_desc(lane == 0 ? cache : lane == 1 ? tree_rows : &p.q);
+  const int boxes = kKeys / p.box, page_step = kKeys / p.page, off_step = kKeys % p.page;
   int j = 0, seg = 0;
   bool ok = true;
   Segment s;
-  while (ok && walk.next(p, s)) {
+#pragma unroll 1
+  while (ok && planned(seg, s)) {
+    const int* table = p.tables + (int64_t)s.b * p.tables_ld;
+    // Lane x knows where rows [x * R, (x + 1) * R) of a tile come from (a page is fetched a tile ahead); one lane issues.
+    const int row = lane * p.box;
+    int key = s.k0 * kKeys + row;
+    int entry = key / p.page, off = key - entry * p.page;  // its table entry and place in the page, carried from tile to tile
+    int page = lane < boxes && key < s.len ? table[entry] : 0;
     if constexpr (!VALUES) {
       const int qb = seg % S::kQ, use = seg / S::kQ;
       if (use > 0) ok = __all_sync(0xffffffffu, wait_for(q_empty + 8 * qb, (use - 1) & 1, failed));
       if (!ok) break;
-      if (lane == 0) {
+      if (elect_one()) {
         mbar_arrive_expect_tx(q_full + 8 * qb, S::kHalves * p.nt * p.group * 128);
         for (int h = 0; h < S::kHalves; ++h)
-          tma_load_3d(base + S::kOffQ + qb * S::kQBytes + h * N * 128, &p.q, q_full + 8 * qb, 64 * h, s.kvh * p.group, s.r.s0 + s.qt * p.nt);
+          tma_load_3d(base + S::kOffQ + qb * S::kQBytes + h * N * 128, &p.q, q_full + 8 * qb, 64 * h, s.kvh * p.group, s.s0 + s.node0);
       }
       __syncwarp();
-      ++seg;
     }
-    const int* table = p.tables + (int64_t)walk.b * p.tables_ld;
-    auto page_of = [&](int kt) {
-      const int key = kt * kKeys + row;
-      return in_use && kt < s.k1 && key < s.r.len ? table[key / p.page] : 0;
-    };
-    int page = page_of(s.k0);
+    ++seg;
+#pragma unroll 1
     for (int kt = s.k0; kt < s.k1; ++kt, ++j) {
-      const int key = kt * kKeys + row, node = key - s.r.pad;
-      const bool cached = in_use && key < s.r.len, tree = in_use && node >= 0 && node < s.r.n;
+      const int node = key - s.pad;
+      const bool cached = lane < boxes && key < s.len, tree = lane < boxes && node >= 0 && node < s.n;
       if (cached && (page < 0 || page >= p.pages)) {
         if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
         page = p.pages;  // out of range: the box reads as zeros
       }
-      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, cached || tree)) * p.box * 128;
-      const int off = cached ? key % p.page : 0;
+      const int from = cached ? off : s.s0 + node, of_page = page;
+      const uint32_t from_cache = __ballot_sync(0xffffffffu, cached), from_tree = __ballot_sync(0xffffffffu, tree);
+      key += kKeys;
+      entry += page_step;
+      off += off_step;
+      if (off >= p.page) {
+        off -= p.page;
+        ++entry;
+      }
+      page = lane < boxes && kt + 1 < s.k1 && key < s.len ? table[entry] : 0;
       const int stage = j % S::kStages, round = j / S::kStages;
       if (round > 0) ok = __all_sync(0xffffffffu, wait_for(empty + 8 * stage, (round - 1) & 1, failed));
       if (!ok) break;
       const uint32_t bar = full + 8 * stage;
-      if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+      const uint32_t dst = base + stage * S::kStage + (VALUES ? S::kKBytes : 0);
+      if (elect_one()) mbar_arrive_expect_tx(bar, __popc(from_cache | from_tree) * p.box * 128 * S::kHalves);
       __syncwarp();
-      const uint32_t dst = base + stage * S::kStage + (VALUES ? S::kKBytes : 0) + half * kHalf + row * 128;
-      if (cached) tma_load_4d(dst, cache, bar, 64 * half, s.kvh, off, page);
-      else if (tree) tma_load_3d(dst, tree_rows, bar, 64 * half, s.kvh, s.r.s0 + node);
-      page = page_of(kt + 1);
+#pragma unroll 1
+      for (int x = 0; x < boxes; ++x) {
+        const int pg = __shfl_sync(0xffffffffu, of_page, x), at = __shfl_sync(0xffffffffu, from, x);
+        const uint32_t to = dst + x * p.box * 128;
+        if ((from_cache >> x) & 1u) {
+          if (elect_one()) {
+            tma_load_4d(to, cache, bar, 0, s.kvh, at, pg);
+            if (S::kHalves == 2) tma_load_4d(to + kHalf, cache, bar, 64, s.kvh, at, pg);
+          }
+        } else if ((from_tree >> x) & 1u) {
+          if (elect_one()) {
+            tma_load_3d(to, tree_rows, bar, 0, s.kvh, at);
+            if (S::kHalves == 2) tma_load_3d(to + kHalf, tree_rows, bar, 64, s.kvh, at);
+          }
+        }
+        __syncwarp();
+      }
     }
   }
   if (!ok) {
@@ -418,11 +486,12 @@ __device__ __forceinline__ bool load_tiles(const Params& p, Walk walk, uint32_t 
   if (*failed && lane == 0) {
     // Copies still in flight land before the CTA's shared memory is given up (bounded).
     volatile int no_abort = 0;
-    for (int i = max(0, j - S::kStages); i < j; ++i) mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
+#pragma unroll 1
+    for (int i = max(0, j - S::kStages); i < j; ++i) wait_for(full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
     if (!VALUES)
-      for (int i = max(0, seg - S::kQ); i < seg; ++i) mbar_wait(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
+#pragma unroll 1
+      for (int i = max(0, seg - S::kQ); i < seg; ++i) wait_for(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
   }
-  return ok;
 }
 
 template <int DT, int N, int HD>
@@ -434,13 +503,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   const uint32_t base = smem_u32(gb), sQ = base + S::kOffQ;
   const uint32_t k_full = base + S::kOffBar, v_full = k_full + 8 * S::kStages, empty = v_full + 8 * S::kStages, q_full = empty + 8 * S::kStages,
                  q_empty = q_full + 16, s_full = q_empty + 16, p_full = s_full + 8 * S::kS, done = p_full + 8 * S::kS, o_full = done + 8 * S::kS,
-                 o_empty = o_full + 16;
-  uint8_t* misc = gb + S::kOffBar + 8 * S::kBars;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc);
-  volatile int* failed = reinterpret_cast<volatile int*>(misc + 4);
-  int* found_b = reinterpret_cast<int*>(misc + 8);
-  int64_t* found = reinterpret_cast<int64_t*>(misc + 16);  // tiles before request found_b
-  int64_t* scan = reinterpret_cast<int64_t*>(misc + 32);   // sums of the warps
+                 o_empty = o_full + 16, plan_full = o_empty + 16;
+  Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(sizeof(Segment) == 48, "plans");
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -459,66 +526,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       mbar_init(o_full + 8 * i, 1);
       mbar_init(o_empty + 8 * i, kSoft);
     }
+    for (int i = 0; i < kPlans; ++i) mbar_init(plan_full + 8 * i, 1);
     *failed = 0;
     fence_barrier_init();
   }
   if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
 
-  // This CTA's share [t0, t1) of the list of tiles, and the request it begins with.
-  const int per = (p.batch + kThreads - 1) / kThreads, b_lo = min(p.batch, tid * per), b_hi = min(p.batch, b_lo + per);
-  int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) {
-    const Request r = request(p, b);
-    mine += r.tiles(p.kv_heads);
-    if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-  }
-  int64_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += y;
-  }
-  if (lane == 31) scan[warp] = upto;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int64_t all = 0, at = upto - mine;
-#pragma unroll 4
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) at += scan[w];
-    all += scan[w];
-  }
-  Shares shares;
-  shares.each = quotient(all, gridDim.x);
-  shares.more = all - shares.each * gridDim.x;
-  const int64_t t0 = shares.begin(blockIdx.x), t1 = shares.begin(blockIdx.x + 1);
-  if (t0 < t1 && at <= t0 && t0 < at + mine) {
-    for (int b = b_lo; b < b_hi; ++b) {
-      const int64_t w = request(p, b).tiles(p.kv_heads);
-      if (t0 < at + w) {
-        *found_b = b;
-        *found = at;
-        break;
-      }
-      at += w;
-    }
-  }
-  __syncthreads();
   const uint32_t tmem = *tmem_slot;
   const Scratch<N, HD> scratch{p.ws, (int)gridDim.x};
-  Walk walk;
-  walk.t = t0;
-  walk.end = t1;
-  walk.b = t0 < t1 ? *found_b : 0;
-  walk.before = t0 < t1 ? *found : 0;
   Segment s;
+  // Segment number `seg` of this CTA as it was planned; false behind the last one.
+  auto planned = [&](int seg, Segment& s) {
+    const bool there = __all_sync(0xffffffffu, wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed));
+    if (!there) *failed = 1;
+    s = plans[seg % kPlans];
+    return there && s.k1 > 0;
+  };
   constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
   auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
 
   if (warp == kLoadK) {
-    load_tiles<N, HD, false>(p, walk, base, k_full, empty, q_full, q_empty, failed);
+    load_tiles<N, HD, false>(p, planned, base, k_full, empty, q_full, q_empty, failed);
   } else if (warp == kLoadV) {
-    load_tiles<N, HD, true>(p, walk, base, v_full, empty, q_full, q_empty, failed);
+    load_tiles<N, HD, true>(p, planned, base, v_full, empty, q_full, q_empty, failed);
   } else if (warp == kMmaS) {
     // ---------------- S^T of every tile ----------------
     // The whole warp keeps the books, one lane issues: descriptors stay in uniform registers.
@@ -526,10 +559,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     const uint64_t d_k = sw128_desc(base), d_q = sw128_desc(sQ);
     bool ok = true;
     int j = 0, seg = 0, stage = 0, stage_phase = 0;
-    while (ok && walk.next(p, s)) {
+#pragma unroll 1
+    while (ok && planned(seg, s)) {
       const int qb = seg % S::kQ;
       ok = agreed(wait_for(q_full + 8 * qb, (seg / S::kQ) & 1, failed));
       const uint64_t b = d_q + (uint32_t)qb * (S::kQBytes >> 4);
+#pragma unroll 1
       for (int kt = s.k0; ok && kt < s.k1; ++kt, ++j) {
         const int sb = j % S::kS;
         ok = agreed(wait_for(k_full + 8 * stage, stage_phase, failed));
@@ -562,9 +597,72 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     const uint64_t d_v = sw128_desc_mn(base + S::kKBytes, kHalf, 1024), d_p = p_desc<N>(base);
     bool ok = true;
     int j = 0, seg = 0, stage = 0, stage_phase = 0;
-    while (ok && walk.next(p, s)) {
+    // The plan. This CTA's share [t0, t1) of the list of tiles, and the request it begins with: two passes over
+    // the requests, 32 at a time.
+    auto sum_up = [&](int x) {  // inclusive sums over the lanes
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      return x;
+    };
+    auto tiles_of = [&](int b) {
+      if (b >= p.batch) return 0;
+      const Request r = request(p, b);
+      if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+      return r.tiles(p.kv_heads);
+    };
+    const int first_tiles = tiles_of(lane);
+    int all = first_tiles;
+#pragma unroll 4
+    for (int b = lane + 32; b < p.batch; b += 32) all += tiles_of(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    Shares shares;
+    shares.each = all / (int)gridDim.x;
+    shares.more = all - shares.each * (int)gridDim.x;
+    Walk walk;
+    walk.t = shares.begin(blockIdx.x);
+    walk.end = shares.begin(blockIdx.x + 1);
+    walk.b = walk.before = 0;
+    if (walk.t < walk.end) {
+#pragma unroll 1
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int upto = sum_up(b0 ? tiles_of(b0 + lane) : first_tiles);
+        const uint32_t behind = __ballot_sync(0xffffffffu, walk.t < walk.before + upto);  // lanes whose request ends behind t
+        if (behind) {
+          const int x = __ffs(behind) - 1;
+          walk.b = b0 + x;
+          walk.before += x ? __shfl_sync(0xffffffffu, upto, x - 1) : 0;
+          break;
+        }
+        walk.before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    int plan = 0;
+    bool more = true;
+    auto plan_on = [&](int upto) {
+#pragma unroll 1
+      for (; more && plan <= upto; ++plan) {
+        more = next_segment(p, walk, s);
+        s.last = s.k1 > 0 && !s.whole && s.k0 == 0 ? shares.owner(s.row_end - 1) : 0;  // the CTA with the row's last tile
+        if (lane == 0) {
+          plans[plan % kPlans] = s;
+          mbar_arrive(plan_full + 8 * (plan % kPlans));
+        }
+        __syncwarp();
+      }
+    };
+    plan_on(1);
+#pragma unroll 1
+    while (true) {
+      // Everyone is done with the plan that this one replaces: P of the segment before this one is there.
+      plan_on(seg + 2);
+      if (!ok || !planned(seg, s)) break;
       const int ob = seg & 1;
       if (seg >= 2) ok = agreed(wait_for(o_empty + 8 * ob, ((seg >> 1) - 1) & 1, failed));
+#pragma unroll 1
       for (int kt = s.k0; ok && kt < s.k1; ++kt, ++j) {
         const int sb = j % S::kS, pipe = j % S::kPipes;
         ok = agreed(wait_for(v_full + 8 * stage, stage_phase, failed)) && agreed(wait_for(p_full + 8 * sb, (j / S::kS) & 1, failed));
@@ -573,9 +671,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         const uint64_t a = d_v + (uint32_t)stage * (S::kStage >> 4), b = d_p + (uint32_t)stage * (S::kStage >> 4);
         const uint32_t o = tmem + (S::kS + ob * S::kPipes + pipe) * N;
         const uint32_t add = kt - s.k0 < S::kPipes ? 0u : 1u;
+        const int steps = min(kKeys / 16, (s.pad + s.n - kt * kKeys + 15) / 16);  // up to the row's last key
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk) tc_mma_bf16(o, a + kk * 128, b + kk * S::kPitch, id_o, kk ? 1u : add);
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            if (kk < steps) tc_mma_bf16(o, a + kk * 128, b + kk * S::kPitch, id_o, kk ? 1u : add);
           tc_commit(empty + 8 * stage);
           tc_commit(done + 8 * sb);
           if (kt + 1 == s.k1) tc_commit(o_full + 8 * ob);
@@ -610,8 +710,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     };
     int j0 = 0, seg = 0;  // tiles before this segment
     bool wrote_start = false;
-    while (walk.next(p, s)) {
-      const int cols = min(p.nt, s.r.n - s.qt * p.nt) * p.group;
+#pragma unroll 1
+    while (planned(seg, s)) {
+      const int cols = min(p.nt, s.n - s.node0) * p.group;
       const int live = min(C, max(0, cols - c0));  // columns of this thread that are rows
       uint64_t l[C / 2];                           // this key's part of the sums
 #pragma unroll
@@ -620,11 +721,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       bool sick = false, begun = false;  // a drafted value that is not finite was set aside; this pipe's O holds something
       named_bar_sync(team, kTeam);
       const int tiles = s.k1 - s.k0;
+#pragma unroll 1
       for (int i0 = (pipe + S::kPipes - j0 % S::kPipes) % S::kPipes; i0 < tiles; i0 += S::kPipes) {
         const int j = j0 + i0, sb = j % S::kS, stage = j % S::kStages;
-        const int key0 = (s.k0 + i0) * kKeys, key = key0 + r, node = key - s.r.pad;
-        const bool masked = key0 + kKeys > s.r.len;
-        const bool in_prefix = key < s.r.len, in_tree = node >= 0 && node < s.r.n;
+        const int key0 = (s.k0 + i0) * kKeys, key = key0 + r, node = key - s.pad;
+        const bool masked = key0 + kKeys > s.len;
+        const bool in_prefix = key < s.len, in_tree = node >= 0 && node < s.n;
         const uint32_t stage_at = base + stage * S::kStage;
         // S of this tile also says that its stage was loaded, so the wait for its V below is at most one phase ahead.
         wait(s_full + 8 * sb, (j / S::kS) & 1);
@@ -632,30 +734,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         uint32_t vis = 0xffffffffu;  // bit i: column c0 + i sees this key
         if (masked) {
           const int c = c0 + lane;
-          vis = transpose_bits(lane < C && c < cols ? seen_bits(p, s.r.s0, s.qt * p.nt + c / p.group, node - lane) : 0u, lane);
+          vis = transpose_bits(lane < C && c < cols ? seen_bits(p, s.s0, s.node0 + c / p.group, node - lane) : 0u, lane);
           vis = in_prefix ? 0xffffffffu : in_tree ? vis : 0u;
-          // Rows of V without a key are whatever lay there: cleared. A drafted value that is not finite would reach
+          // Rows of V without a key (of those that the product takes) are whatever lay there: cleared. A drafted value that is not finite would reach
           // every column as 0 * inf: it is cleared too, and added at the end to the columns that see it.
           wait(v_full + 8 * stage, (j / S::kStages) & 1);
-          if (!in_prefix) {
+          const uint32_t v_row = stage_at + S::kKBytes + r * 128;
+          auto piece = [&](int c16) { return v_row + (c16 >> 3) * kHalf + 16 * ((c16 & 7) ^ (r & 7)); };
+          if (!in_prefix && !in_tree && node < ((s.n + 15) & ~15) + 16) {
+#pragma unroll 4
+            for (int c16 = c0 / C; c16 < 8 * S::kHalves; c16 += S::kGroups)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(piece(c16)), "r"(0) : "memory");
+          } else if (in_tree && (s.n > 1 || p.mask)) {  // (the node of a chain of one is hidden from nobody)
             constexpr uint32_t e = DT == AF_DTYPE_BF16 ? 0x7f80u : 0x7c00u;
-#pragma unroll 1
+#pragma unroll 4
             for (int c16 = c0 / C; c16 < 8 * S::kHalves; c16 += S::kGroups) {
-              const uint32_t where = stage_at + S::kKBytes + (c16 >> 3) * kHalf + r * 128 + 16 * ((c16 & 7) ^ (r & 7));
-              uint32_t w[4] = {0u, 0u, 0u, 0u};
-              bool bad = !in_tree;
-              if (in_tree) {
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(where) : "memory");
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece(c16)) : "memory");
+              bool bad = false;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const bool lo = (w[i] & e) == e, hi = ((w[i] >> 16) & e) == e;
-                  w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-                  bad |= lo || hi;
-                }
-                sick |= bad;
+              for (int i = 0; i < 4; ++i) {
+                const bool lo = (w[i] & e) == e, hi = ((w[i] >> 16) & e) == e;
+                w[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+                bad |= lo || hi;
               }
-              if (bad)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(where), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+              if (bad) {
+                sick = true;
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(c16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+              }
             }
           }
         }
@@ -690,9 +796,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
             }
           }
         };
-        shift();
-        if (vote_any<kTeam>(team, top > kRaise)) {
-          // New maxima of the columns that need one, from the scores themselves.
+        if (begun) shift();
+        if (!begun || vote_any<kTeam>(team, top > kRaise)) {
+          // New maxima of the columns that need one (at first of all of them), from the scores themselves.
           tmem_load<C>(lanes + sb * N + c0, x);
           float y[C];
 #pragma unroll
@@ -753,9 +859,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         if (lane == 0) mbar_arrive(p_full + 8 * sb);
       }
       // ---- the segment's rows: the pipes' sums and O joined; O^T lane = dim, column = row ----
-      const bool whole = s.whole();
+      const bool whole = s.whole != 0;
       const int which = s.k0 == 0 ? 1 : 0;
-      const int64_t first = s.r.s0 + (int64_t)s.qt * p.nt;
+      const int64_t first = s.s0 + (int64_t)s.node0;
       named_bar_sync(team, kTeam);  // the last factors are read
       {
         float y[C];
@@ -790,40 +896,54 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       wait(o_full + 8 * (seg & 1), (seg >> 1) & 1);
       tc_fence_after();
       named_bar_sync(5, kSoft * 32);
-      constexpr int kOut = N >= 32 ? N / 4 : 8;  // columns that a group of 128 threads writes
+      constexpr int kOut = N / 4, kW = kOut < 8 ? kOut : 8;  // columns that a group of 128 threads writes, and at once
       const int o0 = wg * kOut, o1 = min(cols, o0 + kOut);
       if (32 * quad < HD && o0 < o1) {
         float* part = scratch.sums(blockIdx.x, which) + r;
-        int i = o0 / p.group, head = o0 % p.group;
+        int i = o0 / p.group, head = o0 - i * p.group;
         char* out = p.out + (first + i) * p.out_n + (s.kvh * p.group + head) * p.out_h + 2 * r;
         const int64_t wrap = p.out_n - (p.group - 1) * p.out_h;  // from a node's last head to the next node's first
-#pragma unroll 1
-        for (int c8 = o0; c8 < o1; c8 += 8) {
-          float y[8];
+        uint32_t there = 0;  // the pipes with a tile of this segment (the O of another one is anything)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = 0.f;
+        for (int q = 0; q < S::kPipes; ++q) there |= (uint32_t)((q + S::kPipes - j0 % S::kPipes) % S::kPipes < tiles) << q;
+#pragma unroll 1
+        for (int c8 = o0; c8 < o1; c8 += kW) {
+          float y[kW];
+          uint32_t o[kW * S::kPipes];
+          tmem_load_rows<S::kPipes, N, kW>(lanes + (S::kS + (seg & 1) * S::kPipes) * N + c8, o);
+#pragma unroll
+          for (int e = 0; e < kW; ++e) y[e] = 0.f;
 #pragma unroll
           for (int q = 0; q < S::kPipes; ++q) {
-            // A pipe without a tile of this segment has an O of anything.
-            if ((q + S::kPipes - j0 % S::kPipes) % S::kPipes < tiles) {
-              uint32_t o[8];
-              tmem_load<8>(lanes + (S::kS + (seg & 1) * S::kPipes + q) * N + c8, o);
+            if ((there >> q) & 1u) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = fmaf(__uint_as_float(o[e]), fac[q * N + c8 + e], y[e]);
+              for (int e = 0; e < kW; e += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(fac + q * N + c8 + e);
+                y[e] = fmaf(__uint_as_float(o[kW * q + e]), f.x, y[e]);
+                y[e + 1] = fmaf(__uint_as_float(o[kW * q + e + 1]), f.y, y[e + 1]);
+                y[e + 2] = fmaf(__uint_as_float(o[kW * q + e + 2]), f.z, y[e + 2]);
+                y[e + 3] = fmaf(__uint_as_float(o[kW * q + e + 3]), f.w, y[e + 3]);
+              }
             }
           }
+          if (set_aside) {
+            const int x0 = max(0, s.k0 * kKeys - s.pad), x1 = min(s.n, s.k1 * kKeys - s.pad);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (c8 + e < o1) {
-              if (set_aside)
-                y[e] += set_aside_sum<DT>(p, s.r.s0, s.kvh, s.qt * p.nt + i, max(0, s.k0 * kKeys - s.r.pad), min(s.r.n, s.k1 * kKeys - s.r.pad), r);
-              if (whole) *reinterpret_cast<uint16_t*>(out) = to_bits<DT>(y[e]);
-              else part[(c8 + e) * HD] = y[e];
+            for (int e = 0; e < kW; ++e)
+              if (c8 + e < o1) y[e] += set_aside_sum<DT>(p, s.s0, s.kvh, s.node0 + (c8 + e) / p.group, x0, x1, r);
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < kW; ++e) {
+              if (c8 + e < o1) *reinterpret_cast<uint16_t*>(out) = to_bits<DT>(y[e]);
               const bool next = ++head == p.group;
               out += next ? wrap : p.out_h;
               head = next ? 0 : head;
-              i += next;
             }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kW; ++e)
+              if (c8 + e < o1) part[(c8 + e) * HD] = y[e];
           }
         }
       }
@@ -833,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       named_bar_sync(5, kSoft * 32);  // the factors lie where the next maxima go
       if (!whole && s.k0 == 0) {
         wrote_start = true;
-        if (tid == 0) *scratch.started(blockIdx.x) = Started{(int)shares.owner(s.row_end - 1), (int)first, cols, s.kvh};
+        if (tid == 0) *scratch.started(blockIdx.x) = Started{s.last, (int)first, cols, s.kvh};
       }
       j0 += tiles;
       ++seg;
@@ -1013,6 +1133,9 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
   p.nt = n / group;
+  // Tiles are counted in 32 bits: no more than this can come of any device-side values.
+  AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2) < 2147483000.0,
+             "af_tree_attention: more than 2^31 tiles of 128 keys");
   const uint64_t hd = (uint64_t)a.head_dim, kvh = (uint64_t)a.n_kv_heads;
   {
     const uint64_t dims[3] = {hd, (uint64_t)a.n_heads, (uint64_t)a.total};
