@@ -44,6 +44,7 @@ constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMmaS = kSoft + 2, kMmaO = kSo
 constexpr int kThreads = (kSoft + 4) * 32;
 constexpr int kPlans = 4;                   // segments planned in shared memory, up to two ahead of the products of O
 constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
+constexpr int kRow = 2;                     // cost of a row besides its tiles, in tiles (its end drains the pipeline: some 6600 cycles of 3000 a tile)
 constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
 constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
 
@@ -93,11 +94,11 @@ struct Params {
   unsigned* status;
 };
 
-// A request's tree and prefix; tiles = 0 where there is nothing to do or the values are bad.
+// A request's tree and prefix; no cost where there is nothing to do or the values are bad.
 struct Request {
   int s0, n, len, pad, kt, qt;
   bool bad;
-  __device__ __forceinline__ int tiles(int kv_heads) const { return kt * qt * kv_heads; }  // (of all requests below 2^31: checked by the host)
+  __device__ __forceinline__ int cost(int kv_heads) const { return kt ? (kt + kRow) * qt * kv_heads : 0; }  // (of all below 2^31: checked by the host)
 };
 
 __device__ __forceinline__ Request request(const Params& p, int b) {
@@ -113,7 +114,7 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   return r;
 }
 
-// The list of tiles cut into one share per CTA: the first `more` shares have each + 1.
+// The list of rows, each of kRow + kt units, cut into one share per CTA: the first `more` shares have each + 1.
 struct Shares {
   int each, more;
   __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
@@ -128,11 +129,11 @@ struct Shares {
 struct __align__(16) Segment {
   int s0, n, len, pad;       // the request's nodes, cached keys, and where the tree's keys begin
   int b, kvh, node0, k0;     // request, head, first node of the row tile
-  int k1, whole, row_end;    // all tiles of the row?; list index behind its last one
+  int k1, whole, row_end;    // all tiles of the row?; list index behind its last unit
   int last;                  // the CTA with the row's last tile, where this one begins a row that others go on with
 };
 struct Walk {
-  int t, end, before;  // next tile, end of the share, tiles of the requests before b
+  int t, end, before;  // next unit, end of the share, units of the requests before b
   int b;
 };
 
@@ -143,13 +144,12 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
   while (w.t < w.end) {
     Request r = request(p, w.b);
 #pragma unroll 1
-    while (w.t >= w.before + r.tiles(p.kv_heads)) {
-      w.before += r.tiles(p.kv_heads);
+    while (w.t >= w.before + r.cost(p.kv_heads)) {
+      w.before += r.cost(p.kv_heads);
       r = request(p, ++w.b);
     }
-    const int rel = w.t - w.before, row = rel / r.kt;
-    s.k0 = rel - row * r.kt;
-    s.row_end = w.before + (row + 1) * r.kt;
+    const int units = r.kt + kRow, rel = w.t - w.before, row = rel / units, u = rel - row * units;
+    s.row_end = w.before + (row + 1) * units;
     s.kvh = r.qt == 1 ? row : row / r.qt;
     s.node0 = (row - s.kvh * r.qt) * p.nt;
     s.s0 = r.s0;
@@ -157,14 +157,11 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
     s.len = r.len;
     s.pad = r.pad;
     s.b = w.b;
-    if (r.kt <= kWhole) {
-      w.t = s.row_end;
-      if (s.k0 > 0) continue;
-      s.k1 = r.kt;
-    } else {
-      s.k1 = min(r.kt, s.k0 + (w.end - w.t));
-      w.t += s.k1 - s.k0;
-    }
+    const int upto = r.kt <= kWhole ? units : min(units, u + (w.end - w.t));
+    w.t += upto - u;
+    s.k0 = max(0, u - kRow);
+    s.k1 = upto - kRow;
+    if (r.kt <= kWhole ? u > 0 : s.k1 <= s.k0) continue;  // begun by another CTA; no tile in this share
     s.whole = s.k0 == 0 && s.k1 == r.kt;
     return true;
   }
@@ -607,16 +604,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       }
       return x;
     };
-    auto tiles_of = [&](int b) {
+    auto cost_of = [&](int b) {
       if (b >= p.batch) return 0;
       const Request r = request(p, b);
       if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-      return r.tiles(p.kv_heads);
+      return r.cost(p.kv_heads);
     };
-    const int first_tiles = tiles_of(lane);
-    int all = first_tiles;
+    const int first_cost = cost_of(lane);
+    int all = first_cost;
 #pragma unroll 4
-    for (int b = lane + 32; b < p.batch; b += 32) all += tiles_of(b);
+    for (int b = lane + 32; b < p.batch; b += 32) all += cost_of(b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     Shares shares;
@@ -629,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     if (walk.t < walk.end) {
 #pragma unroll 1
       for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int upto = sum_up(b0 ? tiles_of(b0 + lane) : first_tiles);
+        const int upto = sum_up(b0 ? cost_of(b0 + lane) : first_cost);
         const uint32_t behind = __ballot_sync(0xffffffffu, walk.t < walk.before + upto);  // lanes whose request ends behind t
         if (behind) {
           const int x = __ffs(behind) - 1;
@@ -1134,7 +1131,7 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
   p.nt = n / group;
   // Tiles are counted in 32 bits: no more than this can come of any device-side values.
-  AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2) < 2147483000.0,
+  AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + kRow) < 2147483000.0,
              "af_tree_attention: more than 2^31 tiles of 128 keys");
   const uint64_t hd = (uint64_t)a.head_dim, kvh = (uint64_t)a.n_kv_heads;
   {
