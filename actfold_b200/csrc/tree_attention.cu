@@ -27,26 +27,16 @@
 // barrier vote, no maximum across lanes. P then stays below 256, which bf16
 // and fp16 round with the same relative error. Sums and O are fp32. Every wait is
 // bounded; a timeout sets AF_STATUS_TIMEOUT.
-#include <cuda.h>
-
-#include <atomic>
-
-#include "tree.cuh"
+#include "tree_attention.cuh"
 
 namespace af {
+namespace tree_attn {
 
 namespace {
 
-constexpr int kKeys = 128;                  // keys per tile (MMA M)
-constexpr int kHalf = kKeys * 128;          // [128 rows][64 columns] of 16 bits, 128-byte swizzle
 constexpr int kSoft = 16;                   // softmax warps
 constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMmaS = kSoft + 2, kMmaO = kSoft + 3;
 constexpr int kThreads = (kSoft + 4) * 32;
-constexpr int kPlans = 4;                   // segments planned in shared memory, up to two ahead of the products of O
-constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
-constexpr int kRow = 2;                     // cost of a row besides its tiles, in tiles (its end drains the pipeline: some 6600 cycles of 3000 a tile)
-constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
-constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
 
 // Shared memory: stages of (K, V) tiles, Q, and a little state. P^T of a tile
 // goes over its keys, which nobody needs once S is there.
@@ -67,6 +57,7 @@ struct Shape {
   static constexpr int kStages = (192 * 1024) / kStage < kPipes + kS ? (192 * 1024) / kStage : kPipes + kS;
   static constexpr int kQBytes = kHalves * N * 128;
   static constexpr int kQ = kQBytes <= 16384 ? 2 : 1;         // Q buffers
+  static constexpr int kOffK = 0, kOffV = kKBytes, kKStages = kStages, kVStages = kStages, kQTiles = 1, kQRows = N;
   static constexpr int kOffQ = kStages * kStage;
   static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
   static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
@@ -76,107 +67,6 @@ struct Shape {
   static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
 };
 
-struct Params {
-  CUtensorMap q, k, v, kc, vc;
-  const int *tables, *lengths, *starts;
-  const uint32_t* mask;
-  int64_t tables_ld, mask_ld;
-  int words, batch, total, kv_heads, group, pages, page, box, nt;
-  int64_t capacity;  // tokens that a table row can hold
-  float scale;       // times log2(e)
-  const char* v_rows;  // the tree's values, for those that are not finite
-  int64_t v_n, v_h;
-  char* out;
-  int64_t out_n, out_h;
-  float* lse;
-  int heads;
-  char* ws;
-  unsigned* status;
-};
-
-// A request's tree and prefix; no cost where there is nothing to do or the values are bad.
-struct Request {
-  int s0, n, len, pad, kt, qt;
-  bool bad;
-  __device__ __forceinline__ int cost(int kv_heads) const { return kt ? (kt + kRow) * qt * kv_heads : 0; }  // (of all below 2^31: checked by the host)
-};
-
-__device__ __forceinline__ Request request(const Params& p, int b) {
-  Request r;
-  const int s0 = p.starts[b], s1 = p.starts[b + 1];
-  r.len = p.lengths[b];
-  r.bad = s0 < 0 || s1 < s0 || s1 > p.total || r.len < 0 || r.len > p.capacity || (p.mask && s1 - s0 > 32 * (int64_t)p.words);
-  r.s0 = s0;
-  r.n = r.bad ? 0 : s1 - s0;
-  r.pad = (r.len + p.box - 1) & -p.box;
-  r.kt = r.n ? (r.pad + r.n + kKeys - 1) / kKeys : 0;
-  r.qt = r.n <= p.nt ? 1 : (r.n + p.nt - 1) / p.nt;
-  return r;
-}
-
-// The list of rows, each of kRow + kt units, cut into one share per CTA: the first `more` shares have each + 1.
-struct Shares {
-  int each, more;
-  __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
-  __device__ __forceinline__ int owner(int t) const {
-    const int big = more * (each + 1);
-    return t < big ? t / (each + 1) : more + (t - big) / each;
-  }
-};
-
-// The tiles [k0, k1) of one row tile that a CTA works on, as one warp plans
-// it and the others read it (k1 = 0: the share is done).
-struct __align__(16) Segment {
-  int s0, n, len, pad;       // the request's nodes, cached keys, and where the tree's keys begin
-  int b, kvh, node0, k0;     // request, head, first node of the row tile
-  int k1, whole, row_end;    // all tiles of the row?; list index behind its last unit
-  int last;                  // the CTA with the row's last tile, where this one begins a row that others go on with
-};
-struct Walk {
-  int t, end, before;  // next unit, end of the share, units of the requests before b
-  int b;
-};
-
-// The share's next segment. A row of up to kWhole tiles belongs to the CTA
-// whose share it begins in.
-__device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& s) {
-#pragma unroll 1
-  while (w.t < w.end) {
-    Request r = request(p, w.b);
-#pragma unroll 1
-    while (w.t >= w.before + r.cost(p.kv_heads)) {
-      w.before += r.cost(p.kv_heads);
-      r = request(p, ++w.b);
-    }
-    const int units = r.kt + kRow, rel = w.t - w.before, row = rel / units, u = rel - row * units;
-    s.row_end = w.before + (row + 1) * units;
-    s.kvh = r.qt == 1 ? row : row / r.qt;
-    s.node0 = (row - s.kvh * r.qt) * p.nt;
-    s.s0 = r.s0;
-    s.n = r.n;
-    s.len = r.len;
-    s.pad = r.pad;
-    s.b = w.b;
-    const int upto = r.kt <= kWhole ? units : min(units, u + (w.end - w.t));
-    w.t += upto - u;
-    s.k0 = max(0, u - kRow);
-    s.k1 = upto - kRow;
-    if (r.kt <= kWhole ? u > 0 : s.k1 <= s.k0) continue;  // begun by another CTA; no tile in this share
-    s.whole = s.k0 == 0 && s.k1 == r.kt;
-    return true;
-  }
-  s.k1 = 0;
-  return false;
-}
-
-// What CTA c left for k_tree_attention_join: it began a row tile that CTAs
-// c + 1 .. last went on with (last = 0: it did not).
-struct Started {
-  int last, node0, rows, kvh;
-};
-
-// Workspace: Started[ctas], then per CTA two partial rows (0: begun by an
-// earlier CTA, 1: begun here) of [N][HD] fp32 sums and [N] (maximum, sum) pairs.
 // P^T [128 keys][N rows] in shared memory: rows of kPitch bytes whose 16-byte
 // pieces are swizzled over as many bytes (32, 64 or 128), N >= 64 as blocks of 64.
 template <int N>
@@ -190,78 +80,6 @@ __device__ __forceinline__ uint32_t p_piece(int key, int col) {  // byte offset 
   return col / 64 * kHalf + key * (16 * pieces) + 16 * ((col / 8 % pieces) ^ ((key >> shift) % pieces));
 }
 
-template <int N, int HD>
-struct Scratch {
-  char* base;
-  int ctas;
-  __host__ __device__ static int64_t bytes(int ctas) { return ctas * (int64_t)(sizeof(Started) + 2 * N * (HD + 2) * 4); }
-  __device__ Started* started(int c) const { return reinterpret_cast<Started*>(base) + c; }
-  __device__ float* sums(int c, int which) const {
-    return reinterpret_cast<float*>(base + ctas * sizeof(Started)) + ((int64_t)c * 2 + which) * N * HD;
-  }
-  __device__ float2* stats(int c, int which) const {
-    return reinterpret_cast<float2*>(base + ctas * (sizeof(Started) + (int64_t)2 * N * HD * 4)) + ((int64_t)c * 2 + which) * N;
-  }
-};
-
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (DT == AF_DTYPE_BF16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ uint16_t to_bits(float x) {
-  return (uint16_t)pack2<DT>(x, 0.f);
-}
-
-__device__ __forceinline__ bool elect_one() {
-  int r;
-  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
-  return e;
-}
-
-// Pairs of fp32 values in one register pair (two results per instruction).
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-// Bounded wait for a phase: some seconds of attempts (each of which may itself sleep a little).
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* failed) {
-#pragma unroll 1
-  for (int n = 0; !mbar_try_wait(bar, parity); ++n)
-    if (n > (1 << 24) || *failed) return false;
-  return true;
-}
-
 // Lane i's 32 bits become bit i of every lane's word.
 __device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
 #pragma unroll
@@ -272,46 +90,6 @@ __device__ __forceinline__ uint32_t transpose_bits(uint32_t x, int lane) {
   return x;
 }
 
-template <int THREADS>
-__device__ __forceinline__ bool vote_any(int bar, bool mine) {
-  int r;
-  asm volatile(
-      "{\n\t.reg .pred a, b;\n\t"
-      "setp.ne.s32 a, %1, 0;\n\t"
-      "barrier.cta.red.or.pred b, %2, %3, a;\n\t"
-      "selp.s32 %0, 1, 0, b;\n\t}"
-      : "=r"(r)
-      : "r"((int)mine), "r"(bar), "n"(THREADS)
-      : "memory");
-  return r != 0;
-}
-
-// C consecutive columns of the thread's TMEM lane. Load and wait are one
-// statement: nothing that reads the registers can be placed between them.
-template <int C>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t* r) {
-  if constexpr (C == 8) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
-  } else if constexpr (C == 16) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr)
-                 : "memory");
-  } else {
-    static_assert(C == 32, "columns");
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-                   "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                   "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(taddr)
-                 : "memory");
-  }
-}
 // W columns (4 or 8) of each of P blocks of N columns.
 template <int P, int N, int W>
 __device__ __forceinline__ void tmem_load_rows(uint32_t taddr, uint32_t* r) {
@@ -352,13 +130,6 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
                : "memory");
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
-
 // C values per lane (16 or 32) reduced across the warp: lane x returns the
 // result of value x * C / 32. Each step halves the values that a lane keeps
 // (C - 1 exchanges and one more where C is 16; a reduction per value takes 5 C).
@@ -374,121 +145,6 @@ __device__ __forceinline__ float transpose_reduce(float* v, int lane, Op op) {
     }
   }
   return C == 32 ? v[0] : op(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
-}
-
-// Bits of the warp's 32 keys (nodes j0, j0 + 1, ... of the tree) that node i
-// sees; a bit outside the tree means nothing.
-__device__ __forceinline__ uint32_t seen_bits(const Params& p, int s0, int i, int j0) {
-  if (!p.mask) return i < j0 ? 0u : i - j0 >= 31 ? 0xffffffffu : (2u << (i - j0)) - 1u;
-  const uint32_t* row = p.mask + (int64_t)(s0 + i) * p.mask_ld;
-  const int w = j0 >> 5;  // j0 may be negative: rounds down
-  const uint32_t lo = w >= 0 && w < p.words ? row[w] : 0u, hi = w + 1 >= 0 && w + 1 < p.words ? row[w + 1] : 0u;
-  return __funnelshift_r(lo, hi, j0 & 31);
-}
-
-// The values of dim d that are not finite among nodes [x0, x1) that node i sees, added up.
-template <int DT>
-__device__ __noinline__ float set_aside_sum(const Params& p, int s0, int kvh, int i, int x0, int x1, int d) {
-  float sum = 0.f;
-#pragma unroll 1
-  for (int x = x0; x < x1; ++x) {
-    const float y = load_scalar<DT>(p.v_rows + (int64_t)(s0 + x) * p.v_n + kvh * p.v_h, d);
-    if (!isfinite(y) && (seen_bits(p, s0, i, x) & 1u)) sum += y;
-  }
-  return sum;
-}
-
-// Loads of one operand by a warp: K (with the Q of each segment) or V.
-template <int N, int HD, bool VALUES, typename Planned>
-__device__ __forceinline__ void load_tiles(const Params& p, Planned planned, uint32_t base, uint32_t full, uint32_t empty, uint32_t q_full,
-                                           uint32_t q_empty, volatile int* failed) {
-  using S = Shape<N, HD>;
-  const int lane = threadIdx.x & 31;
-  const CUtensorMap* cache = VALUES ? &p.vc : &p.kc;
-  const CUtensorMap* tree_rows = VALUES ? &p.v : &p.k;
-  if (lane < (VALUES ? 2 : 3)) tma_prefetch_desc(lane == 0 ? cache : lane == 1 ? tree_rows : &p.q);
-  const int boxes = kKeys / p.box, page_step = kKeys / p.page, off_step = kKeys % p.page;
-  int j = 0, seg = 0;
-  bool ok = true;
-  Segment s;
-#pragma unroll 1
-  while (ok && planned(seg, s)) {
-    const int* table = p.tables + (int64_t)s.b * p.tables_ld;
-    // Lane x knows where rows [x * R, (x + 1) * R) of a tile come from (a page is fetched a tile ahead); one lane issues.
-    const int row = lane * p.box;
-    int key = s.k0 * kKeys + row;
-    int entry = key / p.page, off = key - entry * p.page;  // its table entry and place in the page, carried from tile to tile
-    int page = lane < boxes && key < s.len ? table[entry] : 0;
-    if constexpr (!VALUES) {
-      const int qb = seg % S::kQ, use = seg / S::kQ;
-      if (use > 0) ok = __all_sync(0xffffffffu, wait_for(q_empty + 8 * qb, (use - 1) & 1, failed));
-      if (!ok) break;
-      if (elect_one()) {
-        mbar_arrive_expect_tx(q_full + 8 * qb, S::kHalves * p.nt * p.group * 128);
-        for (int h = 0; h < S::kHalves; ++h)
-          tma_load_3d(base + S::kOffQ + qb * S::kQBytes + h * N * 128, &p.q, q_full + 8 * qb, 64 * h, s.kvh * p.group, s.s0 + s.node0);
-      }
-      __syncwarp();
-    }
-    ++seg;
-#pragma unroll 1
-    for (int kt = s.k0; kt < s.k1; ++kt, ++j) {
-      const int node = key - s.pad;
-      const bool cached = lane < boxes && key < s.len, tree = lane < boxes && node >= 0 && node < s.n;
-      if (cached && (page < 0 || page >= p.pages)) {
-        if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-        page = p.pages;  // out of range: the box reads as zeros
-      }
-      const int from = cached ? off : s.s0 + node, of_page = page;
-      const uint32_t from_cache = __ballot_sync(0xffffffffu, cached), from_tree = __ballot_sync(0xffffffffu, tree);
-      key += kKeys;
-      entry += page_step;
-      off += off_step;
-      if (off >= p.page) {
-        off -= p.page;
-        ++entry;
-      }
-      page = lane < boxes && kt + 1 < s.k1 && key < s.len ? table[entry] : 0;
-      const int stage = j % S::kStages, round = j / S::kStages;
-      if (round > 0) ok = __all_sync(0xffffffffu, wait_for(empty + 8 * stage, (round - 1) & 1, failed));
-      if (!ok) break;
-      const uint32_t bar = full + 8 * stage;
-      const uint32_t dst = base + stage * S::kStage + (VALUES ? S::kKBytes : 0);
-      if (elect_one()) mbar_arrive_expect_tx(bar, __popc(from_cache | from_tree) * p.box * 128 * S::kHalves);
-      __syncwarp();
-#pragma unroll 1
-      for (int x = 0; x < boxes; ++x) {
-        const int pg = __shfl_sync(0xffffffffu, of_page, x), at = __shfl_sync(0xffffffffu, from, x);
-        const uint32_t to = dst + x * p.box * 128;
-        if ((from_cache >> x) & 1u) {
-          if (elect_one()) {
-            tma_load_4d(to, cache, bar, 0, s.kvh, at, pg);
-            if (S::kHalves == 2) tma_load_4d(to + kHalf, cache, bar, 64, s.kvh, at, pg);
-          }
-        } else if ((from_tree >> x) & 1u) {
-          if (elect_one()) {
-            tma_load_3d(to, tree_rows, bar, 0, s.kvh, at);
-            if (S::kHalves == 2) tma_load_3d(to + kHalf, tree_rows, bar, 64, s.kvh, at);
-          }
-        }
-        __syncwarp();
-      }
-    }
-  }
-  if (!ok) {
-    *failed = 1;
-    if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
-  }
-  __syncwarp();
-  if (*failed && lane == 0) {
-    // Copies still in flight land before the CTA's shared memory is given up (bounded).
-    volatile int no_abort = 0;
-#pragma unroll 1
-    for (int i = max(0, j - S::kStages); i < j; ++i) wait_for(full + 8 * (i % S::kStages), (i / S::kStages) & 1, &no_abort);
-    if (!VALUES)
-#pragma unroll 1
-      for (int i = max(0, seg - S::kQ); i < seg; ++i) wait_for(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
-  }
 }
 
 template <int DT, int N, int HD>
@@ -535,20 +191,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   const uint32_t tmem = *tmem_slot;
   const Scratch<N, HD> scratch{p.ws, (int)gridDim.x};
   Segment s;
-  // Segment number `seg` of this CTA as it was planned; false behind the last one.
-  auto planned = [&](int seg, Segment& s) {
-    const bool there = __all_sync(0xffffffffu, wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed));
-    if (!there) *failed = 1;
-    s = plans[seg % kPlans];
-    return there && s.k1 > 0;
-  };
+  auto planned = [&](int seg, Segment& s) { return read_plan(plans, plan_full, seg, s, failed); };
   constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
   auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
 
   if (warp == kLoadK) {
-    load_tiles<N, HD, false>(p, planned, base, k_full, empty, q_full, q_empty, failed);
+    load_tiles<S, false>(p, planned, base, k_full, empty, q_full, q_empty, failed);
   } else if (warp == kLoadV) {
-    load_tiles<N, HD, true>(p, planned, base, v_full, empty, q_full, q_empty, failed);
+    load_tiles<S, true>(p, planned, base, v_full, empty, q_full, q_empty, failed);
   } else if (warp == kMmaS) {
     // ---------------- S^T of every tile ----------------
     // The whole warp keeps the books, one lane issues: descriptors stay in uniform registers.
@@ -594,68 +244,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     const uint64_t d_v = sw128_desc_mn(base + S::kKBytes, kHalf, 1024), d_p = p_desc<N>(base);
     bool ok = true;
     int j = 0, seg = 0, stage = 0, stage_phase = 0;
-    // The plan. This CTA's share [t0, t1) of the list of tiles, and the request it begins with: two passes over
-    // the requests, 32 at a time.
-    auto sum_up = [&](int x) {  // inclusive sums over the lanes
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      return x;
-    };
-    auto cost_of = [&](int b) {
-      if (b >= p.batch) return 0;
-      const Request r = request(p, b);
-      if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-      return r.cost(p.kv_heads);
-    };
-    const int first_cost = cost_of(lane);
-    int all = first_cost;
-#pragma unroll 4
-    for (int b = lane + 32; b < p.batch; b += 32) all += cost_of(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-    Shares shares;
-    shares.each = all / (int)gridDim.x;
-    shares.more = all - shares.each * (int)gridDim.x;
-    Walk walk;
-    walk.t = shares.begin(blockIdx.x);
-    walk.end = shares.begin(blockIdx.x + 1);
-    walk.b = walk.before = 0;
-    if (walk.t < walk.end) {
-#pragma unroll 1
-      for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int upto = sum_up(b0 ? cost_of(b0 + lane) : first_cost);
-        const uint32_t behind = __ballot_sync(0xffffffffu, walk.t < walk.before + upto);  // lanes whose request ends behind t
-        if (behind) {
-          const int x = __ffs(behind) - 1;
-          walk.b = b0 + x;
-          walk.before += x ? __shfl_sync(0xffffffffu, upto, x - 1) : 0;
-          break;
-        }
-        walk.before += __shfl_sync(0xffffffffu, upto, 31);
-      }
-    }
-    int plan = 0;
-    bool more = true;
-    auto plan_on = [&](int upto) {
-#pragma unroll 1
-      for (; more && plan <= upto; ++plan) {
-        more = next_segment(p, walk, s);
-        s.last = s.k1 > 0 && !s.whole && s.k0 == 0 ? shares.owner(s.row_end - 1) : 0;  // the CTA with the row's last tile
-        if (lane == 0) {
-          plans[plan % kPlans] = s;
-          mbar_arrive(plan_full + 8 * (plan % kPlans));
-        }
-        __syncwarp();
-      }
-    };
-    plan_on(1);
+    Planner planner;
+    planner.begin(p, lane);
+    planner.on(p, plans, plan_full, 1, lane);
 #pragma unroll 1
     while (true) {
       // Everyone is done with the plan that this one replaces: P of the segment before this one is there.
-      plan_on(seg + 2);
+      planner.on(p, plans, plan_full, seg + 2, lane);
       if (!ok || !planned(seg, s)) break;
       const int ob = seg & 1;
       if (seg >= 2) ok = agreed(wait_for(o_empty + 8 * ob, ((seg >> 1) - 1) & 1, failed));
@@ -1031,7 +626,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_tree_attention_join(const __gr
   }
 }
 
-int64_t workspace_bytes() { return Scratch<128, 128>::bytes(sm_count()); }
+int64_t workspace_bytes() { return Scratch<256, 128>::bytes(sm_count()); }
 
 int check_args(const af_tree_attention_args& a) {
   AF_REQUIRE(a.batch >= 0 && a.total >= 0 && a.max_pages >= 0 && a.pages >= 0, "af_tree_attention: bad shape");
@@ -1079,37 +674,42 @@ template <int DT, int N, int HD>
 int launch(const Params& p, cudaStream_t s) {
   using S = Shape<N, HD>;
   static_assert(S::kBytes <= 232448, "shared memory");
-  static std::atomic<uint64_t> allowed{0};  // a bit per device whose copy of the kernel may use this much shared memory
-  int device = 0;
-  cudaGetDevice(&device);
-  const uint64_t bit = 1ull << (device & 63);
-  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    const cudaError_t e = cudaFuncSetAttribute(k_tree_attention<DT, N, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes);
-    if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: ") + cudaGetErrorString(e));
-    allowed.fetch_or(bit, std::memory_order_relaxed);
-  }
+  if (int st = allow_smem<k_tree_attention<DT, N, HD>>(S::kBytes)) return st;
   const int ctas = sm_count();
-  cudaError_t e = launch_ex(k_tree_attention<DT, N, HD>, dim3(ctas), dim3(kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
-  if (e == cudaSuccess && p.capacity + p.total > kWhole * kKeys)  // else no row is shared
-    e = launch_ex(k_tree_attention_join<DT, N, HD>, dim3(ctas, kJoinBlocks), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+  const cudaError_t e = launch_ex(k_tree_attention<DT, N, HD>, dim3(ctas), dim3(kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: launch: ") + cudaGetErrorString(e));
-  return check_launch("af_tree_attention");
+  return join_launch<DT, N, HD>(p, ctas, s);
 }
 
 template <int DT, int HD>
 int launch_rows(const Params& p, int n, cudaStream_t s) {
-  return n == 16 ? launch<DT, 16, HD>(p, s) : n == 32 ? launch<DT, 32, HD>(p, s) : n == 64 ? launch<DT, 64, HD>(p, s) : launch<DT, 128, HD>(p, s);
+  return n == 16 ? launch<DT, 16, HD>(p, s) : n == 32 ? launch<DT, 32, HD>(p, s) : launch<DT, 64, HD>(p, s);
 }
 
-template <int DT>
-int launch_shape(const Params& p, int n, int64_t head_dim, cudaStream_t s) {
-  return head_dim == 128 ? launch_rows<DT, 128>(p, n, s) : launch_rows<DT, 64>(p, n, s);
+int launch_narrow(const Params& p, int n, bool bf16, int64_t head_dim, cudaStream_t s) {
+  if (head_dim == 128) return bf16 ? launch_rows<AF_DTYPE_BF16, 128>(p, n, s) : launch_rows<AF_DTYPE_F16, 128>(p, n, s);
+  return bf16 ? launch_rows<AF_DTYPE_BF16, 64>(p, n, s) : launch_rows<AF_DTYPE_F16, 64>(p, n, s);
 }
 
 }  // namespace
+
+template <int DT, int N, int HD>
+int join_launch(const Params& p, int ctas, cudaStream_t s) {
+  if (p.capacity + p.total <= kWhole * kKeys) return check_launch("af_tree_attention");  // no row is shared
+  const cudaError_t e = launch_ex(k_tree_attention_join<DT, N, HD>, dim3(ctas, kJoinBlocks), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: launch: ") + cudaGetErrorString(e));
+  return check_launch("af_tree_attention");
+}
+template int join_launch<AF_DTYPE_F16, 256, 64>(const Params&, int, cudaStream_t);
+template int join_launch<AF_DTYPE_F16, 256, 128>(const Params&, int, cudaStream_t);
+template int join_launch<AF_DTYPE_BF16, 256, 64>(const Params&, int, cudaStream_t);
+template int join_launch<AF_DTYPE_BF16, 256, 128>(const Params&, int, cudaStream_t);
+
+}  // namespace tree_attn
 }  // namespace af
 
 using namespace af;
+using namespace af::tree_attn;
 
 extern "C" int af_tree_attention_workspace_bytes(int64_t* bytes) {
   AF_REQUIRE(bytes, "af_tree_attention_workspace_bytes: null pointer");
@@ -1125,11 +725,12 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   Params p;
   memset(&p, 0, sizeof(p));
   const int group = (int)(a.n_heads / a.n_kv_heads);
-  // Columns of a tile: the fewest that the average tree fits (the keys are read once per row tile).
+  // Rows of a tile: the fewest that the average tree fits (the keys are read once per row tile); over 64 the wide kernel.
   const int64_t rows = ceil_div(a.total, a.batch) * group;
-  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 256;
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
-  p.nt = n / group;
+  p.nt_q = (n == 256 ? 128 : n) / group;
+  p.nt = n == 256 ? 2 * p.nt_q : p.nt_q;
   // Tiles are counted in 32 bits: no more than this can come of any device-side values.
   AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + kRow) < 2147483000.0,
              "af_tree_attention: more than 2^31 tiles of 128 keys");
@@ -1137,7 +738,7 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   {
     const uint64_t dims[3] = {hd, (uint64_t)a.n_heads, (uint64_t)a.total};
     const int64_t st[2] = {a.q_strides[1], a.q_strides[0]};
-    const uint32_t bx[3] = {64, (uint32_t)group, (uint32_t)p.nt};
+    const uint32_t bx[3] = {64, (uint32_t)group, (uint32_t)p.nt_q};
     if (int e = tree_map(&p.q, a.q, (int)a.dtype, 3, dims, st, bx)) return e;
   }
   for (int x = 0; x < 2; ++x) {
@@ -1180,5 +781,6 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   p.ws = static_cast<char*>(a.workspace);
   p.status = status;
   cudaStream_t s = as_stream(stream);
-  return a.dtype == AF_DTYPE_BF16 ? launch_shape<AF_DTYPE_BF16>(p, n, a.head_dim, s) : launch_shape<AF_DTYPE_F16>(p, n, a.head_dim, s);
+  const bool bf16 = a.dtype == AF_DTYPE_BF16;
+  return n == 256 ? wide_launch(p, bf16, (int)a.head_dim, s) : launch_narrow(p, n, bf16, a.head_dim, s);
 }

@@ -80,8 +80,7 @@ def _same_device(what: str, *tensors: torch.Tensor | None) -> int:
     return index
 
 
-def _vectors(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
-    """Refuse what is not a vector of ``dtype``."""
+def _not_vectors(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) -> None:
     for name, t in tensors.items():
         if t is not None and (t.dtype is not dtype or t.dim() != 1):
             raise ValueError(f"{what}: {name} must be a {dtype} vector, got {t.dtype} {tuple(t.shape)}")
@@ -123,7 +122,9 @@ def block_tables(
     row, inner = tables.stride()
     if (inner != 1 and most > 1) or (row < most and n > 1):
         raise ValueError("block_tables: the rows of tables must be contiguous and must not overlap")
-    _vectors("block_tables", _I32, lengths=lengths, grow=grow, held=held, free_pages=free_pages)
+    if not (lengths.dtype is grow.dtype is free_pages.dtype is _I32 and lengths.dim() == grow.dim() == free_pages.dim() == 1
+            and (held is None or (held.dtype is _I32 and held.dim() == 1))):
+        _not_vectors("block_tables", _I32, lengths=lengths, grow=grow, held=held, free_pages=free_pages)
     if lengths.shape[0] != n or grow.shape[0] != n or (held is not None and held.shape[0] != n):
         raise ValueError(f"block_tables: lengths, grow and held must have one entry for each of {n} requests")
     if not free_pages.is_contiguous():
@@ -162,7 +163,9 @@ def tree_masks(
     base[b] + depth`` (``base`` = the prefix lengths). A tree may hold up to
     ``32 * words`` nodes. Rows behind ``starts[-1]`` are not written.
     """
-    _vectors("tree_masks", _I32, parents=parents, starts=starts, base=base)
+    if not (parents.dtype is starts.dtype is _I32 and parents.dim() == starts.dim() == 1
+            and (base is None or (base.dtype is _I32 and base.dim() == 1))):
+        _not_vectors("tree_masks", _I32, parents=parents, starts=starts, base=base)
     batch, total = starts.shape[0] - 1, parents.shape[0]
     if batch < 0 or words <= 0:
         raise ValueError(f"tree_masks: starts needs one entry more than there are trees, words {words} must be positive")
@@ -200,8 +203,11 @@ def accept_tree(
     (after the prefix when there is none, -1 when that is not given).
     ``max_nodes``: nodes of the largest tree, when known (at most 16384).
     """
-    _vectors("accept_tree", _I32, parents=parents, starts=starts)
-    _vectors("accept_tree", _I64, tokens=tokens, targets=targets, root_targets=root_targets)
+    if not (parents.dtype is starts.dtype is _I32 and tokens.dtype is targets.dtype is _I64
+            and parents.dim() == starts.dim() == tokens.dim() == targets.dim() == 1
+            and (root_targets is None or (root_targets.dtype is _I64 and root_targets.dim() == 1))):
+        _not_vectors("accept_tree", _I32, parents=parents, starts=starts)
+        _not_vectors("accept_tree", _I64, tokens=tokens, targets=targets, root_targets=root_targets)
     batch, total = starts.shape[0] - 1, parents.shape[0]
     if tokens.shape[0] != total or targets.shape[0] != total:
         raise ValueError(f"accept_tree: tokens and targets must have one entry for each of {total} nodes")
@@ -218,11 +224,6 @@ def accept_tree(
             batch, total, 16384 if max_nodes is None else max_nodes, None if root_targets is None else root_targets.data_ptr(), keep,
             rows.data_ptr(), counts.data_ptr(), following.data_ptr(), _status(status))
     return AcceptedPath(rows, counts, following)
-
-
-def _bytes(t: torch.Tensor, size: int) -> list[int]:
-    """Strides of all dimensions but the innermost in bytes, 0 for a dimension of one entry (torch leaves any value there)."""
-    return [x * size if n > 1 else 0 for x, n in zip(t.stride()[:-1], t.shape)]
 
 
 def write_cache(
@@ -261,24 +262,26 @@ def write_cache(
         raise ValueError(f"write_cache: {count} slots for {n} rows")
     if cache[2] == 0:
         raise ValueError("write_cache: page_size must be positive")
-    for c in (k_cache, v_cache):
-        st = c.stride()
-        if dim > 1 and st[4] != 1:
-            raise ValueError("write_cache: the innermost dimension of the caches must be contiguous")
-        if 0 in st and any(x == 0 and m > 1 for x, m in zip(st, cache)):
+    kc0, kc1, kc2, kc3, kc4 = k_cache.stride()
+    vc0, vc1, vc2, vc3, vc4 = v_cache.stride()
+    if (kc4 != 1 or vc4 != 1) and dim > 1:
+        raise ValueError("write_cache: the innermost dimension of the caches must be contiguous")
+    if not (kc0 and kc1 and kc2 and kc3 and vc0 and vc1 and vc2 and vc3):
+        if any(x == 0 and m > 1 for c in (k_cache, v_cache) for x, m in zip(c.stride(), cache)):
             raise ValueError("write_cache: the caches have entries that share memory")
     index = _same_device("write_cache", k, v, k_cache, v_cache, slots, rows)
-    if dim > 1 and k.stride(3) != 1:
-        k = k.contiguous()
-    if dim > 1 and v.stride(3) != 1:
-        v = v.contiguous()
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if (k3 != 1 or v3 != 1) and dim > 1:
+        k, v = k.contiguous(), v.contiguous()
+        k0, k1, k2, k3 = v0, v1, v2, v3 = k.stride()
     slots = slots.contiguous()
     if rows is not None:
         rows = rows.contiguous()
-    size = k.element_size()
-    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *_bytes(k, size), *_bytes(v, size), k_cache.data_ptr(), v_cache.data_ptr(),
-                      *_bytes(k_cache, size), *_bytes(v_cache, size), slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n,
-                      count, cache[1], cache[2], layers, heads, dim * size)
+    e = k.element_size()
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), e * k0, e * k1, e * k2, e * v0, e * v1, e * v2, k_cache.data_ptr(), v_cache.data_ptr(),
+                      e * kc0, e * kc1, e * kc2, e * kc3, e * vc0, e * vc1, e * vc2, e * vc3, slots.data_ptr(),
+                      0 if rows is None else rows.data_ptr(), n, count, cache[1], cache[2], layers, heads, dim * e)
     _launch("write_cache", index, _lib.load().af_write_cache, args, _status(status))
 
 
@@ -296,6 +299,16 @@ def _grid(t: torch.Tensor) -> list[int] | None:
             return None
         out.append(2 * x)
     return out
+
+
+def _row_grid(t: torch.Tensor) -> tuple | list | None:
+    a, b, c = t.stride()
+    return (2 * a, 2 * b) if c == 1 and a > 0 and b > 0 and not ((a | b) & 7 or t.data_ptr() & 15) else _grid(t)
+
+
+def _cache_grid(t: torch.Tensor) -> tuple | list | None:
+    a, b, c, d = t.stride()
+    return (2 * a, 2 * b, 2 * c) if d == 1 and a > 0 and b > 0 and c > 0 and not ((a | b | c) & 7 or t.data_ptr() & 15) else _grid(t)
 
 
 def tree_attention(
@@ -343,7 +356,8 @@ def tree_attention(
     if tables.dim() != 2 or tables.dtype is not _I32:
         raise ValueError(f"tree_attention: tables must be int32 [requests, max_pages], got {tables.dtype} {tuple(tables.shape)}")
     batch, most = tables.shape
-    _vectors("tree_attention", _I32, lengths=lengths, starts=starts)
+    if not (lengths.dtype is starts.dtype is _I32 and lengths.dim() == starts.dim() == 1):
+        _not_vectors("tree_attention", _I32, lengths=lengths, starts=starts)
     if lengths.shape[0] != batch or starts.shape[0] != batch + 1:
         raise ValueError(f"tree_attention: {batch} requests need as many lengths and one entry of starts more")
     index = q.get_device()
@@ -357,12 +371,12 @@ def tree_attention(
             mask = mask.contiguous()
             mask_row = words
         mask_at = mask.data_ptr()
-    k_grid, v_grid = _grid(k_cache), _grid(v_cache)
+    k_grid, v_grid = _cache_grid(k_cache), _cache_grid(v_cache)
     if k_grid is None or v_grid is None:
         raise ValueError("tree_attention: the caches' innermost dimension must be contiguous, their other strides multiples of 16 bytes")
     out_grid = None
     if out is not None:
-        if out.shape != qs or out.dtype is not dtype or (out_grid := _grid(out)) is None:
+        if out.shape != qs or out.dtype is not dtype or (out_grid := _row_grid(out)) is None:
             raise ValueError("tree_attention: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
     if lse is not None and (lse.shape != (total, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
         raise ValueError(f"tree_attention: lse must be contiguous float32 [{total}, {heads}]")
@@ -370,13 +384,13 @@ def tree_attention(
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts = lengths.contiguous(), starts.contiguous()
-    if (q_grid := _grid(q)) is None:
+    if (q_grid := _row_grid(q)) is None:
         q = q.clone(memory_format=torch.contiguous_format)
         q_grid = _grid(q)
-    if (kr_grid := _grid(k)) is None:
+    if (kr_grid := _row_grid(k)) is None:
         k = k.clone(memory_format=torch.contiguous_format)
         kr_grid = _grid(k)
-    if (vr_grid := _grid(v)) is None:
+    if (vr_grid := _row_grid(v)) is None:
         v = v.clone(memory_format=torch.contiguous_format)
         vr_grid = _grid(v)
     if out is None:

@@ -374,6 +374,14 @@ CASES = [
     ([9000, 3, 2500], [1, 1, 1], 8, 2, 128, 64, torch.float16, "chain"),
     ([12, 2000], [300, 200], 2, 1, 128, 16, torch.bfloat16, "chain"),
     ([30000], [20], 4, 4, 128, 16, torch.bfloat16, "tree"),
+    # more than 64 rows per key/value head: one row tile (even and odd key tiles), two, shared by several SMs or not
+    ([7000], [100], 4, 4, 64, 32, torch.bfloat16, "any"),
+    ([129, 4000, 0, 1], [70, 128, 90, 66], 4, 4, 128, 16, torch.bfloat16, "tree"),
+    ([5000, 900], [64, 33], 28, 4, 128, 16, torch.float16, "tree"),
+    ([6000, 40], [300, 5], 8, 2, 128, 64, torch.bfloat16, "any"),
+    ([100, 1700], [129, 200], 6, 2, 64, 8, torch.float16, "chain"),
+    ([0, 0, 3], [80, 200, 100], 2, 2, 128, 16, torch.bfloat16, "none"),
+    ([20000], [64], 16, 1, 128, 48, torch.bfloat16, "tree"),
 ]
 
 
@@ -381,6 +389,19 @@ CASES = [
 def test_attention(lengths, ns, heads, kv, dim, page, dtype, kind):
     args, plain = _case(lengths, ns, heads, kv, dim, page, dtype, seed=len(lengths) + sum(ns), kind=kind)
     _check(args, plain)
+
+
+@pytest.mark.parametrize("case", [CASES[6], CASES[7], CASES[14], CASES[16], *CASES[17:]])
+def test_attention_does_not_depend_on_what_its_scratch_held(case):
+    """Rows that several SMs worked on are joined from scratch memory: only what this call wrote there may count."""
+    from actfold_b200.speculative import tree_attention
+
+    args, _ = _case(*case[:7], seed=2, kind=case[7])
+    first = tree_attention(**args).clone()
+    for i in range(6):
+        junk = torch.full((12_000_000,), (float("nan"), 1e20, -3.0)[i % 3], device="cuda")  # freed at once: the next scratch lies in it
+        del junk
+        assert torch.equal(tree_attention(**args).view(torch.int16), first.view(torch.int16))
 
 
 def test_attention_head_major_cache_and_fused_projections():
@@ -400,16 +421,18 @@ def test_attention_copies_rows_off_the_grid():
     _check(args, plain)
 
 
-@pytest.mark.parametrize("spread,scale", [(8.0, None), (1.0, 1.0), (0.01, None), (30.0, None)])
-def test_attention_sharp_and_flat_rows(spread, scale):
-    args, plain = _case([1500, 200], [20, 70], 8, 2, 128, 64, torch.bfloat16, spread=spread)
+@pytest.mark.parametrize("spread,scale", [(8.0, None), (1.0, 1.0), (0.01, None), (30.0, None), (1.0, -0.2), (1.0, 0.0)])
+@pytest.mark.parametrize("ns", [[3, 5], [20, 70]])
+def test_attention_sharp_and_flat_rows(spread, scale, ns):
+    args, plain = _case([1500, 200], ns, 8, 2, 128, 64, torch.bfloat16, spread=spread)
     _check(args, plain, scale=scale)
 
 
 @pytest.mark.parametrize("step", [+1, -1])
-def test_attention_maximum_that_moves_from_key_to_key(step):
+@pytest.mark.parametrize("nodes", [7, 40, 80, 150])
+def test_attention_maximum_that_moves_from_key_to_key(step, nodes):
     """Scores that rise (the running maximum is raised again and again) or fall along the cache."""
-    args, plain = _case([2000], [7], 4, 4, 128, 16, torch.bfloat16)
+    args, plain = _case([2000], [nodes], 4, 4, 128, 16, torch.bfloat16)
     tables, (t,), _, _ = plain
     ramp = torch.linspace(0, 40, t, device="cuda") if step > 0 else torch.linspace(40, 0, t, device="cuda")
     args["q"][:, :, 0] = 11.3125  # about sqrt(128): the score gains the ramp
@@ -426,9 +449,10 @@ def test_attention_rows_behind_the_last_tree_stay():
     assert got is out and out[34:].eq(3.0).all()
 
 
-def test_attention_hidden_nodes_have_no_influence():
+@pytest.mark.parametrize("heads", [8, 2, 16])
+def test_attention_hidden_nodes_have_no_influence(heads):
     """NaN and infinities in nodes (and in queries of others) that a row does not see."""
-    args, plain = _case([200, 64, 0], [20, 3, 33], 8, 2, 128, 16, torch.bfloat16, kind="tree", seed=5)
+    args, plain = _case([200, 64, 0], [20, 3, 33], heads, 2, 128, 16, torch.bfloat16, kind="tree", seed=5)
     clean = _check(args, plain).clone()
     bits, starts = plain[3], plain[2]
     sick = [starts[0] + 19, starts[2] + 7]
@@ -445,8 +469,9 @@ def test_attention_hidden_nodes_have_no_influence():
 
 
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
-def test_attention_values_that_are_not_finite_reach_the_rows_that_see_them(value):
-    args, plain = _case([130], [12], 4, 2, 128, 16, torch.bfloat16, seed=8)
+@pytest.mark.parametrize("heads", [4, 32])
+def test_attention_values_that_are_not_finite_reach_the_rows_that_see_them(value, heads):
+    args, plain = _case([130], [12], heads, 2, 128, 16, torch.bfloat16, seed=8)
     args["v"][4, :, 3] = value
     from actfold_b200.speculative import tree_attention
 
