@@ -40,8 +40,11 @@ struct Params {
 // A request's tree and prefix; no cost where there is nothing to do or the values are bad.
 struct Request {
   int s0, n, len, pad, kt, qt;
-  bool bad;
-  __device__ __forceinline__ int cost(int kv_heads) const { return kt ? (kt + kRow) * qt * kv_heads : 0; }  // (of all below 2^31: checked by the host)
+  bool bad, narrow;  // narrow: the last row tile has no second Q box, and a wide CTA takes two of its key tiles at a time
+  // Units of a row tile and of a head's row tiles (of all heads and requests below 2^31: checked by the host).
+  __device__ __forceinline__ int units(bool last) const { return kRow + (last && narrow ? (kt + 1) / 2 : kt); }
+  __device__ __forceinline__ int head_units() const { return (qt - 1) * units(false) + units(true); }
+  __device__ __forceinline__ int cost(int kv_heads) const { return kt ? head_units() * kv_heads : 0; }
 };
 
 __device__ __forceinline__ Request request(const Params& p, int b) {
@@ -54,10 +57,11 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.pad = (r.len + p.box - 1) & -p.box;
   r.kt = r.n ? (r.pad + r.n + kKeys - 1) / kKeys : 0;
   r.qt = r.n <= p.nt ? 1 : (r.n + p.nt - 1) / p.nt;
+  r.narrow = p.nt > p.nt_q && r.n - (r.qt - 1) * p.nt <= p.nt_q;
   return r;
 }
 
-// The list of rows, each of kRow + kt units, cut into one share per CTA: the first `more` shares have each + 1.
+// The list of rows, each of kRow units and one per key tile, cut into one share per CTA: the first `more` shares have each + 1.
 struct Shares {
   int each, more;
   __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
@@ -91,10 +95,13 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
       w.before += r.cost(p.kv_heads);
       r = request(p, ++w.b);
     }
-    const int units = r.kt + kRow, rel = w.t - w.before, row = rel / units, u = rel - row * units;
-    s.row_end = w.before + (row + 1) * units;
-    s.kvh = r.qt == 1 ? row : row / r.qt;
-    s.node0 = (row - s.kvh * r.qt) * p.nt;
+    const int full = r.units(false), rel = w.t - w.before;
+    s.kvh = rel / r.head_units();
+    const int in_head = rel - s.kvh * r.head_units(), qt = r.qt == 1 ? 0 : min(in_head / full, r.qt - 1);
+    const bool last = qt == r.qt - 1;
+    const int units = r.units(last), u = in_head - qt * full, step = last && r.narrow ? 2 : 1;
+    s.row_end = w.t - u + units;
+    s.node0 = qt * p.nt;
     s.s0 = r.s0;
     s.n = r.n;
     s.len = r.len;
@@ -102,8 +109,8 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
     s.b = w.b;
     const int upto = r.kt <= kWhole ? units : min(units, u + (w.end - w.t));
     w.t += upto - u;
-    s.k0 = max(0, u - kRow);
-    s.k1 = upto - kRow;
+    s.k0 = max(0, u - kRow) * step;
+    s.k1 = min(r.kt, (upto - kRow) * step);
     if (r.kt <= kWhole ? u > 0 : s.k1 <= s.k0) continue;  // begun by another CTA; no tile in this share
     s.whole = s.k0 == 0 && s.k1 == r.kt;
     return true;

@@ -4,21 +4,21 @@
 // more than 64 rows the tensor cores and the exponentials bound the work and
 // not the keys that are read.
 //
-// A CTA holds two "pipes", each a 128-row S, over which P is written in place (16 bits,
-// TMEM operand of the second product), and an O. With more than 128 rows they are
-// two row tiles over the same keys; with fewer, one row tile over the even and the odd key
-// tiles, joined at the end. A thread owns a row, so a tile needs no exchange
-// between threads at all: 128 scores in registers, their maximum, the
-// exponentials (128 x 128 of them take the SM's 16 per cycle 1024 cycles, as long as the two
-// products), P back to TMEM. While one pipe's softmax runs the tensor cores
-// work for the other. The reference maximum of a row is raised only when a score
-// passes it by 2^8, as in the narrow kernel.
+// A CTA holds two "pipes", each a 128-row O and a 128-row S of 128 keys, over
+// which P is written in place (16 bits, TMEM operand of the second product).
+// With more than 128 rows they are two row tiles over the same keys; with
+// fewer, one row tile over the even and the odd key tiles, joined at the end.
+// A thread owns a row, so no scores are exchanged: 64 of them at a time in
+// registers, their maximum, the exponentials (128 x 128 of them take the SM's 16 per
+// cycle 1024 cycles, as long as the two products of a tile), P back to TMEM. P V of
+// the first 64 keys runs while the softmax works on the others (268 us without
+// that, 255 us with S in halves too, whose products of 64 columns take as long as those
+// of 128, 256 us so, for 4 requests of 64 nodes x 7 heads over up to 65 K keys). The
+// reference maximum of a row is raised only when a score passes it by 2^8, as in
+// the narrow kernel.
 //
 // Warps 0-3 and 4-7: softmax of pipe 0 and 1; warp 8 loads Q and K, warp 9 V,
-// warp 10 plans and issues all products. Products of one thread complete in
-// order, so S of a tile also says that the pipe's last P V is done.
-#include <atomic>
-
+// warp 10 issues S, warp 11 plans and issues O.
 #include "tree_attention.cuh"
 
 namespace af {
@@ -27,8 +27,8 @@ namespace tree_attn {
 namespace {
 
 constexpr int kSoft = 8;
-constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMma = kSoft + 2;
-constexpr int kThreads = (kSoft + 3) * 32;
+constexpr int kLoadK = kSoft, kLoadV = kSoft + 1, kMmaS = kSoft + 2, kMmaO = kSoft + 3;
+constexpr int kThreads = (kSoft + 4) * 32;
 constexpr int kRows = 128;  // of a row tile
 
 template <int HD>
@@ -42,16 +42,16 @@ struct Wide {
   static constexpr int kOffQ = kOffV + kVStages * kStage;
   static constexpr int kOffStat = kOffQ + kQBytes;                   // [2][128] (maximum, sum) of the pipes
   static constexpr int kOffBar = kOffStat + 2 * kRows * 8;
-  static constexpr int kBars = 2 * kKStages + 2 * kVStages + 2 + 4 + 2 + kPlans;
+  static constexpr int kBars = 2 * kKStages + 2 * kVStages + 2 + 12 + 2 + kPlans;
   static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
   static constexpr int kTmemO = 2 * kKeys;                           // O of pipe x at kTmemO + 128 x, S of pipe x at 128 x
 };
 
-// 128 consecutive columns of the thread's TMEM lane.
-__device__ __forceinline__ void tmem_load128(uint32_t taddr, uint32_t* r) {
+// 64 consecutive columns of the thread's TMEM lane.
+__device__ __forceinline__ void tmem_load64(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\ttcgen05.wait::ld.sync.aligned;"
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
@@ -59,16 +59,7 @@ __device__ __forceinline__ void tmem_load128(uint32_t taddr, uint32_t* r) {
         "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
         "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
         "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]),
-        "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]), "=r"(r[71]), "=r"(r[72]),
-        "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]), "=r"(r[80]),
-        "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]),
-        "=r"(r[89]), "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]),
-        "=r"(r[97]), "=r"(r[98]), "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]),
-        "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]), "=r"(r[111]),
-        "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]),
-        "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]),
-        "=r"(r[126]), "=r"(r[127])
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
       : "r"(taddr)
       : "memory");
 }
@@ -85,14 +76,23 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) 
 
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D [tmem] (+)= A [tmem, 16-bit pairs] * B [smem]^T.
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  const uint32_t z = 0;
+// D [tmem] (+)= A [smem] * B [smem]^T (without the lane masks of tc_mma_bf16: a shorter issue).
+__device__ __forceinline__ void mma_from_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// D [tmem] (+)= A [tmem, 16-bit pairs] * B [smem]^T.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   const uint32_t base = smem_u32(gb);
   const uint32_t k_full = base + S::kOffBar, k_empty = k_full + 8 * S::kKStages, v_full = k_empty + 8 * S::kKStages,
                  v_empty = v_full + 8 * S::kVStages, q_full = v_empty + 8 * S::kVStages, q_empty = q_full + 8, s_full = q_empty + 8,
-                 p_full = s_full + 16, o_full = p_full + 16, o_empty = o_full + 8, plan_full = o_empty + 8;
+                 p_full = s_full + 32, done = p_full + 32, o_full = done + 32, o_empty = o_full + 8, plan_full = o_empty + 8;
   Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -119,9 +119,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
       mbar_init(v_full + 8 * i, 1);
       mbar_init(v_empty + 8 * i, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {  // [pipe][half]
       mbar_init(s_full + 8 * i, 1);
       mbar_init(p_full + 8 * i, 4);
+      mbar_init(done + 8 * i, 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     *failed = 0;
     fence_barrier_init();
   }
-  if (warp == kMma) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -139,79 +140,104 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   const Scratch<2 * kRows, HD> scratch{p.ws, (int)gridDim.x};
   Segment s;
   auto planned = [&](int seg, Segment& s) { return read_plan(plans, plan_full, seg, s, failed); };
+  auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
+  constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
 
   if (warp == kLoadK) {
     load_tiles<S, false>(p, planned, base, k_full, k_empty, q_full, q_empty, failed);
   } else if (warp == kLoadV) {
     load_tiles<S, true>(p, planned, base, v_full, v_empty, q_full, q_empty, failed);
-  } else if (warp == kMma) {
-    // ---------------- the plan, and all products ----------------
-    constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
-    constexpr uint32_t id_s = idesc_bf16(kRows, kKeys) ^ kind, id_o = idesc_bf16_bmn(kRows, HD) ^ kind;
-    const uint64_t d_k = sw128_desc(base + S::kOffK), d_q = sw128_desc(base + S::kOffQ), d_v = sw128_desc_mn(base + S::kOffV, kHalf, 1024);
-    auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
+  } else if (warp == kMmaS) {
+    // ---------------- S: two row tiles of a key tile, or one of every other key tile ----------------
+    constexpr uint32_t id_s = idesc_bf16(kRows, kKeys) ^ kind;
+    const uint64_t d_k = sw128_desc(base + S::kOffK), d_q = sw128_desc(base + S::kOffQ);
+    bool ok = true;
+    int seg = 0, stage = 0, k_phase = 0, used0 = 0, used1 = 0;  // tiles of S of the pipes
+#pragma unroll 1
+    while (ok && planned(seg, s)) {
+      const bool two = s.n - s.node0 > p.nt_q;
+      const int tiles = s.k1 - s.k0, steps = two ? 2 : 1;  // of a key tile
+      ok = agreed(wait_for(q_full, seg & 1, failed));
+#pragma unroll 1
+      for (int t = 0; ok && t < tiles; ++t) {
+        ok = agreed(wait_for(k_full + 8 * stage, k_phase, failed));
+#pragma unroll 1
+        for (int x = 0; ok && x < steps; ++x) {
+          const int pipe = two ? x : t & 1, used = pipe ? used1 : used0;
+          if (used) ok = agreed(wait_for(done + 8 * (2 * pipe + 1), (used - 1) & 1, failed));  // P V of the pipe's last keys
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = d_q + (two && pipe ? (uint32_t)(S::kHalves * kRows * 128) >> 4 : 0u), b = d_k + (uint32_t)stage * (S::kStage >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              mma_from_smem(tmem + 128 * pipe, a + (kk >> 2) * (kRows * 8) + 2 * (kk & 3), b + (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3), id_s,
+                            kk ? 1u : 0u);
+            tc_commit(s_full + 8 * pipe);
+            if (x == steps - 1) tc_commit(k_empty + 8 * stage);
+            if (x == steps - 1 && t == tiles - 1) tc_commit(q_empty);
+          }
+          __syncwarp();
+        }
+        used0 += two || !(t & 1);
+        used1 += two || (t & 1);
+        if (++stage == S::kKStages) {
+          stage = 0;
+          k_phase ^= 1;
+        }
+      }
+      ++seg;
+    }
+    if (!ok) {
+      *failed = 1;
+      if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+    }
+  } else if (warp == kMmaO) {
+    // ---------------- the plan, and O += P V of every half ----------------
+    constexpr uint32_t id_o = idesc_bf16_bmn(kRows, HD) ^ kind;
+    const uint64_t d_v = sw128_desc_mn(base + S::kOffV, kHalf, 1024);
     Planner planner;
     planner.begin(p, lane);
     planner.on(p, plans, plan_full, 1, lane);
     bool ok = true;
-    int seg = 0, k_at = 0, v_at = 0;  // tiles of K and V that are used up
-    int issued0 = 0, issued1 = 0;     // S products of the pipes
+    int seg = 0, stage = 0, v_phase = 0, used0 = 0, used1 = 0;
 #pragma unroll 1
     while (true) {
       // The plan that this one replaces has been read by everyone: the segment after it is done.
       planner.on(p, plans, plan_full, seg + 2, lane);
       if (!ok || !planned(seg, s)) break;
-      const bool two = s.n - s.node0 > p.nt_q;  // two row tiles, or one over even and odd key tiles
-      const int tiles = s.k1 - s.k0;
-      ok = agreed(wait_for(q_full, seg & 1, failed));
-      // Step x: P V of the pipe's last tile, then its next S.
-      const int steps = two ? 2 * (tiles + 1) : tiles + 2;
+      const bool two = s.n - s.node0 > p.nt_q;
+      const int tiles = s.k1 - s.k0, steps = two ? 4 : 2;
+      if (seg > 0) ok = agreed(wait_for(o_empty, (seg - 1) & 1, failed));  // the last segment's O is read
 #pragma unroll 1
-      for (int x = 0; ok && x < steps; ++x) {
-        const int pipe = x & 1;
-        const int next = two ? x >> 1 : x, last = two ? next - 1 : x - 2;  // tile of S, tile of P V
-        const int issued = pipe ? issued1 : issued0;
-        if (last >= 0) {
-          const int stage = v_at % S::kVStages;
-          ok = agreed(wait_for(v_full + 8 * stage, (v_at / S::kVStages) & 1, failed)) &&
-               agreed(wait_for(p_full + 8 * pipe, (issued - 1) & 1, failed));
-          if (ok && x == 2 && seg > 0) ok = agreed(wait_for(o_empty, (seg - 1) & 1, failed));  // the last segment's O is read
+      for (int t = 0; ok && t < tiles; ++t) {
+        ok = agreed(wait_for(v_full + 8 * stage, v_phase, failed));
+        const int keys16 = (s.pad + s.n - (s.k0 + t) * kKeys + 15) / 16;  // up to the row's last key
+#pragma unroll 1
+        for (int x = 0; ok && x < steps; ++x) {
+          const int half = two ? x >> 1 : x, pipe = two ? x & 1 : t & 1, bar = 2 * pipe + half, used = pipe ? used1 : used0;
+          ok = agreed(wait_for(p_full + 8 * bar, used & 1, failed));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t b = d_v + (uint32_t)stage * (S::kStage >> 4);
-          const uint32_t o = tmem + S::kTmemO + 128 * pipe, a = tmem + 128 * pipe;
-          const uint32_t add = (two ? last : last >> 1) > 0;
-          const int keys = min(kKeys / 16, (s.pad + s.n - (s.k0 + last) * kKeys + 15) / 16);  // up to the row's last key
-          const bool used = !two || pipe == 1;
+          const uint64_t b = d_v + (uint32_t)stage * (S::kStage >> 4) + half * 4 * 128;
+          const uint32_t o = tmem + S::kTmemO + 128 * pipe, a = tmem + 128 * pipe + 64 * half;
+          const uint32_t add = t > (two ? 0 : 1) || half;
+          const int keys = keys16 - 4 * half;
           if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
+            for (int kk = 0; kk < 4; ++kk)
               if (kk < keys) mma_from_tmem(o, a + 8 * kk, b + kk * 128, id_o, kk ? 1u : add);
-            if (used) tc_commit(v_empty + 8 * stage);
-            if (x == steps - 1) tc_commit(o_full);
+            tc_commit(done + 8 * bar);
+            if (x == steps - 1) tc_commit(v_empty + 8 * stage);
+            if (x == steps - 1 && t == tiles - 1) tc_commit(o_full);
           }
           __syncwarp();
-          v_at += used;
         }
-        if (next < tiles) {
-          const int stage = k_at % S::kKStages;
-          ok = agreed(wait_for(k_full + 8 * stage, (k_at / S::kKStages) & 1, failed));
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t a = d_q + (two && pipe ? (uint32_t)(S::kHalves * kRows * 128) >> 4 : 0u), b = d_k + (uint32_t)stage * (S::kStage >> 4);
-          const bool used = !two || pipe == 1;
-          if (elect_one()) {
-#pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              tc_mma_bf16(tmem + 128 * pipe, a + (kk >> 2) * (kRows * 8) + 2 * (kk & 3), b + (kk >> 2) * (kHalf >> 4) + 2 * (kk & 3), id_s, kk ? 1u : 0u);
-            tc_commit(s_full + 8 * pipe);
-            if (used) tc_commit(k_empty + 8 * stage);
-            if (used && next == tiles - 1) tc_commit(q_empty);
-          }
-          __syncwarp();
-          k_at += used;
-          if (pipe) ++issued1;
-          else ++issued0;
+        used0 += two || !(t & 1);
+        used1 += two || (t & 1);
+        if (++stage == S::kVStages) {
+          stage = 0;
+          v_phase ^= 1;
         }
       }
       ++seg;
@@ -230,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (!wait_for(bar, parity, failed)) *failed = 1;
     };
-    int j0 = 0, seg = 0, taken = 0;  // tiles before this segment; S tiles of this pipe so far
+    int j0 = 0, seg = 0, taken = 0;  // tiles before this segment; halves of S of this pipe so far
     bool wrote_start = false;
 #pragma unroll 1
     while (planned(seg, s)) {
@@ -243,15 +269,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
       uint64_t l0 = 0ull, l1 = 0ull;
       bool sick = false;
 #pragma unroll 1
-      for (int t = two ? 0 : pipe; t < tiles; t += two ? 1 : 2, ++taken) {
+      for (int x2 = two ? 0 : 2 * pipe; x2 < 2 * tiles; x2 += two || !(x2 & 1) ? 1 : 3, ++taken) {
+        const int t = x2 >> 1, half = x2 & 1, bar = 2 * pipe + half;  // a half of a tile at a time
         const int key0 = (s.k0 + t) * kKeys;
         const bool masked = key0 + kKeys > s.len;
-        wait(s_full + 8 * pipe, taken & 1);
+        if (half == 0) wait(s_full + 8 * pipe, (taken >> 1) & 1);
         tc_fence_after();
-        if (masked) {
+        if (masked && half == 0) {
           // Rows of V without a key, and drafted values that are not finite, are cleared (see the narrow kernel). S of
-          // this tile follows the product that freed its V stage, so this wait is at most one phase ahead. With
-          // two pipes both do it: each one's own writes are complete before its own P is.
+          // this tile follows products with the last V of this stage, so this wait is at most one phase ahead. With
+          // two row tiles both pipes do it: each one's own writes are complete before its own P is.
           const int vt = j0 + t, key = key0 + r, x = key - s.pad;
           const bool in_prefix = key < s.len, in_tree = x >= 0 && x < s.n;
           wait(v_full + 8 * (vt % S::kVStages), (vt / S::kVStages) & 1);
@@ -283,16 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
           fence_proxy_async_smem();
         }
         if (busy) {
-          uint32_t x[kKeys];
-          tmem_load128(at_s, x);
+          constexpr int C = kKeys / 2;
+          uint32_t x[C];
+          tmem_load64(at_s + C * half, x);
           if (p.scale <= 0.f) {  // scores in the order of the softmax
 #pragma unroll
-            for (int i = 0; i < kKeys; ++i) x[i] = __float_as_uint(p.scale < 0.f ? -__uint_as_float(x[i]) : __uint_as_float(x[i]) * 0.f);
+            for (int i = 0; i < C; ++i) x[i] = __float_as_uint(p.scale < 0.f ? -__uint_as_float(x[i]) : __uint_as_float(x[i]) * 0.f);
           }
           if (masked) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int k = key0 + 32 * c, j = k - s.pad;  // the word's first key; as a node
+            for (int c = 0; c < C / 32; ++c) {
+              const int k = key0 + C * half + 32 * c, j = k - s.pad;  // the word's first key; as a node
               auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
               const uint32_t tree = below(s.n - j) & ~below(-j);
               const uint32_t vis = below(s.len - k) | (tree && r < rows ? seen_bits(p, s.s0, node, j) & tree : 0u);
@@ -304,17 +332,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
           float top[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            top[c] = __uint_as_float(x[32 * c]);
+            top[c] = __uint_as_float(x[16 * c]);
 #pragma unroll
-            for (int i = 1; i < 31; i += 2) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[32 * c + i]), __uint_as_float(x[32 * c + i + 1])));
-            top[c] = fmaxf(top[c], __uint_as_float(x[32 * c + 31]));
+            for (int i = 1; i < 15; i += 2) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(x[16 * c + i]), __uint_as_float(x[16 * c + i + 1])));
+            top[c] = fmaxf(top[c], __uint_as_float(x[16 * c + 15]));
           }
           const float t_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
           const bool raise = m == kUnset ? t_max > kUnset : t_max > m + kRaise;
           if (__any_sync(0xffffffffu, raise)) {
             const float f = raise ? (m == kUnset ? 0.f : exp2f(m - t_max)) : 1.f;
             if (raise) m = t_max;
-            if (t >= (two ? 1 : 2)) {
+            if (x2 > (two ? 0 : 2 * pipe)) {
+              // O of the halves before this one is complete once the last one's P V is.
+              wait(done + 8 * (bar ^ 1), ((taken - 1) >> 1) & 1);
+              tc_fence_after();
               l0 = fma2(l0, pair(f, f), 0ull);
               l1 = fma2(l1, pair(f, f), 0ull);
 #pragma unroll 1
@@ -330,26 +361,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
             }
           }
           const uint64_t sc2 = pair(sc, sc), nm2 = pair(-m, -m);
+          uint32_t e[C / 2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t e[32];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float2 a = unpair(fma2(pair(__uint_as_float(x[64 * h + 2 * i]), __uint_as_float(x[64 * h + 2 * i + 1])), sc2, nm2));
-              const float2 b = unpair(fma2(pair(__uint_as_float(x[64 * h + 2 * i + 2]), __uint_as_float(x[64 * h + 2 * i + 3])), sc2, nm2));
-              const float a0 = ex2(a.x), a1 = ex2(a.y), b0 = ex2(b.x), b1 = ex2(b.y);
-              l0 = add2(l0, pair(a0, a1));
-              l1 = add2(l1, pair(b0, b1));
-              e[i] = pack2<DT>(a0, a1);
-              e[i + 1] = pack2<DT>(b0, b1);
-            }
-            tmem_store32(at_s + 32 * h, e);
+          for (int i = 0; i < C / 2; i += 2) {
+            const float2 a = unpair(fma2(pair(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), sc2, nm2));
+            const float2 b = unpair(fma2(pair(__uint_as_float(x[2 * i + 2]), __uint_as_float(x[2 * i + 3])), sc2, nm2));
+            const float a0 = ex2(a.x), a1 = ex2(a.y), b0 = ex2(b.x), b1 = ex2(b.y);
+            l0 = add2(l0, pair(a0, a1));
+            l1 = add2(l1, pair(b0, b1));
+            e[i] = pack2<DT>(a0, a1);
+            e[i + 1] = pack2<DT>(b0, b1);
           }
+          tmem_store32(at_s + C * half, e);
           tmem_wait_store();
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + 8 * pipe);
+        if (lane == 0) mbar_arrive(p_full + 8 * bar);
       }
       // ---- the segment's rows ----
       const float2 la = unpair(add2(l0, l1));
@@ -431,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
-  if (warp == kMma) {
+  if (warp == kMmaS) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
