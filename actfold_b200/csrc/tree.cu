@@ -302,16 +302,14 @@ struct WriteArgs {
 
 constexpr int kWriteThreads = 256;
 
-// A warp moves 128 vectors of (keys, then values) of one row: four 16-byte
-// loads per lane in flight, then four stores, so a row of any width keeps
-// HBM's queues full (2 KB per warp, 64 warps per SM).
-template <typename V>
-__global__ void __launch_bounds__(kWriteThreads) k_write_cache(const WriteArgs a, int64_t chunks) {
+// A warp moves 32 U vectors of (keys, then values) of one row: U 16-byte loads
+// per lane in flight, then U stores. Wide rows take U = 8 and x-blocks that lie within one row.
+template <typename V, int U>
+__global__ void __launch_bounds__(kWriteThreads) k_write_cache(const WriteArgs a, int chunks) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);
-  const int64_t m = item / chunks % a.count;
-  const int l = (int)(item / chunks / a.count);
-  if (l >= a.layers) return;
+  const int item = blockIdx.x * (kWriteThreads / 32) + (threadIdx.x >> 5);  // (row, chunk)
+  const int m = item / chunks, chunk = item - m * chunks, l = blockIdx.y;
+  if (m >= a.count) return;
   const int64_t slot = a.slots[m];
   const int64_t row = a.rows ? a.rows[m] : m;
   if (slot < 0 || row < 0) return;
@@ -319,32 +317,38 @@ __global__ void __launch_bounds__(kWriteThreads) k_write_cache(const WriteArgs a
     if (lane == 0 && a.status) atomicOr(a.status, AF_STATUS_BOUNDS);
     return;
   }
-  const int64_t pg = slot / a.page, t = slot - pg * a.page;
+  const int64_t pg = slot < 0x7fffffff ? (int)slot / a.page : slot / a.page, t = slot - pg * a.page;
   const int half = a.heads * a.per_head;
-  const int x0 = (int)(item % chunks) * 128 + lane;
-  V buf[4];
+  const char* k = a.k + l * a.kl + row * a.kn;
+  const char* v = a.v + l * a.vl + row * a.vn;
+  char* kc = a.kc + l * a.kcl + pg * a.kcp + t * a.kct;
+  char* vc = a.vc + l * a.vcl + pg * a.vcp + t * a.vct;
+  const int x0 = chunk * 32 * U + lane;
+  V buf[U];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    int x = x0 + 32 * u;
+  for (int u = 0; u < U; ++u) {
+    const int x = x0 + 32 * u;
     if (x < 2 * half) {
       const bool val = x >= half;
-      x -= val ? half : 0;
-      const int h = x / a.per_head, c = x - h * a.per_head;
-      const char* src = val ? a.v + l * a.vl + row * a.vn + h * a.vh : a.k + l * a.kl + row * a.kn + h * a.kh;
-      buf[u] = reinterpret_cast<const V*>(src)[c];
+      const int y = val ? x - half : x, h = y / a.per_head, c = y - h * a.per_head;
+      buf[u] = reinterpret_cast<const V*>((val ? v : k) + h * (val ? a.vh : a.kh))[c];
     }
   }
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    int x = x0 + 32 * u;
+  for (int u = 0; u < U; ++u) {
+    const int x = x0 + 32 * u;
     if (x < 2 * half) {
       const bool val = x >= half;
-      x -= val ? half : 0;
-      const int h = x / a.per_head, c = x - h * a.per_head;
-      char* dst = val ? a.vc + l * a.vcl + pg * a.vcp + t * a.vct + h * a.vch : a.kc + l * a.kcl + pg * a.kcp + t * a.kct + h * a.kch;
-      reinterpret_cast<V*>(dst)[c] = buf[u];
+      const int y = val ? x - half : x, h = y / a.per_head, c = y - h * a.per_head;
+      reinterpret_cast<V*>((val ? vc : kc) + h * (val ? a.vch : a.kch))[c] = buf[u];
     }
   }
+}
+
+template <typename V, int U>
+void launch_write(const WriteArgs& a, cudaStream_t s) {
+  const int chunks = (int)ceil_div(2 * (int64_t)a.heads * a.per_head, 32 * U);
+  k_write_cache<V, U><<<dim3((unsigned)ceil_div((int64_t)chunks * a.count, kWriteThreads / 32), (unsigned)a.layers), kWriteThreads, 0, s>>>(a, chunks);
 }
 
 template <typename K>
@@ -469,12 +473,11 @@ extern "C" int af_write_cache(const af_cache_rows* w, uint32_t* status, void* st
   for (int i = 0; i < 4; ++i) al |= (uint64_t)w->k_cache_strides[i] | (uint64_t)w->v_cache_strides[i];
   const int unit = (al & 15) == 0 ? 16 : (al & 3) == 0 ? 4 : 1;
   a.per_head = (int)(w->head_bytes / unit);
-  const int64_t chunks = ceil_div(2 * (int64_t)a.heads * a.per_head, 128);
-  const int64_t blocks = ceil_div(chunks * a.count * a.layers, kWriteThreads / 32);
-  AF_REQUIRE(blocks <= 0x7fffffff, "af_write_cache: too many rows");
+  AF_REQUIRE(a.layers <= 65535 && a.count * ceil_div(2 * (int64_t)a.heads * a.per_head, 128) <= 0x7fffffff, "af_write_cache: too many rows");
   cudaStream_t s = as_stream(stream);
-  if (unit == 16) k_write_cache<uint4><<<(unsigned)blocks, kWriteThreads, 0, s>>>(a, chunks);
-  else if (unit == 4) k_write_cache<uint32_t><<<(unsigned)blocks, kWriteThreads, 0, s>>>(a, chunks);
-  else k_write_cache<uint8_t><<<(unsigned)blocks, kWriteThreads, 0, s>>>(a, chunks);
+  if (unit == 16 && a.heads * a.per_head >= 256) launch_write<uint4, 8>(a, s);
+  else if (unit == 16) launch_write<uint4, 4>(a, s);
+  else if (unit == 4) launch_write<uint32_t, 4>(a, s);
+  else launch_write<uint8_t, 4>(a, s);
   return check_launch("af_write_cache");
 }

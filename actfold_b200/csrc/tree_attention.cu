@@ -564,7 +564,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
 }
 
 constexpr int kJoinThreads = 256;
-constexpr int kJoinBlocks = 16;  // per CTA of the main kernel
+template <int N>
+constexpr int kJoinBlocks = N <= 64 ? 8 : 16;  // per CTA of the main kernel (8: all of them resident at once)
 
 // Rows that several CTAs worked on: out = sum_c w_c O_c / sum_c w_c l_c with
 // w_c = 2^(m_c - max m), in the CTAs' order. The block's 8 warps share a row's
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_tree_attention_join(const __gr
   if (st.last <= c) return;
   const int parts = st.last - c + 1;
   const bool share = parts > 8;
-  for (int row = share ? blockIdx.y : blockIdx.y * W + warp; row < st.rows; row += share ? kJoinBlocks : kJoinBlocks * W) {
+  for (int row = share ? blockIdx.y : blockIdx.y * W + warp; row < st.rows; row += share ? kJoinBlocks<N> : kJoinBlocks<N> * W) {
     float m = kUnset;
     for (int i = lane; i < parts; i += 32) m = fmaxf(m, scratch.stats(c + i, i == 0)[row].x);
 #pragma unroll
@@ -696,7 +697,7 @@ int launch_narrow(const Params& p, int n, bool bf16, int64_t head_dim, cudaStrea
 template <int DT, int N, int HD>
 int join_launch(const Params& p, int ctas, cudaStream_t s) {
   if (p.capacity + p.total <= kWhole * kKeys) return check_launch("af_tree_attention");  // no row is shared
-  const cudaError_t e = launch_ex(k_tree_attention_join<DT, N, HD>, dim3(ctas, kJoinBlocks), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+  const cudaError_t e = launch_ex(k_tree_attention_join<DT, N, HD>, dim3(ctas, kJoinBlocks<N>), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention: launch: ") + cudaGetErrorString(e));
   return check_launch("af_tree_attention");
 }
@@ -731,8 +732,10 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
   p.nt_q = (n == 256 ? 128 : n) / group;
   p.nt = n == 256 ? 2 * p.nt_q : p.nt_q;
+  // Measured: a row end costs some 1800 cycles of 2700 a tile with 16 rows, 9000 of 2900 with 64, 8000 of 4500 with 256.
+  p.row_cost = n == 16 ? 1 : n == 64 ? 3 : 2;
   // Tiles are counted in 32 bits: no more than this can come of any device-side values.
-  AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + kRow) < 2147483000.0,
+  AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + p.row_cost) < 2147483000.0,
              "af_tree_attention: more than 2^31 tiles of 128 keys");
   const uint64_t hd = (uint64_t)a.head_dim, kvh = (uint64_t)a.n_kv_heads;
   {

@@ -15,7 +15,6 @@ constexpr int kKeys = 128;                  // keys per tile
 constexpr int kHalf = kKeys * 128;          // [128 rows][64 columns] of 16 bits, 128-byte swizzle
 constexpr int kPlans = 4;                   // segments planned in shared memory, up to two ahead of the products of O
 constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
-constexpr int kRow = 2;                     // cost of a row besides its tiles, in tiles (its end drains the pipeline: some 6600 cycles of 3000 a tile)
 constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
 constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
 
@@ -25,6 +24,7 @@ struct Params {
   const uint32_t* mask;
   int64_t tables_ld, mask_ld;
   int words, batch, total, kv_heads, group, pages, page, box, nt, nt_q;  // nt: nodes of a row tile, nt_q: of one Q box
+  int row_cost;  // of a row tile besides its key tiles, in key tiles: its end drains the pipeline
   int64_t capacity;  // tokens that a table row can hold
   float scale;       // times log2(e)
   const char* v_rows;  // the tree's values, for those that are not finite
@@ -40,9 +40,10 @@ struct Params {
 // A request's tree and prefix; no cost where there is nothing to do or the values are bad.
 struct Request {
   int s0, n, len, pad, kt, qt;
+  int row_cost;
   bool bad, narrow;  // narrow: the last row tile has no second Q box, and a wide CTA takes two of its key tiles at a time
   // Units of a row tile and of a head's row tiles (of all heads and requests below 2^31: checked by the host).
-  __device__ __forceinline__ int units(bool last) const { return kRow + (last && narrow ? (kt + 1) / 2 : kt); }
+  __device__ __forceinline__ int units(bool last) const { return row_cost + (last && narrow ? (kt + 1) / 2 : kt); }
   __device__ __forceinline__ int head_units() const { return (qt - 1) * units(false) + units(true); }
   __device__ __forceinline__ int cost(int kv_heads) const { return kt ? head_units() * kv_heads : 0; }
 };
@@ -53,6 +54,7 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   r.len = p.lengths[b];
   r.bad = s0 < 0 || s1 < s0 || s1 > p.total || r.len < 0 || r.len > p.capacity || (p.mask && s1 - s0 > 32 * (int64_t)p.words);
   r.s0 = s0;
+  r.row_cost = p.row_cost;
   r.n = r.bad ? 0 : s1 - s0;
   r.pad = (r.len + p.box - 1) & -p.box;
   r.kt = r.n ? (r.pad + r.n + kKeys - 1) / kKeys : 0;
@@ -61,7 +63,7 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   return r;
 }
 
-// The list of rows, each of kRow units and one per key tile, cut into one share per CTA: the first `more` shares have each + 1.
+// The list of rows, each of row_cost units and one per key tile, cut into one share per CTA: the first `more` shares have each + 1.
 struct Shares {
   int each, more;
   __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
@@ -109,8 +111,8 @@ __device__ __forceinline__ bool next_segment(const Params& p, Walk& w, Segment& 
     s.b = w.b;
     const int upto = r.kt <= kWhole ? units : min(units, u + (w.end - w.t));
     w.t += upto - u;
-    s.k0 = max(0, u - kRow) * step;
-    s.k1 = min(r.kt, (upto - kRow) * step);
+    s.k0 = max(0, u - r.row_cost) * step;
+    s.k1 = min(r.kt, (upto - r.row_cost) * step);
     if (r.kt <= kWhole ? u > 0 : s.k1 <= s.k0) continue;  // begun by another CTA; no tile in this share
     s.whole = s.k0 == 0 && s.k1 == r.kt;
     return true;

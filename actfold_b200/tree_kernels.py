@@ -137,7 +137,7 @@ def block_tables(
     lengths, grow, free_range = lengths.contiguous(), grow.contiguous(), free_range.contiguous()
     if held is not None:
         held = held.contiguous()
-    starts, totals, out = lengths.new_empty(n + 1), lengths.new_empty(n), free_range.new_empty(2)
+    starts, totals, out = lengths.new_empty(n + 1), torch.empty_like(lengths), torch.empty_like(free_range)
     slots = free_range.new_empty((n, slot_capacity) if padded else slot_capacity)
     if n == 0:
         return BlockTables(starts.zero_(), totals, slots.fill_(-1), out.copy_(free_range))
@@ -175,7 +175,7 @@ def tree_masks(
     parents, starts = parents.contiguous(), starts.contiguous()
     if base is not None:
         base = base.contiguous()
-    mask, positions = parents.new_empty((total, words)), parents.new_empty(total)
+    mask, positions = parents.new_empty((total, words)), torch.empty_like(parents)
     _launch("tree_masks", index, _lib.load().af_tree_masks, parents.data_ptr(), starts.data_ptr(), batch, total, words,
             None if base is None else base.data_ptr(), mask.data_ptr(), positions.data_ptr(), _status(status))
     return mask, positions
@@ -394,7 +394,7 @@ def tree_attention(
         v = v.clone(memory_format=torch.contiguous_format)
         vr_grid = _grid(v)
     if out is None:
-        out = q.new_empty(qs)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_grid = (2 * heads * dim, 2 * dim)
     size = _scratch.get(index) or _workspace_bytes(index)
     workspace = lengths.new_empty(size >> 2)
