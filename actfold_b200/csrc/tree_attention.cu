@@ -52,12 +52,15 @@ struct Shape {
   static constexpr int kPBytes = (N < 64 ? 1 : N / 64) * kKeys * kPitch;
   static constexpr int kKBytes = kHalves * kHalf > kPBytes ? kHalves * kHalf : kPBytes;
   static constexpr int kStage = kKBytes + kHalves * kHalf;
-  // At most kPipes + kS, so that a tile with its S there has all products of O behind it but those of the last kPipes + kS - 1
-  // tiles: a wait for the pipe's last one is then never two phases ahead.
-  static constexpr int kStages = (192 * 1024) / kStage < kPipes + kS ? (192 * 1024) / kStage : kPipes + kS;
+  // At most kS, so that P of a tile is taken before P of the tile that uses the same barrier can be there: no wait is ever
+  // two phases behind its barrier.
+  static constexpr int kStages = (192 * 1024) / kStage < kS ? (192 * 1024) / kStage : kS;
   static constexpr int kQBytes = kHalves * N * 128;
   static constexpr int kQ = kQBytes <= 16384 ? 2 : 1;         // Q buffers
-  static constexpr int kOffK = 0, kOffV = kKBytes, kKStages = kStages, kVStages = kStages, kQTiles = 1, kQRows = N;
+  // V lies before K: the second product always takes 128 dims, so with 64 it reads the 16 KB behind V too (for lanes of O
+  // that nobody looks at), and those have to be there.
+  static constexpr int kOffV = 0, kOffK = kHalves * kHalf, kKStages = kStages, kVStages = kStages, kQTiles = 1, kQRows = N;
+  static_assert(kOffK + kKBytes == kStage && kKBytes >= kHalf, "what the second product reads lies in its stage");
   static constexpr int kOffQ = kStages * kStage;
   static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
   static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     // ---------------- S^T of every tile ----------------
     // The whole warp keeps the books, one lane issues: descriptors stay in uniform registers.
     constexpr uint32_t id_s = idesc_bf16(kKeys, N) ^ kind;
-    const uint64_t d_k = sw128_desc(base), d_q = sw128_desc(sQ);
+    const uint64_t d_k = sw128_desc(base + S::kOffK), d_q = sw128_desc(sQ);
     bool ok = true;
     int j = 0, seg = 0, stage = 0, stage_phase = 0;
 #pragma unroll 1
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   } else if (warp == kMmaO) {
     // ---------------- O^T += V^T P^T of every tile, into its pipe's O ----------------
     constexpr uint32_t id_o = (idesc_bf16(128, N) ^ kind) | (1u << 15) | (1u << 16);  // A and B MN-major
-    const uint64_t d_v = sw128_desc_mn(base + S::kKBytes, kHalf, 1024), d_p = p_desc<N>(base);
+    const uint64_t d_v = sw128_desc_mn(base + S::kOffV, kHalf, 1024), d_p = p_desc<N>(base + S::kOffK);
     bool ok = true;
     int j = 0, seg = 0, stage = 0, stage_phase = 0;
     Planner planner;
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
           // Rows of V without a key (of those that the product takes) are whatever lay there: cleared. A drafted value that is not finite would reach
           // every column as 0 * inf: it is cleared too, and added at the end to the columns that see it.
           wait(v_full + 8 * stage, (j / S::kStages) & 1);
-          const uint32_t v_row = stage_at + S::kKBytes + r * 128;
+          const uint32_t v_row = stage_at + S::kOffV + r * 128;
           auto piece = [&](int c16) { return v_row + (c16 >> 3) * kHalf + 16 * ((c16 & 7) ^ (r & 7)); };
           if (!in_prefix && !in_tree && node < ((s.n + 15) & ~15) + 16) {
 #pragma unroll 4
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
             for (int i = 0; i < 8; ++i) e[i] = ex2(__uint_as_float(x[8 * q8 + i]));
 #pragma unroll
             for (int i = 0; i < 4; ++i) l[4 * q8 + i] = add2(l[4 * q8 + i], pair(e[2 * i], e[2 * i + 1]));
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_at + p_piece<N>(r, c0 + 8 * q8)), "r"(pack2<DT>(e[0], e[1])),
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage_at + S::kOffK + p_piece<N>(r, c0 + 8 * q8)), "r"(pack2<DT>(e[0], e[1])),
                          "r"(pack2<DT>(e[2], e[3])), "r"(pack2<DT>(e[4], e[5])), "r"(pack2<DT>(e[6], e[7]))
                          : "memory");
           }

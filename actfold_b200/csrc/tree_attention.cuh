@@ -177,11 +177,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// Bounded wait for a phase: some seconds of attempts (each of which may itself sleep a little).
+// Bounded wait for a phase: about a second of attempts (each of which sleeps a few microseconds).
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* failed) {
 #pragma unroll 1
   for (int n = 0; !mbar_try_wait(bar, parity); ++n)
-    if (n > (1 << 24) || *failed) return false;
+    if (n > (1 << 18) || *failed) return false;
   return true;
 }
 

@@ -382,6 +382,13 @@ CASES = [
     ([100, 1700], [129, 200], 6, 2, 64, 8, torch.float16, "chain"),
     ([0, 0, 3], [80, 200, 100], 2, 2, 128, 16, torch.bfloat16, "none"),
     ([20000], [64], 16, 1, 128, 48, torch.bfloat16, "tree"),
+    # so long that every SM goes round its stages several times: 16, 32 and 64 rows per tile, and more
+    ([150000], [2], 4, 2, 64, 32, torch.float16, "tree"),
+    ([150000], [12], 4, 2, 64, 128, torch.bfloat16, "tree"),
+    ([150000, 900], [25, 31], 4, 2, 64, 64, torch.float16, "tree"),
+    ([150000], [90], 2, 2, 64, 32, torch.bfloat16, "tree"),
+    ([100000], [2], 4, 2, 128, 32, torch.bfloat16, "tree"),
+    ([100000, 100], [25, 31], 4, 2, 128, 64, torch.float16, "chain"),
 ]
 
 
