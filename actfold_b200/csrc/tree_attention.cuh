@@ -333,7 +333,7 @@ __device__ __forceinline__ void load_tiles(const Params& p, Planned planned, uin
   const int lane = threadIdx.x & 31;
   const CUtensorMap* cache = VALUES ? &p.vc : &p.kc;
   const CUtensorMap* tree_rows = VALUES ? &p.v : &p.k;
-  if (lane < (VALUES ? 2 : 3)) tma_prefetch_desc(lane == 0 ? cache : lane == 1 ? tree_rows : &p.q);
+  if (lane < (VALUES ? 2 : 3) && (lane > 0 || p.capacity > 0)) tma_prefetch_desc(lane == 0 ? cache : lane == 1 ? tree_rows : &p.q);
   const int boxes = kKeys / p.box, page_step = kKeys / p.page, off_step = kKeys % p.page;
   int j = 0, seg = 0;
   bool ok = true;

@@ -2,7 +2,8 @@
 
 The node fields and the tree operations (add, get, get_ancestors, prune,
 best_accepted_leaf) are those of actfold/speculative/branch_tree.py:11-95,
-which callers of ``folded_generate`` and the acceptance policies read.
+which callers of ``folded_generate`` and the acceptance policies read;
+``packed`` lays a tree out for the tree verification operators.
 """
 
 from __future__ import annotations
@@ -67,6 +68,35 @@ class BranchTree:
                     parent.children.remove(node.branch_id)
             first = False
             stack.extend(node.children)
+
+    def packed(self) -> tuple[list[Any], torch.Tensor, torch.Tensor]:
+        """(branch ids, parents, tokens) of the nodes below the root, a parent before its children.
+
+        The form that ``tree_masks``, ``tree_attention`` and ``accept_tree`` take one
+        request's tree in: ``parents`` int32 holds each node's parent as its number in this
+        list, -1 for a child of the root (whose tokens are the prefix), ``tokens`` int64 the
+        one token by which a node extends its parent. The nodes hold a batch of one.
+        """
+        ids: list[Any] = []
+        parents: list[int] = []
+        last: list[torch.Tensor] = []
+        todo = [(c, -1) for c in self._nodes[self.root_id].children]
+        while todo:
+            branch_id, parent = todo.pop(0)
+            node = self._nodes.get(branch_id)
+            if node is None:
+                continue
+            above = self._nodes[ids[parent] if parent >= 0 else self.root_id]
+            if node.tokens.shape[0] != 1 or node.seq_len != above.seq_len + 1:
+                raise ValueError(f"packed: branch {branch_id!r} holds {tuple(node.tokens.shape)} tokens, its parent {tuple(above.tokens.shape)}: "
+                                 "each node must extend its parent by one token, in a batch of one")
+            todo += [(c, len(ids)) for c in node.children]
+            ids.append(branch_id)
+            parents.append(parent)
+            last.append(node.tokens[0, -1])
+        device = self._nodes[self.root_id].tokens.device
+        tokens = torch.stack(last).to(torch.int64) if last else torch.zeros(0, dtype=torch.int64, device=device)
+        return ids, torch.tensor(parents, dtype=torch.int32, device=device), tokens
 
     def best_accepted_leaf(self) -> BranchNode:
         """The deepest accepted node (the root when none is accepted)."""

@@ -110,6 +110,25 @@ def test_accept_ties_and_bad_parents():
         st.check_status()
 
 
+def test_accept_from_a_branch_tree():
+    from actfold_b200 import speculative as S
+
+    tree = S.BranchTree(S.BranchNode("root", None, torch.tensor([[5, 6]], device="cuda")))
+    texts = {"a": [7], "b": [8], "aa": [7, 1], "ba": [8, 2], "bb": [8, 3], "baa": [8, 2, 4]}
+    for name, t in texts.items():
+        tree.add(S.BranchNode(name, name[:-1] or "root", torch.tensor([[5, 6, *t]], device="cuda")))
+    ids, parents, tokens = tree.packed()
+    starts = _i32([0, len(ids)])
+    choice = {"root": 8, "a": 1, "b": 2, "aa": 0, "ba": 9, "bb": 0, "baa": 0}  # what the target model would say after each
+    targets = torch.tensor([choice[i] for i in ids], device="cuda")
+    got = S.accept_tree(parents, tokens, targets, starts, 4, torch.tensor([8], device="cuda"))
+    kept = [ids[i] for i in got.rows[0].tolist() if i >= 0]
+    assert kept == ["b", "ba"] and got.next_tokens.tolist() == [9]
+    mask, _ = S.tree_masks(parents, starts, 1)
+    for i, name in enumerate(ids):
+        assert mask[i, 0].item() == sum(1 << ids.index(name[: k + 1]) for k in range(len(name)))
+
+
 # ------------------------------------------------------------------------------------------------ block tables
 def _pool(batch, most, held, page, spare, rng, head):
     used = [-(-h // page) for h in held]
@@ -488,6 +507,22 @@ def test_attention_values_that_are_not_finite_reach_the_rows_that_see_them(value
     assert torch.equal(bad[:, :, 3].all(1), sees) and not bad[:, :, :3].any() and not bad[:, :, 4:].any() and not bad[~sees].any()
     if value == value:
         assert (out[sees][:, :, 3] == value).all()
+
+
+def test_attention_without_a_cache_or_without_nodes():
+    from actfold_b200.speculative import tree_attention
+
+    args, plain = _case([0, 0], [5, 40], 4, 2, 128, 16, torch.bfloat16)
+    want = _check(args, plain)
+    for pages in (0, 3):
+        none = args["k_cache"][:0] if pages == 0 else args["k_cache"]
+        got = tree_attention(**dict(args, k_cache=none, v_cache=none, tables=_i32([[], []]).view(2, 0)))
+        assert torch.equal(got, want)
+    e = args["q"][:0]
+    assert tree_attention(**dict(args, q=e, k=args["k"][:0], v=args["v"][:0], mask=args["mask"][:0], starts=_i32([0, 0, 0]))).shape == e.shape
+    out = torch.full_like(args["q"], 2.0)
+    tree_attention(**dict(args, starts=_i32([0, 0, 0]), out=out))  # rows, but no tree
+    assert out.eq(2.0).all()
 
 
 def test_attention_reports_bad_pages_and_lengths():

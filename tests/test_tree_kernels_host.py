@@ -112,6 +112,27 @@ def test_wrappers_have_no_cpu_form():
                          _z(3, 16, 2, 64, dtype=b), _z(1, 2), _z(1), _z(2))
 
 
+def test_branch_tree_packed():
+    def node(name, parent, *tokens):
+        return S.BranchNode(name, parent, torch.tensor([tokens]))
+
+    tree = S.BranchTree(node("r", None, 7, 8))
+    for n in (node("a", "r", 7, 8, 1), node("b", "r", 7, 8, 2), node("c", "a", 7, 8, 1, 3), node("d", "b", 7, 8, 2, 4), node("e", "a", 7, 8, 1, 5)):
+        tree.add(n)
+    ids, parents, tokens = tree.packed()
+    assert ids == ["a", "b", "c", "e", "d"] and parents.tolist() == [-1, -1, 0, 0, 1] and tokens.tolist() == [1, 2, 3, 5, 4]
+    assert parents.dtype is torch.int32 and tokens.dtype is torch.int64
+    tree.prune("a")
+    ids, parents, tokens = tree.packed()
+    assert ids == ["b", "d"] and parents.tolist() == [-1, 0] and tokens.tolist() == [2, 4]
+    assert U.accept(parents.tolist(), tokens.tolist(), [4, 9], 2, 8) == ([0, 1], 9)
+    tree.add(node("f", "d", 7, 8, 2, 4, 1, 1))
+    with pytest.raises(ValueError, match="one token"):
+        tree.packed()
+    empty = S.BranchTree(node("r", None, 7)).packed()
+    assert empty[0] == [] and empty[1].numel() == 0 and empty[2].numel() == 0
+
+
 def _attention_args(buf, **kw):
     p = C.addressof(buf)
     p += -p % 16
