@@ -382,10 +382,12 @@ void launch_write(const WriteArgs& a, cudaStream_t s) {
   else k_write_cache<V, U, false><<<grid, kWriteThreads, 0, s>>>(a, chunks);
 }
 
+// Without this a kernel gets 48 KB, its static shared memory (up to 1 KB here) among them. `most` is what any call can
+// need, the same each time: a call on another thread cannot lower it between this one's limit and its launch.
 template <typename K>
-int allow_smem(K kernel, size_t bytes, const char* what) {
-  if (bytes <= 48 * 1024) return AF_OK;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+int allow_smem(K kernel, size_t bytes, size_t most, const char* what) {
+  if (bytes <= 47 * 1024) return AF_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
   return AF_OK;
 }
@@ -406,7 +408,7 @@ extern "C" int af_tree_masks(const int32_t* parents, const int32_t* starts, int6
   const size_t smem = (size_t)most * sizeof(int);
   const auto kernel = words <= 32 ? k_tree_masks<true> : k_tree_masks<false>;
   if (words > 32)  // (up to 32 words: 4 KB of parents)
-    if (int st = allow_smem(kernel, smem, "af_tree_masks")) return st;
+    if (int st = allow_smem(kernel, smem, AF_TREE_MAX_NODES * sizeof(int), "af_tree_masks")) return st;
   kernel<<<dim3((unsigned)ceil_div(most, kMaskThreads), (unsigned)batch), kMaskThreads, smem, as_stream(stream)>>>(
       parents, starts, total, (int)words, base, reinterpret_cast<uint32_t*>(mask), positions, status);
   return check_launch("af_tree_masks");
@@ -423,7 +425,7 @@ extern "C" int af_accept_tree(const int32_t* parents, const int64_t* tokens, con
   AF_REQUIRE(total == 0 || (parents && tokens && targets), "af_accept_tree: null pointer");
   const int64_t most = max_nodes < total ? max_nodes : total;
   const size_t smem = (size_t)most * sizeof(int);
-  if (int st = allow_smem(k_accept_tree, smem, "af_accept_tree")) return st;
+  if (int st = allow_smem(k_accept_tree, smem, AF_TREE_MAX_NODES * sizeof(int), "af_accept_tree")) return st;
   k_accept_tree<<<(unsigned)batch, kAcceptThreads, smem, as_stream(stream)>>>(parents, tokens, targets, starts, total, most, root_targets,
                                                                             (int)keep, rows, counts, next_tokens, status);
   return check_launch("af_accept_tree");
@@ -464,7 +466,7 @@ extern "C" int af_block_tables(int32_t* tables, int64_t tables_stride, int64_t m
   a.range_out = free_range_out;
   a.status = status;
   const size_t smem = 3 * (size_t)(batch + 1) * sizeof(int);
-  if (int st = allow_smem(k_block_tables, smem, "af_block_tables")) return st;
+  if (int st = allow_smem(k_block_tables, smem, 3 * (AF_TABLES_MAX_BATCH + 1) * sizeof(int), "af_block_tables")) return st;
   // A thread writes about two slots; returned pages count as well, where requests end.
   const int64_t want = ceil_div(slot_capacity + batch * max_pages / 16, 2 * kTableThreads);
   const int sms = sm_count();

@@ -225,6 +225,36 @@ def test_block_tables_over_many_steps_keep_every_page_once():
         assert tables.tolist() == plain[0] and [head, tail] == list(plain[3:])
 
 
+@pytest.mark.parametrize("batch", [4031, 4032, 4095, 4096])
+def test_block_tables_where_the_sums_pass_the_default_shared_memory(batch):
+    """Three sums per request and the static state: 48 KB lie between 4031 and 4096 requests."""
+    from actfold_b200.speculative import block_tables
+
+    tables = torch.full((batch, 2), -1, dtype=torch.int32, device="cuda")
+    kept, grow = [0] * batch, [r % 3 for r in range(batch)]
+    ring, span = _i32(list(range(batch))), torch.tensor([0, batch], device="cuda")
+    want = U.tables_step(tables.tolist(), kept, kept, grow, ring.tolist(), 0, batch, 16)
+    got = block_tables(tables, _i32(kept), _i32(grow), ring, span, 16, sum(grow))
+    assert tables.tolist() == want[0] and got.slots.tolist() == [x for r in want[2] for x in r]
+    assert got.free_range.tolist() == list(want[3:])
+
+
+@pytest.mark.parametrize("n", [12270, 12288, 12320])
+def test_trees_whose_parents_pass_the_default_shared_memory(n):
+    """A chain per tree; 48 KB of parents are 12288 nodes."""
+    from actfold_b200.speculative import accept_tree, tree_masks
+
+    parents, starts = _i32(list(range(-1, n - 1))), _i32([0, n])
+    words = -(-n // 32)
+    mask, positions = tree_masks(parents, starts, words)
+    assert positions.tolist() == list(range(n))
+    last = [-1] * (n // 32) + ([(1 << n % 32) - 1] if n % 32 else [])
+    assert mask[-1].tolist() == last
+    tokens = torch.arange(n, device="cuda")
+    path = accept_tree(parents, tokens, tokens + 1, starts, 5, root_targets=torch.tensor([0], device="cuda"))
+    assert path.rows.tolist() == [[0, 1, 2, 3, 4]] and path.counts.tolist() == [5] and path.next_tokens.tolist() == [5]
+
+
 # ------------------------------------------------------------------------------------------------ cache writes
 @pytest.mark.parametrize("layers,heads,dim,dtype,page", [(1, 32, 128, torch.bfloat16, 64), (3, 4, 128, torch.float16, 16), (2, 1, 64, torch.float32, 5),
                                                          (1, 3, 5, torch.bfloat16, 7), (2, 5, 6, torch.int8, 16), (1, 2, 80, torch.float16, 48)])
