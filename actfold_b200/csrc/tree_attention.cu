@@ -24,9 +24,9 @@
 // some 60 cycles), warp 18 issues S, warp 19 plans the CTA's work and issues O. A column's
 // reference maximum m is raised only when a score passes it by more than 2^8
 // (or at the row's first key): steady tiles take one comparison per score and one
-// barrier vote, no maximum across lanes. P then stays below 256, which bf16
-// and fp16 round with the same relative error (half a step of the type per
-// probability: the tensor cores take 16 bits). Sums and O are fp32. Every wait is
+// barrier vote, no maximum across lanes. P then stays below 2^8 (2^15 in fp16, see
+// kLead), rounded to 16 bits for the tensor cores: half a step of the type per
+// probability. Sums and O are fp32. Every wait is
 // bounded; a timeout sets AF_STATUS_TIMEOUT.
 //
 // Measured on B200 (128 dims, joins included): 64 requests of one token over 90 to
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
           }
         };
         if (begun) shift();
-        if (!begun || vote_any<kTeam>(team, top > kRaise)) {
+        if (!begun || vote_any<kTeam>(team, top > kLead<DT> + kRaise)) {
           // New maxima of the columns that need one (at first of all of them), from the scores themselves.
           tmem_load<C>(lanes + sb * N + c0, x);
           float y[C];
@@ -410,9 +410,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
           if (team_tid < C) {
             const float t = fmaxf(fmaxf(red[team_tid], red[N + team_tid]), fmaxf(red[2 * N + team_tid], red[3 * N + team_tid]));
             const float old = -m_neg[team_tid];
-            const bool raise = old == kUnset ? t > kUnset : t > old + kRaise;
-            red[team_tid] = raise ? (old == kUnset ? 0.f : exp2f(old - t)) : 1.f;
-            if (raise) m_neg[team_tid] = -t;
+            const bool raise = old == kUnset ? t > kUnset : t > old + (kLead<DT> + kRaise);
+            red[team_tid] = raise ? (old == kUnset ? 0.f : exp2f(old - (t - kLead<DT>))) : 1.f;
+            if (raise) m_neg[team_tid] = kLead<DT> - t;
           }
           named_bar_sync(team, kTeam);
           if (begun) {

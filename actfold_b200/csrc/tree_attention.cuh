@@ -17,6 +17,11 @@ constexpr int kPlans = 4;                   // segments planned in shared memory
 constexpr int kWhole = 8;                   // a row of at most this many tiles is not shared by CTAs
 constexpr float kUnset = -3.0e38f;          // reference maximum of a row that has seen no key
 constexpr float kRaise = 8.f;               // log2 headroom before a reference maximum is raised
+// A reference maximum is set this far (log2) below the score that it is taken from: probabilities then lie at 2^kLead, and
+// below 2^(kLead + kRaise). fp16 is subnormal below 2^-14 and 0 below 2^-25, which a long cache behind one large score would
+// lose; 2^15 is still a number of that type, so its steps are 2^-31 of the largest probability. bf16 has fp32's range.
+template <int DT>
+constexpr float kLead = DT == AF_DTYPE_F16 ? 7.f : 0.f;
 
 struct Params {
   CUtensorMap q, k, v, kc, vc;

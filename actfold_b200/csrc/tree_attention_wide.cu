@@ -343,10 +343,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
             top[c] = fmaxf(top[c], __uint_as_float(x[16 * c + 15]));
           }
           const float t_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
-          const bool raise = m == kUnset ? t_max > kUnset : t_max > m + kRaise;
+          const bool raise = m == kUnset ? t_max > kUnset : t_max > m + (kLead<DT> + kRaise);
           if (__any_sync(0xffffffffu, raise)) {
-            const float f = raise ? (m == kUnset ? 0.f : exp2f(m - t_max)) : 1.f;
-            if (raise) m = t_max;
+            const float f = raise ? (m == kUnset ? 0.f : exp2f(m - (t_max - kLead<DT>))) : 1.f;
+            if (raise) m = t_max - kLead<DT>;
             if (x2 > (two ? 0 : 2 * pipe)) {
               // O of the halves before this one is complete once the last one's P V is.
               wait(done + 8 * (bar ^ 1), ((taken - 1) >> 1) & 1);

@@ -498,6 +498,35 @@ def test_attention_maximum_that_moves_from_key_to_key(step, nodes):
     _check(args, plain)
 
 
+@pytest.mark.parametrize("dim,nodes", [(128, 1), (64, 20), (128, 50), (128, 90), (64, 200)])
+def test_attention_small_fp16_probabilities_count(dim, nodes):
+    """In every 128 keys one that is far above the others, whose probabilities are 2^-24.9 to 2^-26 of its.
+
+    The large keys' values are 0, the others' 1024, so the output is the sum of the small probabilities. Each is off by at most
+    half a step of a subnormal fp16 number, 2^-25 of a largest one that the kernels hold at 2^7 or more: 1024 * 127 * 2^-32 in
+    all; the result is rounded to fp16 (2^-11 relative), and the scores are off by 2^-24 (dim + 12) |s| in log2 terms.
+    """
+    from actfold_b200.speculative import tree_attention
+
+    t, page = 4096, 64
+    args, plain = _case([t], [nodes], 1, 1, dim, page, torch.float16, kind="none")
+    order = torch.tensor(plain[0][0], device="cuda")
+    keys, values = torch.zeros(t, dim, device="cuda"), torch.full((t, dim), 1024.0, device="cuda")
+    keys[:, 0] = -torch.linspace(24.9, 26.0, t, device="cuda")
+    keys[5::128], values[5::128] = 0.0, 0.0
+    keys = keys.half()
+    args["q"][:] = 0
+    args["q"][:, :, 0] = 1
+    args["k_cache"][order] = keys.view(-1, page, 1, dim)
+    args["v_cache"][order] = values.half().view(-1, page, 1, dim)
+    out = tree_attention(**args, scale=0.6931471805599453).double()  # scores in log2 are the keys' first entries
+    e = torch.exp2(keys[:, 0].double())
+    want = float((e * values[:, 0].double()).sum() / e.sum())
+    allowed = 1024 * 127 * 2.0 ** -32 + want * (2.0 ** -11 + 2.0 ** -24 * (dim + 12) * 26)
+    assert allowed < want / 50
+    assert float((out - want).abs().max()) <= allowed
+
+
 def test_attention_rows_behind_the_last_tree_stay():
     args, plain = _case([60, 5], [4, 30], 4, 2, 128, 16, torch.bfloat16, extra=6)
     out = torch.full_like(args["q"], 3.0)

@@ -73,7 +73,7 @@ def attention(q, k, v, k_cache, v_cache, tables, lengths, starts, bits, scale=No
     dim products summed in fp32, in any order, are off by at most dim * 2^-24 * S with S = scale * sum |q||k|, the scaling, the
     shift by the maximum and exp2 by 2^-24 * 4 (|s| + |max| + 1) more; a weight then moves by at most exp(2 d) - 1, about 2 d,
     and the sum of the weights' rounding in fp32 adds 2^-24 per term, at most keys * 2^-24 relative. fp16 probabilities below
-    2^-14 are off by up to 2^-25 instead (of a largest one of at least 1): f = 2^-25 sum_j |v_j| / l.
+    2^-14 are off by up to 2^-25 instead (of a largest one of at least 2^7): f = 2^-32 sum_j |v_j| / l.
     The log of the sum is off by 2 d, the sum's rounding (keys * 2^-24) and 2^-22 (|lse| + 1) of the logarithm and the shift.
     """
     q64, k64, v64 = q.double(), k.double(), v.double()
@@ -118,7 +118,7 @@ def attention(q, k, v, k_cache, v_cache, tables, lengths, starts, bits, scale=No
                 lse[lo:hi, h] = torch.where(l > 0, top + torch.log(l), torch.full_like(l, -math.inf))[:, 0]
                 big = torch.where(see, (q64[lo:hi, h].abs() @ kk.abs().nan_to_num(0, 0, 0).T) * abs(scale), torch.zeros_like(s)).amax(-1, keepdim=True)
                 d = 2.0 ** -24 * (dim * big + 4 * (2 * big + 1))
-                sub = 2.0 ** -25 * f / l.clamp(min=1e-300) if q.dtype == torch.float16 else 0.0
+                sub = 2.0 ** -32 * f / l.clamp(min=1e-300) if q.dtype == torch.float16 else 0.0
                 tol[lo:hi, h] = (u + 2 * d + (t + n) * 2.0 ** -24) * a + u * o.abs() + sub
                 lse_tol[lo:hi, h] = (2 * d + (t + n) * 2.0 ** -24)[:, 0] + 2.0 ** -22 * (lse[lo:hi, h].abs().nan_to_num(0, 0, 0) + 1)
     return out, lse, tol, lse_tol
