@@ -4,7 +4,7 @@
 // group) of its tree attend to the cached prefix and to the visible nodes of
 // the tree. With few rows per head the work is one pass over the prefix's
 // keys and values, so the products are transposed: the 128 KEYS of a tile are
-// the M side of the tensor-core instruction and the rows (16 to 128 of them)
+// the M side of the tensor-core instruction and the rows (16 to 64 of them)
 // its N side,
 //   S^T [128 keys, rows] = K Q^T,       O^T [dim, rows] += V^T P^T,
 // so a tile with 7 rows costs the exponentials of 8 rows, not of 128.
@@ -52,7 +52,7 @@ struct Shape {
   static constexpr int kCols = N < 32 ? N : 32;     // columns of a softmax thread
   static constexpr int kGroups = N / kCols;         // groups of 128 threads per tile
   static constexpr int kPipes = 4 / kGroups;        // tiles that are worked on at once
-  static constexpr int kS = N == 128 ? 2 : 4;       // S buffers in TMEM
+  static constexpr int kS = 4;                      // S buffers in TMEM
   static constexpr int kTmem = (kS + 2 * kPipes) * N <= 256 ? 256 : 512;  // S, then O [2 segments][kPipes]
   static constexpr int kHalves = HD / 64;
   static constexpr int kPitch = N < 64 ? 2 * N : 128;         // bytes of a key's row of P^T (blocks of 64 rows where there are more)
@@ -744,7 +744,7 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   p.nt = n == 256 ? 2 * p.nt_q : p.nt_q;
   // Measured: a row end costs some 1800 cycles of 2700 a tile with 16 rows, 9000 of 2900 with 64, 8000 of 4500 with 256.
   p.row_cost = n == 16 ? 1 : n == 64 ? 3 : 2;
-  // Tiles are counted in 32 bits: no more than this can come of any device-side values.
+  // Tiles are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
   AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + p.row_cost) < 2147483000.0,
              "af_tree_attention: more than 2^31 tiles of 128 keys");
   const uint64_t hd = (uint64_t)a.head_dim, kvh = (uint64_t)a.n_kv_heads;

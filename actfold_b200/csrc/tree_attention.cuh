@@ -266,21 +266,25 @@ struct Planner {
   int made = 0;
   bool more = true;
 
-  __device__ __forceinline__ static int cost_of(const Params& p, int b) {
+  __device__ __forceinline__ static int cost_of(const Params& p, int b, bool& disorder) {
     if (b >= p.batch) return 0;
     const Request r = request(p, b);
+    disorder |= p.starts[b + 1] < p.starts[b];
     if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
     return r.cost(p.kv_heads);
   }
 
-  // Two passes over the requests, 32 at a time: the list's length, and the request that the share begins with.
+  // Two passes over the requests, 32 at a time: the list's length, and the request that the share begins with. Starts out
+  // of order anywhere are trees that overlap, whose units nothing bounds: then there is no list.
   __device__ __forceinline__ void begin(const Params& p, int lane) {
-    const int first_cost = cost_of(p, lane);
+    bool disorder = false;
+    const int first_cost = cost_of(p, lane, disorder);
     int all = first_cost;
 #pragma unroll 4
-    for (int b = lane + 32; b < p.batch; b += 32) all += cost_of(p, b);
+    for (int b = lane + 32; b < p.batch; b += 32) all += cost_of(p, b, disorder);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (__any_sync(0xffffffffu, disorder)) all = 0;
     shares.each = all / (int)gridDim.x;
     shares.more = all - shares.each * (int)gridDim.x;
     walk.t = shares.begin(blockIdx.x);
@@ -289,7 +293,7 @@ struct Planner {
     if (walk.t >= walk.end) return;
 #pragma unroll 1
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      int upto = b0 ? cost_of(p, b0 + lane) : first_cost;
+      int upto = b0 ? cost_of(p, b0 + lane, disorder) : first_cost;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);

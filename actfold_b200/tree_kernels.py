@@ -105,7 +105,7 @@ def block_tables(
     """Pages and slots for ``grow[r]`` new tokens behind the first ``lengths[r]`` tokens of every request.
 
     ``tables`` [requests, max_pages] int32 (updated in place) holds the pages
-    of each request's first ``held[r]`` tokens (default: ``lengths``). Missing
+    of each request's first ``held[r]`` tokens (default: ``lengths``), each of one request only. Missing
     pages come from the front of the ring ``free_pages`` [pool] int32, pages no
     longer needed go to its end (updated in place). ``free_range`` [2] int64 holds the ring's
     first free entry and the one behind its last, counted without end (entry e
@@ -242,7 +242,7 @@ def write_cache(
     page_size] = x[rows[i]]`` for each ``slot = slots[i]`` (``rows`` None: row
     i); entries with a negative slot or row are skipped. ``slots`` int64 and ``rows`` int32
     may have any shape, the same one. Any dtype, the caches' own; any strides but the
-    innermost. Live slots must differ from one another.
+    innermost. Live slots must differ from one another, and the rows must not lie in the caches.
     """
     shape, cache = k.shape, k_cache.shape
     if v.shape != shape or v_cache.shape != cache or len(shape) not in (3, 4) or len(cache) != len(shape) + 1:
@@ -339,7 +339,8 @@ def tree_attention(
     tree is a chain, in which a node sees the nodes up to itself (a single new
     token, or a prompt behind a cached prefix). ``scale`` defaults to dim **
     -0.5. A row that sees nothing is 0. ``lse`` [nodes, heads] float32 receives the
-    natural log of each row's sum of exponentials. Rows of ``out`` behind ``starts[-1]`` are not written.
+    natural log of each row's sum of exponentials. Rows of ``out`` behind ``starts[-1]`` are not written,
+    none when ``starts`` is out of order. ``out`` shares no memory with the inputs.
     """
     qs, ks, cs = q.shape, k.shape, k_cache.shape
     if len(qs) != 3 or len(ks) != 3 or len(cs) != 4 or v.shape != ks or v_cache.shape != cs:

@@ -538,7 +538,8 @@ int af_write_cache(const af_cache_rows* w, uint32_t* status, void* stream);
  * (they are not in the cache yet). mask null: the nodes of a tree are a chain,
  * node i sees the nodes up to itself. Query head h reads key/value head
  * h / (n_heads / n_kv_heads). A row that sees no key is 0 (lse -inf). Keys and
- * values that a row does not see have no influence on it, whatever they hold.
+ * values that a row does not see have no influence on it, whatever they hold. Starts out of order leave out
+ * as it was; out shares no memory with the inputs.
  * dtype AF_DTYPE_F16 or AF_DTYPE_BF16, head_dim 64 or 128, page_size a
  * multiple of 8, n_heads / n_kv_heads <= 64; every stride (bytes, in the
  * order of the indexes) and address a multiple of 16, the innermost dimension

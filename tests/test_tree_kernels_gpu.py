@@ -606,6 +606,25 @@ def test_attention_reports_bad_pages_and_lengths():
         st.check_status()
 
 
+@pytest.mark.parametrize("heads", [64, 2])
+def test_attention_with_starts_out_of_order_writes_nothing(heads):
+    """Trees that overlap 1500 times: more than 2^31 tiles with 64 key/value heads."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention
+
+    n, batch, page = 3000, 3000, 64
+    x = torch.ones(n, heads, 64, dtype=torch.bfloat16, device="cuda")
+    cache = torch.ones(1, page, heads, 64, dtype=torch.bfloat16, device="cuda")
+    starts = torch.zeros(batch + 1, dtype=torch.int32, device="cuda")
+    starts[1::2] = n
+    tables, lengths = torch.zeros(batch, 256, dtype=torch.int32, device="cuda"), torch.full((batch,), 16384, dtype=torch.int32, device="cuda")
+    out, st = torch.full_like(x, 5.0), DeviceStatus()
+    tree_attention(x, x, x, cache, cache, tables, lengths, starts, out=out, status=st)
+    with pytest.raises(RuntimeError):
+        st.check_status()
+    assert out.eq(5.0).all()
+
+
 def test_attention_same_bits_again_and_on_another_stream():
     from actfold_b200.speculative import tree_attention
 
