@@ -330,14 +330,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         const bool masked = key0 + kKeys > s.len;
         const bool in_prefix = key < s.len, in_tree = node >= 0 && node < s.n;
         const uint32_t stage_at = base + stage * S::kStage;
-        // S of this tile also says that its stage was loaded, so the wait for its V below is at most one phase ahead.
-        wait(s_full + 8 * sb, (j / S::kS) & 1);
-        tc_fence_after();
         uint32_t vis = 0xffffffffu;  // bit i: column c0 + i sees this key
-        if (masked) {
+        if (masked) {  // (read while S is on its way)
           const int c = c0 + lane;
           vis = transpose_bits(lane < C && c < cols ? seen_bits(p, s.s0, s.node0 + c / p.group, node - lane) : 0u, lane);
           vis = in_prefix ? 0xffffffffu : in_tree ? vis : 0u;
+        }
+        // S of this tile also says that its stage was loaded, so the wait for its V below is at most one phase ahead.
+        wait(s_full + 8 * sb, (j / S::kS) & 1);
+        tc_fence_after();
+        if (masked) {
           // Rows of V without a key (of those that the product takes) are whatever lay there: cleared. A drafted value that is not finite would reach
           // every column as 0 * inf: it is cleared too, and added at the end to the columns that see it.
           wait(v_full + 8 * stage, (j / S::kStages) & 1);
