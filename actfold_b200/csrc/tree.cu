@@ -30,8 +30,8 @@ __device__ __forceinline__ int tree_range(const int* __restrict__ starts, int b,
 // thread holds one 32-bit word of its row at a time and writes it when the walk
 // leaves it. Rows of up to 32 words are put together in shared memory and
 // leave in whole lines; wider ones go straight out. Bound by latency (starts, then
-// parents, then the walk): 35726 nodes of 128 trees, 16 words each, take 8.0 us (10.0 us
-// with rows stored straight out and parents loaded one after another), one tree of 26 nodes 2.9 us.
+// parents, then the walk): 35726 nodes of 128 trees, 16 words each, take 8.0 to 8.6 us (10.0 us
+// with rows stored straight out and parents loaded one after another), one tree of 26 nodes 2.9 to 3.3 us.
 template <bool STAGED>
 __global__ void __launch_bounds__(kMaskThreads) k_tree_masks(const int* __restrict__ parents, const int* __restrict__ starts,
                                                              int64_t total, int words, const int* __restrict__ base,
@@ -329,8 +329,8 @@ constexpr int kWriteThreads = 256;
 
 // A warp moves 32 U vectors of (keys, then values) of one row: U 16-byte loads
 // per lane in flight, then U stores. Bound by HBM (every byte is read and written
-// once): 16209 rows of 32 heads x 128 bf16, keys and values, take 53.6 us (6.36 TB/s);
-// with U = 4 and 64-bit divisions they took 64 us. FLAT: a row's heads lie
+// once): 10391 rows of 32 heads x 128 bf16, keys and values, take 53.5 us (6.37 TB/s);
+// with U = 4 and 64-bit divisions they took 64 us, with U = 8 and 32-bit ones 56. FLAT: a row's heads lie
 // next to one another on both sides, so there is no head to divide for.
 template <typename V, int U, bool FLAT>
 __global__ void __launch_bounds__(kWriteThreads) k_write_cache(const WriteArgs a, int chunks) {
