@@ -74,6 +74,9 @@ def attention(q, k, v, k_cache, v_cache, tables, lengths, starts, bits, scale=No
     shift by the maximum and exp2 by 2^-24 * 4 (|s| + |max| + 1) more; a weight then moves by at most exp(2 d) - 1, about 2 d,
     and the sum of the weights' rounding in fp32 adds 2^-24 per term, at most keys * 2^-24 relative. fp16 probabilities below
     2^-14 are off by up to 2^-25 instead (of a largest one of at least 2^7): f = 2^-32 sum_j |v_j| / l.
+    A result below 2^-14 in fp16 is rounded by up to half a subnormal step, 2^-25, instead of u |ref|: f has that as well.
+    (By arithmetic: of an exact -5.9195e-6, between 99 and 100 steps of 2^-24, the nearest number is 99 steps, -5.9009e-6; the
+    right rounding is off by 1.87e-8, u |ref| is 0.29e-8, 2^-25 is 2.98e-8.)
     The log of the sum is off by 2 d, the sum's rounding (keys * 2^-24) and 2^-22 (|lse| + 1) of the logarithm and the shift.
     """
     q64, k64, v64 = q.double(), k.double(), v.double()
@@ -118,7 +121,7 @@ def attention(q, k, v, k_cache, v_cache, tables, lengths, starts, bits, scale=No
                 lse[lo:hi, h] = torch.where(l > 0, top + torch.log(l), torch.full_like(l, -math.inf))[:, 0]
                 big = torch.where(see, (q64[lo:hi, h].abs() @ kk.abs().nan_to_num(0, 0, 0).T) * abs(scale), torch.zeros_like(s)).amax(-1, keepdim=True)
                 d = 2.0 ** -24 * (dim * big + 4 * (2 * big + 1))
-                sub = 2.0 ** -32 * f / l.clamp(min=1e-300) if q.dtype == torch.float16 else 0.0
+                sub = 2.0 ** -32 * f / l.clamp(min=1e-300) + 2.0 ** -25 if q.dtype == torch.float16 else 0.0
                 tol[lo:hi, h] = (u + 2 * d + (t + n) * 2.0 ** -24) * a + u * o.abs() + sub
                 lse_tol[lo:hi, h] = (2 * d + (t + n) * 2.0 ** -24)[:, 0] + 2.0 ** -22 * (lse[lo:hi, h].abs().nan_to_num(0, 0, 0) + 1)
     return out, lse, tol, lse_tol
