@@ -52,6 +52,7 @@ SIGNATURES: dict[str, tuple] = {
     "af_write_cache": (_i32, [_vp, _vp, _vp]),
     "af_tree_attention": (_i32, [_vp, _vp, _vp]),
     "af_tree_attention_workspace_bytes": (_i32, [_vp]),
+    "af_tree_attention_wait_limit": (_i32, [_i64]),
 }
 
 _lib = None

@@ -72,7 +72,7 @@ struct Shape {
   static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
   static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
   static constexpr int kOffBar = kOffRed + kPipes * 4 * N * 4;
-  static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4 + kPlans;
+  static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4 + kPlans + 1;
   static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
 };
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   const uint32_t base = smem_u32(gb), sQ = base + S::kOffQ;
   const uint32_t k_full = base + S::kOffBar, v_full = k_full + 8 * S::kStages, empty = v_full + 8 * S::kStages, q_full = empty + 8 * S::kStages,
                  q_empty = q_full + 16, s_full = q_empty + 16, p_full = s_full + 8 * S::kS, done = p_full + 8 * S::kS, o_full = done + 8 * S::kS,
-                 o_empty = o_full + 16, plan_full = o_empty + 16;
+                 o_empty = o_full + 16, plan_full = o_empty + 16, drained = plan_full + 8 * kPlans;
   Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -190,7 +190,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       mbar_init(o_empty + 8 * i, kSoft);
     }
     for (int i = 0; i < kPlans; ++i) mbar_init(plan_full + 8 * i, 1);
-    *failed = 0;
+    mbar_init(drained, 2);
+    failed[0] = 0;
+    failed[1] = p.patience;
     fence_barrier_init();
   }
   if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
@@ -258,10 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     planner.begin(p, lane);
     planner.on(p, plans, plan_full, 1, lane);
 #pragma unroll 1
-    while (true) {
+    while (ok && planned(seg, s)) {
       // Everyone is done with the plan that this one replaces: P of the segment before this one is there.
       planner.on(p, plans, plan_full, seg + 2, lane);
-      if (!ok || !planned(seg, s)) break;
       const int ob = seg & 1;
       if (seg >= 2) ok = agreed(wait_for(o_empty + 8 * ob, ((seg >> 1) - 1) & 1, failed));
 #pragma unroll 1
@@ -312,8 +313,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     };
     int j0 = 0, seg = 0;  // tiles before this segment
     bool wrote_start = false;
+    // Into the next segment go all softmax warps or none, whatever each has seen of a plan or of a wait that ran out: the
+    // barriers inside have no limit of their own.
+    auto enter = [&]() {
+      const bool there = planned(seg, s);
+      return !vote_any<kSoft * 32>(5, !there || *failed);
+    };
 #pragma unroll 1
-    while (planned(seg, s)) {
+    while (enter()) {
       const int cols = min(p.nt, s.n - s.node0) * p.group;
       const int live = min(C, max(0, cols - c0));  // columns of this thread that are rows
       uint64_t l[C / 2];                           // this key's part of the sums
@@ -554,13 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty + 8 * (seg & 1));
-      named_bar_sync(5, kSoft * 32);  // the factors lie where the next maxima go
       if (!whole && s.k0 == 0) {
         wrote_start = true;
         if (tid == 0) *scratch.started(blockIdx.x) = Started{s.last, (int)first, cols, s.kvh};
       }
       j0 += tiles;
-      ++seg;
+      ++seg;  // (the factors lie where the next maxima go: enter() is a barrier)
     }
     if (!wrote_start && tid == 0) scratch.started(blockIdx.x)->last = 0;
   }
@@ -569,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+  if (*failed && (warp == kMmaS || warp == kMmaO)) drain_products(drained, warp == kMmaS);
   if (warp == kMmaS) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kTmem);
@@ -638,6 +645,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_tree_attention_join(const __gr
     }
   }
 }
+
+std::atomic<int> g_patience{kPatience};
 
 int64_t workspace_bytes() { return Scratch<256, 128>::bytes(sm_count()); }
 
@@ -730,6 +739,12 @@ extern "C" int af_tree_attention_workspace_bytes(int64_t* bytes) {
   return AF_OK;
 }
 
+extern "C" int af_tree_attention_wait_limit(int64_t attempts) {
+  AF_REQUIRE(attempts >= -1 && attempts <= kPatience, "af_tree_attention_wait_limit: attempts must lie between 0 and 2^18, or be -1");
+  g_patience.store(attempts < 0 ? kPatience : (int)attempts, std::memory_order_relaxed);
+  return AF_OK;
+}
+
 extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* status, void* stream) {
   AF_REQUIRE(args, "af_tree_attention: null pointer");
   const af_tree_attention_args& a = *args;
@@ -796,6 +811,7 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   p.lse = a.lse;
   p.ws = static_cast<char*>(a.workspace);
   p.status = status;
+  p.patience = g_patience.load(std::memory_order_relaxed);
   cudaStream_t s = as_stream(stream);
   const bool bf16 = a.dtype == AF_DTYPE_BF16;
   return n == 256 ? wide_launch(p, bf16, (int)a.head_dim, s) : launch_narrow(p, n, bf16, a.head_dim, s);

@@ -40,6 +40,7 @@ struct Params {
   int heads;
   char* ws;
   unsigned* status;
+  int patience;  // attempts of a wait before it gives up
 };
 
 // A request's tree and prefix; no cost where there is nothing to do or the values are bad.
@@ -182,11 +183,13 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// Bounded wait for a phase: about a second of attempts (each of which sleeps a few microseconds).
+// Bounded wait for a phase: failed[0] says that a wait has run out somewhere, failed[1] how many attempts a wait makes
+// (each sleeps a few microseconds; kPatience of them take about a second).
+constexpr int kPatience = 1 << 18;
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* failed) {
 #pragma unroll 1
   for (int n = 0; !mbar_try_wait(bar, parity); ++n)
-    if (n > (1 << 18) || *failed) return false;
+    if (n >= failed[1] || *failed) return false;
   return true;
 }
 
@@ -418,15 +421,28 @@ __device__ __forceinline__ void load_tiles(const Params& p, Planned planned, uin
     if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
   }
   __syncwarp();
-  if (*failed && lane == 0) {
-    // Copies still in flight land before the CTA's shared memory is given up (bounded).
-    volatile int no_abort = 0;
+  if (lane == 0) {
+    // Copies still in flight (there are some only when a wait ran out, here or in another warp, by now or later) land before
+    // the CTA's shared memory is given up (bounded).
+    volatile int by_itself[2] = {0, kPatience};
 #pragma unroll 1
-    for (int i = max(0, j - kStages); i < j; ++i) wait_for(full + 8 * (i % kStages), (i / kStages) & 1, &no_abort);
+    for (int i = max(0, j - kStages); i < j; ++i) wait_for(full + 8 * (i % kStages), (i / kStages) & 1, by_itself);
     if (!VALUES)
 #pragma unroll 1
-      for (int i = max(0, seg - S::kQ); i < seg; ++i) wait_for(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, &no_abort);
+      for (int i = max(0, seg - S::kQ); i < seg; ++i) wait_for(q_full + 8 * (i % S::kQ), (i / S::kQ) & 1, by_itself);
   }
+  __syncwarp();
+}
+
+// After a wait has run out: the products that the two issue warps have in flight end before the CTA's tensor and shared
+// memory is given up. Called by both (converged) behind the CTA's last barrier; the one that frees tensor memory waits, for
+// both (bounded): a commit follows the products of the thread that makes it.
+__device__ __forceinline__ void drain_products(uint32_t drained, bool waits) {
+  if (elect_one()) tc_commit(drained);
+  __syncwarp();
+  volatile int by_itself[2] = {0, kPatience};
+  if (waits) wait_for(drained, 0, by_itself);
+  __syncwarp();
 }
 
 // Workspace: Started[ctas], then per CTA two partial rows (0: begun by an

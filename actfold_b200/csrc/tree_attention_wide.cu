@@ -47,7 +47,7 @@ struct Wide {
   static constexpr int kOffQ = kOffV + kVStages * kStage;
   static constexpr int kOffStat = kOffQ + kQBytes;                   // [2][128] (maximum, sum) of the pipes
   static constexpr int kOffBar = kOffStat + 2 * kRows * 8;
-  static constexpr int kBars = 2 * kKStages + 2 * kVStages + 2 + 12 + 2 + kPlans;
+  static constexpr int kBars = 2 * kKStages + 2 * kVStages + 2 + 12 + 2 + kPlans + 1;
   static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
   static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
   static constexpr int kTmemO = 2 * kKeys;                           // O of pipe x at kTmemO + 128 x, S of pipe x at 128 x
@@ -110,7 +110,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   const uint32_t base = smem_u32(gb);
   const uint32_t k_full = base + S::kOffBar, k_empty = k_full + 8 * S::kKStages, v_full = k_empty + 8 * S::kKStages,
                  v_empty = v_full + 8 * S::kVStages, q_full = v_empty + 8 * S::kVStages, q_empty = q_full + 8, s_full = q_empty + 8,
-                 p_full = s_full + 32, done = p_full + 32, o_full = done + 32, o_empty = o_full + 8, plan_full = o_empty + 8;
+                 p_full = s_full + 32, done = p_full + 32, o_full = done + 32, o_empty = o_full + 8, plan_full = o_empty + 8,
+                 drained = plan_full + 8 * kPlans;
   Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -134,7 +135,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     mbar_init(o_full, 1);
     mbar_init(o_empty, kSoft);
     for (int i = 0; i < kPlans; ++i) mbar_init(plan_full + 8 * i, 1);
-    *failed = 0;
+    mbar_init(drained, 2);
+    failed[0] = 0;
+    failed[1] = p.patience;
     fence_barrier_init();
   }
   if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), 512);
@@ -207,10 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     bool ok = true;
     int seg = 0, stage = 0, v_phase = 0, used0 = 0, used1 = 0;
 #pragma unroll 1
-    while (true) {
+    while (ok && planned(seg, s)) {
       // The plan that this one replaces has been read by everyone: the segment after it is done.
       planner.on(p, plans, plan_full, seg + 2, lane);
-      if (!ok || !planned(seg, s)) break;
       const bool two = s.n - s.node0 > p.nt_q;
       const int tiles = s.k1 - s.k0, steps = two ? 4 : 2;
       if (seg > 0) ok = agreed(wait_for(o_empty, (seg - 1) & 1, failed));  // the last segment's O is read
@@ -263,8 +265,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     };
     int j0 = 0, seg = 0, taken = 0;  // tiles before this segment; halves of S of this pipe so far
     bool wrote_start = false;
+    // Into the next segment go all softmax warps or none (see the narrow kernel).
+    auto enter = [&]() {
+      const bool there = planned(seg, s);
+      return !vote_any<kSoft * 32>(1, !there || *failed);
+    };
 #pragma unroll 1
-    while (planned(seg, s)) {
+    while (enter()) {
       const bool two = s.n - s.node0 > p.nt_q;
       const int tiles = s.k1 - s.k0;
       const int first_node = s.node0 + (two && pipe ? p.nt_q : 0), rows = min(p.nt_q, s.n - first_node) * p.group;
@@ -449,13 +456,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(o_empty);
-      named_bar_sync(1, kSoft * 32);  // the next segment's maxima go where these ones are
       if (!whole && s.k0 == 0) {
         wrote_start = true;
         if (tid == 0) *scratch.started(blockIdx.x) = Started{s.last, s.s0 + s.node0, min(p.nt, s.n - s.node0) * p.group, s.kvh};
       }
       j0 += tiles;
-      ++seg;
+      ++seg;  // (the next segment's maxima go where these ones are: enter() is a barrier)
     }
     if (!wrote_start && tid == 0) scratch.started(blockIdx.x)->last = 0;
   }
@@ -464,6 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+  if (*failed && (warp == kMmaS || warp == kMmaO)) drain_products(drained, warp == kMmaS);
   if (warp == kMmaS) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);

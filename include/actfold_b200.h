@@ -573,6 +573,14 @@ int af_tree_attention(const af_tree_attention_args* a, uint32_t* status, void* s
 /* Bytes of scratch that af_tree_attention needs on the current device. */
 int af_tree_attention_workspace_bytes(int64_t* bytes);
 
+/*
+ * Attempts (of a few microseconds each) after which a wait inside later
+ * af_tree_attention calls of this process gives up: the call then ends with
+ * AF_STATUS_TIMEOUT in *status and rows of out that mean nothing. -1: the
+ * default, 2^18 attempts or about a second, which is also the most.
+ */
+int af_tree_attention_wait_limit(int64_t attempts);
+
 #ifdef __cplusplus
 }
 #endif

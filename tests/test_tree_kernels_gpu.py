@@ -653,6 +653,72 @@ def test_attention_far_offsets():
     _check(args, ([far], lengths, starts, bits))
 
 
+@pytest.fixture
+def wait_limit():
+    """Sets how many attempts a wait inside the attention kernels makes; the default comes back at the end."""
+    from actfold_b200 import _lib
+
+    lib = _lib.load()
+    yield lambda attempts: _lib.check(lib.af_tree_attention_wait_limit(attempts))
+    torch.cuda.synchronize()
+    _lib.check(lib.af_tree_attention_wait_limit(-1))
+
+
+def _one_long_chain(n, heads, kv, dim, batch):
+    """One chain of n nodes among empty requests, so that the average, which picks the kernel, is n / batch."""
+    args, plain = _case([70], [n], heads, kv, dim, 16, torch.bfloat16, kind="chain")
+    more = batch - 1
+    args["tables"] = torch.cat([args["tables"], torch.zeros(more, args["tables"].shape[1], dtype=torch.int32, device="cuda")])
+    args["lengths"] = torch.cat([args["lengths"], _i32([0] * more)])
+    args["starts"] = torch.cat([args["starts"], _i32([n] * more)])
+    return args, plain
+
+
+@pytest.mark.parametrize("group", [1, 4, 8, 16])  # tiles of 16, 32 and 64 rows, and the wide kernel
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_whose_waits_run_out_ends_with_a_status(group, dim, wait_limit):
+    """Values that are not finite make the ends of rows long (every node is looked through for them): with a limit of one
+    attempt the other warps' waits run out in the middle. The call ends and says so, and the next one is as always."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention
+
+    n = 8000
+    args, _ = _one_long_chain(n, 2 * group, 2, dim, n // 8)
+    want = tree_attention(**args)
+    sick = dict(args, v=args["v"].clone())
+    sick["v"][0], sick["v"][n - 1] = float("inf"), float("inf")
+    st = DeviceStatus()
+    torch.cuda.synchronize()
+    wait_limit(0)
+    tree_attention(**sick, status=st)
+    with pytest.raises(TimeoutError):
+        st.check_status()
+    wait_limit(-1)
+    assert torch.equal(tree_attention(**args, status=st), want)
+    st.check_status()
+
+
+@pytest.mark.parametrize("case", [CASES[4], CASES[6], CASES[7], *CASES[13:19], CASES[22], *CASES[24:28]])
+def test_attention_with_short_waits_is_right_or_says_so(case, wait_limit):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention
+
+    args, _ = _case(*case[:7], seed=4, kind=case[7])
+    want, st = tree_attention(**args), DeviceStatus()
+    for attempts in (0, 1, 2, 4, 16, 0):
+        torch.cuda.synchronize()
+        wait_limit(attempts)
+        got = tree_attention(**args, status=st)
+        try:
+            st.check_status()
+            assert torch.equal(got, want)
+        except TimeoutError:
+            pass
+    wait_limit(-1)
+    assert torch.equal(tree_attention(**args, status=st), want)
+    st.check_status()
+
+
 # ------------------------------------------------------------------------------------------------ the step as a whole
 def _model(token, position, heads, dim):
     """Deterministic rows of a toy layer: one vector per (token, position)."""

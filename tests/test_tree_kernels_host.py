@@ -178,3 +178,10 @@ def test_entry_points_refuse_before_any_launch(lib):
         assert lib.af_write_cache(packed(**kw), None, None) == _lib.AF_ERR_ARG, kw
     assert lib.af_write_cache(None, None, None) == _lib.AF_ERR_ARG
     assert lib.af_write_cache(packed(count=0), None, None) == _lib.AF_OK
+
+
+def test_wait_limit_refusals(lib):
+    for attempts in (-2, (1 << 18) + 1, 1 << 40):
+        assert lib.af_tree_attention_wait_limit(attempts) == _lib.AF_ERR_ARG
+    for attempts in (0, 1 << 18, -1):
+        assert lib.af_tree_attention_wait_limit(attempts) == _lib.AF_OK
