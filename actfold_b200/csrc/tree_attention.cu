@@ -539,9 +539,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
           }
           if (set_aside) {
             const int x0 = max(0, s.k0 * kKeys - s.pad), x1 = min(s.n, s.k1 * kKeys - s.pad);
+            float more[kW];
+            set_aside_rows<DT, kW>(p, s.s0, s.kvh, s.node0, c8, min(o1, c8 + kW), x0, x1, r, more);
 #pragma unroll
-            for (int e = 0; e < kW; ++e)
-              if (c8 + e < o1) y[e] += set_aside_sum<DT>(p, s.s0, s.kvh, s.node0 + (c8 + e) / p.group, x0, x1, r);
+            for (int e = 0; e < kW; ++e) y[e] += more[e];
           }
           if (whole) {
 #pragma unroll

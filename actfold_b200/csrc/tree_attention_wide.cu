@@ -437,8 +437,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
           if (r < rows) {
             if (set_aside) {
               const int x0 = max(0, s.k0 * kKeys - s.pad), x1 = min(s.n, s.k1 * kKeys - s.pad);
+              float more[8];
+              set_aside_dims<DT>(p, s.s0, s.kvh, node, x0, x1, d, more);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] += set_aside_sum<DT>(p, s.s0, s.kvh, node, x0, x1, d + i);
+              for (int i = 0; i < 8; ++i) y[i] += more[i];
             }
             if (whole) {
               *reinterpret_cast<uint4*>(out + 2 * d) = make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));

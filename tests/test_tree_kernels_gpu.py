@@ -666,7 +666,8 @@ def wait_limit():
 
 def _one_long_chain(n, heads, kv, dim, batch):
     """One chain of n nodes among empty requests, so that the average, which picks the kernel, is n / batch."""
-    args, plain = _case([70], [n], heads, kv, dim, 16, torch.bfloat16, kind="chain")
+    args, plain = _case([70], [n], heads, kv, dim, 16, torch.bfloat16, kind="none")
+    args["mask"] = None
     more = batch - 1
     args["tables"] = torch.cat([args["tables"], torch.zeros(more, args["tables"].shape[1], dtype=torch.int32, device="cuda")])
     args["lengths"] = torch.cat([args["lengths"], _i32([0] * more)])
@@ -717,6 +718,43 @@ def test_attention_with_short_waits_is_right_or_says_so(case, wait_limit):
     wait_limit(-1)
     assert torch.equal(tree_attention(**args, status=st), want)
     st.check_status()
+
+
+@pytest.mark.parametrize("group,batch", [(1, 12500), (16, 12500), (8, 12500), (1, 1)])  # 16, 128 (wide), 64 rows; wide with one head per key/value head
+def test_attention_of_a_long_chain_with_values_that_are_not_finite(group, batch):
+    """Two values that are not finite among 100000 nodes: looking for them at a row's end must not outlast the other warps' waits.
+
+    Rows that see none of them, or only the first, are compared with the formula; the allowance is tree_util.attention's (see there).
+    """
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention
+
+    n, dim = 100_000, 64
+    g = torch.Generator(device="cuda").manual_seed(group)
+    q, k, v = (torch.randn(n, h, dim, device="cuda", generator=g).to(torch.bfloat16) for h in (group, 1, 1))
+    v[7, 0, 3], v[n - 9, 0, 5] = float("inf"), float("nan")
+    cache = torch.zeros(1, 16, 1, dim, dtype=torch.bfloat16, device="cuda")
+    starts = _i32([0] + [n] * batch)
+    st = DeviceStatus()
+    out = tree_attention(q, k, v, cache, cache, torch.zeros(batch, 1, dtype=torch.int32, device="cuda"), _i32([0] * batch), starts, status=st)
+    st.check_status()
+    clean = v.clone()
+    clean[7, 0, 3] = clean[n - 9, 0, 5] = 0
+    for i in (0, 6, 7, 500, 49_999, n - 10, n - 9, n - 1):
+        # The last node of a chain of i + 1 nodes, as a tree of one node behind i cached ones: the plain form's single row.
+        pad = -(i % -16)
+        kc, vc = (torch.cat([x[:i], x.new_zeros(pad, 1, dim)]).view(-1, 16, 1, dim) for x in (k, clean))
+        row = slice(i, i + 1)
+        ref, _, tol, _ = U.attention(q[row], k[row], clean[row], kc, vc, [list(range(len(kc)))], [i], [0, 1], [None])
+        bad = torch.zeros(group, dim, dtype=torch.bool, device="cuda")
+        if i >= 7:
+            assert (out[i, :, 3] == float("inf")).all()
+            bad[:, 3] = True
+        if i >= n - 9:
+            assert out[i, :, 5].isnan().all()
+            bad[:, 5] = True
+        err = (out[i].double() - ref[0]).abs()
+        assert bool((err <= tol[0])[~bad].all()), i
 
 
 # ------------------------------------------------------------------------------------------------ the step as a whole
