@@ -15,8 +15,8 @@ Nodes are packed: tree b holds nodes ``starts[b] .. starts[b + 1]`` and a
 parent comes before its children. Sizes that change from step to step
 (``starts``, lengths, counts) stay on the device, and no call synchronises, so a
 step can be captured into a CUDA graph. Pass a
-:class:`~actfold_b200.kernels.DeviceStatus` to learn of values that the device
-found out of range or out of capacity (``check_status()`` raises). Each call is ordered on
+:class:`~actfold_b200.kernels.DeviceStatus` on the tensors' device to learn of values that the
+kernels found out of range or out of capacity (``check_status()`` raises). Each call is ordered on
 the current stream of its tensors' device; its scratch comes from torch's
 allocator on that stream.
 """
@@ -86,8 +86,8 @@ def _not_vectors(what: str, dtype: torch.dtype, **tensors: torch.Tensor | None) 
             raise ValueError(f"{what}: {name} must be a {dtype} vector, got {t.dtype} {tuple(t.shape)}")
 
 
-def _status(status: DeviceStatus | None) -> int | None:
-    return None if status is None else status.status.data_ptr()
+def _word(status: DeviceStatus | None) -> torch.Tensor | None:
+    return None if status is None else status.status
 
 
 def block_tables(
@@ -133,7 +133,7 @@ def block_tables(
         raise ValueError(f"block_tables: free_range must be two int64 numbers, got {free_range.dtype} {tuple(free_range.shape)}")
     if page_size <= 0 or slot_capacity < 0:
         raise ValueError(f"block_tables: page_size {page_size} must be positive and slot_capacity {slot_capacity} not negative")
-    index = _same_device("block_tables", tables, lengths, grow, free_pages, free_range, held)
+    index = _same_device("block_tables", tables, lengths, grow, free_pages, free_range, held, word := _word(status))
     lengths, grow, free_range = lengths.contiguous(), grow.contiguous(), free_range.contiguous()
     if held is not None:
         held = held.contiguous()
@@ -144,7 +144,7 @@ def block_tables(
     _launch("block_tables", index, _lib.load().af_block_tables, tables.data_ptr(), row if n > 1 else most, most,
             None if held is None else held.data_ptr(), lengths.data_ptr(), grow.data_ptr(), n, free_pages.data_ptr(), free_pages.shape[0],
             free_range.data_ptr(), page_size, n * slot_capacity if padded else slot_capacity, slot_capacity if padded else 0,
-            starts.data_ptr(), totals.data_ptr(), slots.data_ptr(), out.data_ptr(), _status(status))
+            starts.data_ptr(), totals.data_ptr(), slots.data_ptr(), out.data_ptr(), _lib.ptr(word))
     return BlockTables(starts, totals, slots, out)
 
 
@@ -171,13 +171,13 @@ def tree_masks(
         raise ValueError(f"tree_masks: starts needs one entry more than there are trees, words {words} must be positive")
     if base is not None and base.shape[0] != batch:
         raise ValueError(f"tree_masks: base must have one entry for each of {batch} trees")
-    index = _same_device("tree_masks", parents, starts, base)
+    index = _same_device("tree_masks", parents, starts, base, word := _word(status))
     parents, starts = parents.contiguous(), starts.contiguous()
     if base is not None:
         base = base.contiguous()
     mask, positions = parents.new_empty((total, words)), torch.empty_like(parents)
     _launch("tree_masks", index, _lib.load().af_tree_masks, parents.data_ptr(), starts.data_ptr(), batch, total, words,
-            None if base is None else base.data_ptr(), mask.data_ptr(), positions.data_ptr(), _status(status))
+            None if base is None else base.data_ptr(), mask.data_ptr(), positions.data_ptr(), _lib.ptr(word))
     return mask, positions
 
 
@@ -215,14 +215,14 @@ def accept_tree(
         raise ValueError(f"accept_tree: starts needs one entry more than there are trees, keep {keep} must be positive")
     if root_targets is not None and root_targets.shape[0] != batch:
         raise ValueError(f"accept_tree: root_targets must have one entry for each of {batch} trees")
-    index = _same_device("accept_tree", parents, tokens, targets, starts, root_targets)
+    index = _same_device("accept_tree", parents, tokens, targets, starts, root_targets, word := _word(status))
     parents, tokens, targets, starts = parents.contiguous(), tokens.contiguous(), targets.contiguous(), starts.contiguous()
     if root_targets is not None:
         root_targets = root_targets.contiguous()
     rows, counts, following = parents.new_empty((batch, keep)), parents.new_empty(batch), tokens.new_empty(batch)
     _launch("accept_tree", index, _lib.load().af_accept_tree, parents.data_ptr(), tokens.data_ptr(), targets.data_ptr(), starts.data_ptr(),
             batch, total, 16384 if max_nodes is None else max_nodes, None if root_targets is None else root_targets.data_ptr(), keep,
-            rows.data_ptr(), counts.data_ptr(), following.data_ptr(), _status(status))
+            rows.data_ptr(), counts.data_ptr(), following.data_ptr(), _lib.ptr(word))
     return AcceptedPath(rows, counts, following)
 
 
@@ -269,7 +269,7 @@ def write_cache(
     if not (kc0 and kc1 and kc2 and kc3 and vc0 and vc1 and vc2 and vc3):
         if any(x == 0 and m > 1 for c in (k_cache, v_cache) for x, m in zip(c.stride(), cache)):
             raise ValueError("write_cache: the caches have entries that share memory")
-    index = _same_device("write_cache", k, v, k_cache, v_cache, slots, rows)
+    index = _same_device("write_cache", k, v, k_cache, v_cache, slots, rows, word := _word(status))
     k0, k1, k2, k3 = k.stride()
     v0, v1, v2, v3 = v.stride()
     if (k3 != 1 or v3 != 1) and dim > 1:
@@ -282,7 +282,7 @@ def write_cache(
     args = _ROWS.pack(k.data_ptr(), v.data_ptr(), e * k0, e * k1, e * k2, e * v0, e * v1, e * v2, k_cache.data_ptr(), v_cache.data_ptr(),
                       e * kc0, e * kc1, e * kc2, e * kc3, e * vc0, e * vc1, e * vc2, e * vc3, slots.data_ptr(),
                       0 if rows is None else rows.data_ptr(), n, count, cache[1], cache[2], layers, heads, dim * e)
-    _launch("write_cache", index, _lib.load().af_write_cache, args, _status(status))
+    _launch("write_cache", index, _lib.load().af_write_cache, args, _lib.ptr(word))
 
 
 def _grid(t: torch.Tensor) -> list[int] | None:
@@ -381,7 +381,7 @@ def tree_attention(
             raise ValueError("tree_attention: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
     if lse is not None and (lse.shape != (total, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
         raise ValueError(f"tree_attention: lse must be contiguous float32 [{total}, {heads}]")
-    _same_device("tree_attention", q, k, v, k_cache, v_cache, tables, lengths, starts, mask, out, lse)
+    _same_device("tree_attention", q, k, v, k_cache, v_cache, tables, lengths, starts, mask, out, lse, word := _word(status))
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts = lengths.contiguous(), starts.contiguous()
@@ -404,7 +404,7 @@ def tree_attention(
         cs[0], cs[1], tables.data_ptr(), tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(), starts.data_ptr(),
         mask_at, mask_row if total > 1 else words, words, batch, total, heads, ks[1], dim, _lib.DTYPE[dtype],
         dim ** -0.5 if scale is None else scale, out.data_ptr(), *out_grid, 0 if lse is None else lse.data_ptr(), workspace.data_ptr(), size)
-    _launch("tree_attention", index, _lib.load().af_tree_attention, args, _status(status))
+    _launch("tree_attention", index, _lib.load().af_tree_attention, args, _lib.ptr(word))
     return out
 
 

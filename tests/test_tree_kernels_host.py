@@ -185,3 +185,27 @@ def test_wait_limit_refusals(lib):
         assert lib.af_tree_attention_wait_limit(attempts) == _lib.AF_ERR_ARG
     for attempts in (0, 1 << 18, -1):
         assert lib.af_tree_attention_wait_limit(attempts) == _lib.AF_OK
+
+
+def test_a_status_on_another_device_is_refused(monkeypatch):
+    """Tensors that only claim to be on a device: no call gets as far as a pointer."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from actfold_b200.kernels import DeviceStatus
+
+    monkeypatch.setattr(T, "_cache_grid", lambda t: (16, 16, 16))
+    i64, b = torch.int64, torch.bfloat16
+    with FakeTensorMode():
+        def z(*shape, dtype=torch.int32):
+            return torch.empty(*shape, dtype=dtype, device="cuda:1")
+
+        rows, cache = z(5, 2, 64, dtype=b), z(3, 16, 2, 64, dtype=b)
+        for where, error in (("cuda:0", ValueError), ("cpu", RuntimeError)):
+            st = DeviceStatus(where)
+            for call in (lambda: S.tree_masks(z(4), z(2), 1, status=st),
+                         lambda: S.accept_tree(z(4), z(4, dtype=i64), z(4, dtype=i64), z(2), 3, status=st),
+                         lambda: S.block_tables(z(2, 3), z(2), z(2), z(6), z(2, dtype=i64), 16, 4, status=st),
+                         lambda: S.write_cache(rows, rows, cache, cache, z(5, dtype=i64), status=st),
+                         lambda: S.tree_attention(rows, rows, rows, cache, cache, z(2, 2), z(2), z(3), status=st)):
+                with pytest.raises(error, match="cuda:0|CUDA device"):
+                    call()
