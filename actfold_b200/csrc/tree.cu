@@ -480,7 +480,8 @@ extern "C" int af_write_cache(const af_cache_rows* w, uint32_t* status, void* st
   AF_REQUIRE(w->layers >= 0 && w->n_rows >= 0 && w->count >= 0 && w->pages >= 0 && w->page_size > 0 && w->heads >= 0 && w->head_bytes >= 0,
              "af_write_cache: bad shape");
   if (w->layers == 0 || w->count == 0 || w->heads == 0 || w->head_bytes == 0) return AF_OK;
-  AF_REQUIRE(w->k && w->v && w->k_cache && w->v_cache && w->slots, "af_write_cache: null pointer");
+  AF_REQUIRE(w->slots && (w->n_rows == 0 || (w->k && w->v)) && (w->pages == 0 || (w->k_cache && w->v_cache)),
+             "af_write_cache: null pointer");  // (of no rows or no pages every entry is skipped)
   AF_REQUIRE(w->heads <= (1 << 20) && w->head_bytes <= (1 << 20) && w->heads * w->head_bytes <= (1 << 28) && w->page_size <= (1 << 20) &&
                  w->layers <= 0x7fffffff,
              "af_write_cache: size too large");

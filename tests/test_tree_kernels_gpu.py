@@ -319,6 +319,26 @@ def test_write_cache_skips_slots_and_rows_out_of_range():
     assert cache[1, 1].eq(1).all() and cache.sum().item() == 128
 
 
+@pytest.mark.parametrize("none", ["rows", "pages"])
+def test_write_cache_of_a_step_without_rows_or_pages(none):
+    """No node in any tree, or a pool without pages: every entry is skipped, and one that is not negative is reported."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import write_cache
+
+    k = torch.ones(2, 0 if none == "rows" else 4, 2, 64, dtype=torch.float16, device="cuda")
+    cache = torch.zeros(2, 0 if none == "pages" else 3, 8, 2, 64, dtype=torch.float16, device="cuda")
+    slots, rows, st = torch.full((3, 5), -1, device="cuda"), torch.full((3, 5), -1, dtype=torch.int32, device="cuda"), DeviceStatus()
+    write_cache(k, k, cache, cache.clone(), slots, rows=rows, status=st)
+    st.check_status()
+    write_cache(k, k, cache, cache.clone(), torch.full_like(slots, 3), rows=rows, status=st)
+    st.check_status()
+    rows[1, 2], slots[1, 2] = 1, 3
+    write_cache(k, k, cache, cache.clone(), slots, rows=rows, status=st)
+    with pytest.raises(RuntimeError):
+        st.check_status()
+    assert not cache.any()
+
+
 def test_write_cache_far_offsets():
     """A cache of more than 2^32 bytes: its last slots."""
     from actfold_b200.speculative import write_cache
