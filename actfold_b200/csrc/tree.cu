@@ -197,8 +197,9 @@ __device__ __forceinline__ int request_of(const int* edge, int batch, int x) {
 // by another one: taken entries lie behind the held ones of their row, a slot
 // in a taken page reads the ring, and the ring's places for returned pages
 // are no free ones (returned <= held = pool - free). Bound by latency (lengths, the
-// scan, a search per slot): 10.3 us for 1000 requests with 84700 new tokens (0.8 MB, 0.1 us of
-// HBM), 5.9 us for 5 requests.
+// scan, the look through what changes hands, a search per slot) and by 64-bit divisions per page and slot: 14.7 us for
+// 1000 requests with 84700 new tokens, 2613 pages taken and 3832 returned (0.8 MB, 0.1 us of HBM), 6.4 us for 5
+// requests; without the look for negative entries 10.2 and 5.6 us, but then they would go round in the ring unseen.
 __global__ void __launch_bounds__(kTableThreads) k_block_tables(const TableArgs a) {
   extern __shared__ int sh[];
   const int B = a.batch, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -207,7 +208,8 @@ __global__ void __launch_bounds__(kTableThreads) k_block_tables(const TableArgs 
   int* s_tok = sh + 2 * (B + 1); // [B + 1]
   __shared__ int64_t part[3][32];
   __shared__ unsigned s_bad;
-  if (tid == 0) s_bad = 0;
+  __shared__ int s_lost;
+  if (tid == 0) s_bad = s_lost = 0;
   __syncthreads();
   int64_t run[3] = {0, 0, 0};
   unsigned bad = 0;
@@ -268,14 +270,43 @@ __global__ void __launch_bounds__(kTableThreads) k_block_tables(const TableArgs 
     s_tok[B] = (int)min(run[2], (int64_t)0x7fffffff);
   }
   __syncthreads();
-  const bool ok = s_bad == 0;
+  if (s_bad == 0) {
+    // A negative entry among those that change hands is no page: it would come into a table, or into the ring and out of it
+    // again. Every CTA looks through all of them before it writes (no CTA writes any of them), so all find the same.
+    // Four loads at a time; of the returned ones a thread looks at neighbours, so that it searches for a request about once.
+    const uint32_t take = s_take[B], give = s_give[B], pool = (uint32_t)a.pool;
+    const uint32_t first = head < (1LL << 32) ? (uint32_t)head % pool : (uint32_t)(head % a.pool);
+    int lost = 0;  // negative where one of them is
+    for (uint32_t x = tid; x < take; x += 4 * kTableThreads) {
+#pragma unroll
+      for (uint32_t u = 0; u < 4 * kTableThreads; u += kTableThreads) {
+        const uint32_t at = first + x + u;
+        if (x + u < take) lost |= a.ring[at < pool ? at : at - pool];
+      }
+    }
+    const uint32_t each = (give + kTableThreads - 1) / kTableThreads, end = min(give, (tid + 1) * each);
+    for (uint32_t x = tid * each; x < end;) {
+      const int r = request_of(s_give, B, (int)x);
+      const uint32_t stop = min(end, (uint32_t)s_give[r + 1]), want = ((uint32_t)a.lengths[r] + a.grow[r] + a.page - 1) / (uint32_t)a.page;
+      const int* row = a.tables + r * a.t_ld + want - s_give[r];
+      for (; x < stop; x += 4) {
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+          if (x + u < stop) lost |= row[x + u];
+      }
+      x = stop;
+    }
+    if (lost < 0) s_lost = 1;
+  }
+  __syncthreads();
+  const bool ok = s_bad == 0 && s_lost == 0;
   if (blockIdx.x == 0) {
     for (int r = tid; r <= B; r += kTableThreads) a.starts[r] = ok ? s_tok[r] : 0;
     for (int r = tid; r < B; r += kTableThreads) a.totals[r] = ok ? a.lengths[r] + a.grow[r] : (a.held ? a.held[r] : a.lengths[r]);
     if (tid == 0) {
       a.range_out[0] = ok ? head + run[0] : head;
       a.range_out[1] = ok ? tail + run[1] : tail;
-      if (!ok && a.status) atomicOr(a.status, s_bad);
+      if (!ok && a.status) atomicOr(a.status, s_bad ? s_bad : AF_STATUS_BOUNDS);
     }
   }
   const int64_t me = (int64_t)blockIdx.x * kTableThreads + tid, step = (int64_t)gridDim.x * kTableThreads;
@@ -306,7 +337,8 @@ __global__ void __launch_bounds__(kTableThreads) k_block_tables(const TableArgs 
       const int64_t kept = a.lengths[r], held = a.held ? a.held[r] : kept, pos = kept + i;
       const int64_t k = pos / a.page, had = (held + a.page - 1) / a.page;
       const int page = k < had ? a.tables[r * a.t_ld + k] : a.ring[(head + s_take[r] + (k - had)) % a.pool];
-      slot = page < 0 ? -1 : (int64_t)page * a.page + (pos - k * a.page);
+      if (page >= 0) slot = (int64_t)page * a.page + (pos - k * a.page);
+      else if (a.status) atomicOr(a.status, AF_STATUS_BOUNDS);  // a held entry that is no page
     }
     a.slots[x] = slot;
   }

@@ -114,7 +114,9 @@ def block_tables(
     [slot_capacity], packed at ``starts``, or with ``padded`` [requests,
     slot_capacity], -1 behind a request's last new token. Requests that do
     not fit leave everything as it was, with empty ``starts`` and -1 slots, and
-    set the capacity bit of ``status``.
+    set the capacity bit of ``status``; so do, with the bounds bit, a negative number
+    and a negative entry (no page) among those that would change hands. New tokens of a
+    held page that is negative get slot -1 and set the bounds bit. The ring has at least one place.
     """
     if tables.dim() != 2 or tables.dtype is not _I32:
         raise ValueError(f"block_tables: tables must be int32 [requests, max_pages], got {tables.dtype} {tuple(tables.shape)}")

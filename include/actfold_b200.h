@@ -472,7 +472,10 @@ int af_fold_get_timing(void* plan, double* ms, int64_t* counts, int n_kinds, int
  * + i (slots_per_request 0) or at r * slots_per_request + i, -1 elsewhere.
  * When the pages, a table row or the slots do not suffice nothing is taken or
  * returned: starts is 0, totals = held, every slot -1, and AF_STATUS_CAPACITY
- * is set.
+ * is set. The same, with AF_STATUS_BOUNDS, when a number is negative, the range
+ * is none of the ring's, or an entry to be taken or returned is negative (no
+ * page). A negative entry among those that a request holds and keeps gives its
+ * tokens slot -1 and sets AF_STATUS_BOUNDS. pool >= 1, also where no page moves.
  */
 int af_block_tables(int32_t* tables, int64_t tables_stride, int64_t max_pages, const int32_t* held, const int32_t* lengths,
                     const int32_t* grow, int64_t batch, int32_t* free_pages, int64_t pool, const int64_t* free_range,

@@ -203,6 +203,49 @@ def test_block_tables_that_do_not_fit_change_nothing(why):
         st.check_status()
 
 
+@pytest.mark.parametrize("where", ["taken", "returned", "last returned"])
+@pytest.mark.parametrize("batch", [3, 1500])
+def test_block_tables_with_an_entry_that_is_no_page_change_nothing(where, batch):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import block_tables
+
+    rng = np.random.default_rng(5)
+    page = 8
+    held = [20, 0, 33] * (batch // 3)
+    kept, grow = [18, 0, 3] * (batch // 3), [9, 25, 2] * (batch // 3)  # of three requests one grows, one is new, one gives pages back
+    tables, ring, head, tail = _pool(batch, 6, held, page, 5 * batch, rng, 7)
+    pool = len(ring)
+    if where == "taken":
+        ring[(head + 2 * batch // 3) % pool] = -1
+    elif where == "returned":
+        tables[2][3] = -3
+    else:
+        tables[batch - 1][4] = -1
+    tt, rr, st = _i32(tables), _i32(ring), DeviceStatus()
+    got = block_tables(tt, _i32(kept), _i32(grow), rr, torch.tensor([head, tail], device="cuda"), page, sum(grow), held=_i32(held), status=st)
+    assert tt.tolist() == tables and rr.tolist() == ring and got.free_range.tolist() == [head, tail]
+    assert set(got.starts.tolist()) == {0} and got.totals.tolist() == held and set(got.slots.tolist()) == {-1}
+    with pytest.raises(RuntimeError):
+        st.check_status()
+
+
+def test_block_tables_report_a_held_entry_that_is_no_page():
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import block_tables
+
+    # The page that request 0 goes on in is missing; request 1 is sound.
+    tables, ring, st = _i32([[4, -1, -1], [2, -1, -1]]), _i32([5, 6, 7]), DeviceStatus()
+    got = block_tables(tables, _i32([12, 6]), _i32([6, 3]), ring, torch.tensor([0, 3], device="cuda"), 8, 9, status=st)
+    assert got.slots.tolist() == [-1] * 4 + [40, 41, 22, 23, 48] and got.totals.tolist() == [18, 9]
+    assert tables.tolist() == [[4, -1, 5], [2, 6, -1]] and got.free_range.tolist() == [2, 3]
+    with pytest.raises(RuntimeError):
+        st.check_status()
+    # An entry in front of the kept tokens' last page is not looked at.
+    tables = _i32([[-1, 3]])
+    assert block_tables(tables, _i32([9]), _i32([2]), ring, torch.tensor([0, 3], device="cuda"), 8, 2, status=st).slots.tolist() == [25, 26]
+    st.check_status()
+
+
 def test_block_tables_over_many_steps_keep_every_page_once():
     from actfold_b200.speculative import block_tables
 
