@@ -55,9 +55,10 @@ class AcceptedPath(NamedTuple):
 
 
 # These calls are short, so what the host does per call counts: plain
-# comparisons, no helper objects, and the stream's handle without a Stream object.
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# comparisons, no helper objects, and the stream's handle without a Stream object
+# (where torch has these two names; it need not: one built without CUDA has neither).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _lib.stream_ptr)
 
 
 def _launch(what: str, index: int, fn, *args) -> None:

@@ -69,6 +69,21 @@ def test_masks_report_bad_trees_and_do_the_others():
         st2.check_status()
 
 
+def test_masks_with_torchs_public_names_of_device_and_stream(monkeypatch):
+    from actfold_b200 import _lib
+    from actfold_b200 import tree_kernels as T
+
+    monkeypatch.setattr(T, "_current_device", torch.cuda.current_device)
+    monkeypatch.setattr(T, "_current_stream", _lib.stream_ptr)
+    parents, starts = _i32([-1, 0, 1]), _i32([0, 3])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        mask, _ = T.tree_masks(parents, starts, 1)
+    s.synchronize()
+    assert mask[:, 0].tolist() == [1, 3, 7]
+
+
 # ------------------------------------------------------------------------------------------------ acceptance
 @pytest.mark.parametrize("ns,keep,vocab,with_root", [([26], 6, 3, True), ([1, 0, 7, 300], 4, 2, True), ([40, 41], 64, 1, True),
                                                      ([300, 5], 300, 1, False), ([9, 0, 12], 1, 2, False), ([600], 8, 5, True)])

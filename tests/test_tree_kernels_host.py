@@ -4,6 +4,8 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -209,3 +211,15 @@ def test_a_status_on_another_device_is_refused(monkeypatch):
                          lambda: S.tree_attention(rows, rows, rows, cache, cache, z(2, 2), z(2), z(3), status=st)):
                 with pytest.raises(error, match="cuda:0|CUDA device"):
                     call()
+
+
+def test_host_classes_import_where_torch_has_no_cuda_names():
+    """A torch without CUDA has neither name; the trees and policies of a host need none of them."""
+    code = ("import torch\n"
+            "for name in ('_cuda_getDevice', '_cuda_getCurrentRawStream'):\n"
+            "    delattr(torch._C, name)\n"
+            "from actfold_b200.speculative import BranchNode, BranchTree, GreedyAcceptancePolicy\n"
+            "GreedyAcceptancePolicy()\n"
+            "assert BranchTree(BranchNode('r', None, torch.tensor([[1]]))).packed()[0] == []\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr
