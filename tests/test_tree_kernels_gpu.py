@@ -84,6 +84,12 @@ def test_masks_with_torchs_public_names_of_device_and_stream(monkeypatch):
     assert mask[:, 0].tolist() == [1, 3, 7]
 
 
+@pytest.mark.parametrize("ns,words", [([1200, 5, 1100], 38), ([1025, 0, 2000, 1], 64), ([31, 1056, 32], 33)])
+def test_masks_of_branching_trees_with_more_than_32_words(ns, words):
+    """Rows that go straight out: every word of every row, the zero ones among them, of several trees."""
+    test_masks_and_positions(ns, words)
+
+
 # ------------------------------------------------------------------------------------------------ acceptance
 @pytest.mark.parametrize("ns,keep,vocab,with_root", [([26], 6, 3, True), ([1, 0, 7, 300], 4, 2, True), ([40, 41], 64, 1, True),
                                                      ([300, 5], 300, 1, False), ([9, 0, 12], 1, 2, False), ([600], 8, 5, True)])
@@ -729,6 +735,72 @@ def test_attention_far_offsets():
         kc[y], vc[y] = args["k_cache"][x], args["v_cache"][x]
     args.update(k_cache=kc, v_cache=vc, tables=_i32([far]))
     _check(args, ([far], lengths, starts, bits))
+
+
+JOINED = [CASES[6], CASES[14], CASES[16], *CASES[17:20], *CASES[23:]]  # cases with rows that several SMs work on
+
+
+@pytest.mark.parametrize("case", JOINED)
+@pytest.mark.parametrize("junk", [0x7fc00000, 0x60ad78ec, -1, 0x3f800000])  # NaN, 1e20, all ones, 1
+def test_attention_writes_all_of_its_scratch_that_it_reads(case, junk, monkeypatch):
+    """The scratch memory is this test's own, filled with junk, and nothing behind its end is written."""
+    from actfold_b200 import tree_kernels as T
+
+    args, _ = _case(*case[:7], seed=2, kind=case[7])
+    want = T.tree_attention(**args)
+    size = T._workspace_bytes(0)
+    scratch = torch.full((size // 4 + 64,), junk, dtype=torch.int32, device="cuda")
+    launch, used = T._launch, []
+
+    def with_own_scratch(what, index, fn, packed, *rest):
+        fields = list(T._ATTENTION.unpack(packed))
+        assert fields[-1] == size
+        fields[-2] = scratch.data_ptr()
+        used.append(what)
+        launch(what, index, fn, T._ATTENTION.pack(*fields), *rest)
+
+    monkeypatch.setattr(T, "_launch", with_own_scratch)
+    got = T.tree_attention(**args)
+    assert used == ["tree_attention"] and torch.equal(got, want)
+    assert scratch[size // 4:].eq(junk).all() and not scratch[: size // 4].eq(junk).all()
+
+
+def test_attention_of_many_requests_with_trees():
+    rng = np.random.default_rng(9)
+    lengths, ns = rng.integers(0, 700, 300).tolist(), rng.integers(0, 41, 300).tolist()
+    _check(*_case(lengths, ns, 4, 2, 64, 16, torch.bfloat16))
+
+
+def test_attention_on_two_streams_at_once_and_from_two_graphs():
+    """Different inputs on each stream, calls in flight together; then the same from a graph each."""
+    from actfold_b200.speculative import tree_attention
+
+    cases = [_case([3000, 800], [64, 20], 8, 4, 128, 16, torch.bfloat16, seed=1)[0], _case([9000], [3], 8, 2, 128, 64, torch.float16, seed=2)[0],
+             _case([2000, 77], [100, 90], 4, 4, 128, 32, torch.bfloat16, seed=3)[0]]
+    want = [tree_attention(**a) for a in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[] for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for s, a, g in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                g.append(tree_attention(**a))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w, x) for x in g)
+    graphs, outs = [], []
+    for a in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(tree_attention(**a))
+        graphs.append(graph)
+    for _ in range(10):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, x) for w, x in zip(want, outs))
 
 
 @pytest.fixture
