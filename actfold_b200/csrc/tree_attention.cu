@@ -55,19 +55,18 @@ struct Shape {
   static constexpr int kS = 4;                      // S buffers in TMEM
   static constexpr int kTmem = (kS + 2 * kPipes) * N <= 256 ? 256 : 512;  // S, then O [2 segments][kPipes]
   static constexpr int kHalves = HD / 64;
-  static constexpr int kPitch = N < 64 ? 2 * N : 128;         // bytes of a key's row of P^T (blocks of 64 rows where there are more)
-  static constexpr int kPBytes = (N < 64 ? 1 : N / 64) * kKeys * kPitch;
-  static constexpr int kKBytes = kHalves * kHalf > kPBytes ? kHalves * kHalf : kPBytes;
+  static constexpr int kPitch = 2 * N;                        // bytes of a key's row of P^T
+  static constexpr int kKBytes = kHalves * kHalf;             // (P^T, at most kHalf, goes over them)
   static constexpr int kStage = kKBytes + kHalves * kHalf;
   // At most kS, so that P of a tile is taken before P of the tile that uses the same barrier can be there: no wait is ever
   // two phases behind its barrier.
   static constexpr int kStages = (192 * 1024) / kStage < kS ? (192 * 1024) / kStage : kS;
   static constexpr int kQBytes = kHalves * N * 128;
-  static constexpr int kQ = kQBytes <= 16384 ? 2 : 1;         // Q buffers
+  static constexpr int kQ = 2;                                // Q buffers
   // V lies before K: the second product always takes 128 dims, so with 64 it reads the 16 KB behind V too (for lanes of O
   // that nobody looks at), and those have to be there.
   static constexpr int kOffV = 0, kOffK = kHalves * kHalf, kKStages = kStages, kVStages = kStages, kQTiles = 1, kQRows = N;
-  static_assert(kOffK + kKBytes == kStage && kKBytes >= kHalf, "what the second product reads lies in its stage");
+  static_assert(N <= 64 && kOffK + kKBytes == kStage && kKBytes >= kHalf, "what the second product reads lies in its stage");
   static constexpr int kOffQ = kStages * kStage;
   static constexpr int kOffM = kOffQ + kQ * kQBytes;          // [kPipes][N] reference maxima, negated; then the factors of O
   static constexpr int kOffRed = kOffM + kPipes * N * 4;      // [kPipes][4][N] per-warp maxima or sums
@@ -78,16 +77,16 @@ struct Shape {
 };
 
 // P^T [128 keys][N rows] in shared memory: rows of kPitch bytes whose 16-byte
-// pieces are swizzled over as many bytes (32, 64 or 128), N >= 64 as blocks of 64.
+// pieces are swizzled over as many bytes (32, 64 or 128).
 template <int N>
 __device__ __forceinline__ uint64_t p_desc(uint32_t at) {
-  constexpr uint64_t pitch = N < 64 ? 2 * N : 128, swizzle = N == 16 ? 6 : N == 32 ? 4 : 2;
+  constexpr uint64_t pitch = 2 * N, swizzle = N == 16 ? 6 : N == 32 ? 4 : 2;
   return (uint64_t)((at & 0x3ffffu) >> 4) | (uint64_t)(kHalf >> 4) << 16 | (8 * pitch >> 4) << 32 | (uint64_t)1 << 46 | swizzle << 61;
 }
 template <int N>
 __device__ __forceinline__ uint32_t p_piece(int key, int col) {  // byte offset of columns col .. col + 7 (a multiple of 8)
-  constexpr int pieces = N < 64 ? N / 8 : 8, shift = N == 16 ? 2 : N == 32 ? 1 : 0;
-  return col / 64 * kHalf + key * (16 * pieces) + 16 * ((col / 8 % pieces) ^ ((key >> shift) % pieces));
+  constexpr int pieces = N / 8, shift = N == 16 ? 2 : N == 32 ? 1 : 0;
+  return key * (16 * pieces) + 16 * ((col / 8) ^ ((key >> shift) % pieces));
 }
 
 // Lane i's 32 bits become bit i of every lane's word.
@@ -105,9 +104,8 @@ template <int P, int N, int W>
 __device__ __forceinline__ void tmem_load_rows(uint32_t taddr, uint32_t* r) {
 #define AF_LD4(a, b) "tcgen05.ld.sync.aligned.32x32b.x4.b32 {" a "}, [" b "];\n\t"
 #define AF_LD8(a, b) "tcgen05.ld.sync.aligned.32x32b.x8.b32 {" a "}, [" b "];\n\t"
-  if constexpr (P == 1) {
-    tmem_load<8>(taddr, r);
-  } else if constexpr (P == 2) {
+  static_assert((P == 2 && W == 8) || P == 4, "pipes");
+  if constexpr (P == 2) {
     asm volatile(AF_LD8("%0,%1,%2,%3,%4,%5,%6,%7", "%16") AF_LD8("%8,%9,%10,%11,%12,%13,%14,%15", "%17") "tcgen05.wait::ld.sync.aligned;"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
                    "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
