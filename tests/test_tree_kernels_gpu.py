@@ -765,6 +765,33 @@ def test_attention_writes_all_of_its_scratch_that_it_reads(case, junk, monkeypat
     assert scratch[size // 4:].eq(junk).all() and not scratch[: size // 4].eq(junk).all()
 
 
+@pytest.mark.parametrize("heads", [4, 64])  # narrow tiles and wide ones
+def test_attention_with_a_mask_of_ones(heads):
+    """Every bit of every word is set, those behind a tree's last node too: a node sees its own tree and nothing else."""
+    ns = [33, 1, 7, 40]
+    args, (tables, lengths, starts, _) = _case([100, 0, 300, 64], ns, heads, 2, 64, 16, torch.bfloat16)
+    args["mask"] = torch.full((sum(ns), 3), -1, dtype=torch.int32, device="cuda")
+    _check(args, (tables, lengths, starts, [torch.ones(n, n, dtype=torch.bool) for n in ns]))
+
+
+def test_attention_of_the_most_requests():
+    """16384 requests of one token (every seventh has none), a few keys each."""
+    rng = np.random.default_rng(4)
+    lengths, ns = rng.integers(0, 40, 16384).tolist(), [int(i % 7 > 0) for i in range(16384)]
+    args, plain = _case(lengths, ns, 2, 1, 64, 8, torch.bfloat16, kind="chain")
+    from actfold_b200.speculative import tree_attention
+
+    out = tree_attention(**args)
+    starts, some = plain[2], [0, 1, 2, 8, 5000, 11111, 16382, 16383]
+    for b in some:
+        if ns[b]:
+            row = slice(starts[b], starts[b + 1])
+            ref, _, tol, _ = U.attention(args["q"][row], args["k"][row], args["v"][row], args["k_cache"], args["v_cache"], [plain[0][b]], [lengths[b]],
+                                         [0, 1], [None])
+            assert bool(((out[row].double() - ref).abs() <= tol).all()), b
+    assert out.isfinite().all()
+
+
 def test_attention_of_many_requests_with_trees():
     rng = np.random.default_rng(9)
     lengths, ns = rng.integers(0, 700, 300).tolist(), rng.integers(0, 41, 300).tolist()
