@@ -73,7 +73,7 @@ struct Shape {
   static constexpr int kOffBar = kOffRed + kPipes * 4 * N * 4;
   static constexpr int kBars = 3 * kStages + 4 + 3 * kS + 4 + kPlans + 1;
   static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
-  static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
+  static constexpr int kBytes = kOffPlan + kPlans * 48 + 32;
 };
 
 // P^T [128 keys][N rows] in shared memory: rows of kPitch bytes whose 16-byte
@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
   Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* found = tmem_slot + 4;  // of even and of odd segments: tiles with values that are not finite
   static_assert(sizeof(Segment) == 48, "plans");
 
   if (tid == 0) {
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
     mbar_init(drained, 2);
     failed[0] = 0;
     failed[1] = p.patience;
+    found[0] = found[1] = 0;
     fence_barrier_init();
   }
   if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
@@ -325,7 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
 #pragma unroll
       for (int i = 0; i < C / 2; ++i) l[i] = 0ull;
       if (team_tid < C) m_neg[team_tid] = -kUnset;
-      bool sick = false, begun = false;  // a drafted value that is not finite was set aside; this pipe's O holds something
+      uint32_t sick = 0;   // tiles whose drafted values that are not finite were set aside (see found_shift)
+      bool begun = false;  // this pipe's O holds something
       named_bar_sync(team, kTeam);
       const int tiles = s.k1 - s.k0;
 #pragma unroll 1
@@ -368,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
                 bad |= lo || hi;
               }
               if (bad) {
-                sick = true;
+                sick |= 1u << (i0 >> found_shift(tiles));
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(c16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
               }
             }
@@ -483,7 +486,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
         const float sum = transpose_reduce<C>(y, lane, [](float a, float b) { return a + b; });
         red[red_at] = sum;
       }
-      const bool set_aside = vote_any<kSoft * 32>(5, sick);  // (and the sums are there)
+      if (sick) atomicOr(found + (seg & 1), sick);
+      const bool set_aside = vote_any<kSoft * 32>(5, sick != 0);  // (and the sums are there)
+      if (tid == 0) found[(seg + 1) & 1] = 0;  // (read last before this segment was entered)
       if (tid < cols) {
         float m = kUnset, sum = 0.f, f[S::kPipes];
 #pragma unroll
@@ -536,9 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention(const __grid_con
             }
           }
           if (set_aside) {
-            const int x0 = max(0, s.k0 * kKeys - s.pad), x1 = min(s.n, s.k1 * kKeys - s.pad);
             float more[kW];
-            set_aside_rows<DT, kW>(p, s.s0, s.kvh, s.node0, c8, min(o1, c8 + kW), x0, x1, r, more);
+            set_aside_rows<DT, kW>(p, plans + seg % kPlans, found + (seg & 1), c8, min(o1, c8 + kW), r, more);
 #pragma unroll
             for (int e = 0; e < kW; ++e) y[e] += more[e];
           }

@@ -49,7 +49,7 @@ struct Wide {
   static constexpr int kOffBar = kOffStat + 2 * kRows * 8;
   static constexpr int kBars = 2 * kKStages + 2 * kVStages + 2 + 12 + 2 + kPlans + 1;
   static constexpr int kOffPlan = (kOffBar + kBars * 8 + 15) / 16 * 16;
-  static constexpr int kBytes = kOffPlan + kPlans * 48 + 16;
+  static constexpr int kBytes = kOffPlan + kPlans * 48 + 32;
   static constexpr int kTmemO = 2 * kKeys;                           // O of pipe x at kTmemO + 128 x, S of pipe x at 128 x
 };
 
@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
   Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffPlan + kPlans * 48);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* found = tmem_slot + 4;  // of even and of odd segments: tiles with values that are not finite
 
   if (tid == 0) {
     for (int i = 0; i < S::kKStages; ++i) {
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
     mbar_init(drained, 2);
     failed[0] = 0;
     failed[1] = p.patience;
+    found[0] = found[1] = 0;
     fence_barrier_init();
   }
   if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), 512);
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
       const bool busy = 32 * quad < rows;  // any of the warp's rows is one
       float m = kUnset;
       uint64_t l0 = 0ull, l1 = 0ull;
-      bool sick = false;
+      uint32_t sick = 0;
 #pragma unroll 1
       for (int x2 = two ? 0 : 2 * pipe; x2 < 2 * tiles; x2 += two || !(x2 & 1) ? 1 : 3, ++taken) {
         const int t = x2 >> 1, half = x2 & 1, bar = 2 * pipe + half;  // a half of a tile at a time
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
                 bad |= lo || hi;
               }
               if (bad) {
-                sick = true;
+                sick |= 1u << (t >> found_shift(tiles));
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(c16)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
               }
             }
@@ -395,7 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
       const float2 la = unpair(add2(l0, l1));
       const float mine = la.x + la.y;
       stat[pipe * kRows + r] = make_float2(m, mine);
-      const bool set_aside = vote_any<kSoft * 32>(1, sick);  // (and both pipes' maxima and sums are there)
+      if (sick) atomicOr(found + (seg & 1), sick);
+      const bool set_aside = vote_any<kSoft * 32>(1, sick != 0);  // (and both pipes' maxima and sums are there)
+      if (tid == 0) found[(seg + 1) & 1] = 0;  // (read last before this segment was entered)
       float own = 1.f, other = 0.f, sum = mine;  // factors of this pipe's O and of the other one's
       if (!two) {
         const float2 y = stat[(1 - pipe) * kRows + r];
@@ -436,9 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tree_attention_wide(const __gri
           }
           if (r < rows) {
             if (set_aside) {
-              const int x0 = max(0, s.k0 * kKeys - s.pad), x1 = min(s.n, s.k1 * kKeys - s.pad);
               float more[8];
-              set_aside_dims<DT>(p, s.s0, s.kvh, node, x0, x1, d, more);
+              set_aside_dims<DT>(p, plans + seg % kPlans, found + (seg & 1), node, d, more);
 #pragma unroll
               for (int i = 0; i < 8; ++i) y[i] += more[i];
             }
