@@ -27,13 +27,14 @@
 // barrier vote, no maximum across lanes. P then stays below 2^8 (2^15 in fp16, see
 // kLead), rounded to 16 bits for the tensor cores: half a step of the type per
 // probability. Sums and O are fp32. Every wait is
-// bounded; a timeout sets AF_STATUS_TIMEOUT.
+// bounded; a timeout sets AF_STATUS_TIMEOUT and all warps leave: the ones that meet at
+// barriers by a common vote before each row (0.2 us of a call).
 //
 // Measured on B200 (128 dims, joins included): 64 requests of one token over 90 to
-// 8000 keys, 28 heads over 4: 91.7 us, 5.8 TB/s of the 6.55 that a copy reaches. 8 trees of 20 to
-// 64 nodes over 300 to 4100 keys, 32 heads: 78.1 us (4.2 TB/s; every row's end, some 9000
-// cycles of masks, joins and output, drains the pipeline). One token over 523 keys: 12.3
-// us, all of it latency (plan, page table, first tile, five tiles, output).
+// 8000 keys, 28 heads over 4: 92.2 us, 5.8 TB/s of the 6.55 that a copy reaches. 8 trees of 20 to
+// 64 nodes over 300 to 4100 keys, 32 heads: 78.8 us (4.2 TB/s; at every row's end the softmax warps,
+// which write the output too, spend some 9000 cycles that no next row overlaps). One token over 523 keys:
+// 12.6 us, all of it latency (plan, page table, first tile, five tiles, output) on 4 of the SMs.
 #include "tree_attention.cuh"
 
 namespace af {
@@ -762,8 +763,9 @@ extern "C" int af_tree_attention(const af_tree_attention_args* args, uint32_t* s
   const int box = (int)(a.page_size % 32 == 0 ? 32 : a.page_size % 16 == 0 ? 16 : 8);
   p.nt_q = (n == 256 ? 128 : n) / group;
   p.nt = n == 256 ? 2 * p.nt_q : p.nt_q;
-  // Measured: a row end costs some 1800 cycles of 2700 a tile with 16 rows, 9000 of 2900 with 64, 8000 of 4500 with 256; 32
-  // rows, which were not, take a value between.
+  // Measured: a row end costs some 1800 cycles of 2700 a tile with 16 rows, 9000 of 2900 with 64, 8000 of 4500 with 256. With
+  // 32 rows, 1 / 2 / 3 / 4 key tiles a row end: 32 requests of 28 rows over 300 to 4100 keys 56.7 / 55.2 / 53.9 / 52.4 us, 8
+  // requests of 20 to 30 rows, 32 heads 92.3 / 91.4 / 82.7 / 72.8 us: 2 is low for them.
   p.row_cost = n == 16 ? 1 : n == 64 ? 3 : 2;
   // Tiles are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
   AF_REQUIRE((double)a.n_kv_heads * (ceil_div(a.total, p.nt) + a.batch) * ((a.max_pages * a.page_size + a.total) / kKeys + 2 + p.row_cost) < 2147483000.0,

@@ -18,9 +18,9 @@
 // the narrow kernel. Half of the exponentials as a polynomial on the multiply-add pipe made it
 // slower (282 us).
 //
-// Measured on B200: that case 252 to 259 us in bursts (0.70 PFLOP/s), 292 to 296 us in long runs at
-// the 1 kW power cap; ncu shows the tensor cores busy 39 %, the exponentials 39 %, DRAM
-// 33 % (keys are read once per 256 rows): the chain of softmax, P V and Q K of two pipes bounds it.
+// Measured on B200: that case 250 to 258 us in bursts (0.70 PFLOP/s), 291 to 296 us in long runs at
+// the 1 kW power cap; ncu shows the tensor cores busy 40 %, the exponentials 40 %, DRAM
+// 34 % (keys are read once per 256 rows): the chain of softmax, P V and Q K of two pipes bounds it.
 //
 // Warps 0-3 and 4-7: softmax of pipe 0 and 1; warp 8 loads Q and K, warp 9 V,
 // warp 10 issues S, warp 11 plans and issues O.

@@ -340,7 +340,8 @@ def tree_attention(
     words] int32, see :func:`tree_masks`; any bits are allowed, so a block that
     sees itself in both directions is a mask of ones). ``mask`` None: each
     tree is a chain, in which a node sees the nodes up to itself (a single new
-    token, or a prompt behind a cached prefix). ``scale`` defaults to dim **
+    token, or a prompt behind a cached prefix; the work of a long one is that of a
+    full square, about twice what its nodes see). ``scale`` defaults to dim **
     -0.5. A row that sees nothing is 0. ``lse`` [nodes, heads] float32 receives the
     natural log of each row's sum of exponentials. Rows of ``out`` behind ``starts[-1]`` are not written,
     none when ``starts`` is out of order. ``out`` shares no memory with the inputs.
