@@ -855,7 +855,7 @@ def _one_long_chain(n, heads, kv, dim, batch):
 @pytest.mark.parametrize("group", [1, 4, 8, 16])  # tiles of 16, 32 and 64 rows, and the wide kernel
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_whose_waits_run_out_ends_with_a_status(group, dim, wait_limit):
-    """Values that are not finite make the ends of rows long (every node is looked through for them): with a limit of one
+    """Values that are not finite make the ends of rows long (their tiles are looked through for them): with a limit of one
     attempt the other warps' waits run out in the middle. The call ends and says so, and the next one is as always."""
     from actfold_b200.kernels import DeviceStatus
     from actfold_b200.speculative import tree_attention
@@ -864,7 +864,7 @@ def test_attention_whose_waits_run_out_ends_with_a_status(group, dim, wait_limit
     args, _ = _one_long_chain(n, 2 * group, 2, dim, n // 8)
     want = tree_attention(**args)
     sick = dict(args, v=args["v"].clone())
-    sick["v"][0], sick["v"][n - 1] = float("inf"), float("inf")
+    sick["v"][::100] = float("inf")  # in every tile
     st = DeviceStatus()
     torch.cuda.synchronize()
     wait_limit(0)
