@@ -53,6 +53,9 @@ SIGNATURES: dict[str, tuple] = {
     "af_tree_attention": (_i32, [_vp, _vp, _vp]),
     "af_tree_attention_workspace_bytes": (_i32, [_vp]),
     "af_tree_attention_wait_limit": (_i32, [_i64]),
+    "af_write_cache_int4": (_i32, [_vp, _vp, _vp]),
+    "af_read_cache_int4": (_i32, [_vp, _vp, _vp]),
+    "af_evict_cache": (_i32, [_vp, _vp, _vp]),
 }
 
 _lib = None

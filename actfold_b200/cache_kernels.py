@@ -1,0 +1,252 @@
+"""Long requests in less memory: a paged key/value cache in 4 bits, windowed attention over it, and eviction.
+
+Next to the 16-bit cache of :mod:`actfold_b200.tree_kernels`, with the same
+pages, tables and slots (:func:`~actfold_b200.tree_kernels.block_tables` serves both):
+
+* :class:`Int4Cache` holds keys and values in 4 bits, with a 16-bit scale and offset for every 32 dims:
+  160 bytes a token and head of 128 dims instead of 512;
+* :func:`write_cache_int4` and :func:`read_cache_int4` move rows into their slots and back;
+* :func:`tree_attention_int4` is tree attention over it, with an optional sliding window and first tokens ("sinks") that stay visible;
+* :func:`attention_weights` adds up the attention that every cached token is given, in either cache;
+* :func:`evict_cache` keeps, of a request that has outgrown its budget, the tokens that were given the most, in either cache.
+
+No call synchronises; sizes that change from step to step stay on the device,
+so a step can be captured into a CUDA graph. Pass a
+:class:`~actfold_b200.kernels.DeviceStatus` on the tensors' device to learn of
+values that the kernels found out of range. Each call is ordered on the
+current stream of its tensors' device; its scratch comes from torch's
+allocator on that stream.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import struct
+from typing import NamedTuple
+
+import torch
+
+from actfold_b200 import _lib
+from actfold_b200.kernels import DeviceStatus
+from actfold_b200.tree_kernels import _launch, _not_vectors, _same_device, _word
+
+_I32, _I64 = torch.int32, torch.int64
+_CACHE = "q3q6q"
+_ROWS = struct.Struct("2q3q3q2q2q" + _CACHE)
+_EVICT = struct.Struct(_CACHE + "2q4q4q5q3q2qq3qq3q3q")
+_NO_CACHE = (0,) * 10
+
+
+class Int4Cache:
+    """A paged key/value cache in 4 bits.
+
+    ``data`` is uint8 [pages, kv_heads, page_size / 8, 10 * dim], or with a leading dimension of layers, dim 64 or 128; ``dtype``
+    (fp16 or bf16) is that of the rows that go in and come out, and of the scales and offsets. Its last two dimensions are
+    contiguous, its other strides multiples of 16 bytes. :meth:`empty` makes one; ``cache[l]`` is layer l. The pages hold what
+    :func:`write_cache_int4` wrote; places that were never written are never used.
+    """
+
+    __slots__ = ("data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
+
+    def __init__(self, data: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> None:
+        if data.dtype is not torch.uint8 or data.dim() not in (4, 5) or data.shape[-1] not in (640, 1280):
+            raise ValueError(f"Int4Cache: data must be uint8 [(layers,) pages, kv_heads, page_size / 8, 640 or 1280], got {data.dtype} {tuple(data.shape)}")
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
+            raise ValueError(f"Int4Cache: dtype must be fp16 or bf16, got {dtype}")
+        *outer, blocks, size = data.shape
+        if blocks == 0:
+            raise ValueError("Int4Cache: page_size must be positive")
+        strides = list(data.stride())
+        if strides[-1] != 1 or (blocks > 1 and strides[-2] != size):
+            raise ValueError("Int4Cache: the blocks of a page's head must be contiguous")
+        outer_strides = [0 if n <= 1 else s for n, s in zip(outer, strides)]
+        if any(s <= 0 and n > 1 for n, s in zip(outer, outer_strides)):
+            raise ValueError("Int4Cache: data has entries that share memory")
+        if any(s & 15 for s in outer_strides) or data.data_ptr() & 15:
+            raise ValueError("Int4Cache: data's address and strides must be multiples of 16 bytes")
+        self.data, self.dtype, self.dim = data, dtype, size // 10
+        self.layers = outer[0] if len(outer) == 3 else None
+        self.pages, self.kv_heads = outer[-2], outer[-1]
+        self.page_size = 8 * blocks
+        if self.layers is None:
+            outer_strides = [0, *outer_strides]
+        self._packed = (data.data_ptr(), *outer_strides, 1 if self.layers is None else self.layers, self.pages, self.page_size, self.kv_heads, self.dim,
+                        _lib.DTYPE[dtype])
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, dtype: torch.dtype = torch.bfloat16, layers: int | None = None,
+              device: torch.device | str = "cuda") -> "Int4Cache":
+        """A cache with nothing in it."""
+        if page_size <= 0 or page_size % 8 or dim not in (64, 128) or pages < 0 or kv_heads <= 0:
+            raise ValueError(f"Int4Cache: page_size {page_size} must be a positive multiple of 8, dim {dim} 64 or 128, pages and kv_heads positive")
+        shape = (pages, kv_heads, page_size // 8, 10 * dim)
+        return cls(torch.empty(shape if layers is None else (layers, *shape), dtype=torch.uint8, device=device), dtype)
+
+    def __getitem__(self, layer: int) -> "Int4Cache":
+        if self.layers is None:
+            raise ValueError("Int4Cache: the cache has no layers")
+        return Int4Cache(self.data[layer], self.dtype)
+
+
+class EvictedCache(NamedTuple):
+    """Result of :func:`evict_cache` (device tensors)."""
+
+    lengths: torch.Tensor  # [requests] int32: tokens that are left
+    kept: torch.Tensor     # [(layers,) requests, kv_heads, keep] int32: the places that they came from, -1 behind the last
+    weights: torch.Tensor  # like the call's weights: theirs, 0 behind the last
+
+
+def _row_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
+    """Strides in bytes of 16-bit rows [layers, n, heads, dim], or None where they or the address are not multiples of 16."""
+    e = t.element_size()
+    a, b, c, d = t.stride()
+    if (d != 1 and t.shape[3] > 1) or t.data_ptr() & 15:
+        return None
+    out = tuple(0 if n <= 1 else s * e for n, s in zip(t.shape, (a, b, c)))
+    return None if any(s & 15 for s in out) else out
+
+
+def write_cache_int4(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: Int4Cache,
+    slots: torch.Tensor,
+    rows: torch.Tensor | None = None,
+    status: DeviceStatus | None = None,
+) -> None:
+    """Write key and value rows into their slots of a 4-bit cache, in place.
+
+    ``k``, ``v`` [n, kv_heads, dim], or with the cache's leading dimension of layers that share the slots, of the cache's dtype
+    and any strides. Entry i puts row ``rows[i]`` (``rows`` None: row i) into ``slots[i]`` (page * page_size + offset, as
+    :func:`~actfold_b200.tree_kernels.block_tables` gives them); entries with a negative slot or row are skipped. ``slots`` int64
+    and ``rows`` int32 may have any shape, the same one. Live slots must differ from one another. Of every 32 dims of a row the
+    smallest value is kept as it is, the others lie within half a step of a fifteenth of their range (and the rounding to dtype);
+    32 dims with a value that is not finite become NaN throughout.
+    """
+    layered = cache.layers is not None
+    if v.shape != k.shape or k.dim() != (4 if layered else 3) or k.shape[-2:] != (cache.kv_heads, cache.dim) or (layered and k.shape[0] != cache.layers):
+        raise ValueError(f"write_cache_int4: k, v {tuple(k.shape)}, {tuple(v.shape)} do not match a cache {tuple(cache.data.shape)}")
+    if k.dtype is not cache.dtype or v.dtype is not cache.dtype:
+        raise ValueError(f"write_cache_int4: rows {k.dtype}, {v.dtype} differ from the cache's {cache.dtype}")
+    if slots.dtype is not _I64 or (rows is not None and (rows.dtype is not _I32 or rows.shape != slots.shape)):
+        raise ValueError("write_cache_int4: slots must be int64, rows int32 of the same shape")
+    if not layered:
+        k, v = k[None], v[None]
+    n, count = k.shape[1], slots.numel()
+    if rows is None and count > n:
+        raise ValueError(f"write_cache_int4: {count} slots for {n} rows")
+    index = _same_device("write_cache_int4", k, v, cache.data, slots, rows, word := _word(status))
+    if (ks := _row_strides(k)) is None:
+        k = k.clone(memory_format=torch.contiguous_format)
+        ks = _row_strides(k)
+    if (vs := _row_strides(v)) is None:
+        v = v.clone(memory_format=torch.contiguous_format)
+        vs = _row_strides(v)
+    slots = slots.contiguous()
+    if rows is not None:
+        rows = rows.contiguous()
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *ks, *vs, slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n, count, *cache._packed)
+    _launch("write_cache_int4", index, _lib.load().af_write_cache_int4, args, _lib.ptr(word))
+
+
+def read_cache_int4(
+    cache: Int4Cache,
+    slots: torch.Tensor,
+    status: DeviceStatus | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values [(layers,) *slots.shape, kv_heads, dim] of the cache's dtype that lie in ``slots`` (int64; negative ones read as 0)."""
+    if slots.dtype is not _I64:
+        raise ValueError(f"read_cache_int4: slots must be int64, got {slots.dtype}")
+    index = _same_device("read_cache_int4", cache.data, slots, word := _word(status))
+    slots = slots.contiguous()
+    outer = () if cache.layers is None else (cache.layers,)
+    k, v = (torch.empty((*outer, *slots.shape, cache.kv_heads, cache.dim), dtype=cache.dtype, device=slots.device) for _ in range(2))
+    count, row = slots.numel(), 2 * cache.kv_heads * cache.dim
+    st = (count * row, row, 2 * cache.dim)
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *st, *st, slots.data_ptr(), 0, count, count, *cache._packed)
+    _launch("read_cache_int4", index, _lib.load().af_read_cache_int4, args, _lib.ptr(word))
+    return k, v
+
+
+def _check_tables(what: str, tables: torch.Tensor, lengths: torch.Tensor) -> tuple[int, int]:
+    if tables.dim() != 2 or tables.dtype is not _I32:
+        raise ValueError(f"{what}: tables must be int32 [requests, max_pages], got {tables.dtype} {tuple(tables.shape)}")
+    if lengths.dtype is not _I32 or lengths.dim() != 1:
+        _not_vectors(what, _I32, lengths=lengths)
+    if lengths.shape[0] != tables.shape[0]:
+        raise ValueError(f"{what}: lengths must have one entry for each of {tables.shape[0]} requests")
+    return tables.shape
+
+
+def evict_cache(
+    cache: Int4Cache | tuple[torch.Tensor, torch.Tensor],
+    tables: torch.Tensor,
+    lengths: torch.Tensor,
+    weights: torch.Tensor,
+    keep: int,
+    sinks: int = 0,
+    recent: int = 0,
+    status: DeviceStatus | None = None,
+) -> EvictedCache:
+    """Of every request with more than ``keep`` cached tokens, keep those that were given the most attention.
+
+    ``cache`` is an :class:`Int4Cache` or the pair (k_cache, v_cache) of :func:`~actfold_b200.tree_kernels.write_cache` (any dtype),
+    in both cases with or without a leading dimension of layers; ``weights`` float32 [(layers,) requests, kv_heads, places], as
+    :func:`attention_weights` adds them up. For each layer, request and head by itself the first ``sinks`` tokens, the last
+    ``recent`` and, of those between, the ones with the largest weights stay (equal weights: the earlier tokens; NaN counts as the
+    largest), ``keep`` in all. They move, in their order, to the request's first ``keep`` places, in place, so lengths stay the
+    same for all layers and heads. Other requests stay as they are. The tables are not changed: a
+    :func:`~actfold_b200.tree_kernels.block_tables` call with ``lengths`` the result's and ``held`` the old ones returns the pages.
+    Keys are moved as they are, so they have to hold their positions (as rotated keys do); a window of
+    :func:`tree_attention_int4` counts places.
+    """
+    packed = isinstance(cache, Int4Cache)
+    if not packed:
+        k_cache, v_cache = cache
+        if k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype or k_cache.dim() not in (4, 5):
+            raise ValueError(f"evict_cache: caches {k_cache.dtype} {tuple(k_cache.shape)} and {v_cache.dtype} {tuple(v_cache.shape)} do not match")
+        layered = k_cache.dim() == 5
+        if not layered:
+            k_cache, v_cache = k_cache[None], v_cache[None]
+        layers, pages, page, heads, dim = k_cache.shape
+        if page == 0:
+            raise ValueError("evict_cache: page_size must be positive")
+        e = k_cache.element_size()
+        strides = []
+        for t in (k_cache, v_cache):
+            if t.stride(4) != 1 and dim > 1:
+                raise ValueError("evict_cache: the innermost dimension of the caches must be contiguous")
+            st = [0 if n <= 1 else s * e for n, s in zip(t.shape[:4], t.stride()[:4])]
+            if any(s <= 0 and n > 1 for n, s in zip(t.shape[:4], st)):
+                raise ValueError("evict_cache: the caches have entries that share memory")
+            if any(s & 15 for s in st) or t.data_ptr() & 15 or dim * e & 15:
+                raise ValueError("evict_cache: the caches' rows and strides must be multiples of 16 bytes")
+            strides += st
+        held = (k_cache, v_cache)
+        parts = (*_NO_CACHE, k_cache.data_ptr(), v_cache.data_ptr(), *strides, layers, pages, page, heads, dim * e)
+    else:
+        layered, layers, heads = cache.layers is not None, 1 if cache.layers is None else cache.layers, cache.kv_heads
+        held = (cache.data, None)
+        parts = (*cache._packed, *((0,) * 15))
+    n, most = _check_tables("evict_cache", tables, lengths)
+    if weights.dtype is not torch.float32 or weights.dim() != (4 if layered else 3) or weights.shape[-3:-1] != (n, heads) \
+            or (layered and weights.shape[0] != layers):
+        raise ValueError(f"evict_cache: weights must be float32 [{'layers, ' if layered else ''}{n}, {heads}, places], got {weights.dtype} {tuple(weights.shape)}")
+    if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError(f"evict_cache: sinks {sinks} and recent {recent} must not be negative, and together not more than keep {keep}")
+    index = _same_device("evict_cache", *held, tables, lengths, weights, word := _word(status))
+    if most > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lengths = lengths.contiguous()
+    places = weights.shape[-1]
+    if places > 1 and weights.stride(-1) != 1:
+        weights = weights.contiguous()
+    kept = lengths.new_empty((*weights.shape[:-1], keep))
+    left, out = torch.empty_like(lengths), torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
+    if layers == 0 or heads == 0:
+        return EvictedCache(torch.clamp(lengths, max=keep), kept, out)
+    ws = weights.stride()
+    args = _EVICT.pack(*parts, tables.data_ptr(), tables.stride(0) if n > 1 else most, most, lengths.data_ptr(), n, weights.data_ptr(),
+                       *(ws[:3] if layered else (0, *ws[:2])), places, keep, sinks, recent, kept.data_ptr(), out.data_ptr(), left.data_ptr())
+    _launch("evict_cache", index, _lib.load().af_evict_cache, args, _lib.ptr(word))
+    return EvictedCache(left, kept, out)

@@ -1,0 +1,365 @@
+// Eviction of cached tokens by the attention weight that they were given (sm_100a).
+//
+// Every (layer, request, head) is a segment of its own. k_select finds, one CTA
+// per segment, the smallest weight that stays: a radix selection over the
+// weights' bits, 11, 11 and 10 of them at a time, each a histogram of the
+// tokens that still tie, and then writes the places that stay in order. k_move
+// brings their rows to the front, in place: row r comes from kept[r] >= r,
+// and a step stores rows that no later step loads, so between a step's loads
+// and its stores lies one barrier and nothing else; the loads of the next steps
+// are in flight meanwhile. Columns of a row are independent: keys and
+// values, and with few segments 64-byte pieces, are CTAs of their own, and
+// with fewer still a cluster shares each step's rows. Bound by HBM: every
+// moved byte is read and written once.
+#include <string>
+
+#include "int4_cache.cuh"
+#include "tree.cuh"
+
+namespace af {
+namespace kv_evict {
+namespace {
+
+struct SelectArgs {
+  const int* lengths;
+  const float* weights;
+  int64_t wl, wr, wh;  // strides: layer, request, head
+  int* kept;
+  float* weights_out;
+  int* lengths_out;
+  int batch, heads, places, keep, sinks, recent;
+  int64_t capacity;
+  unsigned* status;
+};
+
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32, kBins = 2048;
+
+// Ascending whole numbers for ascending weights; -0 equals 0, and NaN is above all numbers.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  if (isnan(w)) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(w + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
+  __shared__ int s_hist[kBins];
+  __shared__ int s_sum[2][kSelWarps];
+  __shared__ int s_bin, s_need;
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t seg = blockIdx.x;
+  const int h = (int)(seg % a.heads), b = (int)(seg / a.heads % a.batch);
+  const int64_t l = seg / a.heads / a.batch;
+  const int given = a.lengths[b];
+  const bool bad = given < 0 || given > a.capacity || given > a.places;
+  const int t = bad ? 0 : given;
+  const float* w = a.weights + l * a.wl + b * a.wr + h * a.wh;
+  int* kept = a.kept + seg * a.keep;
+  float* out = a.weights_out + seg * a.places;
+  if (tid == 0 && l == 0 && h == 0) {
+    a.lengths_out[b] = bad ? given : min(t, a.keep);
+    if (bad && a.status) atomicOr(a.status, AF_STATUS_BOUNDS);
+  }
+  if (t <= a.keep) {  // all stay
+    for (int i = tid; i < a.keep; i += kSelThreads) kept[i] = i < t ? i : -1;
+    for (int i = tid; i < a.places; i += kSelThreads) out[i] = i < t ? w[i] : 0.f;
+    return;
+  }
+  // The weights of places [lo, hi) decide; need of them stay (keep >= sinks + recent, t > keep: hi - lo > need).
+  const int lo = a.sinks, hi = t - a.recent, need0 = a.keep - a.sinks - a.recent;
+  uint32_t prefix = 0;
+  int need = need0;
+  if (need0 > 0) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : shift + (pass == 1 ? 11 : 10);
+      const uint32_t mask = pass == 2 ? 1023u : 2047u;
+      s_hist[tid] = s_hist[tid + kSelThreads] = 0;
+      __syncthreads();
+#pragma unroll 4
+      for (int i = lo + tid; i < hi; i += kSelThreads) {
+        const uint32_t k = order_of(w[i]);
+        if (pass == 0 || k >> above == prefix >> above) atomicAdd(&s_hist[(k >> shift) & mask], 1);
+      }
+      __syncthreads();
+      // Thread x has the bins 2047 - 2 x and 2046 - 2 x; from the top down, the one in which the need-th token lies.
+      const int c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
+      int upto = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      if (lane == 31) s_sum[0][warp] = upto;
+      __syncthreads();
+      int before = lane < warp ? s_sum[0][lane] : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      const int end = before + upto, begin = end - c0 - c1;
+      if (begin < need && need <= end) {
+        const bool first = need <= begin + c0;
+        s_bin = kBins - 1 - 2 * tid - (first ? 0 : 1);
+        s_need = need - begin - (first ? 0 : c0);
+      }
+      __syncthreads();
+      prefix |= (uint32_t)s_bin << shift;
+      need = s_need;
+    }
+  }
+  // Tokens above `prefix` stay, and the first `need` of those that equal it. In order: the number of certain ones and of equal
+  // ones before each, both in one word (a chunk has 1024 places).
+  int certain = 0, equal = 0;
+#pragma unroll 1
+  for (int i0 = 0, turn = 0; i0 < t; i0 += kSelThreads, turn ^= 1) {
+    const int i = i0 + tid;
+    const float x = i < t ? w[i] : 0.f;
+    const bool middle = i >= lo && i < hi;
+    const uint32_t k = order_of(x);
+    const bool sure = i < t && (!middle || (need0 > 0 && k > prefix)), tie = middle && need0 > 0 && k == prefix;
+    const uint32_t sures = __ballot_sync(0xffffffffu, sure), ties = __ballot_sync(0xffffffffu, tie);
+    if (lane == 0) s_sum[turn][warp] = __popc(sures) | __popc(ties) << 16;
+    __syncthreads();
+    const int all = s_sum[turn][lane];
+    int before = lane < warp ? all : 0, total = all;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    const uint32_t below = (1u << lane) - 1u;
+    const int sure_at = certain + (before & 0xffff) + __popc(sures & below), tie_at = equal + (before >> 16) + __popc(ties & below);
+    if (sure || (tie && tie_at < need)) {
+      const int at = sure_at + min(tie_at, need);
+      kept[at] = i;
+      out[at] = x;
+    }
+    certain += total & 0xffff;
+    equal += total >> 16;
+  }
+  for (int i = a.keep + tid; i < a.places; i += kSelThreads) out[i] = 0.f;
+}
+
+struct MoveArgs {
+  char *k, *v;                                      // 16-bit rows; 4 bits: k alone
+  int64_t kl, kp, kt, kh, vl, vp, vt, vh;           // byte strides: layer, page, token (16-bit rows), head
+  const int *tables, *lengths, *kept;
+  int64_t tables_ld, capacity;
+  int batch, heads, pages, page, places, keep;
+  int columns, pieces;                              // CTAs side by side of a row; pieces of 16 (of 4 bits and 64 dims: 8) bytes of each
+  uint32_t by_pieces;                               // p / pieces = p * by_pieces >> 20 for p < 2048, pieces <= 256
+  unsigned* status;
+};
+
+constexpr int kMoveThreads = 256, kPer = 8, kStages = 3;  // pieces of a thread and step; steps in flight
+constexpr int kStepPieces = kMoveThreads * kPer;
+
+template <int BYTES>
+__device__ __forceinline__ void copy_in(uint32_t dst, const char* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// HD = 0: rows of 16 bits (or any other) type; 64 or 128: 4-bit blocks of that many dims. CLUSTER CTAs share each step's rows.
+template <int HD, int CLUSTER>
+__global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
+  constexpr int kBytes = HD == 64 ? 8 : 16;
+  using B = kv4::Block<HD == 0 ? 64 : HD>;
+  extern __shared__ __align__(16) uint8_t buf[];
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int64_t item = blockIdx.x / CLUSTER;
+  const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
+  const int column = (int)(item % a.columns);
+  const int64_t seg = item / a.columns;
+  const int h = (int)(seg % a.heads), b = (int)(seg / a.heads % a.batch);
+  const int64_t l = seg / a.heads / a.batch;
+  const int t = a.lengths[b];
+  if (t <= a.keep || t > a.capacity || t > a.places) return;
+  const int* kept = a.kept + seg * a.keep;
+  const int* table = a.tables + b * a.tables_ld;
+  // Rows before the first gap stay where they are: kept[r] - r never falls.
+  int first = 0;
+  for (int n = a.keep; n > 0;) {
+    const int half = n / 2;
+    if (kept[first + half] == first + half) {
+      first += half + 1;
+      n -= half + 1;
+    } else {
+      n = half;
+    }
+  }
+  const int step_rows = kStepPieces / a.pieces * CLUSTER;  // of the cluster
+  const int steps = (a.keep - first + step_rows - 1) / step_rows;
+  char* base;
+  int64_t page_step, token_step = 0;
+  const int half = a.columns / 2;
+  if constexpr (HD == 0) {
+    const bool val = column >= half;
+    base = (val ? a.v + l * a.vl + h * a.vh : a.k + l * a.kl + h * a.kh) + (int64_t)(val ? column - half : column) * a.pieces * 16;
+    page_step = val ? a.vp : a.kp;
+    token_step = val ? a.vt : a.kt;
+  } else {
+    base = a.k + l * a.kl + h * a.kh + (int64_t)column * B::kPart;  // columns: keys and values
+    page_step = a.kp;
+  }
+  // Where piece `piece` of the token at `place` lies, or null.
+  auto locate = [&](int place, int piece) -> char* {
+    const int entry = place / a.page, off = place - entry * a.page, pg = table[entry];
+    if (pg < 0 || pg >= a.pages) return nullptr;
+    char* at = base + pg * page_step;
+    if constexpr (HD == 0) return at + off * token_step + piece * 16;
+    const int r = off % kv4::kBlockTokens;
+    at += (int64_t)(off / kv4::kBlockTokens) * B::kBytes;
+    return at + (piece == 4 ? B::pair(r, 0) : B::word(r, piece * (kBytes / 4)));
+  };
+  // Piece number u of this thread in a step: (row, piece) or row = keep.
+  auto mine = [&](int step, int u, int& row, int& piece) {
+    const int p = tid + kMoveThreads * u, q = (int)((uint32_t)p * a.by_pieces >> 20);
+    piece = p - q * a.pieces;
+    const int rows = kStepPieces / a.pieces;
+    row = q < rows ? min(a.keep, first + step * step_rows + rank * rows + q) : a.keep;
+  };
+  const uint32_t smem = smem_u32(buf);
+  bool bad = false;
+  auto load = [&](int step) {
+    if (step < steps) {
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        int row, piece;
+        mine(step, u, row, piece);
+        if (row < a.keep) {
+          const char* src = locate(kept[row], piece);
+          if (src) copy_in<kBytes>(smem + ((step % kStages) * kStepPieces + tid + kMoveThreads * u) * kBytes, src);
+          else bad = true;
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) load(s);
+#pragma unroll 1
+  for (int s = 0; s < steps; ++s) {
+    load(s + kStages - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    // All loads of this step have landed: its stores may go over them.
+    if constexpr (CLUSTER > 1) cluster_sync_all();
+    else __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      int row, piece;
+      mine(s, u, row, piece);
+      if (row < a.keep) {
+        char* dst = locate(row, piece);
+        const bool there = dst && locate(kept[row], 0);
+        const uint8_t* from = buf + (int64_t)((s % kStages) * kStepPieces + tid + kMoveThreads * u) * kBytes;
+        if (!there) bad = true;
+        else if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(from);
+      }
+    }
+  }
+  if (bad && a.status) atomicOr(a.status, AF_STATUS_BOUNDS);
+}
+
+template <int HD, int CLUSTER>
+cudaError_t launch_move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
+  constexpr int bytes = kStages * kStepPieces * (HD == 64 ? 8 : 16);
+  // The same for every call: set each time, which costs less than keeping track of the devices.
+  const cudaError_t e = cudaFuncSetAttribute(k_move<HD, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  return launch_ex(k_move<HD, CLUSTER>, dim3((unsigned)(segments * a.columns * CLUSTER)), dim3(kMoveThreads), (size_t)bytes, s, true, dim3(CLUSTER), a);
+}
+
+template <int HD>
+cudaError_t move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
+  return segments * a.columns < 148 ? launch_move<HD, 8>(a, segments, s) : launch_move<HD, 1>(a, segments, s);
+}
+
+}  // namespace
+}  // namespace kv_evict
+}  // namespace af
+
+using namespace af;
+
+extern "C" int af_evict_cache(const af_evict_args* args, uint32_t* status, void* stream) {
+  AF_REQUIRE(args, "af_evict_cache: null pointer");
+  const af_evict_args& w = *args;
+  const bool packed = w.int4.head_dim != 0;
+  const int64_t layers = packed ? w.int4.layers : w.layers, pages = packed ? w.int4.pages : w.pages, heads = packed ? w.int4.heads : w.heads,
+                page = packed ? w.int4.page_size : w.page_size;
+  AF_REQUIRE(layers >= 0 && pages >= 0 && heads >= 0 && w.batch >= 0 && w.max_pages >= 0 && w.places >= 0, "af_evict_cache: bad shape");
+  AF_REQUIRE(w.sinks >= 0 && w.recent >= 0 && w.keep >= 0 && w.sinks <= w.keep && w.recent <= w.keep - w.sinks,
+             "af_evict_cache: sinks and recent must not be negative, and together not more than keep");
+  AF_REQUIRE(page > 0 && page <= (1 << 20), "af_evict_cache: bad page_size");
+  if (packed) {
+    AF_REQUIRE(page % 8 == 0, "af_evict_cache: page_size must be a multiple of 8");
+    AF_REQUIRE(w.int4.head_dim == 64 || w.int4.head_dim == 128, "af_evict_cache: head_dim must be 64 or 128");
+  } else {
+    AF_REQUIRE(w.head_bytes >= 0 && w.head_bytes <= 4096, "af_evict_cache: at most 4096 bytes per head");
+  }
+  const int64_t segments = layers * w.batch * heads;
+  if (w.batch == 0 || layers == 0 || heads == 0) return AF_OK;
+  AF_REQUIRE(layers <= (1 << 20) && heads <= (1 << 16) && w.batch <= (1 << 20) && segments <= (1 << 24) && pages <= 0x7fffffff &&
+                 w.places <= (1 << 30) && w.keep <= (1 << 30) && w.max_pages <= (1 << 30) && w.max_pages * page <= (1 << 30),
+             "af_evict_cache: size too large");
+  const bool moves = pages > 0 && w.max_pages > 0 && w.keep > 0 && (packed || w.head_bytes > 0);
+  AF_REQUIRE(w.lengths && w.lengths_out && (w.places == 0 || (w.weights && w.weights_out)) && (w.keep == 0 || w.kept), "af_evict_cache: null pointer");
+  AF_REQUIRE(!moves || (w.tables && (packed ? w.int4.data != nullptr : w.k_cache && w.v_cache)), "af_evict_cache: null pointer");
+  kv_evict::SelectArgs a;
+  a.lengths = w.lengths;
+  a.weights = w.weights;
+  a.wl = w.weights_strides[0], a.wr = w.weights_strides[1], a.wh = w.weights_strides[2];
+  a.kept = w.kept;
+  a.weights_out = w.weights_out;
+  a.lengths_out = w.lengths_out;
+  a.batch = (int)w.batch;
+  a.heads = (int)heads;
+  a.places = (int)w.places;
+  a.keep = (int)w.keep;
+  a.sinks = (int)w.sinks;
+  a.recent = (int)w.recent;
+  a.capacity = pages ? w.max_pages * page : 0;
+  a.status = status;
+  kv_evict::MoveArgs m;
+  memset(&m, 0, sizeof(m));
+  uint64_t al;
+  if (packed) {
+    m.k = static_cast<char*>(w.int4.data);
+    m.kl = w.int4.strides[0], m.kp = w.int4.strides[1], m.kh = w.int4.strides[2];
+    al = reinterpret_cast<uintptr_t>(m.k) | (uint64_t)m.kl | (uint64_t)m.kp | (uint64_t)m.kh;
+    m.columns = 2;
+    m.pieces = 5;
+  } else {
+    m.k = static_cast<char*>(w.k_cache), m.v = static_cast<char*>(w.v_cache);
+    m.kl = w.k_cache_strides[0], m.kp = w.k_cache_strides[1], m.kt = w.k_cache_strides[2], m.kh = w.k_cache_strides[3];
+    m.vl = w.v_cache_strides[0], m.vp = w.v_cache_strides[1], m.vt = w.v_cache_strides[2], m.vh = w.v_cache_strides[3];
+    al = reinterpret_cast<uintptr_t>(m.k) | reinterpret_cast<uintptr_t>(m.v) | (uint64_t)w.head_bytes;
+    for (int i = 0; i < 4; ++i) al |= (uint64_t)w.k_cache_strides[i] | (uint64_t)w.v_cache_strides[i];
+    const int whole = (int)(w.head_bytes / 16);
+    // Whole rows a CTA where there are enough segments for all SMs, else 64 bytes.
+    m.pieces = 2 * segments < 296 && whole % 4 == 0 ? 4 : whole > 0 ? whole : 1;
+    m.columns = whole > 0 ? 2 * (whole / m.pieces) : 2;
+  }
+  AF_REQUIRE(!moves || (al & 15) == 0, "af_evict_cache: addresses and strides must be multiples of 16 bytes");
+  m.by_pieces = (uint32_t)(((1 << 20) + m.pieces - 1) / m.pieces);
+  m.tables = w.tables;
+  m.tables_ld = w.tables_stride;
+  m.lengths = w.lengths;
+  m.kept = w.kept;
+  m.capacity = a.capacity;
+  m.batch = a.batch;
+  m.heads = a.heads;
+  m.pages = (int)pages;
+  m.page = (int)page;
+  m.places = a.places;
+  m.keep = a.keep;
+  m.status = status;
+  cudaStream_t s = as_stream(stream);
+  kv_evict::k_select<<<(unsigned)segments, kv_evict::kSelThreads, 0, s>>>(a);
+  if (int st = check_launch("af_evict_cache")) return st;
+  if (!moves) return AF_OK;
+  const cudaError_t e = !packed ? kv_evict::move<0>(m, segments, s) : w.int4.head_dim == 128 ? kv_evict::move<128>(m, segments, s) : kv_evict::move<64>(m, segments, s);
+  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_evict_cache: ") + cudaGetErrorString(e));
+  return check_launch("af_evict_cache");
+}

@@ -584,6 +584,92 @@ int af_tree_attention_workspace_bytes(int64_t* bytes);
  */
 int af_tree_attention_wait_limit(int64_t attempts);
 
+/* ------------------------------------------------------------------------
+ * A paged key/value cache in 4 bits, and the operators that keep long
+ * requests in less memory. No counterpart in the reference.
+ *
+ * The cache of a layer is [pages][heads][page_size / 8] blocks of 10 *
+ * head_dim bytes (contiguous within a page's head), each the keys and values
+ * of 8 tokens of one head: 8 rows of head_dim / 2 bytes of key codes, 8 rows
+ * of 16-bit (scale, offset) pairs of the keys, one per 32 dims, then the same
+ * of the values. Word w of a row of codes holds dims 8 w .. 8 w + 7: bits 4 i
+ * of its low half dim 8 w + 2 i, of its high half dim 8 w + 2 i + 1. With 128
+ * dims the two halves of a row of codes are swapped in rows 2, 3, 6 and 7 of
+ * a block. A value is code * scale + offset, rounded once to dtype, that of
+ * the pairs (fp16 or bf16).
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  void* data;
+  int64_t strides[3]; /* layer, page, head: bytes, multiples of 16 */
+  int64_t layers, pages, page_size, heads, head_dim, dtype;
+} af_int4_cache;
+
+/*
+ * af_write_cache_int4 -- key and value rows into their slots, in 4 bits.
+ * af_read_cache_int4 -- the values of slots, as 16-bit rows.
+ *
+ * As af_write_cache: for every layer and i < count with slots[i] >= 0 (and
+ * rows[i] >= 0, rows null: row i). Per row and group of 32 dims: offset = the
+ * smallest value, scale = (largest - smallest) / 15 rounded to dtype (one step
+ * less where 15 * scale + offset would overflow), code = (x - offset) / scale
+ * rounded half to even, in 0 .. 15 (0 where scale is 0). A group with a value
+ * that is not finite, or with a range past fp32's, stands for NaN throughout.
+ * Two rows for one slot leave an unspecified mixture. Reading writes row i
+ * of k and v for slot i, zeros for a negative slot; rows is not used. Strides in bytes
+ * (layer, row, head); they, and the addresses, are multiples of 16.
+ */
+typedef struct {
+  void *k, *v;
+  int64_t k_strides[3], v_strides[3]; /* layer, row, head */
+  const int64_t* slots;
+  const int32_t* rows;
+  int64_t n_rows, count;
+  af_int4_cache cache;
+} af_int4_rows;
+
+int af_write_cache_int4(const af_int4_rows* w, uint32_t* status, void* stream);
+int af_read_cache_int4(const af_int4_rows* w, uint32_t* status, void* stream);
+
+/*
+ * af_evict_cache -- of every request's cached tokens, those that were given
+ * the most attention stay.
+ *
+ * Per layer, request and head with more than `keep` tokens: the first `sinks`
+ * places, the last `recent` and, of those between, the ones with the largest
+ * weights (equal ones: the lowest places; NaN counts as the largest) stay,
+ * `keep` in all; they move to places 0 .. keep - 1 in their order, in place. A
+ * request with at most `keep` tokens stays as it is. kept [layers, batch,
+ * heads, keep]: the places that the tokens came from, -1 behind the last;
+ * weights_out [layers, batch, heads, places]: their weights, 0 behind the
+ * last; lengths_out[b] = min(lengths[b], keep). weights [layers, batch, heads,
+ * places] (strides in elements: layer, request, head). A length that is
+ * negative or above places or the table's capacity, or a page out of range, sets
+ * AF_STATUS_BOUNDS: such a request keeps its length and its rows, kept is
+ * -1; rows of such a page are not moved. The tables are not changed
+ * (af_block_tables with `held` gives the pages behind the kept tokens back).
+ * With int4.head_dim 0 the cache is k_cache and v_cache: rows of head_bytes
+ * (at most 4096), strides in bytes (layer, page, token, head). Strides in bytes, head_bytes
+ * and addresses are multiples of 16. Pages of one request must not be another's.
+ */
+typedef struct {
+  af_int4_cache int4;
+  void *k_cache, *v_cache;
+  int64_t k_cache_strides[4], v_cache_strides[4];
+  int64_t layers, pages, page_size, heads, head_bytes; /* of k_cache and v_cache */
+  const int32_t* tables;
+  int64_t tables_stride, max_pages; /* elements */
+  const int32_t* lengths;
+  int64_t batch;
+  const float* weights;
+  int64_t weights_strides[3], places;
+  int64_t keep, sinks, recent;
+  int32_t* kept;
+  float* weights_out;
+  int32_t* lengths_out;
+} af_evict_args;
+
+int af_evict_cache(const af_evict_args* a, uint32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,259 @@
+"""Operators of the 4-bit cache against plain 64-bit forms. What is held in 4 bits, places and moved rows must be equal."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import cache_util as U
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _i64(x):
+    return torch.tensor(x, dtype=torch.int64, device="cuda")
+
+
+def _bits(x):
+    return x.contiguous().view(torch.int16) if x.dtype in (BF, HF) else x
+
+
+def _same(a, b):
+    """Equal values (0 and -0 alike), NaN in the same places."""
+    return bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+# ------------------------------------------------------------------------------------------------ rows in and out
+@pytest.mark.parametrize("layers,n,heads,dim,page,dtype", [(None, 1, 1, 64, 8, BF), (None, 37, 4, 128, 16, BF), (3, 20, 5, 64, 48, HF), (2, 9, 32, 128, 64, HF),
+                                                           (None, 130, 3, 64, 8, HF), (28, 6, 1, 128, 128, BF)])
+def test_write_and_read(layers, n, heads, dim, page, dtype):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import Int4Cache, read_cache_int4, write_cache_int4
+
+    g = torch.Generator(device="cuda").manual_seed(n + heads)
+    pages = -(-n // page) + 2
+    cache = Int4Cache.empty(pages, page, heads, dim, dtype, layers)
+    cache.data.random_(0, 256, generator=g)
+    before = cache.data.clone()
+    lead = () if layers is None else (layers,)
+    k, v = ((torch.randn(*lead, n, heads, dim, device="cuda", generator=g) * torch.exp(2 * torch.randn(n, heads, 1, device="cuda", generator=g))).to(dtype)
+            for _ in range(2))
+    slots = torch.randperm(pages * page, device="cuda", generator=g)[:n]
+    slots[n // 3] = -1
+    st = DeviceStatus()
+    write_cache_int4(k, v, cache, slots, status=st)
+    got = read_cache_int4(cache, slots, status=st)
+    st.check_status()
+    live = [i for i in range(n) if i != n // 3]
+    for x, y in zip((k, v), got):
+        want = U.values(*U.encode(x))
+        assert _same(y[..., live, :, :], want[..., live, :, :]) and not y[..., n // 3, :, :].any()
+    # The bytes are those of the layout, and no others are touched.
+    want = before if layers is not None else before[None]
+    for l in range(layers or 1):
+        for part, x in enumerate((k, v)):
+            codes, scales, offsets = U.encode(x[l] if layers is not None else x)
+            for i in live:
+                U.put(want[l], int(slots[i]), part, codes[i], scales[i], offsets[i])
+    assert torch.equal(cache.data, want if layers is not None else want[0])
+    assert _same(U.decoded(want[0], dtype)[0][slots[live]], got[0][..., live, :, :] if layers is None else got[0][0, live])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_groups_of_every_kind(dtype):
+    """Equal values, zeros, halves of a step (ties), the type's extremes, subnormal numbers, infinities and NaN."""
+    from actfold_b200.speculative import Int4Cache, read_cache_int4, write_cache_int4
+
+    top, tiny = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    sub = 2.0 ** -24 if dtype is HF else 2.0 ** -133
+    i = torch.arange(32, dtype=torch.float64)
+    rows = [torch.zeros(32), torch.full((32,), 3.25), -i, i / 2, i * 15 / 31, torch.where(i == 0, top, -top), torch.where(i == 5, top, 0.0),
+            torch.where(i < 16, -top, -top / 2), i * tiny, i * sub, i * sub * 4, torch.where(i == 31, math.inf, i), torch.where(i == 0, -math.inf, i),
+            torch.where(i == 9, math.nan, i), torch.full((32,), math.inf), torch.where(i % 2 == 0, -0.0, 0.0), 7.5 * (i % 3), i % 31 - 7.5,
+            torch.where(i == 0, -15.0, torch.where(i == 1, 2.0 ** -20, -(i % 16))), torch.where(i == 0, -7.5, torch.where(i == 1, 7.5, 2.0 ** -24)),
+            torch.where(i == 3, 15.0, 0.5 + i % 15), 1000 + i]
+    x = torch.stack([r.to(torch.float64) for r in rows]).to(dtype).cuda()
+    n = x.shape[0]
+    k = x.repeat(1, 2).view(n, 1, 64).contiguous()
+    k[:, 0, 32:] = k[:, 0, 32:].flip(-1)
+    v = k.flip(0).contiguous()
+    cache = Int4Cache.empty(3, 8, 1, 64, dtype)
+    slots = torch.arange(n, device="cuda")
+    write_cache_int4(k, v, cache, slots)
+    for a, b in zip(read_cache_int4(cache, slots), (k, v)):
+        want = U.values(*U.encode(b))
+        assert _same(a, want), (a != want).nonzero()
+    got = read_cache_int4(cache, slots)[0][:, 0, :32]
+    # (Row 5's range, twice the largest number, is past fp32's where the type is bf16.)
+    assert got.isnan().all(1).nonzero()[:, 0].tolist() == ([5] if dtype is BF else []) + [11, 12, 13, 14] and not got.isinf().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_error_is_half_a_step(dtype):
+    """Off by at most half a step, and the roundings: of the scale by u of 15 steps, of the value by u of itself."""
+    from actfold_b200.speculative import Int4Cache, read_cache_int4, write_cache_int4
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(4000, 2, 128, device="cuda", generator=g).to(dtype)
+    cache = Int4Cache.empty(250, 16, 2, 128, dtype)
+    slots = torch.randperm(4000, device="cuda", generator=g)
+    write_cache_int4(k, k, cache, slots)
+    u = torch.finfo(dtype).eps / 2
+    x = k.double().unflatten(-1, (4, 32))
+    step = (x.amax(-1, keepdim=True) - x.amin(-1, keepdim=True)) / 15
+    for y in read_cache_int4(cache, slots):
+        y = y.double().unflatten(-1, (4, 32))
+        assert bool(((y - x).abs() <= step * (1 + u) / 2 + 15 * u * step + u * y.abs()).all())
+
+
+def test_rows_by_number_strides_and_bad_slots():
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import Int4Cache, read_cache_int4, write_cache_int4
+
+    g = torch.Generator(device="cuda").manual_seed(4)
+    full = torch.randn(2, 40, 2, 5, 130, device="cuda", generator=g).to(HF)
+    odd = full[:, :, 0, :, 1:129]                                   # rows that are not 16-byte aligned
+    even = full.new_empty(2, 5, 40, 136).normal_(generator=g)[..., :128].transpose(1, 2)  # heads outside the rows
+    big = torch.zeros(2, 6, 7, 2, 1280, dtype=torch.uint8, device="cuda")
+    cache = Int4Cache(big[:, 1:5, 1:6], HF)                         # a part of a larger pool
+    slots = _i64([[3, -1, 17], [63, 9, 30]])
+    rows = _i32([[39, 0, -1], [0, 7, 7]])
+    st = DeviceStatus()
+    write_cache_int4(odd, even, cache, slots, rows=rows, status=st)
+    st.check_status()
+    k, v = read_cache_int4(cache, slots)
+    assert k.shape == (2, 2, 3, 5, 128)
+    for a, b in ((k, odd), (v, even)):
+        want = U.values(*U.encode(b[:, rows.clamp(min=0).long()]))
+        want[:, 0, 1:] = 0                                          # a negative slot; a negative row: the zeros that were there
+        assert _same(a, want)
+    assert not big[:, 0].any() and not big[:, 5].any() and not big[:, :, 0].any() and not big[:, :, 6].any()
+    for call in (lambda: write_cache_int4(odd, even, cache, _i64([64]), rows=_i32([0]), status=st),
+                 lambda: write_cache_int4(odd, even, cache, _i64([5]), rows=_i32([40]), status=st), lambda: read_cache_int4(cache, _i64([2 ** 40]), status=st)):
+        call()
+        with pytest.raises(RuntimeError):
+            st.check_status()
+    write_cache_int4(odd[:, :0], even[:, :0], cache, slots[:0, 0], status=st)
+    assert read_cache_int4(cache, slots[:0])[0].shape == (2, 0, 3, 5, 128)
+    st.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+def _evict_case(layers, ls, heads, dim, page, dtype, held, seed, extra=3):
+    from actfold_b200.speculative import Int4Cache
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    used = [-(-t // page) for t in ls]
+    pool = sum(used) + 2
+    order = torch.randperm(pool, device="cuda", generator=g).to(torch.int32)
+    tables = torch.full((len(ls), max(1, *used) + 1), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, u in enumerate(used):
+        tables[r, :u] = order[at:at + u]
+        at += u
+    lead = () if layers is None else (layers,)
+    if held == 4:
+        cache = Int4Cache.empty(pool, page, heads, dim, dtype, layers)
+        cache.data.random_(0, 256, generator=g)
+        rows = cache.data
+        # One row of bytes per token and head: [.., pool * page, heads, 2, codes and pairs].
+    else:
+        cache = tuple(torch.randn(*lead, pool, page, heads, dim, device="cuda", generator=g).to(dtype) for _ in range(2))
+        rows = cache
+    w = torch.rand(*lead, len(ls), heads, max(1, *ls) + extra, device="cuda", generator=g)
+    w = torch.where(w < 0.1, torch.zeros_like(w), (w * 50).round() / 50)  # many equal ones
+    return cache, rows, tables, w
+
+
+def _flat(cache, held, dtype):
+    """[2 (keys, values), layers, slots, heads, dim]: what the cache holds, as whole numbers where they are codes."""
+    if held == 16:
+        return torch.stack([c if c.dim() == 5 else c[None] for c in cache]).flatten(2, 3)
+    data = cache.data if cache.layers is not None else cache.data[None]
+    out = []
+    for d in data:
+        pages, heads, blocks, size = d.shape
+        dim = size // 10
+        parts = d.reshape(pages, heads, blocks, 2, 5 * dim)
+        codes = parts[..., : 4 * dim].reshape(pages, heads, blocks, 2, 8, dim // 2).clone()
+        if dim == 128:
+            codes[..., [2, 3, 6, 7], :] = codes[..., [2, 3, 6, 7], :].roll(32, -1)
+        pairs = parts[..., 4 * dim:].reshape(pages, heads, blocks, 2, 8, dim // 8)
+        out.append(torch.cat([codes, pairs], -1).permute(3, 0, 2, 4, 1, 5).reshape(2, -1, heads, dim // 2 + dim // 8))
+    return torch.stack(out, 1)
+
+
+@pytest.mark.parametrize("layers,ls,heads,dim,page,dtype,held,keep,sinks,recent", [
+    (None, [40], 1, 64, 8, BF, 16, 20, 4, 5), (None, [40], 1, 64, 8, BF, 4, 20, 4, 5), (3, [100, 7, 0, 64, 65], 2, 128, 16, HF, 4, 64, 3, 10),
+    (3, [100, 7, 0, 64, 65], 2, 128, 16, HF, 16, 64, 3, 10), (2, [5000, 3001], 1, 64, 48, BF, 4, 2999, 0, 0), (1, [9000], 2, 128, 64, BF, 4, 1, 0, 1),
+    (1, [9000], 1, 128, 64, BF, 16, 8999, 1, 700), (28, [300, 280], 4, 128, 128, HF, 4, 150, 4, 30), (28, [1500] * 3, 4, 128, 16, BF, 16, 777, 2, 32),
+    (None, [33, 12], 3, 64, 8, HF, 4, 0, 0, 0), (None, [20, 21], 2, 128, 8, BF, 4, 20, 12, 8), (40, [260, 500], 4, 64, 16, HF, 4, 200, 4, 8),
+    (None, [3000], 1, 40, 24, torch.float32, 16, 1024, 4, 256)])
+def test_evict(layers, ls, heads, dim, page, dtype, held, keep, sinks, recent):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import evict_cache
+
+    cache, _, tables, w = _evict_case(layers, ls, heads, dim, page, dtype, held, keep + len(ls))
+    before = _flat(cache, held, dtype)
+    st = DeviceStatus()
+    r = evict_cache(cache, tables, _i32(ls), w, keep, sinks=sinks, recent=recent, status=st)
+    st.check_status()
+    after = _flat(cache, held, dtype)
+    assert r.lengths.tolist() == [min(t, keep) for t in ls]
+    assert r.kept.shape == (*w.shape[:-1], keep) and r.weights.shape == w.shape
+    kept, given, old = (x if layers is not None else x[None] for x in (r.kept, r.weights, w))
+    want = before.clone()
+    for l in range(layers or 1):
+        for b, t in enumerate(ls):
+            place = torch.arange(max(t, 1), device="cuda")
+            slot = tables[b].long()[place // page] * page + place % page
+            for h in range(heads):
+                places = U.evict(old[l, b, h, :t].tolist(), keep, sinks, recent)
+                assert kept[l, b, h].tolist() == places + [-1] * (keep - len(places))
+                assert torch.equal(given[l, b, h, :len(places)], old[l, b, h, places]) and not given[l, b, h, len(places):].any()
+                if t > keep:
+                    want[:, l, slot[:keep], h] = before[:, l, slot[places], h]
+    assert torch.equal(_bits(after), _bits(want))
+
+
+def test_evict_weights_of_every_kind():
+    """Negative weights, zeros of both signs, infinities and NaN; a weight that all tokens share."""
+    from actfold_b200.speculative import evict_cache
+
+    for w in ([0.0, -0.0, 1.0, -1.0, math.inf, -math.inf, math.nan, 0.0, -0.0, 2.0, math.nan, 1e-45], [1.5] * 12, [-0.0, 0.0] * 6):
+        cache, _, tables, _ = _evict_case(None, [12], 1, 64, 8, BF, 4, 1)
+        for keep in range(12):
+            r = evict_cache(cache, tables, _i32([12]), torch.tensor(w, device="cuda").view(1, 1, 12), keep, sinks=min(1, keep))
+            assert r.kept[0, 0].tolist() == U.evict(w, keep, min(1, keep), 0), (w, keep)
+
+
+def test_evict_reports_bad_lengths_and_pages():
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import evict_cache
+
+    st = DeviceStatus()
+    for ls in ([-1, 30], [10 ** 6, 30], [34, 30]):  # negative, past the table, past the weights
+        cache, _, tables, w = _evict_case(None, [32, 30], 2, 64, 8, BF, 4, 2, extra=1)
+        before = cache.data.clone()
+        r = evict_cache(cache, tables, _i32(ls), w, 20, status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+        assert r.lengths.tolist() == [ls[0], 20] and (r.kept[0] == -1).all() and (r.kept[1] >= 0).all()
+        mine = tables[0, :4].long()
+        assert torch.equal(cache.data[mine], before[mine])
+    for page in (-1, 10 ** 6):
+        cache, _, tables, w = _evict_case(None, [32, 30], 2, 64, 8, BF, 4, 2)
+        tables[0, 3] = page
+        r = evict_cache(cache, tables, _i32([32, 30]), w, 20, status=st)
+        assert r.lengths.tolist() == [20, 20]
+        with pytest.raises(RuntimeError):
+            st.check_status()
