@@ -56,6 +56,8 @@ SIGNATURES: dict[str, tuple] = {
     "af_write_cache_int4": (_i32, [_vp, _vp, _vp]),
     "af_read_cache_int4": (_i32, [_vp, _vp, _vp]),
     "af_evict_cache": (_i32, [_vp, _vp, _vp]),
+    "af_tree_attention_int4": (_i32, [_vp, _vp, _vp]),
+    "af_tree_attention_int4_workspace_bytes": (_i32, [_vp]),
 }
 
 _lib = None

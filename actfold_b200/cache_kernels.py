@@ -28,11 +28,12 @@ import torch
 
 from actfold_b200 import _lib
 from actfold_b200.kernels import DeviceStatus
-from actfold_b200.tree_kernels import _launch, _not_vectors, _same_device, _word
+from actfold_b200.tree_kernels import _launch, _not_vectors, _row_grid, _same_device, _word
 
 _I32, _I64 = torch.int32, torch.int64
 _CACHE = "q3q6q"
 _ROWS = struct.Struct("2q3q3q2q2q" + _CACHE)
+_ATTENTION = struct.Struct("3q2q2q2q" + _CACHE + "3q2q3q5qdq2qq2q")
 _EVICT = struct.Struct(_CACHE + "2q4q4q5q3q2qq3qq3q3q")
 _NO_CACHE = (0,) * 10
 
@@ -250,3 +251,113 @@ def evict_cache(
                        *(ws[:3] if layered else (0, *ws[:2])), places, keep, sinks, recent, kept.data_ptr(), out.data_ptr(), left.data_ptr())
     _launch("evict_cache", index, _lib.load().af_evict_cache, args, _lib.ptr(word))
     return EvictedCache(left, kept, out)
+
+
+def _check_window(what: str, window: int | None, sinks: int) -> int:
+    """The window as the C entry points take it (0: none)."""
+    if window is None:
+        if sinks:
+            raise ValueError(f"{what}: sinks need a window")
+        return 0
+    if window <= 0 or sinks < 0:
+        raise ValueError(f"{what}: window {window} must be positive and sinks {sinks} not negative")
+    return window
+
+
+def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, tuple | list]:
+    """16-bit rows [n, heads, dim] and their strides in bytes, copied where these or the address are not multiples of 16."""
+    if (grid := _row_grid(t)) is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        grid = _row_grid(t)
+    return t, grid
+
+
+def tree_attention_int4(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cache: Int4Cache,
+    tables: torch.Tensor,
+    lengths: torch.Tensor,
+    starts: torch.Tensor,
+    mask: torch.Tensor | None = None,
+    window: int | None = None,
+    sinks: int = 0,
+    scale: float | None = None,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    status: DeviceStatus | None = None,
+) -> torch.Tensor:
+    """Attention of packed tree nodes over their requests' 4-bit caches and their own trees.
+
+    As :func:`~actfold_b200.tree_kernels.tree_attention` over what :func:`read_cache_int4` gives for the prefix: ``q`` [nodes,
+    heads, dim], ``k`` / ``v`` [nodes, kv_heads, dim] of this step (16 bits, not in the cache), all of the cache's dtype;
+    ``cache`` without layers, or one layer of it. Request b's first ``lengths[b]`` tokens lie in pages ``tables[b]``; node i also
+    sees the nodes whose bits are set in ``mask[i]`` ([nodes, words] int32), without a mask the nodes of its chain up to itself.
+
+    With a ``window`` a node that sees c nodes (itself among them) sees the last ``window - c`` tokens of the prefix (none where
+    that is negative) and the prefix's first ``sinks`` tokens; in a chain, which has no mask, it sees the last ``window`` nodes.
+    Nodes that a mask shows stay visible whatever the window. Only pages with visible tokens are read.
+
+    ``scale`` defaults to dim ** -0.5. A row that sees nothing is 0. ``lse`` [nodes, heads] float32 receives the natural log of
+    each row's sum of exponentials, as :func:`attention_weights` takes it. Rows of ``out`` behind ``starts[-1]`` are not written,
+    none when ``starts`` is out of order. ``out`` shares no memory with the inputs.
+    """
+    if cache.layers is not None:
+        raise ValueError("tree_attention_int4: cache must be one layer (cache[l])")
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or v.shape != ks or ks[0] != qs[0] or ks[1] != cache.kv_heads or ks[2] != cache.dim or qs[2] != cache.dim:
+        raise ValueError(f"tree_attention_int4: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} and cache {tuple(cache.data.shape)} do not match")
+    total, heads, dim = qs
+    dtype = cache.dtype
+    if q.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError(f"tree_attention_int4: q, k, v must be of the cache's {dtype}, got {q.dtype}, {k.dtype}, {v.dtype}")
+    batch, most = _check_tables("tree_attention_int4", tables, lengths)
+    if starts.dtype is not _I32 or starts.dim() != 1:
+        _not_vectors("tree_attention_int4", _I32, starts=starts)
+    if starts.shape[0] != batch + 1:
+        raise ValueError(f"tree_attention_int4: {batch} requests need one entry of starts more")
+    window = _check_window("tree_attention_int4", window, sinks)
+    mask_at = mask_row = words = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.dtype is not _I32 or mask.shape[0] != total or mask.shape[1] == 0:
+            raise ValueError(f"tree_attention_int4: mask must be int32 [{total}, words], got {mask.dtype} {tuple(mask.shape)}")
+        words = mask.shape[1]
+        mask_row, inner = mask.stride()
+        if (words > 1 and inner != 1) or mask_row < words:
+            mask = mask.contiguous()
+            mask_row = words
+        mask_at = mask.data_ptr()
+    out_grid = None
+    if out is not None and (out.shape != qs or out.dtype is not dtype or (out_grid := _row_grid(out)) is None):
+        raise ValueError("tree_attention_int4: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
+    if lse is not None and (lse.shape != (total, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
+        raise ValueError(f"tree_attention_int4: lse must be contiguous float32 [{total}, {heads}]")
+    index = _same_device("tree_attention_int4", q, k, v, cache.data, tables, lengths, starts, mask, out, lse, word := _word(status))
+    if most > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lengths, starts = lengths.contiguous(), starts.contiguous()
+    (q, q_grid), (k, k_grid), (v, v_grid) = _rows16(q), _rows16(k), _rows16(v)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_grid = (2 * heads * dim, 2 * dim)
+    size = _scratch.get(index) or _workspace_bytes(index)
+    workspace = lengths.new_empty(size >> 2)
+    args = _ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q_grid, *k_grid, *v_grid, *cache._packed, tables.data_ptr(),
+        tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(), starts.data_ptr(), mask_at, mask_row if total > 1 else words, words, batch, total,
+        heads, window, sinks, dim ** -0.5 if scale is None else scale, out.data_ptr(), *out_grid, 0 if lse is None else lse.data_ptr(),
+        workspace.data_ptr(), size)
+    _launch("tree_attention_int4", index, _lib.load().af_tree_attention_int4, args, _lib.ptr(word))
+    return out
+
+
+_scratch: dict[int, int] = {}  # bytes of scratch per device
+
+
+def _workspace_bytes(index: int) -> int:
+    n = C.c_int64()
+    with torch.cuda.device(index):
+        _lib.check(_lib.load().af_tree_attention_int4_workspace_bytes(C.byref(n)), "tree_attention_int4")
+    _scratch[index] = (n.value + 15) & ~15
+    return _scratch[index]

@@ -732,6 +732,9 @@ template int join_launch<AF_DTYPE_BF16, 256, 64>(const Params&, int, cudaStream_
 template int join_launch<AF_DTYPE_BF16, 256, 128>(const Params&, int, cudaStream_t);
 
 }  // namespace tree_attn
+
+int attention_patience() { return tree_attn::g_patience.load(std::memory_order_relaxed); }
+
 }  // namespace af
 
 using namespace af;

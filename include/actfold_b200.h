@@ -578,7 +578,7 @@ int af_tree_attention_workspace_bytes(int64_t* bytes);
 
 /*
  * Attempts (of a few microseconds each) after which a wait inside later
- * af_tree_attention calls of this process gives up: the call then ends with
+ * af_tree_attention and af_tree_attention_int4 calls of this process gives up: the call then ends with
  * AF_STATUS_TIMEOUT in *status and rows of out that mean nothing. -1: the
  * default, 2^18 attempts or about a second, which is also the most.
  */
@@ -669,6 +669,46 @@ typedef struct {
 } af_evict_args;
 
 int af_evict_cache(const af_evict_args* a, uint32_t* status, void* stream);
+
+/*
+ * af_tree_attention_int4 -- af_tree_attention over a 4-bit cache, with an
+ * optional sliding window and first tokens that stay visible.
+ *
+ * Nodes, mask, scale, out, lse and status as in af_tree_attention; the prefix
+ * comes from one layer of a 4-bit cache (cache.strides[0] is not used), k and
+ * v of the step's own nodes are 16-bit rows of the cache's dtype. Any group
+ * n_heads / cache.heads. window 0: a node sees all of the prefix. Else it
+ * sees the last max(0, window - c) tokens of the prefix, where c counts the
+ * nodes that it sees (itself among them), and the prefix's first `sinks`
+ * tokens; without a mask only the last `window` nodes of its chain. Nodes
+ * that a mask shows stay visible whatever the window. Values that a row
+ * does not see have no influence on it. workspace:
+ * af_tree_attention_int4_workspace_bytes() bytes, not shared by calls that
+ * may run at once. Sums, maxima and the output rows are held in 32 bits;
+ * probabilities are rounded to dtype.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_strides[2], k_strides[2], v_strides[2]; /* node, head */
+  af_int4_cache cache;
+  const int32_t* tables;
+  int64_t tables_stride, max_pages; /* elements */
+  const int32_t *lengths, *starts;
+  const int32_t* mask;
+  int64_t mask_stride, words; /* elements */
+  int64_t batch, total, n_heads, window, sinks;
+  double scale;
+  void* out;
+  int64_t out_strides[2]; /* node, head */
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+} af_tree_attention_int4_args;
+
+int af_tree_attention_int4(const af_tree_attention_int4_args* a, uint32_t* status, void* stream);
+
+/* Bytes of scratch that af_tree_attention_int4 needs on the current device. */
+int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
 
 #ifdef __cplusplus
 }

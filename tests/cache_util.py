@@ -79,3 +79,82 @@ def evict(weights: list[float], keep: int, sinks: int, recent: int) -> list[int]
     middle = range(sinks, t - recent)
     best = sorted(middle, key=lambda i: (0 if math.isnan(weights[i]) else 1, -weights[i] if not math.isnan(weights[i]) else 0.0, i))
     return sorted([*range(sinks), *best[: keep - sinks - recent], *range(t - recent, t)])
+
+
+def visible(n: int, t: int, bits: torch.Tensor | None, window: int, sinks: int) -> torch.Tensor:
+    """[n, t + n]: what the n nodes behind t cached tokens see. bits: their own tree's [n, n], None for a chain; window 0: none."""
+    i = torch.arange(n)
+    if bits is None:
+        tree = i[None] <= i[:, None]
+        if window:
+            tree &= i[None] > i[:, None] - window
+    else:
+        tree = bits.cpu()
+    see = torch.ones(n, t + n, dtype=torch.bool)
+    see[:, t:] = tree
+    if window:
+        for r in range(n):
+            see[r, min(sinks, t): max(min(sinks, t), t - max(0, window - int(tree[r].sum())))] = False
+    return see
+
+
+def attention(q, k, v, data, dtype, tables, lengths, starts, bits, window=0, sinks=0, scale=None):
+    """(out, lse, allowed error of out, of lse) in 64 bits, request by request, over the values that 4-bit pages stand for.
+
+    bits: per request a bool [n, n] array of what a node sees, or None for a chain. The error that fp32 scores and sums with
+    probabilities rounded to the inputs' type allow, with u = eps / 2 of that type:
+      |out - ref| <= (u + 2 d) A + u |ref| + f,   A = sum_j w_j |v_j|  (w: exact weights)
+    where u A is the rounding of the probabilities, u |ref| that of the result, and d bounds how far a score is off (in
+    natural units): dim products summed in fp32, where the tensor cores may cut a sum instead of rounding it, are off by at most dim * 2^-23 * S
+    with S = scale * sum |q||k|; the scaling, the shift by the maximum and exp2 by 2^-24 * 4 (|s| + |max| + 1) and by 2^-22 more. A
+    weight then moves by about 2 d (its own score and the sum's). The products with the values are summed in fp32: 2^-23 a
+    term and relative, as is the sum of the weights. fp16 probabilities below 2^-14 are off by up to 2^-25 (of a largest one of at least 2^7):
+    f = 2^-32 sum_j |v_j| / l, and a result below 2^-14 is rounded by up to 2^-25 instead of u |ref|. The log of the sum is off
+    by 2 d, the sum's rounding and 2^-22 (|lse| + 1).
+    """
+    total, heads, dim = q.shape
+    kv = k.shape[1]
+    page = 8 * data.shape[2]
+    scale = dim ** -0.5 if scale is None else scale
+    u = torch.finfo(q.dtype).eps / 2
+    held = decoded(data, dtype).double()
+    out = torch.zeros(total, heads, dim, dtype=torch.float64, device=q.device)
+    lse = torch.full((total, heads), -math.inf, dtype=torch.float64, device=q.device)
+    tol, lse_tol = torch.zeros_like(out), torch.zeros_like(lse)
+    for b, t in enumerate(lengths):
+        lo, hi = starts[b], starts[b + 1]
+        n = hi - lo
+        if n == 0:
+            continue
+        place = torch.arange(t)
+        slots = torch.tensor([int(tables[b][x // page]) * page + x % page for x in place.tolist()], dtype=torch.int64, device=q.device)
+        see = visible(n, t, None if bits is None else bits[b], window, sinks).to(q.device)
+        used = see.any(0)
+        for g in range(kv):
+            kk, vv = (torch.where(used[:, None], torch.cat([held[x][slots, g], y[lo:hi, g].double()]), 0.0) for x, y in ((0, k), (1, v)))
+            for h in range(g * heads // kv, (g + 1) * heads // kv):
+                x = q[lo:hi, h].double()
+                s = torch.where(see, (x @ kk.T) * scale, -math.inf)
+                top = s.amax(-1, keepdim=True)
+                top = torch.where(torch.isfinite(top), top, 0.0)
+                e = torch.where(see, torch.exp(s - top), 0.0)
+                l = e.sum(-1, keepdim=True)
+                w = torch.where(l > 0, e / l, torch.zeros_like(e))
+                if bool(torch.isfinite(vv).all()):
+                    o, a, f = w @ vv, w @ vv.abs(), see.double() @ vv.abs()
+                else:  # a hidden value has no influence, not even as 0 * NaN
+                    o, a, f = (torch.stack([y[i][see[i]] @ z[see[i]] for i in range(n)]) for y, z in ((w, vv), (w, vv.abs()), (see.double(), vv.abs())))
+                out[lo:hi, h] = o
+                lse[lo:hi, h] = torch.where(l > 0, top + torch.log(l), -math.inf)[:, 0]
+                big = torch.where(see, (x.abs() @ kk.abs().nan_to_num(0, 0, 0).T) * abs(scale), 0.0).amax(-1, keepdim=True).nan_to_num(0, 0, 0)
+                d = 2.0 ** -23 * dim * big + 2.0 ** -24 * 4 * (2 * big + 1) + 2.0 ** -22
+                sub = 2.0 ** -32 * f / l.clamp(min=1e-300) + 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+                tol[lo:hi, h] = (u + 2 * d + 2 * (t + n) * 2.0 ** -23) * a + u * o.abs() + sub
+                lse_tol[lo:hi, h] = (2 * d + (t + n) * 2.0 ** -23)[:, 0] + 2.0 ** -22 * (lse[lo:hi, h].abs().nan_to_num(0, 0, 0) + 1)
+    return out, lse, tol, lse_tol
+
+
+def close(got, want, tol) -> bool:
+    """Within the allowed error; NaN and infinities in the same places."""
+    same = (got.double() == want) | (got.isnan() & want.isnan())
+    return bool((same | ((got.double() - want).abs() <= tol)).all())

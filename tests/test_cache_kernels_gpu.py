@@ -257,3 +257,85 @@ def test_evict_reports_bad_lengths_and_pages():
         assert r.lengths.tolist() == [20, 20]
         with pytest.raises(RuntimeError):
             st.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def _attention_case(ns, ls, heads, kv, dim, page, dtype, tree, seed, extra_rows=0):
+    """Keys with a few strong channels; scattered pages; random bytes in the places behind a request's last token."""
+    import tree_util as T
+    from actfold_b200.speculative import Int4Cache, write_cache_int4
+
+    rng = np.random.default_rng(seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    used = [-(-t // page) for t in ls]
+    pool = sum(used) + 2
+    order = torch.randperm(pool, device="cuda", generator=g).to(torch.int32)
+    tables = torch.full((len(ls), max(1, *used) + 1), -1, dtype=torch.int32, device="cuda")
+    slots, at = [], 0
+    for r, (u, t) in enumerate(zip(used, ls)):
+        tables[r, :u] = order[at:at + u]
+        at += u
+        place = torch.arange(t, device="cuda")
+        slots.append(tables[r].long()[place // page] * page + place % page)
+    slots = torch.cat(slots)
+    cache = Int4Cache.empty(pool, page, kv, dim, dtype)
+    cache.data.random_(0, 256, generator=g)
+    strong = torch.where(torch.rand(kv, dim, device="cuda", generator=g) < 0.05, 3.0, 1.0)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    write_cache_int4((rand(slots.numel(), kv, dim) * strong).to(dtype), rand(slots.numel(), kv, dim).to(dtype), cache, slots)
+    total = sum(ns) + extra_rows
+    starts = [0, *np.cumsum(ns).tolist()]
+    bits = mask = None
+    if tree:
+        paths = [T.ancestors(T.random_parents(n, rng)) for n in ns]
+        words = max(1, -(-max(ns) // 32))
+        mask = torch.zeros(total, words, dtype=torch.int32, device="cuda")
+        bits = []
+        for b, p in enumerate(paths):
+            m = torch.zeros(ns[b], ns[b], dtype=torch.bool)
+            for i, row in enumerate(p):
+                m[i, row] = True
+            bits.append(m)
+            if ns[b]:
+                mask[starts[b]:starts[b + 1]] = torch.from_numpy(T.pack_bits(p, words)).cuda()
+    a = dict(q=rand(total, heads, dim).to(dtype), k=(rand(total, kv, dim) * strong).to(dtype), v=rand(total, kv, dim).to(dtype), cache=cache,
+             tables=tables, lengths=_i32(ls), starts=_i32(starts), mask=mask)
+    return a, starts, bits
+
+
+def _check_attention(a, ls, starts, bits, window=None, sinks=0, **kw):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention_int4
+
+    st = DeviceStatus()
+    total, heads = a["q"].shape[:2]
+    lse = torch.full((total, heads), 7.0, device="cuda")
+    out = tree_attention_int4(**a, window=window, sinks=sinks, lse=lse, status=st, **kw)
+    st.check_status()
+    n = starts[-1]
+    want, want_lse, tol, lse_tol = U.attention(a["q"], a["k"], a["v"], a["cache"].data, a["cache"].dtype, a["tables"].tolist(), ls, starts, bits,
+                                               window or 0, sinks, kw.get("scale"))
+    assert U.close(out[:n], want[:n], tol[:n]), ((out[:n].double() - want[:n]).abs() / tol[:n]).nan_to_num(0).max()
+    assert U.close(lse[:n], want_lse[:n], lse_tol[:n])
+    assert bool((lse[n:] == 7.0).all())
+    return out
+
+
+@pytest.mark.parametrize("ns,ls,heads,kv,dim,page,dtype,tree", [
+    ([1], [523], 28, 4, 128, 16, BF, False), ([1], [0], 4, 4, 64, 8, HF, False), ([1, 1, 1, 1], [1, 31, 32, 33], 8, 2, 128, 8, BF, False),
+    ([1] * 9, [2000, 90, 0, 700, 64, 1, 1024, 1025, 300], 28, 4, 128, 64, BF, False), ([1] * 3, [6000, 5, 4000], 12, 1, 64, 48, HF, False),
+    ([5, 0, 17, 1], [100, 50, 333, 2000], 32, 32, 128, 64, BF, True), ([64, 40], [900, 4100], 8, 8, 128, 64, BF, True),
+    ([33, 70], [40, 1500], 28, 4, 128, 16, HF, True), ([3, 2], [500, 0], 16, 2, 64, 24, HF, False), ([100, 31, 0], [77, 0, 9], 5, 5, 128, 128, BF, False),
+    ([1, 2], [300, 1200], 64, 1, 64, 16, BF, False), ([2], [3000], 80, 1, 128, 32, HF, True), ([8] * 40, list(range(0, 400, 10)), 4, 4, 64, 16, BF, True)])
+def test_attention(ns, ls, heads, kv, dim, page, dtype, tree):
+    a, starts, bits = _attention_case(ns, ls, heads, kv, dim, page, dtype, tree, sum(ns) + heads)
+    _check_attention(a, ls, starts, bits)
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (7, 0), (16, 1), (32, 4), (100, 0), (100, 40), (128, 128), (1000, 8), (5000, 4)])
+@pytest.mark.parametrize("ns,ls,heads,kv,dim,page,dtype,tree", [
+    ([1] * 6, [0, 1, 40, 129, 2000, 1023], 8, 2, 128, 16, BF, False), ([6, 40, 1], [90, 300, 1500], 4, 4, 64, 8, HF, False),
+    ([20, 64, 3], [0, 700, 1300], 14, 2, 128, 48, BF, True)])
+def test_attention_window(ns, ls, heads, kv, dim, page, dtype, tree, window, sinks):
+    a, starts, bits = _attention_case(ns, ls, heads, kv, dim, page, dtype, tree, sum(ns) + window)
+    _check_attention(a, ls, starts, bits, window, sinks)
