@@ -58,6 +58,7 @@ SIGNATURES: dict[str, tuple] = {
     "af_evict_cache": (_i32, [_vp, _vp, _vp]),
     "af_tree_attention_int4": (_i32, [_vp, _vp, _vp]),
     "af_tree_attention_int4_workspace_bytes": (_i32, [_vp]),
+    "af_attention_weights": (_i32, [_vp, _vp, _vp]),
 }
 
 _lib = None

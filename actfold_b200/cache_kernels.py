@@ -28,12 +28,13 @@ import torch
 
 from actfold_b200 import _lib
 from actfold_b200.kernels import DeviceStatus
-from actfold_b200.tree_kernels import _launch, _not_vectors, _row_grid, _same_device, _word
+from actfold_b200.tree_kernels import _grid, _launch, _not_vectors, _row_grid, _same_device, _word
 
 _I32, _I64 = torch.int32, torch.int64
 _CACHE = "q3q6q"
 _ROWS = struct.Struct("2q3q3q2q2q" + _CACHE)
 _ATTENTION = struct.Struct("3q2q2q2q" + _CACHE + "3q2q3q5qdq2qq2q")
+_WEIGHTS = struct.Struct("q2q" + _CACHE + "q3q2q5qdqq2qq")
 _EVICT = struct.Struct(_CACHE + "2q4q4q5q3q2qq3qq3q3q")
 _NO_CACHE = (0,) * 10
 
@@ -350,6 +351,71 @@ def tree_attention_int4(
         workspace.data_ptr(), size)
     _launch("tree_attention_int4", index, _lib.load().af_tree_attention_int4, args, _lib.ptr(word))
     return out
+
+
+def attention_weights(
+    q: torch.Tensor,
+    cache: Int4Cache | torch.Tensor,
+    tables: torch.Tensor,
+    lengths: torch.Tensor,
+    starts: torch.Tensor,
+    lse: torch.Tensor,
+    weights: torch.Tensor,
+    window: int | None = None,
+    sinks: int = 0,
+    scale: float | None = None,
+    status: DeviceStatus | None = None,
+) -> torch.Tensor:
+    """Add the attention that rows give to every cached token to ``weights``, in place; returns ``weights``.
+
+    ``weights`` float32 [requests, kv_heads, places]: entry (b, h, p) grows by the sum, over request b's rows and the query heads
+    of group h, of ``exp(scale * q . k_p - lse)`` for the places p < ``lengths[b]`` that the row sees. ``q`` [nodes, heads, dim]
+    and ``lse`` float32 [nodes, heads], as :func:`~actfold_b200.tree_kernels.tree_attention` or :func:`tree_attention_int4` left
+    them for these rows; request b's rows ``starts[b] .. starts[b + 1]`` follow one another (a prompt, one token, or the accepted path
+    of a tree), and ``window``, ``sinks`` and ``scale`` are that call's. ``cache`` is one layer: an :class:`Int4Cache` or a 16-bit
+    k_cache [pages, page_size, kv_heads, dim]. :func:`evict_cache` takes the weights.
+    """
+    packed = isinstance(cache, Int4Cache)
+    if packed:
+        if cache.layers is not None:
+            raise ValueError("attention_weights: cache must be one layer (cache[l])")
+        keys, dtype, kv, dim, parts, token = cache.data, cache.dtype, cache.kv_heads, cache.dim, cache._packed, 0
+    else:
+        if cache.dim() != 4 or cache.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"attention_weights: cache must be an Int4Cache or 16-bit [pages, page_size, kv_heads, dim], got {cache.dtype} {tuple(cache.shape)}")
+        pages, page, kv, dim = cache.shape
+        if page == 0 or page % 8 or dim not in (64, 128) or kv == 0:
+            raise ValueError(f"attention_weights: page_size {page} must be a positive multiple of 8, dim {dim} 64 or 128")
+        if (grid := _grid(cache)) is None:
+            raise ValueError("attention_weights: the cache's innermost dimension must be contiguous, its other strides multiples of 16 bytes")
+        keys, dtype = cache, cache.dtype
+        parts, token = (cache.data_ptr(), 0, grid[0], grid[2], 1, pages, page, kv, dim, _lib.DTYPE[dtype]), grid[1]
+    total, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+    if q.dim() != 3 or q.dtype is not dtype or q.shape[2] != dim or heads == 0 or heads % kv:
+        raise ValueError(f"attention_weights: q {q.dtype} {tuple(q.shape)} and cache {dtype} {tuple(keys.shape)} do not match")
+    batch, most = _check_tables("attention_weights", tables, lengths)
+    if starts.dtype is not _I32 or starts.dim() != 1:
+        _not_vectors("attention_weights", _I32, starts=starts)
+    if starts.shape[0] != batch + 1:
+        raise ValueError(f"attention_weights: {batch} requests need one entry of starts more")
+    if lse.dtype is not torch.float32 or lse.shape != (total, heads):
+        raise ValueError(f"attention_weights: lse must be float32 [{total}, {heads}], got {lse.dtype} {tuple(lse.shape)}")
+    if weights.dtype is not torch.float32 or weights.dim() != 3 or weights.shape[:2] != (batch, kv):
+        raise ValueError(f"attention_weights: weights must be float32 [{batch}, {kv}, places], got {weights.dtype} {tuple(weights.shape)}")
+    places = weights.shape[2]
+    if (places > 1 and weights.stride(2) != 1) or any(s == 0 and n > 1 for s, n in zip(weights.stride(), weights.shape)):
+        raise ValueError("attention_weights: the innermost dimension of weights must be contiguous, and its entries must not share memory")
+    window = _check_window("attention_weights", window, sinks)
+    index = _same_device("attention_weights", q, keys, tables, lengths, starts, lse, weights, word := _word(status))
+    if most > 1 and tables.stride(1) != 1:
+        tables = tables.contiguous()
+    lengths, starts, lse = lengths.contiguous(), starts.contiguous(), lse.contiguous()
+    q, q_grid = _rows16(q)
+    args = _WEIGHTS.pack(q.data_ptr(), *q_grid, *parts, token, tables.data_ptr(), tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(),
+                         starts.data_ptr(), batch, total, heads, window, sinks, dim ** -0.5 if scale is None else scale, lse.data_ptr(),
+                         weights.data_ptr(), weights.stride(0), weights.stride(1), places)
+    _launch("attention_weights", index, _lib.load().af_attention_weights, args, _lib.ptr(word))
+    return weights
 
 
 _scratch: dict[int, int] = {}  # bytes of scratch per device

@@ -1,0 +1,260 @@
+// The attention that cached tokens are given, added up (sm_100a).
+//
+//   weights[b, h, p] += sum over the request's rows i and the query heads of group h of exp(scale q_i . k_p - lse_i)
+//
+// over the places p that row i sees. The rows' sums are known (lse), so keys
+// are independent: a warp takes 32 of them, all rows of the request against
+// 16 at a time in registers (m16n8k16, the keys as the M side: few rows waste little), and adds to their
+// weights without atomics. With few rows HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and
+// 8 of its weight; with many the products do. See int4_attention.cu for the fragments' order.
+#include <string>
+
+#include "int4_attention.cuh"
+
+namespace af {
+namespace kv4 {
+namespace {
+
+constexpr int kUnit = 32, kThreads = 256, kCtas = 3;  // keys of a unit; CTAs per SM
+
+struct WeightArgs {
+  Params p;                     // q, tables, lengths, starts, window, sinks, scale; data: the cache
+  int64_t d_token;              // 16-bit keys: byte stride of a token
+  const float* lse;             // [total, heads]
+  float* weights;
+  int64_t w_request, w_head;    // strides in elements
+  int64_t places;
+};
+
+__device__ __forceinline__ int units_of(const WeightArgs& a, int b, Request<kUnit>& r) {
+  r = request<kUnit>(a.p, b);
+  r.bad |= r.len > a.places;
+  return r.bad || r.n == 0 ? 0 : r.cached * a.p.kv_heads;
+}
+
+template <int DT>
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (DT == AF_DTYPE_BF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+
+template <int DT, int HD, bool INT4>
+__global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_constant__ WeightArgs a) {
+  using B = Block<HD>;
+  constexpr int W = kThreads / 32, KS = HD / 16;
+  __shared__ int s_share[4];  // first unit, the one behind the last; the request that the share begins with, and the units before it
+  const Params& p = a.p;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  Request<kUnit> r;
+  if (warp == 0) {
+    bool disorder = false;
+    int all = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+      all += units_of(a, b, r);
+      disorder |= p.starts[b + 1] < p.starts[b];
+      if (r.bad && blockIdx.x == 0 && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (__any_sync(0xffffffffu, disorder)) all = 0;  // rows of several requests: no work
+    const int each = all / (int)gridDim.x, more = all - each * (int)gridDim.x, c = blockIdx.x;
+    const int first = each * c + min(c, more), end = each * (c + 1) + min(c + 1, more);
+    int before = 0, b0 = 0;
+    if (first < end) {
+      for (;; b0 += 32) {
+        int upto = b0 + lane < p.batch ? units_of(a, b0 + lane, r) : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += y;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, first < before + upto);
+        if (behind) {
+          const int x = __ffs(behind) - 1;
+          b0 += x;
+          before += x ? __shfl_sync(0xffffffffu, upto, x - 1) : 0;
+          break;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) s_share[0] = first, s_share[1] = end, s_share[2] = b0, s_share[3] = before;
+  }
+  __syncthreads();
+  const int end = s_share[1];
+  int b = s_share[2], before = s_share[3];
+  if (s_share[0] + warp >= end) return;
+  int of = units_of(a, b, r);
+  const int kap = !INT4 ? g : g & 1 ? 4 + ((g >> 1) ^ 1) : g >> 1;
+#pragma unroll 1
+  for (int u = s_share[0] + warp; u < end; u += W) {
+#pragma unroll 1
+    while (u >= before + of) {
+      before += of;
+      of = units_of(a, ++b, r);
+    }
+    const int h = (u - before) / r.cached, x = (u - before) - h * r.cached;
+    const int place = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from);
+    const int* table = p.tables + (int64_t)b * p.tables_ld;
+    // The lane adds up the weight of one key: row kap of block t.
+    const int mine = place + 8 * t + kap;
+    float* at_weight = a.weights + b * a.w_request + h * a.w_head + mine;
+    const float old = mine < r.len ? *at_weight : 0.f;
+    float given = 0.f;
+    const int rows = r.n * p.group, first_all = p.window ? max(0, r.len - max(0, p.window - r.n)) : 0;
+    const bool masked = place + kUnit > r.len || (p.window && place < first_all && place + kUnit > p.sinks);
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      if (place + 16 * half >= r.len) break;
+      uint32_t k[KS][4];  // the operand: keys kap of two blocks, the 32 (16) dims that the lane takes
+      bool bad = false;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int at = place + 16 * half + 8 * y, entry = at / p.page, off = at - entry * p.page;
+        const int page = at < r.len ? table[entry] : 0;
+        const bool there = page >= 0 && page < p.pages && at < r.len;
+        bad |= page < 0 || page >= p.pages;
+        const char* from = p.data + (there ? page : 0) * p.d_page + h * p.d_head;
+        if constexpr (INT4) {
+          from += (int64_t)(off / kBlockTokens) * B::kBytes;
+          uint32_t w[HD / 32], pr = 0;
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) w[i] = 0;
+          if (there) {
+            const char* words = from + B::word(kap, HD / 32 * t);
+            if constexpr (HD == 128) {
+              const uint4 v = *reinterpret_cast<const uint4*>(words);
+              w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(words);
+              w[0] = v.x, w[1] = v.y;
+            }
+            pr = *reinterpret_cast<const uint32_t*>(from + B::pair(kap, (HD / 4) * t / kGroup));
+          }
+          const uint32_t s2 = __byte_perm(pr, 0, 0x1010), o2 = __byte_perm(pr, 0, 0x3232);
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            k[2 * i][y] = two_values<DT, 0>(w[i], s2, o2);
+            k[2 * i][2 + y] = two_values<DT, 1>(w[i], s2, o2);
+            k[2 * i + 1][y] = two_values<DT, 2>(w[i], s2, o2);
+            k[2 * i + 1][2 + y] = two_values<DT, 3>(w[i], s2, o2);
+          }
+        } else {
+          from += (int64_t)(off + kap) * a.d_token + t * (HD / 2);
+          const bool row = there && at + kap < r.len;
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) {
+            const uint4 v = row ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+            k[2 * i][y] = v.x, k[2 * i][2 + y] = v.y, k[2 * i + 1][y] = v.z, k[2 * i + 1][2 + y] = v.w;
+          }
+        }
+      }
+      if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+      float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+      for (int row0 = 0; row0 < rows; row0 += 8) {
+        const int flat = row0 + g;
+        const char* q_at = p.q + (int64_t)(r.s0 + flat / p.group) * p.q_n + (h * p.group + flat % p.group) * p.q_h + t * (HD / 2);
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < KS / 2; ++i) {
+          const uint4 v = flat < rows ? *reinterpret_cast<const uint4*>(q_at + 16 * i) : make_uint4(0, 0, 0, 0);
+          mma<DT>(c, k[2 * i], v.x, v.y);
+          mma<DT>(c, k[2 * i + 1], v.z, v.w);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = row0 + 2 * t + e, node = row / p.group;
+          const float lse = row < rows ? a.lse[(int64_t)(r.s0 + node) * p.heads + h * p.group + row % p.group] : -INFINITY;
+          const int first = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int at = place + 16 * half + 8 * y + kap;
+            const bool sees = !masked || (at < r.len && (at >= first || at < p.sinks));
+            if (sees && lse != -INFINITY) sum[y] += ex2(fmaf(c[2 * y + e], p.scale, lse * -1.4426950408889634f));
+          }
+        }
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
+        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
+        if (t == 2 * half + y) given = sum[y];
+      }
+    }
+    if (mine < r.len) *at_weight = old + given;
+  }
+}
+
+template <int DT, int HD>
+void launch(const WeightArgs& a, bool int4, cudaStream_t s) {
+  const int ctas = sm_count() * kCtas;
+  if (int4) k_weights<DT, HD, true><<<ctas, kThreads, 0, s>>>(a);
+  else k_weights<DT, HD, false><<<ctas, kThreads, 0, s>>>(a);
+}
+
+}  // namespace
+}  // namespace kv4
+}  // namespace af
+
+using namespace af;
+
+extern "C" int af_attention_weights(const af_attention_weights_args* args, uint32_t* status, void* stream) {
+  AF_REQUIRE(args, "af_attention_weights: null pointer");
+  const af_attention_weights_args& w = *args;
+  const af_int4_cache& c = w.cache;
+  AF_REQUIRE(w.batch >= 0 && w.total >= 0 && w.max_pages >= 0 && w.places >= 0 && c.pages >= 0, "af_attention_weights: bad shape");
+  AF_REQUIRE(w.n_heads > 0 && c.heads > 0 && w.n_heads % c.heads == 0, "af_attention_weights: n_heads must be a multiple of the cache's heads");
+  AF_REQUIRE(c.head_dim == 64 || c.head_dim == 128, "af_attention_weights: head_dim must be 64 or 128");
+  AF_REQUIRE(c.dtype == AF_DTYPE_F16 || c.dtype == AF_DTYPE_BF16, "af_attention_weights: dtype must be fp16 or bf16");
+  AF_REQUIRE(c.page_size > 0 && c.page_size % kv4::kBlockTokens == 0 && c.page_size <= (1 << 20), "af_attention_weights: page_size must be a multiple of 8");
+  AF_REQUIRE(w.window >= 0 && w.sinks >= 0 && w.window <= (1 << 30) && w.sinks <= (1 << 30), "af_attention_weights: window and sinks must not be negative");
+  AF_REQUIRE(w.total <= (1 << 28) && c.pages <= 0x7fffffff && w.n_heads <= (1 << 16) && w.max_pages <= (1 << 30) && w.max_pages * c.page_size <= (1 << 30) &&
+                 w.total * (w.n_heads / c.heads) <= (1 << 30) && w.batch <= (1 << 20),
+             "af_attention_weights: size too large");
+  if (w.batch == 0 || w.total == 0 || w.max_pages == 0 || c.pages == 0) return AF_OK;
+  AF_REQUIRE(w.q && c.data && w.tables && w.lengths && w.starts && w.lse && (w.places == 0 || w.weights), "af_attention_weights: null pointer");
+  AF_REQUIRE((double)c.heads * w.batch * (w.max_pages * c.page_size / kv4::kUnit + 2) < 2147483000.0, "af_attention_weights: more than 2^31 units of 32 keys");
+  uint64_t al = reinterpret_cast<uintptr_t>(w.q) | reinterpret_cast<uintptr_t>(c.data) | (uint64_t)w.q_strides[0] | (uint64_t)w.q_strides[1] |
+                (uint64_t)c.strides[1] | (uint64_t)c.strides[2] | (uint64_t)w.token_stride;
+  AF_REQUIRE((al & 15) == 0, "af_attention_weights: addresses and strides must be multiples of 16 bytes");
+  kv4::WeightArgs a;
+  memset(&a, 0, sizeof(a));
+  kv4::Params& p = a.p;
+  p.q = static_cast<const char*>(w.q), p.q_n = w.q_strides[0], p.q_h = w.q_strides[1];
+  p.data = static_cast<const char*>(c.data), p.d_page = c.strides[1], p.d_head = c.strides[2];
+  p.tables = w.tables;
+  p.tables_ld = w.tables_stride;
+  p.lengths = w.lengths;
+  p.starts = w.starts;
+  p.batch = (int)w.batch;
+  p.total = (int)w.total;
+  p.heads = (int)w.n_heads;
+  p.kv_heads = (int)c.heads;
+  p.group = (int)(w.n_heads / c.heads);
+  p.pages = (int)c.pages;
+  p.page = (int)c.page_size;
+  p.capacity = w.max_pages * c.page_size;
+  p.window = (int)w.window;
+  p.sinks = (int)w.sinks;
+  p.scale = (float)(w.scale * 1.4426950408889634);
+  p.rows = 8;
+  p.status = status;
+  a.d_token = w.token_stride;
+  a.lse = w.lse;
+  a.weights = w.weights;
+  a.w_request = w.weights_strides[0], a.w_head = w.weights_strides[1];
+  a.places = w.places;
+  cudaStream_t s = as_stream(stream);
+  const bool int4 = w.token_stride == 0;
+  if (c.dtype == AF_DTYPE_BF16) c.head_dim == 128 ? kv4::launch<AF_DTYPE_BF16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_BF16, 64>(a, int4, s);
+  else c.head_dim == 128 ? kv4::launch<AF_DTYPE_F16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_F16, 64>(a, int4, s);
+  return check_launch("af_attention_weights");
+}

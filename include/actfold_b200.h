@@ -710,6 +710,38 @@ int af_tree_attention_int4(const af_tree_attention_int4_args* a, uint32_t* statu
 /* Bytes of scratch that af_tree_attention_int4 needs on the current device. */
 int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
 
+/*
+ * af_attention_weights -- the attention that cached tokens are given.
+ *
+ * weights[b, h, p] += sum over the request's rows i (a chain: [starts[b],
+ * starts[b + 1])) and the query heads of group h of exp(scale * q_i . k_p -
+ * lse_i), for the places p < lengths[b] that row i sees (window and sinks as
+ * in af_tree_attention_int4 without a mask). lse [total, n_heads]: natural log
+ * of each row's sum of exponentials, as the attention leaves it; a row of
+ * -inf gives nothing. The cache is one layer: 4-bit blocks where token_stride is 0, else
+ * 16-bit keys [page, token, head] with strides cache.strides[1], token_stride,
+ * cache.strides[2] (bytes). weights strides in elements: request, head; places entries. A
+ * length above places or the table's capacity, or a page out of range, sets AF_STATUS_BOUNDS: the
+ * request is skipped, such a page's keys read as zeros. Sums are held in 32 bits,
+ * in an order that does not change.
+ */
+typedef struct {
+  const void* q;
+  int64_t q_strides[2]; /* node, head: bytes */
+  af_int4_cache cache;
+  int64_t token_stride;
+  const int32_t* tables;
+  int64_t tables_stride, max_pages; /* elements */
+  const int32_t *lengths, *starts;
+  int64_t batch, total, n_heads, window, sinks;
+  double scale;
+  const float* lse;
+  float* weights;
+  int64_t weights_strides[2], places;
+} af_attention_weights_args;
+
+int af_attention_weights(const af_attention_weights_args* a, uint32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

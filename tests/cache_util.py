@@ -158,3 +158,30 @@ def close(got, want, tol) -> bool:
     """Within the allowed error; NaN and infinities in the same places."""
     same = (got.double() == want) | (got.isnan() & want.isnan())
     return bool((same | ((got.double() - want).abs() <= tol)).all())
+
+
+def weights(q, keys, slots, lengths, starts, lse, old, window=0, sinks=0, scale=None):
+    """(sums, allowed error) in 64 bits of the attention that cached tokens are given. keys [slots, kv, dim], slots: per request.
+
+    A term exp(s - lse) is off by a factor of e^d, d = dim * 2^-23 * S + 2^-24 * 4 (|s| + |lse| + 1) + 2^-22 (see attention),
+    each addition by 2^-24 of what has been added up.
+    """
+    total, heads, dim = q.shape
+    kv = keys.shape[1]
+    scale = dim ** -0.5 if scale is None else scale
+    out, tol = old.double().clone(), torch.zeros(old.shape, dtype=torch.float64, device=q.device)
+    for b, t in enumerate(lengths):
+        lo, hi = starts[b], starts[b + 1]
+        see = visible(hi - lo, t, None, window, sinks)[:, :t].to(q.device)
+        for h in range(heads):
+            g = h * kv // heads
+            k = torch.where(see.any(0)[:, None], keys[slots[b], g].double(), 0.0)
+            x = q[lo:hi, h].double()
+            s = (x @ k.T) * scale
+            y = lse[lo:hi, h, None].double()
+            p = torch.where(see & (y != -math.inf), torch.exp(s - y), 0.0)
+            d = dim * 2.0 ** -23 * (x.abs() @ k.abs().T) * abs(scale) + 2.0 ** -22 * (s.abs() + y.abs().nan_to_num(0, 0, 0) + 1) + 2.0 ** -22
+            out[b, g, :t] += p.sum(0)
+            tol[b, g, :t] += torch.where(p > 0, p * d.exp() * d, 0.0).sum(0)
+    rows = (max((hi - lo for lo, hi in zip(starts, starts[1:])), default=0)) * heads // kv
+    return out, tol + (rows + 2) * 2.0 ** -24 * out.abs()

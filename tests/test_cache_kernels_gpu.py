@@ -339,3 +339,51 @@ def test_attention(ns, ls, heads, kv, dim, page, dtype, tree):
 def test_attention_window(ns, ls, heads, kv, dim, page, dtype, tree, window, sinks):
     a, starts, bits = _attention_case(ns, ls, heads, kv, dim, page, dtype, tree, sum(ns) + window)
     _check_attention(a, ls, starts, bits, window, sinks)
+
+
+# ------------------------------------------------------------------------------------------------ weights
+@pytest.mark.parametrize("ns,ls,heads,kv,dim,page,dtype,held,window,sinks", [
+    ([1], [1500], 28, 4, 128, 16, BF, 4, None, 0), ([1, 0, 5, 12], [1, 40, 0, 700], 8, 2, 64, 8, HF, 4, None, 0),
+    ([3] * 9, [2000, 90, 0, 700, 64, 1, 1024, 33, 31], 28, 4, 128, 64, BF, 4, None, 0), ([3] * 5, [2000, 90, 15, 16, 17], 32, 32, 128, 64, BF, 16, None, 0),
+    ([9, 1, 2], [300, 1, 77], 12, 1, 64, 48, HF, 16, None, 0), ([4, 9, 1], [600, 100, 40], 10, 5, 128, 24, HF, 4, 50, 4),
+    ([4, 9, 1], [600, 100, 40], 10, 5, 64, 24, BF, 16, 5, 0), ([40, 2], [3000, 5], 4, 4, 128, 16, BF, 4, 700, 100), ([200], [129], 14, 2, 128, 8, BF, 4, None, 0)])
+def test_weights(ns, ls, heads, kv, dim, page, dtype, held, window, sinks):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import attention_weights, read_cache_int4
+
+    a, starts, _ = _attention_case(ns, ls, heads, kv, dim, page, dtype, False, sum(ls) + heads, extra_rows=2)
+    slots = [a["tables"][b].long()[torch.arange(t, device="cuda") // page] * page + torch.arange(t, device="cuda") % page for b, t in enumerate(ls)]
+    pool = a["cache"].pages * page
+    keys = read_cache_int4(a["cache"], torch.arange(pool, device="cuda"))[0]
+    cache = a["cache"] if held == 4 else keys.view(-1, page, kv, dim)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    lse = 5 + 2 * torch.randn(starts[-1] + 2, heads, device="cuda", generator=g)
+    lse[0, 0] = -math.inf
+    wide = torch.rand(len(ls), kv + 1, max(ls) + 40, device="cuda", generator=g)
+    w = wide[:, :kv, 1: max(ls) + 4]
+    before = wide.clone()
+    st = DeviceStatus()
+    got = attention_weights(a["q"], cache, a["tables"], a["lengths"], a["starts"], lse, w, window=window, sinks=sinks, status=st)
+    st.check_status()
+    assert got is w
+    want, tol = U.weights(a["q"], keys, slots, ls, starts, lse, before[:, :kv, 1: max(ls) + 4], window or 0, sinks)
+    assert U.close(w, want, tol), ((w.double() - want).abs() / tol).nan_to_num(0).max()
+    wide[:, :kv, 1: max(ls) + 4] = before[:, :kv, 1: max(ls) + 4]
+    assert torch.equal(wide, before)  # nothing beside
+    for b, t in enumerate(ls):
+        assert torch.equal(got[b, :, t:], before[b, :kv, 1 + t: max(ls) + 4])
+
+
+def test_weights_are_those_of_the_attention():
+    """Every row's weights over the prefix and its own nodes sum to one: what the prefix is given is what the chain's tree is not."""
+    from actfold_b200.speculative import attention_weights, tree_attention_int4
+
+    ls, heads, kv = [700, 64, 1], 8, 2
+    a, starts, _ = _attention_case([1, 1, 1], ls, heads, kv, 128, 16, BF, False, 5)
+    lse = torch.empty(3, heads, device="cuda")
+    tree_attention_int4(**a, lse=lse)
+    w = torch.zeros(3, kv, 700, device="cuda")
+    attention_weights(a["q"], a["cache"], a["tables"], a["lengths"], a["starts"], lse, w)
+    own = torch.einsum("bhd,bhd->bh", a["q"].double(), a["k"].double().repeat_interleave(heads // kv, 1)) * 128 ** -0.5
+    left = (1 - torch.exp(own - lse.double())).view(3, kv, -1).sum(-1)
+    assert bool(((w.double().sum(-1) - left).abs() <= 2.0 ** -14).all())  # 700 keys, scores below 32: 2^-23 * 128 * 32 * 4 terms
