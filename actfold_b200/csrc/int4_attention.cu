@@ -89,7 +89,7 @@ __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t b
   planner.begin(p, lane);
   Segment s;
   bool ok = true;
-  int j = 0;  // units so far
+  int j = 0, issued = 0;  // units so far; the number behind the lane's last one
 #pragma unroll 1
   for (int seg = 0; ok; ++seg) {
     const bool more = planner.next(p, s);
@@ -105,59 +105,55 @@ __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t b
     const char* head = p.data + s.kvh * p.d_head;
 #pragma unroll 1
     for (int x0 = s.x0; ok && x0 < s.x1; x0 += 32) {
-      // Lane x knows the pages of unit x0 + x; the lanes issue in turn, as slots fall empty.
-      const int x = x0 + lane, count = min(32, s.x1 - x0);
+      // Lane x knows where unit x0 + x lies: the first run of blocks within a page, and the entries of the others.
+      const int x = x0 + lane;
       const int place = kUnit * (x < s.sink_units ? x : x - s.sink_units + s.from);
       const int tokens = x < s.x1 && x < s.cached ? min(kUnit, s.len - place) : 0;
-      int pages[kMostRuns], blocks[kMostRuns];  // runs of blocks within a page
-      const int entry0 = tokens ? place / p.page : 0, off0 = place - entry0 * p.page;
-      {
-        int left = (tokens + kBlockTokens - 1) / kBlockTokens, entry = entry0, room = (p.page - off0) / kBlockTokens;
-#pragma unroll
-        for (int i = 0; i < kMostRuns; ++i) {
-          blocks[i] = min(left, room);
-          pages[i] = blocks[i] ? table[entry] : 0;
-          left -= blocks[i];
-          ++entry;
-          room = p.page / kBlockTokens;
-        }
-      }
+      const int all = (tokens + kBlockTokens - 1) / kBlockTokens;
+      const int entry = tokens ? place / p.page : 0, at = (place - entry * p.page) / kBlockTokens;
+      const int run = min(all, p.page / kBlockTokens - at);
+      const int page = tokens ? table[entry] : 0;
+      bool sound = page >= 0 && page < p.pages;
+      const char* from = head + page * p.d_page + (int64_t)at * kBlock;
+      const int me = j + lane, slot = me % kSlots;
+      const uint32_t bar = full + 8 * slot, to = base + slot * S::kUnitBytes;
+      const int count = min(32, s.x1 - x0);
+      // Eight slots at a time, so that the others stay filled meanwhile.
 #pragma unroll 1
-      for (int i = 0; i < count; ++i, ++j) {
-        const int slot = j % kSlots;
-        if (j >= kSlots) ok = __all_sync(0xffffffffu, wait_for(empty + 8 * slot, (j / kSlots - 1) & 1, failed));
+      for (int i = 0; i < count; i += 8) {
+        const bool mine = lane >= i && lane < min(count, i + 8);
+        ok = __all_sync(0xffffffffu, !mine || me < kSlots || wait_for(empty + 8 * slot, (me / kSlots - 1) & 1, failed));
         if (!ok) break;
-        if (lane == i) {
-          const uint32_t bar = full + 8 * slot;
-          if (tokens == 0) {
+        if (mine) {
+          if (all == 0) {
             mbar_arrive(bar);  // the step's own nodes: nothing to bring
+          } else if (run == all && sound) {
+            mbar_arrive_expect_tx(bar, all * kBlock);
+            bulk_copy(to, from, all * kBlock, bar);
           } else {
+            // Several pages, or one out of range, which reads as zeros.
             uint32_t bytes = 0;
-            bool bad = false;
-#pragma unroll
-            for (int y = 0; y < kMostRuns; ++y) {
-              const bool there = pages[y] >= 0 && pages[y] < p.pages;
-              bad |= blocks[y] && !there;
-              if (there) bytes += blocks[y] * kBlock;
+            for (int y = 0, e = entry, n = run; y < all; y += n, ++e, n = min(all - y, p.page / kBlockTokens)) {
+              const int pg = table[e];
+              if (pg >= 0 && pg < p.pages) bytes += n * kBlock;
             }
-            if (bad) {  // a page out of range reads as zeros
+            if (bytes < (uint32_t)(all * kBlock)) {
               if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
               uint4* z = reinterpret_cast<uint4*>(gb + slot * S::kUnitBytes);
               for (int y = 0; y < S::kUnitBytes / 16; ++y) z[y] = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
             }
             mbar_arrive_expect_tx(bar, bytes);
-            uint32_t dst = base + slot * S::kUnitBytes;
-#pragma unroll
-            for (int y = 0; y < kMostRuns; ++y) {
-              if (blocks[y] && pages[y] >= 0 && pages[y] < p.pages)
-                bulk_copy(dst, head + pages[y] * p.d_page + (int64_t)(y ? 0 : off0 / kBlockTokens) * kBlock, blocks[y] * kBlock, bar);
-              dst += blocks[y] * kBlock;
+            for (int y = 0, e = entry, n = run; y < all; y += n, ++e, n = min(all - y, p.page / kBlockTokens)) {
+              const int pg = table[e];
+              if (pg >= 0 && pg < p.pages) bulk_copy(to + y * kBlock, head + pg * p.d_page + (int64_t)(y ? 0 : at) * kBlock, n * kBlock, bar);
             }
           }
+          issued = me + 1;
         }
         __syncwarp();
       }
+      j += count;
     }
   }
   if (!ok) {
@@ -165,12 +161,11 @@ __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t b
     if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
   }
   __syncwarp();
-  if (lane == 0) {
-    // Copies still in flight (there are some only when a wait ran out) land before the CTA's shared memory is given up (bounded).
-    volatile int by_itself[2] = {0, kPatience};
-#pragma unroll 1
-    for (int i = max(0, j - kSlots); i < j; ++i) wait_for(full + 8 * (i % kSlots), (i / kSlots) & 1, by_itself);
-  }
+  // Copies still in flight (there are some only when a wait ran out) land before the CTA's shared memory is given up (bounded):
+  // of the last kSlots units, one a lane.
+  const int last = __reduce_max_sync(0xffffffffu, issued), mine = last - kSlots + lane;
+  volatile int by_itself[2] = {0, kPatience};
+  if (mine >= 0) wait_for(full + 8 * (mine % kSlots), (mine / kSlots) & 1, by_itself);
   __syncwarp();
 }
 
@@ -589,19 +584,6 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
 }
 
-template <auto Kernel>
-int allow_smem(int bytes) {
-  static std::atomic<uint64_t> allowed{0};  // a bit per device
-  int device = 0;
-  cudaGetDevice(&device);
-  const uint64_t bit = 1ull << (device & 63);
-  if (allowed.load(std::memory_order_relaxed) & bit) return AF_OK;
-  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: ") + cudaGetErrorString(e));
-  allowed.fetch_or(bit, std::memory_order_relaxed);
-  return AF_OK;
-}
-
 template <int DT, int HD, int NT, int W>
 int launch(const Params& p, cudaStream_t s) {
   using S = Shape<HD, NT, W>;
@@ -620,7 +602,7 @@ int launch_rows(const Params& p, cudaStream_t s) {
   return p.rows == 8 ? launch<DT, HD, 1, 11>(p, s) : launch<DT, HD, 2, 7>(p, s);
 }
 
-int64_t workspace_bytes() { return Scratch<16, 128>::bytes(sm_count()); }
+int64_t workspace_bytes() { return Scratch<256, 128>::bytes(sm_count()); }
 
 int check_args(const af_tree_attention_int4_args& a) {
   const af_int4_cache& c = a.cache;
@@ -695,14 +677,19 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.ws = static_cast<char*>(a.workspace);
   p.status = status;
   p.patience = attention_patience();
-  p.rows = ceil_div(a.total, a.batch) * p.group <= 8 ? 8 : 16;
-  p.row_cost = 10;
-  p.whole = 32;
+  const int64_t rows = ceil_div(a.total, a.batch) * p.group;  // of the average request and head
+  const bool wide = rows > 16;
+  p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+  p.row_cost = wide ? 3 : 10;
+  p.whole = wide ? 8 : 32;
   // Units are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
-  AF_REQUIRE((double)c.heads * (ceil_div(a.total * p.group, p.rows) + a.batch) * ((a.max_pages * c.page_size + a.total) / kv4::kUnit + 3 + p.row_cost) < 2147483000.0,
-             "af_tree_attention_int4: more than 2^31 units of 32 keys");
+  AF_REQUIRE((double)c.heads * (ceil_div(a.total * p.group, p.rows) + a.batch) *
+                     ((a.max_pages * c.page_size + a.total) / (wide ? kv4::kWideUnit : kv4::kUnit) + 3 + p.row_cost) <
+                 2147483000.0,
+             "af_tree_attention_int4: more than 2^31 units of keys");
   cudaStream_t s = as_stream(stream);
   const bool bf16 = c.dtype == AF_DTYPE_BF16;
+  if (wide) return kv4::wide_launch(p, bf16, (int)c.head_dim, s);
   if (c.head_dim == 128) return bf16 ? kv4::launch_rows<AF_DTYPE_BF16, 128>(p, s) : kv4::launch_rows<AF_DTYPE_F16, 128>(p, s);
   return bf16 ? kv4::launch_rows<AF_DTYPE_BF16, 64>(p, s) : kv4::launch_rows<AF_DTYPE_F16, 64>(p, s);
 }

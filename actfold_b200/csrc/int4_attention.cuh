@@ -267,6 +267,23 @@ struct Scratch {
   }
 };
 
+constexpr int kWideUnit = 128;
+// The kernel for many rows (int4_attention_wide.cu).
+int wide_launch(const Params& p, bool bf16, int head_dim, cudaStream_t s);
+
+template <auto Kernel>
+int allow_smem(int bytes) {
+  static std::atomic<uint64_t> allowed{0};  // a bit per device
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (allowed.load(std::memory_order_relaxed) & bit) return AF_OK;
+  const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: ") + cudaGetErrorString(e));
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return AF_OK;
+}
+
 constexpr int kJoinThreads = 256;
 
 // Rows that several CTAs worked on: out = sum_c w_c O_c / sum_c w_c l_c with w_c = 2^(m_c - max m), in the CTAs' order. The

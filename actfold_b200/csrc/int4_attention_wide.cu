@@ -1,0 +1,743 @@
+// Attention over the 4-bit paged cache with many rows per key/value head
+// (sm_100a, tcgen05): the list of work and the joins of int4_attention.cuh, but the
+// rows are the M side (S [128 rows, 128 keys] = Q K^T, O += P V), because with
+// more than 16 rows a tile of keys is worth turning into 16 bits once, in
+// shared memory, for all rows.
+//
+// A CTA holds two "pipes", each a 128-row O and a 128-row S of 128 keys, over
+// which P is written in place (16 bits, TMEM operand of the second product).
+// With more than 128 rows they are two row tiles over the same keys; with
+// fewer, one row tile over the even and the odd key tiles, joined at the end.
+// Eight warps read the codes of the next tile into registers while they turn this
+// one's into values and write them where the tensor cores take them (a thread has half a key's
+// dims; 16-byte pieces, 128-byte swizzle): 64 KB a tile that go through shared memory twice, some
+// 1000 cycles of its 128 bytes, next to 512 cycles of products per pipe and of exponentials.
+// A softmax thread owns a row, so no scores are exchanged. The reference
+// maximum of a row is raised only when a score passes it by 2^8.
+//
+// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-15: keys and values;
+// warp 16 issues S, warp 17 O, warp 18 plans.
+#include "int4_attention.cuh"
+
+namespace af {
+namespace kv4 {
+
+namespace {
+
+constexpr int kUnit = kWideUnit;           // keys of a tile
+constexpr int kRows = 128;                 // rows of a pipe
+constexpr int kSoft = 8, kTurn = 8;        // warps
+constexpr int kMmaS = kSoft + kTurn, kMmaO = kMmaS + 1, kPlan = kMmaS + 2;
+constexpr int kThreads = 32 * (kPlan + 1);
+constexpr int kReaders = kSoft + kTurn + 2;  // of a plan
+constexpr int kStages = 2;                 // of keys, and of values
+constexpr int kPanel = kUnit * 128;        // [128 rows][64 columns] of 16 bits, 128-byte swizzle
+
+template <int HD>
+struct Wide {
+  static constexpr int kHalves = HD / 64;
+  static constexpr int kTile = kHalves * kPanel;  // a K, V or Q tile
+  static constexpr int kOffK = 0, kOffV = kStages * kTile, kOffQ = 2 * kStages * kTile;
+  static constexpr int kOffStat = kOffQ + 2 * kTile;                 // [2][128] (maximum, sum) of the pipes
+  static constexpr int kOffBar = kOffStat + 2 * kRows * 8;
+  static constexpr int kBars = 4 * kStages + 1 + 12 + 2 + 2 * kPlans + 1;
+  static constexpr int kOffPlan = (kOffBar + 8 * kBars + 15) / 16 * 16;
+  static constexpr int kOffMisc = kOffPlan + kPlans * (int)sizeof(Segment);  // tensor memory's address; failed, patience; found[kPlans]
+  static constexpr int kBytes = kOffMisc + 4 * (4 + kPlans);
+  static constexpr int kTmemO = 2 * kUnit;                           // O of pipe x at kTmemO + 128 x, S of pipe x at 128 x
+};
+
+__device__ __forceinline__ bool elect_one() {
+  int r;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.s32 %0, 1, 0, q;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// Pairs of fp32 values in one register pair (two results per instruction).
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// C consecutive columns of the thread's TMEM lane. Load and wait are one
+// statement: nothing that reads the registers can be placed between them.
+__device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+               "r"(r[13]), "r"(r[14]), "r"(r[15])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D [tmem] (+)= A [smem] * B [smem]^T.
+__device__ __forceinline__ void mma_from_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D [tmem] (+)= A [tmem, 16-bit pairs] * B [smem]^T.
+__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
+// Place of unit x of a segment's cached keys.
+__device__ __forceinline__ int place_of(const Segment& s, int x) { return kUnit * (x < s.sink_units ? x : x - s.sink_units + s.from); }
+
+// Not every row of the request sees all of these keys: the prefix's last ones, ones that only some windows hold, and nodes.
+__device__ __forceinline__ bool is_masked(const Params& p, const Segment& s, int x) {
+  if (x >= s.cached) return true;
+  const int place = place_of(s, x);
+  return place + kUnit > s.len || (p.window && place < s.len - max(0, p.window - s.n) && place + kUnit > p.sinks);
+}
+
+// Units of a segment that hold values that are not finite and that not all rows see: bit i stands for units i * 2^shift and on,
+// 2^shift of them, from the segment's first.
+__device__ __forceinline__ int found_shift(int units) { return max(0, 27 - __clz(units - 1 | 1)); }
+
+// Such values of dims d .. d + 7, added up for a row of node i, whose window begins at `first`.
+template <int DT, int HD>
+__device__ __noinline__ void set_aside(const Params& p, const Segment* plan, uint32_t found, int i, int first, int d, float* sum) {
+  using B = Block<HD>;
+  const Segment& s = *plan;
+  const int units = s.x1 - s.x0, shift = found_shift(units);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+#pragma unroll 1
+  for (; found; found &= found - 1) {
+    const int u0 = (__ffs(found) - 1) << shift;
+#pragma unroll 1
+    for (int x = s.x0 + u0; x < s.x0 + min(units, u0 + (1 << shift)); ++x) {
+      if (!is_masked(p, s, x)) continue;
+      if (x < s.cached) {
+        const int place0 = place_of(s, x);
+#pragma unroll 1
+        for (int at = place0; at < min(s.len, place0 + kUnit); ++at) {
+          if (at < first && at >= p.sinks) continue;
+          const int page = p.tables[(int64_t)s.b * p.tables_ld + at / p.page], off = at % p.page;
+          if (page < 0 || page >= p.pages) continue;
+          const uint32_t pr = *reinterpret_cast<const uint32_t*>(p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes +
+                                                                B::kPart + B::pair(off % kBlockTokens, d / kGroup));
+          if (not_finite<DT>(pr) || not_finite<DT>(pr >> 16))
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[e] = NAN;
+        }
+      } else {
+        const int n0 = kUnit * (x - s.cached);
+#pragma unroll 1
+        for (int j = n0; j < min(s.n, n0 + kUnit); ++j) {
+          if (!((seen_nodes(p, s.s0, s.n, i, j & ~31) >> (j & 31)) & 1u)) continue;
+          const uint4 v = *reinterpret_cast<const uint4*>(p.v + (int64_t)(s.s0 + j) * p.v_n + s.kvh * p.v_h + 2 * d);
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t b = (w[e / 2] >> (16 * (e & 1))) & 0xffffu;
+            if (not_finite<DT>(b)) sum[e] += from_bits<DT>(b);
+          }
+        }
+      }
+    }
+  }
+}
+
+// What a thread holds of a tile: the codes and pairs of half the dims of one key and value, or of a node's rows nothing yet.
+template <int HD>
+struct Codes {
+  static constexpr int kWords = HD / 16, kPairs = HD / 64;
+  uint32_t k[kWords], v[kWords], kp[kPairs], vp[kPairs];
+};
+
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __grid_constant__ Params p) {
+  using S = Wide<HD>;
+  using B = Block<HD>;
+  extern __shared__ __align__(1024) uint8_t gb[];
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = smem_u32(gb);
+  const uint32_t k_full = base + S::kOffBar, k_empty = k_full + 8 * kStages, v_full = k_empty + 8 * kStages, v_empty = v_full + 8 * kStages,
+                 q_full = v_empty + 8 * kStages, s_full = q_full + 8, p_full = s_full + 32, done = p_full + 32, o_full = done + 32, o_empty = o_full + 8,
+                 plan_full = o_empty + 8, plan_empty = plan_full + 8 * kPlans, drained = plan_empty + 8 * kPlans;
+  Segment* plans = reinterpret_cast<Segment*>(gb + S::kOffPlan);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gb + S::kOffMisc);
+  volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint32_t* found = tmem_slot + 4;  // per plan: units with values that are not finite
+
+  if (tid == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(k_full + 8 * i, kTurn);
+      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v_full + 8 * i, kTurn);
+      mbar_init(v_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {  // [pipe][half]
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4);
+      mbar_init(done + 8 * i, 1);
+    }
+    mbar_init(q_full, kSoft);
+    mbar_init(o_full, 1);
+    mbar_init(o_empty, kSoft);
+    for (int i = 0; i < kPlans; ++i) {
+      mbar_init(plan_full + 8 * i, 1);
+      mbar_init(plan_empty + 8 * i, kReaders);
+    }
+    mbar_init(drained, 2);
+    failed[0] = 0;
+    failed[1] = p.patience;
+    fence_barrier_init();
+  }
+  if (warp == kMmaS) tmem_alloc(smem_u32(tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Scratch<2 * kRows, HD> scratch{p.ws, (int)gridDim.x};
+  Segment s;
+  auto agreed = [](bool mine) { return (bool)__all_sync(0xffffffffu, mine); };
+  // Segment number `seg` as it was planned; false behind the last one. Its reader gives it back with read().
+  auto planned = [&](int seg, Segment& s) {
+    const bool there = agreed(wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed));
+    if (!there) *failed = 1;
+    s = plans[seg % kPlans];
+    return there && s.x1 > 0;
+  };
+  auto read = [&](int seg) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(plan_empty + 8 * (seg % kPlans));
+  };
+  auto give_up = [&]() {
+    *failed = 1;
+    if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+  };
+  constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
+
+  if (warp == kPlan) {
+    Planner<kUnit> planner;
+    planner.begin(p, lane);
+    bool ok = true;
+#pragma unroll 1
+    for (int seg = 0; ok; ++seg) {
+      const bool more = planner.next(p, s);
+      if (seg >= kPlans) ok = agreed(wait_for(plan_empty + 8 * (seg % kPlans), (seg / kPlans - 1) & 1, failed));
+      if (!ok) break;
+      if (lane == 0) {
+        plans[seg % kPlans] = s;
+        found[seg % kPlans] = 0;
+        mbar_arrive(plan_full + 8 * (seg % kPlans));
+      }
+      __syncwarp();
+      if (!more) break;
+    }
+    if (!ok) give_up();
+  } else if (warp == kMmaS) {
+    // ---------------- S: two row tiles of a key tile, or one of every other key tile ----------------
+    constexpr uint32_t id_s = idesc_bf16(kRows, kUnit) ^ kind;
+    const uint64_t d_k = sw128_desc(base + S::kOffK), d_q = sw128_desc(base + S::kOffQ);
+    bool ok = true;
+    int seg = 0, j = 0, used0 = 0, used1 = 0;  // tiles; tiles of S of the pipes
+#pragma unroll 1
+    while (ok && planned(seg, s)) {
+      const bool two = s.n * p.group - s.row0 > kRows && p.rows > kRows;
+      const int tiles = s.x1 - s.x0, steps = two ? 2 : 1;  // of a key tile
+      ok = agreed(wait_for(q_full, seg & 1, failed));
+#pragma unroll 1
+      for (int t = 0; ok && t < tiles; ++t, ++j) {
+        const int stage = j % kStages;
+        ok = agreed(wait_for(k_full + 8 * stage, (j / kStages) & 1, failed));
+#pragma unroll 1
+        for (int x = 0; ok && x < steps; ++x) {
+          const int pipe = two ? x : t & 1, used = pipe ? used1 : used0;
+          if (used) ok = agreed(wait_for(done + 8 * (2 * pipe + 1), (used - 1) & 1, failed));  // P V of the pipe's last keys
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = d_q + (two && pipe ? (uint32_t)S::kTile >> 4 : 0u), b = d_k + (uint32_t)stage * (S::kTile >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              mma_from_smem(tmem + 128 * pipe, a + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3), b + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3), id_s, kk ? 1u : 0u);
+            tc_commit(s_full + 8 * pipe);
+            if (x == steps - 1) tc_commit(k_empty + 8 * stage);
+          }
+          __syncwarp();
+          if (pipe) ++used1;
+          else ++used0;
+        }
+      }
+      read(seg++);
+    }
+    if (!ok) give_up();
+  } else if (warp == kMmaO) {
+    // ---------------- O += P V of every half ----------------
+    constexpr uint32_t id_o = idesc_bf16_bmn(kRows, HD) ^ kind;
+    const uint64_t d_v = sw128_desc_mn(base + S::kOffV, kPanel, 1024);
+    bool ok = true;
+    int seg = 0, j = 0, used0 = 0, used1 = 0;
+#pragma unroll 1
+    while (ok && planned(seg, s)) {
+      const bool two = s.n * p.group - s.row0 > kRows && p.rows > kRows;
+      const int tiles = s.x1 - s.x0, steps = two ? 4 : 2;
+      if (seg > 0) ok = agreed(wait_for(o_empty, (seg - 1) & 1, failed));  // the last segment's O is read
+#pragma unroll 1
+      for (int t = 0; ok && t < tiles; ++t, ++j) {
+        const int stage = j % kStages, x1 = s.x0 + t;
+        ok = agreed(wait_for(v_full + 8 * stage, (j / kStages) & 1, failed));
+        const int keys16 = ((x1 < s.cached ? s.len - place_of(s, x1) : s.n - kUnit * (x1 - s.cached)) + 15) / 16;  // up to the tile's last key
+#pragma unroll 1
+        for (int x = 0; ok && x < steps; ++x) {
+          const int half = two ? x >> 1 : x, pipe = two ? x & 1 : t & 1, bar = 2 * pipe + half, used = pipe ? used1 : used0;
+          ok = agreed(wait_for(p_full + 8 * bar, used & 1, failed));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t b = d_v + (uint32_t)stage * (S::kTile >> 4) + half * 4 * 128;
+          const uint32_t o = tmem + S::kTmemO + 128 * pipe, a = tmem + 128 * pipe + 64 * half;
+          const uint32_t add = t > (two ? 0 : 1) || half;
+          const int keys = keys16 - 4 * half;
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              if (kk < keys) mma_from_tmem(o, a + 8 * kk, b + kk * 128, id_o, kk ? 1u : add);
+            tc_commit(done + 8 * bar);
+            if (x == steps - 1) tc_commit(v_empty + 8 * stage);
+            if (x == steps - 1 && t == tiles - 1) tc_commit(o_full);
+          }
+          __syncwarp();
+        }
+        used0 += two || !(t & 1);
+        used1 += two || (t & 1);
+      }
+      read(seg++);
+    }
+    if (!ok) give_up();
+  } else if (warp >= kSoft) {
+    // ---------------- keys and values into 16 bits: thread = half the dims of a key of every tile ----------------
+    const int key = (tid - 32 * kSoft) >> 1, half = tid & 1;
+    using C = Codes<HD>;
+    const uint32_t row = key * 128, swz = key & 7;
+    // Byte of the thread's word i in a tile: 16 bytes of values. With 128 dims a thread with the second half takes its words in
+    // another order (i ^ 4), so that eight threads write different banks.
+    auto piece = [&](int i) {
+      if constexpr (HD == 128) return half * kPanel + row + 16 * ((uint32_t)(i ^ (half ? 4 : 0)) ^ swz);
+      else return row + 16 * ((uint32_t)(half * 4 + i) ^ swz);
+    };
+    auto write = [&](uint32_t at, uint4 v) {
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    };
+    // The page of the thread's key of unit x (-1: not a cached key; out of range: reads as zeros).
+    auto page_at = [&](const Segment& s, int x) -> int {
+      const int at = x < s.cached ? place_of(s, x) + key : s.len;
+      return at < s.len ? p.tables[(int64_t)s.b * p.tables_ld + at / p.page] : -1;
+    };
+    auto fetch = [&](const Segment& s, int x, int page, C& c) {
+      const int at = x < s.cached ? place_of(s, x) + key : s.len;
+#pragma unroll
+      for (int i = 0; i < C::kWords; ++i) c.k[i] = c.v[i] = 0;
+#pragma unroll
+      for (int i = 0; i < C::kPairs; ++i) c.kp[i] = c.vp[i] = 0;
+      if (at >= s.len) return;
+      if (page < 0 || page >= p.pages) {
+        if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+        return;
+      }
+      const int off = at % p.page, r = off % kBlockTokens;
+      const char* from = p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes;
+#pragma unroll
+      for (int val = 0; val < 2; ++val) {
+        uint32_t* w = val ? c.v : c.k;
+        uint32_t* pr = val ? c.vp : c.kp;
+#pragma unroll
+        for (int i = 0; i < C::kWords / 4; ++i) {
+          const int first = HD == 128 ? half * 8 + 4 * (i ^ half) : half * 4;
+          const uint4 y = *reinterpret_cast<const uint4*>(from + val * B::kPart + B::word(r, first));
+          w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
+          pr[i] = *reinterpret_cast<const uint32_t*>(from + val * B::kPart + B::pair(r, first / 4));
+        }
+      }
+    };
+    auto turn = [&](uint32_t to, const uint32_t* w, const uint32_t* pr) {
+#pragma unroll
+      for (int i = 0; i < C::kWords; ++i) {
+        const uint32_t s2 = __byte_perm(pr[i / 4], 0, 0x1010), o2 = __byte_perm(pr[i / 4], 0, 0x3232);
+        write(to + piece(i), make_uint4(two_values<DT, 0>(w[i], s2, o2), two_values<DT, 1>(w[i], s2, o2), two_values<DT, 2>(w[i], s2, o2),
+                                        two_values<DT, 3>(w[i], s2, o2)));
+      }
+    };
+    // A node's row: the thread's half, zeros behind the last node; of values the ones that are not finite set aside.
+    auto copy_row = [&](const Segment& s, int x, uint32_t to, bool values) {
+      const int j = kUnit * (x - s.cached) + key;
+      const char* from = (values ? p.v + (int64_t)(s.s0 + j) * p.v_n + s.kvh * p.v_h : p.k + (int64_t)(s.s0 + j) * p.k_n + s.kvh * p.k_h) + half * HD;
+      bool sick = false;
+#pragma unroll
+      for (int i = 0; i < C::kWords; ++i) {
+        const int at = HD == 128 ? i ^ (half ? 4 : 0) : i;
+        uint4 v = j < s.n ? *reinterpret_cast<const uint4*>(from + 16 * at) : make_uint4(0, 0, 0, 0);
+        if (values) {
+          uint32_t* w = &v.x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool lo = not_finite<DT>(w[e]), hi = not_finite<DT>(w[e] >> 16);
+            sick |= lo || hi;
+            w[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          }
+        }
+        write(to + piece(i), v);
+      }
+      return sick;
+    };
+    bool ok = true;
+    int seg = 0, j = 0;
+    Segment next;
+    ok = planned(0, s);
+    bool more = ok;
+    C c;
+    int page = more ? page_at(s, s.x0) : -1;
+    if (more) fetch(s, s.x0, page, c);
+    int seg_next = 0, x_next = s.x0;  // the tile that comes after: its segment's number, its unit
+    next = s;
+    auto advance = [&]() {
+      if (x_next + 1 < next.x1) {
+        ++x_next;
+        return true;
+      }
+      if (!planned(++seg_next, next)) return false;
+      x_next = next.x0;
+      return true;
+    };
+    ok = true;
+    int x = s.x0;
+#pragma unroll 1
+    while (more && ok) {
+      const bool follows = advance();
+      const int next_page = follows ? page_at(next, x_next) : -1;
+      const int stage = j % kStages;
+      const bool cached = x < s.cached, masked = is_masked(p, s, x);
+      const uint32_t at_k = base + S::kOffK + stage * S::kTile, at_v = base + S::kOffV + stage * S::kTile;
+      if (j >= kStages) ok = agreed(wait_for(k_empty + 8 * stage, (j / kStages - 1) & 1, failed));
+      if (!ok) break;
+      if (cached) turn(at_k, c.k, c.kp);
+      else copy_row(s, x, at_k, false);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_full + 8 * stage);
+      bool sick = false;
+      if (cached && masked) {
+        // What no row sees is 0; NaN that only some rows see is set aside.
+        const int at = place_of(s, x) + key;
+        const bool hidden = at >= s.len || (p.window && at < s.len - (p.window - 1) && at >= p.sinks);
+#pragma unroll
+        for (int i = 0; i < C::kPairs; ++i) {
+          if (hidden) c.vp[i] = 0;
+          if (not_finite<DT>(c.vp[i]) || not_finite<DT>(c.vp[i] >> 16)) {
+            sick = true;
+            c.vp[i] = 0;
+          }
+        }
+      }
+      if (j >= kStages) ok = agreed(wait_for(v_empty + 8 * stage, (j / kStages - 1) & 1, failed));
+      if (!ok) break;
+      if (cached) turn(at_v, c.v, c.vp);
+      else sick = copy_row(s, x, at_v, true);
+      if (sick) atomicOr(&found[seg % kPlans], 1u << ((x - s.x0) >> found_shift(s.x1 - s.x0)));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_full + 8 * stage);
+      ++j;
+      if (x + 1 == s.x1) read(seg);
+      more = follows;
+      if (more) {
+        if (seg != seg_next) s = next;
+        seg = seg_next;
+        x = x_next;
+        fetch(s, x, next_page, c);
+      }
+    }
+    if (!ok) give_up();
+  } else {
+    // ---------------- softmax of row r of the pipe's tiles ----------------
+    const int quad = warp & 3, pipe = warp >> 2, r = 32 * quad + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
+    const uint32_t at_s = lanes + 128 * pipe, at_o = lanes + S::kTmemO + 128 * pipe;
+    float2* stat = reinterpret_cast<float2*>(gb + S::kOffStat);
+    const float sc = p.scale == 0.f ? 1.f : fabsf(p.scale);
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (!wait_for(bar, parity, failed)) *failed = 1;
+    };
+    int seg = 0, taken = 0;  // halves of S of this pipe so far
+    bool wrote_start = false;
+    // Into the next segment go all softmax warps or none, whatever each has seen of a plan or of a wait that ran out: the
+    // barriers inside have no limit of their own.
+    auto enter = [&]() {
+      const bool there = planned(seg, s);
+      return !vote_any<kSoft * 32>(1, !there || *failed);
+    };
+#pragma unroll 1
+    while (enter()) {
+      const int all = min(p.rows, s.n * p.group - s.row0);   // rows of the tile
+      const bool two = all > kRows;
+      const int tiles = s.x1 - s.x0;
+      const int row = (two && pipe ? kRows : 0) + r;          // of the tile
+      const int rows = min(kRows, two && pipe ? all - kRows : all);
+      const int flat = s.row0 + min(row, all - 1), node = flat / p.group, head = s.kvh * p.group + flat % p.group;
+      const bool busy = 32 * quad < rows;                     // any of the warp's rows is one
+      // Q: its row, 16-byte pieces swizzled over 128 bytes; zeros where there is no row. (S of the segment before is complete: all pipes have read it.)
+      if (two || pipe == 0) {
+        const char* from = p.q + (int64_t)(s.s0 + node) * p.q_n + head * p.q_h;
+        const uint32_t to = base + S::kOffQ + pipe * S::kTile + r * 128;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          const uint4 v = r < rows ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * kPanel + 16 * ((i & 7) ^ (r & 7))), "r"(v.x), "r"(v.y), "r"(v.z),
+                       "r"(v.w)
+                       : "memory");
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      const int first = first_place(p, s.s0, s.n, s.len, node);
+      float m = kUnset;
+      uint64_t l0 = 0ull, l1 = 0ull;
+#pragma unroll 1
+      for (int x2 = two ? 0 : 2 * pipe; x2 < 2 * tiles; x2 += two || !(x2 & 1) ? 1 : 3, ++taken) {
+        const int x = s.x0 + (x2 >> 1), half = x2 & 1, bar = 2 * pipe + half;  // a half of a tile at a time
+        const bool cached = x < s.cached, masked = is_masked(p, s, x);
+        const int key0 = (cached ? place_of(s, x) : kUnit * (x - s.cached)) + 64 * half;
+        if (half == 0) wait(s_full + 8 * pipe, (taken >> 1) & 1);
+        tc_fence_after();
+        if (busy) {
+          uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int k = key0 + 32 * c;
+              if (cached) vis[c] = below(s.len - k) & (~below(first - k) | below(p.sinks - k));
+              else vis[c] = r < rows && k < s.n ? seen_nodes(p, s.s0, s.n, node, k) : 0u;
+            }
+          }
+          // Scores in the order of the softmax; hidden ones -inf.
+          auto load = [&](int c, uint32_t* y) {
+            tmem_load32(at_s + 64 * half + 32 * c, y);
+            if (p.scale <= 0.f) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(p.scale < 0.f ? -__uint_as_float(y[i]) : __uint_as_float(y[i]) * 0.f);
+            }
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((vis[c] >> i) & 1u)) y[i] = 0xff800000u;
+            }
+          };
+          uint32_t y[32];
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 1; c >= 0; --c) {  // (the first 32 last: they stay in the registers)
+            load(c, y);
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1])));
+          }
+          const float t_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
+          const bool raise = m == kUnset ? t_max > kUnset : t_max > m + (kLead<DT> + kRaise);
+          if (__any_sync(0xffffffffu, raise)) {
+            const float f = raise ? (m == kUnset ? 0.f : exp2f(m - (t_max - kLead<DT>))) : 1.f;
+            if (raise) m = t_max - kLead<DT>;
+            if (x2 > (two ? 0 : 2 * pipe)) {
+              // O of the halves before this one is complete once the last one's P V is.
+              wait(done + 8 * (bar ^ 1), ((taken - 1) >> 1) & 1);
+              tc_fence_after();
+              l0 = fma2(l0, pair(f, f), 0ull);
+              l1 = fma2(l1, pair(f, f), 0ull);
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 8) {
+                uint32_t o[8];
+                tmem_load8(at_o + c, o);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_store8(at_o + c, o);
+              }
+            }
+          }
+          const uint64_t sc2 = pair(sc, sc), nm2 = pair(-m, -m);
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            if (c) load(1, y);
+            uint32_t e[16];
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float2 a = unpair(fma2(pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), sc2, nm2));
+              const float2 b = unpair(fma2(pair(__uint_as_float(y[2 * i + 2]), __uint_as_float(y[2 * i + 3])), sc2, nm2));
+              const float a0 = ex2(a.x), a1 = ex2(a.y), b0 = ex2(b.x), b1 = ex2(b.y);
+              l0 = add2(l0, pair(a0, a1));
+              l1 = add2(l1, pair(b0, b1));
+              e[i] = pack2<DT>(a0, a1);
+              e[i + 1] = pack2<DT>(b0, b1);
+            }
+            tmem_store16(at_s + 64 * half + 16 * c, e);
+          }
+          tmem_wait_store();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8 * bar);
+      }
+      // ---- the segment's rows ----
+      const float2 la = unpair(add2(l0, l1));
+      const float mine = la.x + la.y;
+      stat[pipe * kRows + r] = make_float2(m, mine);
+      named_bar_sync(1, kSoft * 32);
+      float own = 1.f, other = 0.f, sum = mine;  // factors of this pipe's O and of the other one's
+      if (!two) {
+        const float2 y = stat[(1 - pipe) * kRows + r];
+        const float top = fmaxf(m, y.x);
+        own = m == top ? 1.f : exp2f(m - top);
+        other = y.x == top ? 1.f : exp2f(y.x - top);
+        // (the same operations in the same order on both sides)
+        sum = pipe ? other * y.y + own * mine : own * mine + other * y.y;
+        m = top;
+      }
+      const bool whole = s.whole != 0;
+      const int which = s.x0 == 0 ? 1 : 0;
+      const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+      own *= inv;
+      other *= inv;
+      const bool single = two || tiles == 1;  // only one pipe's O holds anything of these rows
+      wait(o_full, seg & 1);
+      tc_fence_after();
+      const uint32_t aside = found[seg % kPlans];
+      const int d0 = two ? 0 : pipe * (HD / 2), d1 = two ? HD : d0 + HD / 2;  // the columns that this thread writes
+      const uint32_t from = two ? at_o : lanes + S::kTmemO;                   // (pipe 0's O, then pipe 1's)
+      const float f0 = two || !pipe ? own : other, f1 = pipe ? own : other;
+      if (busy) {
+        char* out = p.out + (int64_t)(s.s0 + node) * p.out_n + head * p.out_h;
+        float* part = scratch.sums(blockIdx.x, which) + (int64_t)row * HD;
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 8) {
+          uint32_t o[8];
+          float y[8];
+          tmem_load8(from + d, o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(o[i]) * f0;
+          if (!single) {
+            tmem_load8(from + 128 + d, o);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = fmaf(__uint_as_float(o[i]), f1, y[i]);
+          }
+          if (r < rows) {
+            if (aside) {
+              float more[8];
+              set_aside<DT, HD>(p, plans + seg % kPlans, aside, node, first, d, more);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) y[i] += more[i];
+            }
+            if (whole) {
+              *reinterpret_cast<uint4*>(out + 2 * d) = make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+            } else {
+              *reinterpret_cast<float4*>(part + d) = make_float4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<float4*>(part + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            }
+          }
+        }
+      }
+      if (r < rows && (two || pipe == 0)) {
+        if (!whole) scratch.stats(blockIdx.x, which)[row] = make_float2(m, sum);
+        else if (p.lse) p.lse[(int64_t)(s.s0 + node) * p.heads + head] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+      if (!whole && s.x0 == 0) {
+        wrote_start = true;
+        if (tid == 0) *scratch.started(blockIdx.x) = Started{s.last, s.s0, s.row0, all, s.kvh};
+      }
+      read(seg);
+      ++seg;  // (the next segment's maxima go where these ones are: enter() is a barrier)
+    }
+    if (!wrote_start && tid == 0) scratch.started(blockIdx.x)->last = 0;
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+  if (*failed && (warp == kMmaS || warp == kMmaO)) {
+    // After a wait has run out: the products that the two issue warps have in flight end before the CTA's tensor and shared
+    // memory is given up (bounded): a commit follows the products of the thread that makes it.
+    if (elect_one()) tc_commit(drained);
+    __syncwarp();
+    volatile int by_itself[2] = {0, kPatience};
+    if (warp == kMmaS) wait_for(drained, 0, by_itself);
+    __syncwarp();
+  }
+  if (warp == kMmaS) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DT, int HD>
+int launch(const Params& p, cudaStream_t s) {
+  static_assert(Wide<HD>::kBytes <= 232448, "shared memory");
+  if (int st = allow_smem<k_int4_attention_wide<DT, HD>>(Wide<HD>::kBytes)) return st;
+  const int ctas = sm_count();
+  cudaError_t e = launch_ex(k_int4_attention_wide<DT, HD>, dim3(ctas), dim3(kThreads), (size_t)Wide<HD>::kBytes, s, false, dim3(1), p);
+  if (e == cudaSuccess && p.capacity + p.total > (int64_t)(p.whole - 2) * kUnit)  // else no row is shared
+    e = launch_ex(k_join<DT, 2 * kRows, HD>, dim3(ctas, 16), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: launch: ") + cudaGetErrorString(e));
+  return check_launch("af_tree_attention_int4");
+}
+
+}  // namespace
+
+int wide_launch(const Params& p, bool bf16, int head_dim, cudaStream_t s) {
+  if (head_dim == 128) return bf16 ? launch<AF_DTYPE_BF16, 128>(p, s) : launch<AF_DTYPE_F16, 128>(p, s);
+  return bf16 ? launch<AF_DTYPE_BF16, 64>(p, s) : launch<AF_DTYPE_F16, 64>(p, s);
+}
+
+}  // namespace kv4
+}  // namespace af
