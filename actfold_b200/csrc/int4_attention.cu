@@ -18,6 +18,8 @@
 // copy per page run, into a ring of 32 slots; consumer warps take units in turn, each with maxima,
 // sums and an O of its own, joined through shared memory at the end of a row tile. The step's own nodes are
 // units too, read from their 16-bit rows. Every wait is bounded; a timeout sets AF_STATUS_TIMEOUT.
+#include <math.h>
+
 #include "int4_attention.cuh"
 
 namespace af {
@@ -29,12 +31,14 @@ namespace kv4 {
 namespace {
 
 constexpr int kUnit = 32;    // keys of a unit
-constexpr int kSlots = 32;
 
-template <int HD, int NT, int W>
+// NT: 8-row tiles of a warp; W: consumer warps; CTAS: on an SM.
+template <int HD, int NT, int W, int CTAS>
 struct Shape {
+  static constexpr int kSlots = 32 / CTAS;
   static constexpr int kRows = 8 * NT;
   static constexpr int kUnitBytes = kUnit / kBlockTokens * Block<HD>::kBytes;
+  static_assert(kSlots >= 16 && kSlots <= 32, "a producer fills eight at a time, others stay filled");
   static constexpr int kThreads = 32 * (W + 1);
   static constexpr int kOffAcc = kSlots * kUnitBytes;               // [W][kRows][HD] sums of the warps
   static constexpr int kOffStat = kOffAcc + W * kRows * HD * 4;     // [W][kRows] (maximum, sum)
@@ -79,11 +83,11 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const char* src, uint32_
 }
 
 // Plans the CTA's share, and brings its units of cached keys into the ring.
-template <int HD, int NT, int W>
+template <int HD, int NT, int W, int CTAS>
 __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t base, uint32_t full, uint32_t empty, uint32_t plan_full,
                                         uint32_t plan_empty, Segment* plans, volatile int* failed) {
-  using S = Shape<HD, NT, W>;
-  constexpr int kBlock = Block<HD>::kBytes, kMostRuns = kUnit / kBlockTokens;
+  using S = Shape<HD, NT, W, CTAS>;
+  constexpr int kBlock = Block<HD>::kBytes, kSlots = S::kSlots;
   const int lane = threadIdx.x & 31;
   Planner<kUnit> planner;
   planner.begin(p, lane);
@@ -165,14 +169,15 @@ __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t b
   // of the last kSlots units, one a lane.
   const int last = __reduce_max_sync(0xffffffffu, issued), mine = last - kSlots + lane;
   volatile int by_itself[2] = {0, kPatience};
-  if (mine >= 0) wait_for(full + 8 * (mine % kSlots), (mine / kSlots) & 1, by_itself);
+  if (lane < kSlots && mine >= 0) wait_for(full + 8 * (mine % kSlots), (mine / kSlots) & 1, by_itself);
   __syncwarp();
 }
 
-template <int DT, int HD, int NT, int W>
-__global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid_constant__ Params p) {
-  using S = Shape<HD, NT, W>;
+template <int DT, int HD, int NT, int W, int CTAS>
+__global__ void __launch_bounds__(32 * (W + 1), CTAS) k_int4_attention(const __grid_constant__ Params p) {
+  using S = Shape<HD, NT, W, CTAS>;
   using B = Block<HD>;
+  constexpr int kSlots = S::kSlots;
   constexpr int KW = HD / 32, KS = HD / 16;   // code words of a key that a lane takes; steps of the first product
   constexpr int VW = HD / 64, VT = HD / 16;   // code words of a value; 16-dim tiles of the second product
   constexpr int kTeam = 32 * W;
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
   const Scratch<S::kRows, HD> scratch{p.ws, (int)gridDim.x};
 
   if (warp == W) {
-    produce<HD, NT, W>(p, gb, base, full, empty, plan_full, plan_empty, plans, failed);
+    produce<HD, NT, W, CTAS>(p, gb, base, full, empty, plan_full, plan_empty, plans, failed);
   } else {
     const int g = lane >> 2, t = lane & 3;
     // The key of a block that index g of the first product's M side stands for: indices 2 x and 2 x + 1, which a lane of the second
@@ -236,7 +241,9 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
 #pragma unroll
         for (int i = 0; i < KS / 2; ++i) {
           const uint4 x = row < rows ? *reinterpret_cast<const uint4*>(at + 16 * i) : make_uint4(0, 0, 0, 0);
-          q[nt][4 * i] = x.x, q[nt][4 * i + 1] = x.y, q[nt][4 * i + 2] = x.z, q[nt][4 * i + 3] = x.w;
+          // (p.scale is positive: the sign of the caller's goes to q, and 0 makes q 0)
+          q[nt][4 * i] = (x.x ^ p.q_flip) & p.q_keep, q[nt][4 * i + 1] = (x.y ^ p.q_flip) & p.q_keep;
+          q[nt][4 * i + 2] = (x.z ^ p.q_flip) & p.q_keep, q[nt][4 * i + 3] = (x.w ^ p.q_flip) & p.q_keep;
         }
       }
       // Rows 8 nt + 2 t and the next one: their nodes, and the first place of their windows.
@@ -261,38 +268,29 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
       }
-      // Scores of the unit's keys (h: half of 16; c: key g of its block 0, rows 2 t and 2 t + 1, then of block 1) into probabilities of the
-      // second product's operand. seen(h, r, nt, e): does row e see key r of half h.
-      auto softmax = [&](float (&x)[2][NT][4], uint32_t (&pf)[2][NT][2], bool masked, auto seen) {
-        float top = -INFINITY;
+      // Scores of 16 keys (c: key g of their block 0, rows 2 t and 2 t + 1, then of block 1) into probabilities, the second product's
+      // operand. seen(r, nt, e): does row e see key g of block r.
+      auto softmax = [&](float (&x)[NT][4], uint32_t (&pf)[NT][2], bool masked, auto seen) {
         if (masked) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) x[h][nt][c] = seen(h, c >> 1, nt, c & 1) ? x[h][nt][c] * p.scale : -INFINITY;
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) x[h][nt][c] *= p.scale;
+            for (int c = 0; c < 4; ++c) x[nt][c] = seen(c >> 1, nt, c & 1) ? x[nt][c] : -INFINITY;
         }
+        float top = -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            top = fmaxf(top, fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]), fmaxf(x[1][nt][e], x[1][nt][2 + e])) - m[nt][e]);
+          for (int e = 0; e < 2; ++e) top = fmaxf(top, fmaf(fmaxf(x[nt][e], x[nt][2 + e]), p.scale, -m[nt][e]));
         if (__any_sync(0xffffffffu, top > kLead<DT> + kRaise)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float y = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]), fmaxf(x[1][nt][e], x[1][nt][2 + e]));
+              float y = fmaxf(x[nt][e], x[nt][2 + e]);
 #pragma unroll
               for (int d = 4; d < 32; d <<= 1) y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+              y *= p.scale;
               const float old = m[nt][e];
               if (old == kUnset ? y > kUnset : y > old + (kLead<DT> + kRaise)) {
                 m[nt][e] = y - kLead<DT>;
@@ -307,18 +305,16 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
             }
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int nt = 0; nt < NT; ++nt) {
+          float y[4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float y[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              y[c] = ex2(x[h][nt][c] - m[nt][c & 1]);
-              l[nt][c & 1] += y[c];
-            }
-            pf[h][nt][0] = transposed(pack2<DT>(y[0], y[1]));
-            pf[h][nt][1] = transposed(pack2<DT>(y[2], y[3]));
+          for (int c = 0; c < 4; ++c) {
+            y[c] = ex2(fmaf(x[nt][c], p.scale, -m[nt][c & 1]));
+            l[nt][c & 1] += y[c];
           }
+          pf[nt][0] = transposed(pack2<DT>(y[0], y[1]));
+          pf[nt][1] = transposed(pack2<DT>(y[2], y[3]));
+        }
       };
       const int x0 = s.x0 + (W + warp - s.j0 % W) % W;
 #pragma unroll 1
@@ -328,55 +324,53 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
           *failed = 1;
           break;
         }
-        float sc[2][NT][4];
-        uint32_t pf[2][NT][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sc[h][nt][c] = 0.f;
         if (x < s.cached) {
           // ---------------- 32 cached keys ----------------
           const int place = kUnit * (x < s.sink_units ? x : x - s.sink_units + s.from);
           const bool masked = place + kUnit > s.len || (p.window && place < first_all && place + kUnit > p.sinks);
           const uint32_t unit = base + slot * S::kUnitBytes;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[2][KW], pr[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              lds<4 * KW>(unit + (2 * h + r) * B::kBytes + k_at, w[r]);
-              lds<4>(unit + (2 * h + r) * B::kBytes + kp_at, &pr[r]);
-            }
-            const uint32_t s0 = __byte_perm(pr[0], 0, 0x1010), o0 = __byte_perm(pr[0], 0, 0x3232);
-            const uint32_t s1 = __byte_perm(pr[1], 0, 0x1010), o1 = __byte_perm(pr[1], 0, 0x3232);
-#pragma unroll
-            for (int i = 0; i < KW; ++i) {
-              const uint32_t a0 = two_values<DT, 0>(w[0][i], s0, o0), a1 = two_values<DT, 0>(w[1][i], s1, o1);
-              const uint32_t a2 = two_values<DT, 1>(w[0][i], s0, o0), a3 = two_values<DT, 1>(w[1][i], s1, o1);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[h][nt], a0, a1, a2, a3, q[nt][4 * i], q[nt][4 * i + 1]);
-              const uint32_t b0 = two_values<DT, 2>(w[0][i], s0, o0), b1 = two_values<DT, 2>(w[1][i], s1, o1);
-              const uint32_t b2 = two_values<DT, 3>(w[0][i], s0, o0), b3 = two_values<DT, 3>(w[1][i], s1, o1);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[h][nt], b0, b1, b2, b3, q[nt][4 * i + 2], q[nt][4 * i + 3]);
-            }
-          }
           auto sees = [&](int at, int nt, int e) { return at < s.len && (at >= first[nt][e] || at < p.sinks); };
-          softmax(sc, pf, masked, [&](int h, int r, int nt, int e) { return sees(place + 16 * h + 8 * r + kap, nt, e); });
           bool sick = false;
-#pragma unroll
+#pragma unroll 1
           for (int h = 0; h < 2; ++h) {
+            const uint32_t blocks = unit + 2 * h * B::kBytes;
+            float sc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sc[nt][c] = 0.f;
+            uint32_t pf[NT][2];
+            {
+              uint32_t w[2][KW], pr[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                lds<4 * KW>(blocks + r * B::kBytes + k_at, w[r]);
+                lds<4>(blocks + r * B::kBytes + kp_at, &pr[r]);
+              }
+              const uint32_t s0 = __byte_perm(pr[0], 0, 0x1010), o0 = __byte_perm(pr[0], 0, 0x3232);
+              const uint32_t s1 = __byte_perm(pr[1], 0, 0x1010), o1 = __byte_perm(pr[1], 0, 0x3232);
+#pragma unroll
+              for (int i = 0; i < KW; ++i) {
+                const uint32_t a0 = two_values<DT, 0>(w[0][i], s0, o0), a1 = two_values<DT, 0>(w[1][i], s1, o1);
+                const uint32_t a2 = two_values<DT, 1>(w[0][i], s0, o0), a3 = two_values<DT, 1>(w[1][i], s1, o1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], a0, a1, a2, a3, q[nt][4 * i], q[nt][4 * i + 1]);
+                const uint32_t b0 = two_values<DT, 2>(w[0][i], s0, o0), b1 = two_values<DT, 2>(w[1][i], s1, o1);
+                const uint32_t b2 = two_values<DT, 3>(w[0][i], s0, o0), b3 = two_values<DT, 3>(w[1][i], s1, o1);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], b0, b1, b2, b3, q[nt][4 * i + 2], q[nt][4 * i + 3]);
+              }
+            }
             uint32_t w[2][2][VW], pr[2][2];  // [block][key of the lane's two]
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-              const uint32_t at = unit + (2 * h + r) * B::kBytes;
+              const uint32_t at = blocks + r * B::kBytes;
               lds<4 * VW>(at + v_at0, w[r][0]);
               lds<4 * VW>(at + v_at1, w[r][1]);
               lds<4>(at + vp_at0, &pr[r][0]);
               lds<4>(at + vp_at1, &pr[r][1]);
             }
+            softmax(sc, pf, masked, [&](int r, int nt, int e) { return sees(place + 16 * h + 8 * r + kap, nt, e); });
             if (masked) {
               // What no row sees is 0 (behind the last token lies whatever was there); NaN that only some see is set aside.
 #pragma unroll
@@ -405,11 +399,11 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
                 lo[r] = __byte_perm(w[r][0][i], w[r][1][i], 0x5410);
                 hi[r] = __byte_perm(w[r][0][i], w[r][1][i], 0x7632);
               }
-#define AF_STEP(I)                                                                                                                     \
-  {                                                                                                                                    \
-    const uint32_t a0 = two_values<DT, I>(lo[0], s2[0], o2[0]), a1 = two_values<DT, I>(hi[0], s2[0], o2[0]);                           \
-    const uint32_t a2 = two_values<DT, I>(lo[1], s2[1], o2[1]), a3 = two_values<DT, I>(hi[1], s2[1], o2[1]);                           \
-    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) mma<DT>(o[4 * i + I][nt], a0, a1, a2, a3, pf[h][nt][0], pf[h][nt][1]);           \
+#define AF_STEP(I)                                                                                                                   \
+  {                                                                                                                                  \
+    const uint32_t a0 = two_values<DT, I>(lo[0], s2[0], o2[0]), a1 = two_values<DT, I>(hi[0], s2[0], o2[0]);                         \
+    const uint32_t a2 = two_values<DT, I>(lo[1], s2[1], o2[1]), a3 = two_values<DT, I>(hi[1], s2[1], o2[1]);                         \
+    _Pragma("unroll") for (int nt = 0; nt < NT; ++nt) mma<DT>(o[4 * i + I][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);               \
   }
               AF_STEP(0) AF_STEP(1) AF_STEP(2) AF_STEP(3)
 #undef AF_STEP
@@ -447,31 +441,35 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
           if (__any_sync(0xffffffffu, any != 0)) {  // (most units of a long chain are seen by no row of the tile)
             const char* k_row = p.k + (int64_t)s.s0 * p.k_n + s.kvh * p.k_h + t * (HD / 2);
             const char* v_row = p.v + (int64_t)s.s0 * p.v_n + s.kvh * p.v_h + g * (HD / 4);
-#pragma unroll
+            bool sick = false;
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
+              if (j0 + 16 * h >= s.n) break;
               const int n0 = j0 + 16 * h + g, n1 = n0 + 8;
+              float sc[NT][4];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sc[nt][c] = 0.f;
+              uint32_t pf[NT][2];
 #pragma unroll
               for (int i = 0; i < KS / 2; ++i) {
                 const uint4 a = n0 < s.n ? *reinterpret_cast<const uint4*>(k_row + n0 * p.k_n + 16 * i) : make_uint4(0, 0, 0, 0);
                 const uint4 b = n1 < s.n ? *reinterpret_cast<const uint4*>(k_row + n1 * p.k_n + 16 * i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                  mma<DT>(sc[h][nt], a.x, b.x, a.y, b.y, q[nt][4 * i], q[nt][4 * i + 1]);
-                  mma<DT>(sc[h][nt], a.z, b.z, a.w, b.w, q[nt][4 * i + 2], q[nt][4 * i + 3]);
+                  mma<DT>(sc[nt], a.x, b.x, a.y, b.y, q[nt][4 * i], q[nt][4 * i + 1]);
+                  mma<DT>(sc[nt], a.z, b.z, a.w, b.w, q[nt][4 * i + 2], q[nt][4 * i + 3]);
                 }
               }
-            }
-            softmax(sc, pf, true, [&](int h, int r, int nt, int e) { return ((bits[nt][e] >> (16 * h + 8 * r + g)) & 1u) != 0; });
-            bool sick = false;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
+              softmax(sc, pf, true, [&](int r, int nt, int e) { return ((bits[nt][e] >> (16 * h + 8 * r + g)) & 1u) != 0; });
 #pragma unroll
               for (int i = 0; i < VT / 4; ++i) {
                 uint32_t w[4][4];  // keys 2 t, 2 t + 1, and the same of the second block: 8 dims each
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
-                  const int n0 = j0 + 16 * h + 8 * (y >> 1) + 2 * t + (y & 1);
-                  const uint4 a = n0 < s.n ? *reinterpret_cast<const uint4*>(v_row + n0 * p.v_n + 16 * i) : make_uint4(0, 0, 0, 0);
+                  const int at = j0 + 16 * h + 8 * (y >> 1) + 2 * t + (y & 1);
+                  const uint4 a = at < s.n ? *reinterpret_cast<const uint4*>(v_row + at * p.v_n + 16 * i) : make_uint4(0, 0, 0, 0);
                   w[y][0] = a.x, w[y][1] = a.y, w[y][2] = a.z, w[y][3] = a.w;
 #pragma unroll
                   for (int c = 0; c < 4; ++c) {
@@ -486,7 +484,7 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
                   const uint32_t a0 = __byte_perm(w[0][c], w[1][c], 0x5410), a1 = __byte_perm(w[0][c], w[1][c], 0x7632);
                   const uint32_t a2 = __byte_perm(w[2][c], w[3][c], 0x5410), a3 = __byte_perm(w[2][c], w[3][c], 0x7632);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) mma<DT>(o[4 * i + c][nt], a0, a1, a2, a3, pf[h][nt][0], pf[h][nt][1]);
+                  for (int nt = 0; nt < NT; ++nt) mma<DT>(o[4 * i + c][nt], a0, a1, a2, a3, pf[nt][0], pf[nt][1]);
                 }
               }
             }
@@ -584,13 +582,13 @@ __global__ void __launch_bounds__(32 * (W + 1), 1) k_int4_attention(const __grid
   if (tid == 0 && *failed && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
 }
 
-template <int DT, int HD, int NT, int W>
+template <int DT, int HD, int NT, int W, int CTAS>
 int launch(const Params& p, cudaStream_t s) {
-  using S = Shape<HD, NT, W>;
-  static_assert(S::kBytes <= 232448, "shared memory");
-  if (int st = allow_smem<k_int4_attention<DT, HD, NT, W>>(S::kBytes)) return st;
-  const int ctas = sm_count();
-  cudaError_t e = launch_ex(k_int4_attention<DT, HD, NT, W>, dim3(ctas), dim3(S::kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
+  using S = Shape<HD, NT, W, CTAS>;
+  static_assert(CTAS * (S::kBytes + 1024) <= 233472, "shared memory");
+  if (int st = allow_smem<k_int4_attention<DT, HD, NT, W, CTAS>>(S::kBytes)) return st;
+  const int ctas = CTAS * sm_count();
+  cudaError_t e = launch_ex(k_int4_attention<DT, HD, NT, W, CTAS>, dim3(ctas), dim3(S::kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
   if (e == cudaSuccess && p.capacity + p.total > (int64_t)(p.whole - 2) * kUnit)  // else no row is shared
     e = launch_ex(k_join<DT, S::kRows, HD>, dim3(ctas, S::kRows / 8 * 4), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: launch: ") + cudaGetErrorString(e));
@@ -599,7 +597,7 @@ int launch(const Params& p, cudaStream_t s) {
 
 template <int DT, int HD>
 int launch_rows(const Params& p, cudaStream_t s) {
-  return p.rows == 8 ? launch<DT, HD, 1, 11>(p, s) : launch<DT, HD, 2, 7>(p, s);
+  return p.rows == 8 ? launch<DT, HD, 1, 7, 2>(p, s) : launch<DT, HD, 2, 7, 1>(p, s);
 }
 
 int64_t workspace_bytes() { return Scratch<256, 128>::bytes(sm_count()); }
@@ -671,7 +669,9 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.capacity = c.pages ? a.max_pages * c.page_size : 0;
   p.window = (int)a.window;
   p.sinks = (int)a.sinks;
-  p.scale = (float)(a.scale * 1.4426950408889634);
+  p.scale = a.scale == 0. ? 1.f : (float)(fabs(a.scale) * 1.4426950408889634);
+  p.q_flip = a.scale < 0. ? 0x80008000u : 0u;
+  p.q_keep = a.scale == 0. ? 0u : 0xffffffffu;
   p.out = static_cast<char*>(a.out), p.out_n = a.out_strides[0], p.out_h = a.out_strides[1];
   p.lse = a.lse;
   p.ws = static_cast<char*>(a.workspace);

@@ -31,7 +31,8 @@ struct Params {
   int words, batch, total, heads, kv_heads, group, pages, page;
   int64_t capacity;                             // tokens that a table row can hold
   int window, sinks;                            // window 0: all of the prefix is visible
-  float scale;                                  // times log2(e)
+  float scale;                                  // times log2(e); of the attention kernels positive: q is flipped, or made 0, instead
+  uint32_t q_flip, q_keep;                      // q = (q ^ flip) & keep, in pairs
   char* out;
   int64_t out_n, out_h;
   float* lse;

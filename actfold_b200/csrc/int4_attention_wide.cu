@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
     const uint32_t at_s = lanes + 128 * pipe, at_o = lanes + S::kTmemO + 128 * pipe;
     float2* stat = reinterpret_cast<float2*>(gb + S::kOffStat);
-    const float sc = p.scale == 0.f ? 1.f : fabsf(p.scale);
+    const float sc = p.scale;
     auto wait = [&](uint32_t bar, uint32_t parity) {
       if (!wait_for(bar, parity, failed)) *failed = 1;
     };
@@ -531,8 +531,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) {
           const uint4 v = r < rows ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * kPanel + 16 * ((i & 7) ^ (r & 7))), "r"(v.x), "r"(v.y), "r"(v.z),
-                       "r"(v.w)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * kPanel + 16 * ((i & 7) ^ (r & 7))), "r"((v.x ^ p.q_flip) & p.q_keep),
+                       "r"((v.y ^ p.q_flip) & p.q_keep), "r"((v.z ^ p.q_flip) & p.q_keep), "r"((v.w ^ p.q_flip) & p.q_keep)
                        : "memory");
         }
         fence_proxy_async_smem();
@@ -559,13 +559,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
               else vis[c] = r < rows && k < s.n ? seen_nodes(p, s.s0, s.n, node, k) : 0u;
             }
           }
-          // Scores in the order of the softmax; hidden ones -inf.
+          // Scores; hidden ones -inf.
           auto load = [&](int c, uint32_t* y) {
             tmem_load32(at_s + 64 * half + 32 * c, y);
-            if (p.scale <= 0.f) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(p.scale < 0.f ? -__uint_as_float(y[i]) : __uint_as_float(y[i]) * 0.f);
-            }
             if (masked) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
