@@ -589,7 +589,7 @@ int launch(const Params& p, cudaStream_t s) {
   if (int st = allow_smem<k_int4_attention<DT, HD, NT, W, CTAS>>(S::kBytes)) return st;
   const int ctas = CTAS * sm_count();
   cudaError_t e = launch_ex(k_int4_attention<DT, HD, NT, W, CTAS>, dim3(ctas), dim3(S::kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
-  if (e == cudaSuccess && p.capacity + p.total > (int64_t)(p.whole - 2) * kUnit)  // else no row is shared
+  if (e == cudaSuccess && p.joins)
     e = launch_ex(k_join<DT, S::kRows, HD>, dim3(ctas, S::kRows / 8 * 4), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: launch: ") + cudaGetErrorString(e));
   return check_launch("af_tree_attention_int4");
@@ -682,11 +682,13 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
   p.row_cost = wide ? 3 : 10;
   p.whole = wide ? 8 : 32;
+  p.whole_long = 8;
+  p.least = wide ? 2 : 14;
   // Units are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
-  AF_REQUIRE((double)c.heads * (ceil_div(a.total * p.group, p.rows) + a.batch) *
-                     ((a.max_pages * c.page_size + a.total) / (wide ? kv4::kWideUnit : kv4::kUnit) + 3 + p.row_cost) <
-                 2147483000.0,
-             "af_tree_attention_int4: more than 2^31 units of keys");
+  const int64_t most = (a.max_pages * c.page_size + a.total) / (wide ? kv4::kWideUnit : kv4::kUnit) + 3;  // of a row tile
+  const double all = (double)c.heads * (ceil_div(a.total * p.group, p.rows) + a.batch) * (most + p.row_cost);
+  AF_REQUIRE(all < 2147483000.0, "af_tree_attention_int4: more than 2^31 units of keys");
+  p.joins = most > (all >= 2.0 * p.whole * sm_count() ? p.whole_long : p.whole);
   cudaStream_t s = as_stream(stream);
   const bool bf16 = c.dtype == AF_DTYPE_BF16;
   if (wide) return kv4::wide_launch(p, bf16, (int)c.head_dim, s);

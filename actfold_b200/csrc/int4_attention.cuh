@@ -29,6 +29,7 @@ struct Params {
   const uint32_t* mask;
   int64_t tables_ld, mask_ld;
   int words, batch, total, heads, kv_heads, group, pages, page;
+  int runs;                                     // that 32 tokens of a cache lie in: of 32, 16 or 8 tokens, so that none leaves a page
   int64_t capacity;                             // tokens that a table row can hold
   int window, sinks;                            // window 0: all of the prefix is visible
   float scale;                                  // times log2(e); of the attention kernels positive: q is flipped, or made 0, instead
@@ -38,7 +39,9 @@ struct Params {
   float* lse;
   int rows;                                     // of a row tile: consecutive (node, head of the group) pairs of a request
   int row_cost;                                 // of a row tile besides its units
-  int whole;                                    // a row tile of at most this many units is not shared by CTAs
+  int whole, whole_long;                        // a row tile of at most this many units is not shared by CTAs; where shares are long
+  int least;                                    // units of a share
+  int joins;                                    // may a row tile be shared?
   char* ws;
   unsigned* status;
   int patience;                                 // attempts of a wait before it gives up
@@ -76,10 +79,11 @@ __device__ __forceinline__ Request<UNIT> request(const Params& p, int b) {
   return r;
 }
 
-// The list of row tiles, cut into one share per CTA: the first `more` shares have each + 1 units.
+// The list of row tiles, cut into one share per CTA: the first `more` shares have each + 1 units. Short lists are cut into
+// shares of p.least units, for as many CTAs as that takes: a part of a row costs its CTA and the join more than a few units do.
 struct Shares {
-  int each, more;
-  __device__ __forceinline__ int begin(int i) const { return each * i + min(i, more); }
+  int each, more, all;
+  __device__ __forceinline__ int begin(int i) const { return (int)min((int64_t)all, (int64_t)each * i + min(i, more)); }
   __device__ __forceinline__ int owner(int t) const {
     const int big = more * (each + 1);
     return t < big ? t / (each + 1) : more + (t - big) / each;
@@ -104,7 +108,8 @@ struct Started {
 template <int UNIT>
 struct Planner {
   Shares shares;
-  int t, end, before, b, j = 0;  // units of the requests before b; of the CTA so far
+  int t, end, before, b, j;  // units of the requests before b; of the CTA so far
+  int whole;                 // a row tile of at most this many units is not shared: fewer where shares are long, which it would make uneven
   Request<UNIT> r;
 
   __device__ __forceinline__ static int cost_of(const Params& p, int b, bool& disorder) {
@@ -126,11 +131,14 @@ struct Planner {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
     if (__any_sync(0xffffffffu, disorder)) all = 0;
+    shares.all = all;
     shares.each = all / (int)gridDim.x;
     shares.more = all - shares.each * (int)gridDim.x;
+    whole = shares.each >= 2 * p.whole ? p.whole_long : p.whole;
+    if (shares.each < p.least) shares.each = p.least, shares.more = 0;
     t = shares.begin(blockIdx.x);
     end = shares.begin(blockIdx.x + 1);
-    b = before = 0;
+    b = before = j = 0;
     if (t >= end) return;
 #pragma unroll 1
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -166,7 +174,7 @@ struct Planner {
       s.row0 = (row - s.kvh * r.tiles) * p.rows;
       s.s0 = r.s0, s.n = r.n, s.len = r.len, s.b = b;
       s.sink_units = r.sink_units, s.from = r.from, s.cached = r.cached;
-      const bool alone = r.units <= p.whole;
+      const bool alone = r.units <= whole;
       const int row_end = t - u + r.cost, upto = alone ? r.cost : min(r.cost, u + (end - t));
       t += upto - u;
       s.x0 = max(0, u - p.row_cost);
