@@ -5,8 +5,9 @@
 // over the places p that row i sees. The rows' sums are known (lse), so keys
 // are independent: a warp takes 32 of them, all rows of the request against
 // 16 at a time in registers (m16n8k16, the keys as the M side: few rows waste little), and adds to their
-// weights without atomics. With few rows HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and
-// 8 of its weight; with many the products do. See int4_attention.cu for the fragments' order.
+// weights without atomics. The rows of a request and head, 64 at a time, lie in shared memory with their sums. With few rows
+// HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and 8 of its weight; with many the products
+// do. See int4_attention.cu for the fragments' order.
 #include <string>
 
 #include "int4_attention.cuh"
@@ -15,7 +16,7 @@ namespace af {
 namespace kv4 {
 namespace {
 
-constexpr int kUnit = 32, kThreads = 256, kCtas = 3;  // keys of a unit; CTAs per SM
+constexpr int kUnit = 32, kThreads = 256, kCtas = 3, kRows = 64;  // keys of a unit; CTAs per SM; rows in shared memory at once
 
 struct WeightArgs {
   Params p;                     // q, tables, lengths, starts, window, sinks, scale; data: the cache
@@ -50,6 +51,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
   using B = Block<HD>;
   constexpr int W = kThreads / 32, KS = HD / 16;
   __shared__ int s_share[4];  // first unit, the one behind the last; the request that the share begins with, and the units before it
+  __shared__ __align__(16) uint4 s_q[kRows * (HD / 8)];
+  __shared__ float s_sum[kRows];  // -lse in log2 units; -inf where there is no row
+  __shared__ int s_first[kRows];  // first place of the row's window
   const Params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   Request<kUnit> r;
@@ -89,107 +93,133 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
   }
   __syncthreads();
   const int end = s_share[1];
-  int b = s_share[2], before = s_share[3];
-  if (s_share[0] + warp >= end) return;
+  int b = s_share[2], before = s_share[3], u0 = s_share[0];
+  if (u0 >= end) return;
   int of = units_of(a, b, r);
   const int kap = !INT4 ? g : g & 1 ? 4 + ((g >> 1) ^ 1) : g >> 1;
 #pragma unroll 1
-  for (int u = s_share[0] + warp; u < end; u += W) {
+  while (u0 < end) {
 #pragma unroll 1
-    while (u >= before + of) {
+    while (u0 >= before + of) {
       before += of;
       of = units_of(a, ++b, r);
     }
-    const int h = (u - before) / r.cached, x = (u - before) - h * r.cached;
-    const int place = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from);
+    // The share's units of one request and head: x0 .. x1 - 1.
+    const int h = (u0 - before) / r.cached, x0 = (u0 - before) - h * r.cached, x1 = min(r.cached, x0 + end - u0);
+    u0 += x1 - x0;
     const int* table = p.tables + (int64_t)b * p.tables_ld;
-    // The lane adds up the weight of one key: row kap of block t.
-    const int mine = place + 8 * t + kap;
-    float* at_weight = a.weights + b * a.w_request + h * a.w_head + mine;
-    const float old = mine < r.len ? *at_weight : 0.f;
-    float given = 0.f;
     const int rows = r.n * p.group, first_all = p.window ? max(0, r.len - max(0, p.window - r.n)) : 0;
-    const bool masked = place + kUnit > r.len || (p.window && place < first_all && place + kUnit > p.sinks);
 #pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      if (place + 16 * half >= r.len) break;
-      uint32_t k[KS][4];  // the operand: keys kap of two blocks, the 32 (16) dims that the lane takes
-      bool bad = false;
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int at = place + 16 * half + 8 * y, entry = at / p.page, off = at - entry * p.page;
-        const int page = at < r.len ? table[entry] : 0;
-        const bool there = page >= 0 && page < p.pages && at < r.len;
-        bad |= page < 0 || page >= p.pages;
-        const char* from = p.data + (there ? page : 0) * p.d_page + h * p.d_head;
-        if constexpr (INT4) {
-          from += (int64_t)(off / kBlockTokens) * B::kBytes;
-          uint32_t w[HD / 32], pr = 0;
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) w[i] = 0;
-          if (there) {
-            const char* words = from + B::word(kap, HD / 32 * t);
-            if constexpr (HD == 128) {
-              const uint4 v = *reinterpret_cast<const uint4*>(words);
-              w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2*>(words);
-              w[0] = v.x, w[1] = v.y;
-            }
-            pr = *reinterpret_cast<const uint32_t*>(from + B::pair(kap, (HD / 4) * t / kGroup));
-          }
-          const uint32_t s2 = __byte_perm(pr, 0, 0x1010), o2 = __byte_perm(pr, 0, 0x3232);
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            k[2 * i][y] = two_values<DT, 0>(w[i], s2, o2);
-            k[2 * i][2 + y] = two_values<DT, 1>(w[i], s2, o2);
-            k[2 * i + 1][y] = two_values<DT, 2>(w[i], s2, o2);
-            k[2 * i + 1][2 + y] = two_values<DT, 3>(w[i], s2, o2);
-          }
-        } else {
-          from += (int64_t)(off + kap) * a.d_token + t * (HD / 2);
-          const bool row = there && at + kap < r.len;
-#pragma unroll
-          for (int i = 0; i < KS / 2; ++i) {
-            const uint4 v = row ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
-            k[2 * i][y] = v.x, k[2 * i][2 + y] = v.y, k[2 * i + 1][y] = v.z, k[2 * i + 1][2 + y] = v.w;
-          }
-        }
+    for (int row0 = 0; row0 < rows; row0 += kRows) {
+      // A row's 16-byte pieces in the order in which the lanes of a quad take them, exchanged by halves of 128 bytes in odd rows:
+      // eight lanes read different banks.
+      const int count = min(kRows, rows - row0), tiles = (count + 7) / 8;
+      __syncthreads();
+      for (int i = tid; i < tiles * 8 * (HD / 8); i += kThreads) {
+        const int row = i / (HD / 8), c = i % (HD / 8), flat = row0 + row;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < count)
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(r.s0 + flat / p.group) * p.q_n + (h * p.group + flat % p.group) * p.q_h + 16 * c);
+        s_q[row * (HD / 8) + ((c % (KS / 2) * 4 + c / (KS / 2)) ^ (4 * (row & 1)))] = v;
       }
-      if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-      float sum[2] = {0.f, 0.f};
+      if (tid < tiles * 8) {
+        const int flat = row0 + tid, node = flat / p.group;
+        const float lse = tid < count ? a.lse[(int64_t)(r.s0 + node) * p.heads + h * p.group + flat % p.group] : -INFINITY;
+        s_sum[tid] = lse == -INFINITY ? -INFINITY : lse * -1.4426950408889634f;
+        s_first[tid] = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
+      }
+      __syncthreads();
 #pragma unroll 1
-      for (int row0 = 0; row0 < rows; row0 += 8) {
-        const int flat = row0 + g;
-        const char* q_at = p.q + (int64_t)(r.s0 + flat / p.group) * p.q_n + (h * p.group + flat % p.group) * p.q_h + t * (HD / 2);
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-          const uint4 v = flat < rows ? *reinterpret_cast<const uint4*>(q_at + 16 * i) : make_uint4(0, 0, 0, 0);
-          mma<DT>(c, k[2 * i], v.x, v.y);
-          mma<DT>(c, k[2 * i + 1], v.z, v.w);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = row0 + 2 * t + e, node = row / p.group;
-          const float lse = row < rows ? a.lse[(int64_t)(r.s0 + node) * p.heads + h * p.group + row % p.group] : -INFINITY;
-          const int first = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
+      for (int x = x0 + warp; x < x1; x += W) {
+        const int place = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from);
+        // The lane adds up the weight of one key: row kap of block t.
+        const int mine = place + 8 * t + kap;
+        float* at_weight = a.weights + b * a.w_request + h * a.w_head + mine;
+        const float old = mine < r.len ? *at_weight : 0.f;
+        float given = 0.f;
+        const bool masked = place + kUnit > r.len || (p.window && place < first_all && place + kUnit > p.sinks);
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (place + 16 * half >= r.len) break;
+          uint32_t k[KS][4];  // the operand: keys kap of two blocks, the 32 (16) dims that the lane takes
+          bool bad = false;
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int at = place + 16 * half + 8 * y + kap;
-            const bool sees = !masked || (at < r.len && (at >= first || at < p.sinks));
-            if (sees && lse != -INFINITY) sum[y] += ex2(fmaf(c[2 * y + e], p.scale, lse * -1.4426950408889634f));
+            const int at = place + 16 * half + 8 * y, entry = at / p.page, off = at - entry * p.page;
+            const int page = at < r.len ? table[entry] : 0;
+            const bool there = page >= 0 && page < p.pages && at < r.len;
+            bad |= page < 0 || page >= p.pages;
+            const char* from = p.data + (there ? page : 0) * p.d_page + h * p.d_head;
+            if constexpr (INT4) {
+              from += (int64_t)(off / kBlockTokens) * B::kBytes;
+              uint32_t w[HD / 32], pr = 0;
+#pragma unroll
+              for (int i = 0; i < HD / 32; ++i) w[i] = 0;
+              if (there) {
+                const char* words = from + B::word(kap, HD / 32 * t);
+                if constexpr (HD == 128) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(words);
+                  w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                } else {
+                  const uint2 v = *reinterpret_cast<const uint2*>(words);
+                  w[0] = v.x, w[1] = v.y;
+                }
+                pr = *reinterpret_cast<const uint32_t*>(from + B::pair(kap, (HD / 4) * t / kGroup));
+              }
+              const uint32_t s2 = __byte_perm(pr, 0, 0x1010), o2 = __byte_perm(pr, 0, 0x3232);
+#pragma unroll
+              for (int i = 0; i < HD / 32; ++i) {
+                k[2 * i][y] = two_values<DT, 0>(w[i], s2, o2);
+                k[2 * i][2 + y] = two_values<DT, 1>(w[i], s2, o2);
+                k[2 * i + 1][y] = two_values<DT, 2>(w[i], s2, o2);
+                k[2 * i + 1][2 + y] = two_values<DT, 3>(w[i], s2, o2);
+              }
+            } else {
+              from += (int64_t)(off + kap) * a.d_token + t * (HD / 2);
+              const bool row = there && at + kap < r.len;
+#pragma unroll
+              for (int i = 0; i < KS / 2; ++i) {
+                const uint4 v = row ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+                k[2 * i][y] = v.x, k[2 * i][2 + y] = v.y, k[2 * i + 1][y] = v.z, k[2 * i + 1][2 + y] = v.w;
+              }
+            }
+          }
+          if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+          float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+          for (int tile = 0; tile < tiles; ++tile) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) {
+              const uint4 v = s_q[(8 * tile + g) * (HD / 8) + ((4 * i + t) ^ (4 * (g & 1)))];
+              mma<DT>(c, k[2 * i], v.x, v.y);
+              mma<DT>(c, k[2 * i + 1], v.z, v.w);
+            }
+            const float2 less = *reinterpret_cast<const float2*>(s_sum + 8 * tile + 2 * t);
+            if (masked) {
+              const int2 first = *reinterpret_cast<const int2*>(s_first + 8 * tile + 2 * t);
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const int at = place + 16 * half + 8 * y + kap;
+                const bool in = at < r.len, sink = at < p.sinks;
+                if (in && (sink || at >= first.x)) sum[y] += ex2(fmaf(c[2 * y], p.scale, less.x));
+                if (in && (sink || at >= first.y)) sum[y] += ex2(fmaf(c[2 * y + 1], p.scale, less.y));
+              }
+            } else {
+#pragma unroll
+              for (int y = 0; y < 2; ++y) sum[y] += ex2(fmaf(c[2 * y], p.scale, less.x)) + ex2(fmaf(c[2 * y + 1], p.scale, less.y));
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
+            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
+            if (t == 2 * half + y) given = sum[y];
           }
         }
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
-        sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
-        if (t == 2 * half + y) given = sum[y];
+        if (mine < r.len) *at_weight = old + given;
       }
     }
-    if (mine < r.len) *at_weight = old + given;
   }
 }
 

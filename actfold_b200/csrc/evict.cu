@@ -146,12 +146,26 @@ struct MoveArgs {
   int64_t tables_ld, capacity;
   int batch, heads, pages, page, places, keep;
   int columns, pieces;                              // CTAs side by side of a row; pieces of 16 (of 4 bits and 64 dims: 8) bytes of each
+  int rows;                                         // of a warp's step: at most 32, and kWarpPieces pieces
   uint32_t by_pieces;                               // p / pieces = p * by_pieces >> 20 for p < 2048, pieces <= 256
   unsigned* status;
 };
 
-constexpr int kMoveThreads = 256, kPer = 8, kStages = 3;  // pieces of a thread and step; steps in flight
-constexpr int kStepPieces = kMoveThreads * kPer;
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32, kStages = 3;  // steps in flight
+constexpr int kWarpPieces = 256, kPer = kWarpPieces / 32;  // of a step
+
+// Where a row lies: its first piece, and its row of a 4-bit block.
+struct Place {
+  char* at;
+  int r;
+};
+
+template <int BYTES>
+struct MoveShared {
+  static constexpr int kData = kStages * kMoveWarps * kWarpPieces * BYTES;
+  static constexpr int kPlaces = kMoveWarps * 32 * (int)sizeof(Place);  // of a step's rows: where from, and per stage where to
+  static constexpr int kBytes = kData + (1 + kStages) * kPlaces;
+};
 
 template <int BYTES>
 __device__ __forceinline__ void copy_in(uint32_t dst, const char* src) {
@@ -160,13 +174,15 @@ __device__ __forceinline__ void copy_in(uint32_t dst, const char* src) {
 }
 
 // HD = 0: rows of 16 bits (or any other) type; 64 or 128: 4-bit blocks of that many dims. CLUSTER CTAs share each step's rows.
+// A warp's step: its lanes look up a row each (page and place, where from and where to), then move the rows' pieces together.
 template <int HD, int CLUSTER>
 __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
   constexpr int kBytes = HD == 64 ? 8 : 16;
   using B = kv4::Block<HD == 0 ? 64 : HD>;
+  using M = MoveShared<kBytes>;
   extern __shared__ __align__(16) uint8_t buf[];
   pdl_wait();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t item = blockIdx.x / CLUSTER;
   const int rank = CLUSTER > 1 ? blockIdx.x % CLUSTER : 0;
   const int column = (int)(item % a.columns);
@@ -188,8 +204,9 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
       n = half;
     }
   }
-  const int step_rows = kStepPieces / a.pieces * CLUSTER;  // of the cluster
+  const int step_rows = CLUSTER * kMoveWarps * a.rows;
   const int steps = (a.keep - first + step_rows - 1) / step_rows;
+  const int mine = first + (rank * kMoveWarps + warp) * a.rows;  // the warp's first row of step 0
   char* base;
   int64_t page_step, token_step = 0;
   const int half = a.columns / 2;
@@ -202,35 +219,42 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
     base = a.k + l * a.kl + h * a.kh + (int64_t)column * B::kPart;  // columns: keys and values
     page_step = a.kp;
   }
-  // Where piece `piece` of the token at `place` lies, or null.
-  auto locate = [&](int place, int piece) -> char* {
+  auto locate = [&](int place) -> Place {
     const int entry = place / a.page, off = place - entry * a.page, pg = table[entry];
-    if (pg < 0 || pg >= a.pages) return nullptr;
+    if (pg < 0 || pg >= a.pages) return {nullptr, 0};
     char* at = base + pg * page_step;
-    if constexpr (HD == 0) return at + off * token_step + piece * 16;
-    const int r = off % kv4::kBlockTokens;
-    at += (int64_t)(off / kv4::kBlockTokens) * B::kBytes;
-    return at + (piece == 4 ? B::pair(r, 0) : B::word(r, piece * (kBytes / 4)));
+    if constexpr (HD == 0) return {at + off * token_step, 0};
+    return {at + (int64_t)(off / kv4::kBlockTokens) * B::kBytes, off % kv4::kBlockTokens};
   };
-  // Piece number u of this thread in a step: (row, piece) or row = keep.
-  auto mine = [&](int step, int u, int& row, int& piece) {
-    const int p = tid + kMoveThreads * u, q = (int)((uint32_t)p * a.by_pieces >> 20);
-    piece = p - q * a.pieces;
-    const int rows = kStepPieces / a.pieces;
-    row = q < rows ? min(a.keep, first + step * step_rows + rank * rows + q) : a.keep;
+  auto piece_of = [&](const Place& p, int piece) -> char* {
+    if constexpr (HD == 0) return p.at + piece * 16;
+    return p.at + (piece == 4 ? B::pair(p.r, 0) : B::word(p.r, piece * (kBytes / 4)));
   };
-  const uint32_t smem = smem_u32(buf);
+  uint8_t* data = buf + warp * kWarpPieces * kBytes;                     // + stage * kMoveWarps * kWarpPieces * kBytes
+  Place* from = reinterpret_cast<Place*>(buf + M::kData) + warp * 32;
+  Place* to = from + kMoveWarps * 32;                                    // + stage * kMoveWarps * 32
   bool bad = false;
   auto load = [&](int step) {
     if (step < steps) {
+      const int row = mine + step * step_rows + lane;
+      __syncwarp();
+      if (lane < a.rows) {
+        Place src{nullptr, 0}, dst{nullptr, 0};
+        if (row < a.keep) {
+          src = locate(kept[row]);
+          dst = locate(row);
+          if (!src.at || !dst.at) bad = true, src.at = nullptr;
+        }
+        from[lane] = src;
+        to[(step % kStages) * kMoveWarps * 32 + lane] = {src.at ? dst.at : nullptr, dst.r};
+      }
+      __syncwarp();
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
-        int row, piece;
-        mine(step, u, row, piece);
-        if (row < a.keep) {
-          const char* src = locate(kept[row], piece);
-          if (src) copy_in<kBytes>(smem + ((step % kStages) * kStepPieces + tid + kMoveThreads * u) * kBytes, src);
-          else bad = true;
+        const int p = lane + 32 * u, row = (int)((uint32_t)p * a.by_pieces >> 20);
+        if (row < a.rows) {
+          const Place src = from[row];
+          if (src.at) copy_in<kBytes>(smem_u32(data) + ((step % kStages) * kMoveWarps * kWarpPieces + p) * kBytes, piece_of(src, p - row * a.pieces));
         }
       }
     }
@@ -247,15 +271,15 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
     else __syncthreads();
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
-      int row, piece;
-      mine(s, u, row, piece);
-      if (row < a.keep) {
-        char* dst = locate(row, piece);
-        const bool there = dst && locate(kept[row], 0);
-        const uint8_t* from = buf + (int64_t)((s % kStages) * kStepPieces + tid + kMoveThreads * u) * kBytes;
-        if (!there) bad = true;
-        else if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(from);
-        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(from);
+      const int p = lane + 32 * u, row = (int)((uint32_t)p * a.by_pieces >> 20);
+      if (row < a.rows) {
+        const Place dst = to[(s % kStages) * kMoveWarps * 32 + row];
+        if (dst.at) {
+          char* at = piece_of(dst, p - row * a.pieces);
+          const uint8_t* x = data + ((s % kStages) * kMoveWarps * kWarpPieces + p) * kBytes;  // (what this lane itself brought)
+          if constexpr (kBytes == 16) *reinterpret_cast<uint4*>(at) = *reinterpret_cast<const uint4*>(x);
+          else *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(x);
+        }
       }
     }
   }
@@ -264,7 +288,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
 
 template <int HD, int CLUSTER>
 cudaError_t launch_move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
-  constexpr int bytes = kStages * kStepPieces * (HD == 64 ? 8 : 16);
+  constexpr int bytes = MoveShared<HD == 64 ? 8 : 16>::kBytes;
   // The same for every call: set each time, which costs less than keeping track of the devices.
   const cudaError_t e = cudaFuncSetAttribute(k_move<HD, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
@@ -343,6 +367,7 @@ extern "C" int af_evict_cache(const af_evict_args* args, uint32_t* status, void*
   }
   AF_REQUIRE(!moves || (al & 15) == 0, "af_evict_cache: addresses and strides must be multiples of 16 bytes");
   m.by_pieces = (uint32_t)(((1 << 20) + m.pieces - 1) / m.pieces);
+  m.rows = kv_evict::kWarpPieces / m.pieces < 32 ? kv_evict::kWarpPieces / m.pieces : 32;
   m.tables = w.tables;
   m.tables_ld = w.tables_stride;
   m.lengths = w.lengths;
