@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
           bool bad = false;
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int at = place + 16 * half + 8 * y, entry = at / p.page, off = at - entry * p.page;
+            const int at = place + 16 * half + 8 * y, entry = entry_of(p, at), off = at - entry * p.page;
             const int page = at < r.len ? table[entry] : 0;
             const bool there = page >= 0 && page < p.pages && at < r.len;
             bad |= page < 0 || page >= p.pages;
@@ -270,7 +270,7 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   p.kv_heads = (int)c.heads;
   p.group = (int)(w.n_heads / c.heads);
   p.pages = (int)c.pages;
-  p.page = (int)c.page_size;
+  kv4::set_page(p, c.page_size);
   p.capacity = w.max_pages * c.page_size;
   p.window = (int)w.window;
   p.sinks = (int)w.sinks;

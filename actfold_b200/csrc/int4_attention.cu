@@ -114,7 +114,7 @@ __device__ __forceinline__ void produce(const Params& p, uint8_t* gb, uint32_t b
       const int place = kUnit * (x < s.sink_units ? x : x - s.sink_units + s.from);
       const int tokens = x < s.x1 && x < s.cached ? min(kUnit, s.len - place) : 0;
       const int all = (tokens + kBlockTokens - 1) / kBlockTokens;
-      const int entry = tokens ? place / p.page : 0, at = (place - entry * p.page) / kBlockTokens;
+      const int entry = tokens ? entry_of(p, place) : 0, at = (place - entry * p.page) / kBlockTokens;
       const int run = min(all, p.page / kBlockTokens - at);
       const int page = tokens ? table[entry] : 0;
       bool sound = page >= 0 && page < p.pages;
@@ -665,7 +665,7 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.kv_heads = (int)c.heads;
   p.group = (int)(a.n_heads / c.heads);
   p.pages = (int)c.pages;
-  p.page = (int)c.page_size;
+  kv4::set_page(p, c.page_size);
   p.capacity = c.pages ? a.max_pages * c.page_size : 0;
   p.window = (int)a.window;
   p.sinks = (int)a.sinks;

@@ -29,6 +29,8 @@ struct Params {
   const uint32_t* mask;
   int64_t tables_ld, mask_ld;
   int words, batch, total, heads, kv_heads, group, pages, page;
+  uint32_t page_mul;                            // see entry_of
+  int page_shift;
   int runs;                                     // that 32 tokens of a cache lie in: of 32, 16 or 8 tokens, so that none leaves a page
   int64_t capacity;                             // tokens that a table row can hold
   int window, sinks;                            // window 0: all of the prefix is visible
@@ -46,6 +48,19 @@ struct Params {
   unsigned* status;
   int patience;                                 // attempts of a wait before it gives up
 };
+
+// place / p.page, for places up to 2^30 and pages of 8 d tokens: with s = ceil(log2 d) and m = ceil(2^(31 + s) / d) < 2^32 it is
+// (2 (place / 8) m) >> (32 + s), since m is too large by less than d / 2^(31 + s) and place / 8 < 2^27.
+__device__ __forceinline__ int entry_of(const Params& p, int place) {
+  return (int)(__umulhi((uint32_t)(place >> 3) << 1, p.page_mul) >> p.page_shift);
+}
+inline void set_page(Params& p, int64_t page) {
+  const uint64_t d = (uint64_t)page / kBlockTokens;
+  p.page = (int)page;
+  p.page_shift = 0;
+  while ((1ull << p.page_shift) < d) ++p.page_shift;
+  p.page_mul = (uint32_t)(((1ull << (31 + p.page_shift)) + d - 1) / d);
+}
 
 // A request's nodes and the units of UNIT keys that any of its rows can see: those of the first tokens, those of the
 // window, then those of its own tree.

@@ -8,14 +8,15 @@
 // which P is written in place (16 bits, TMEM operand of the second product).
 // With more than 128 rows they are two row tiles over the same keys; with
 // fewer, one row tile over the even and the odd key tiles, joined at the end.
-// Eight warps read the codes of the next tile into registers while they turn this
-// one's into values and write them where the tensor cores take them (a thread has half a key's
-// dims; 16-byte pieces, 128-byte swizzle): 64 KB a tile that go through shared memory twice, some
-// 1000 cycles of its 128 bytes, next to 512 cycles of products per pipe and of exponentials.
-// A softmax thread owns a row, so no scores are exchanged. The reference
-// maximum of a row is raised only when a score passes it by 2^8.
+// Four warps turn a tile's keys into values and write them where the tensor cores take them (a thread has a key; 16-byte
+// pieces, 128-byte swizzle), with the next tile's codes on their way to registers, and four its values, on their own: with
+// one after the other in eight warps the keys of a tile waited for the products with the values two tiles before
+// (8 trees of 20 to 64 nodes, 32 heads: 114 us). 64 KB a tile go through shared memory twice, some 1000 cycles of its
+// 128 bytes, next to 512 cycles of products per pipe. A softmax thread owns a row, so no scores are exchanged; 64 of
+// them at a time in registers, of which these warps get 152 each, and the others 64 and 48. The reference maximum of a row is
+// raised only when a score passes it by 2^8.
 //
-// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-15: keys and values;
+// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-11: keys; 12-15: values;
 // warp 16 issues S, warp 17 O, warp 18 plans.
 #include "int4_attention.cuh"
 
@@ -26,9 +27,9 @@ namespace {
 
 constexpr int kUnit = kWideUnit;           // keys of a tile
 constexpr int kRows = 128;                 // rows of a pipe
-constexpr int kSoft = 8, kTurn = 8;        // warps
+constexpr int kSoft = 8, kTurn = 8;        // warps (of the latter half for keys, half for values)
 constexpr int kMmaS = kSoft + kTurn, kMmaO = kMmaS + 1, kPlan = kMmaS + 2;
-constexpr int kThreads = 32 * (kPlan + 1);
+constexpr int kThreads = 32 * (kPlan + 2);  // (whole groups of four warps share out registers)
 constexpr int kReaders = kSoft + kTurn + 2;  // of a plan
 constexpr int kStages = 2;                 // of keys, and of values
 constexpr int kPanel = kUnit * 128;        // [128 rows][64 columns] of 16 bits, 128-byte swizzle
@@ -83,26 +84,37 @@ __device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t* r) {
                : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(taddr)
-               : "memory");
-}
 __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-               "r"(r[13]), "r"(r[14]), "r"(r[15])
-               : "memory");
+// 64 consecutive columns of the thread's TMEM lane.
+__device__ __forceinline__ void tmem_load64(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
+        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
+        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
+        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr)
+      : "memory");
 }
+
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D [tmem] (+)= A [smem] * B [smem]^T.
@@ -185,12 +197,16 @@ __device__ __noinline__ void set_aside(const Params& p, const Segment* plan, uin
   }
 }
 
-// What a thread holds of a tile: the codes and pairs of half the dims of one key and value, or of a node's rows nothing yet.
-template <int HD>
-struct Codes {
-  static constexpr int kWords = HD / 16, kPairs = HD / 64;
-  uint32_t k[kWords], v[kWords], kp[kPairs], vp[kPairs];
-};
+template <int R>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+constexpr int kRegsSoft = 152, kRegsTurn = 64, kRegsRest = 48;  // of a thread; at launch all have 96
+static_assert(8 * kRegsSoft + 8 * kRegsTurn + 4 * kRegsRest <= 20 * 96, "no more than the launch has");
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __grid_constant__ Params p) {
@@ -210,9 +226,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(k_full + 8 * i, kTurn);
+      mbar_init(k_full + 8 * i, kTurn / 2);
       mbar_init(k_empty + 8 * i, 1);
-      mbar_init(v_full + 8 * i, kTurn);
+      mbar_init(v_full + 8 * i, kTurn / 2);
       mbar_init(v_empty + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) {  // [pipe][half]
@@ -257,6 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
   };
   constexpr uint32_t kind = DT == AF_DTYPE_BF16 ? 0u : ((1u << 7) | (1u << 10));  // operand formats: bf16 = 1, f16 = 0
 
+  if (warp >= kMmaS) registers_down<kRegsRest>();
   if (warp == kPlan) {
     Planner<kUnit> planner;
     planner.begin(p, lane);
@@ -354,150 +371,125 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       read(seg++);
     }
     if (!ok) give_up();
-  } else if (warp >= kSoft) {
-    // ---------------- keys and values into 16 bits: thread = half the dims of a key of every tile ----------------
-    const int key = (tid - 32 * kSoft) >> 1, half = tid & 1;
-    using C = Codes<HD>;
-    const uint32_t row = key * 128, swz = key & 7;
-    // Byte of the thread's word i in a tile: 16 bytes of values. With 128 dims a thread with the second half takes its words in
-    // another order (i ^ 4), so that eight threads write different banks.
-    auto piece = [&](int i) {
-      if constexpr (HD == 128) return half * kPanel + row + 16 * ((uint32_t)(i ^ (half ? 4 : 0)) ^ swz);
-      else return row + 16 * ((uint32_t)(half * 4 + i) ^ swz);
+  } else if (warp >= kSoft && warp < kMmaS) {
+    registers_down<kRegsTurn>();
+    // ---------------- keys or values into 16 bits: thread = a key of every tile ----------------
+    constexpr int kWords = HD / 8, kPairs = HD / 32;
+    const bool values = warp >= kSoft + kTurn / 2;
+    const int key = tid & 127, part = values ? B::kPart : 0;
+    const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty, tiles_at = base + (values ? S::kOffV : S::kOffK) + key * 128;
+    auto write = [&](uint32_t tile, int i, uint4 v) {  // dims 8 i .. 8 i + 7
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + (i >> 3) * kPanel + 16 * ((i & 7) ^ (key & 7))), "r"(v.x), "r"(v.y), "r"(v.z),
+                   "r"(v.w)
+                   : "memory");
     };
-    auto write = [&](uint32_t at, uint4 v) {
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-    };
-    // The page of the thread's key of unit x (-1: not a cached key; out of range: reads as zeros).
+    // The page of the thread's key of unit x (nothing where it is no cached key).
     auto page_at = [&](const Segment& s, int x) -> int {
       const int at = x < s.cached ? place_of(s, x) + key : s.len;
-      return at < s.len ? p.tables[(int64_t)s.b * p.tables_ld + at / p.page] : -1;
+      return at < s.len ? p.tables[(int64_t)s.b * p.tables_ld + entry_of(p, at)] : 0;
     };
-    auto fetch = [&](const Segment& s, int x, int page, C& c) {
+    uint32_t w[kWords], pr[kPairs];
+    // The thread's codes and pairs of unit x; zeros where there is no cached key, and of a page out of range.
+    auto fetch = [&](const Segment& s, int x, int page) {
       const int at = x < s.cached ? place_of(s, x) + key : s.len;
 #pragma unroll
-      for (int i = 0; i < C::kWords; ++i) c.k[i] = c.v[i] = 0;
+      for (int i = 0; i < kWords; ++i) w[i] = 0;
 #pragma unroll
-      for (int i = 0; i < C::kPairs; ++i) c.kp[i] = c.vp[i] = 0;
+      for (int i = 0; i < kPairs; ++i) pr[i] = 0;
       if (at >= s.len) return;
       if (page < 0 || page >= p.pages) {
         if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
         return;
       }
-      const int off = at % p.page, r = off % kBlockTokens;
-      const char* from = p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes;
+      const int off = at - entry_of(p, at) * p.page, r = off % kBlockTokens;
+      const char* from = p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes + part;
 #pragma unroll
-      for (int val = 0; val < 2; ++val) {
-        uint32_t* w = val ? c.v : c.k;
-        uint32_t* pr = val ? c.vp : c.kp;
-#pragma unroll
-        for (int i = 0; i < C::kWords / 4; ++i) {
-          const int first = HD == 128 ? half * 8 + 4 * (i ^ half) : half * 4;
-          const uint4 y = *reinterpret_cast<const uint4*>(from + val * B::kPart + B::word(r, first));
-          w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
-          pr[i] = *reinterpret_cast<const uint32_t*>(from + val * B::kPart + B::pair(r, first / 4));
-        }
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 y = *reinterpret_cast<const uint4*>(from + B::word(r, 4 * i));
+        w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
       }
-    };
-    auto turn = [&](uint32_t to, const uint32_t* w, const uint32_t* pr) {
-#pragma unroll
-      for (int i = 0; i < C::kWords; ++i) {
-        const uint32_t s2 = __byte_perm(pr[i / 4], 0, 0x1010), o2 = __byte_perm(pr[i / 4], 0, 0x3232);
-        write(to + piece(i), make_uint4(two_values<DT, 0>(w[i], s2, o2), two_values<DT, 1>(w[i], s2, o2), two_values<DT, 2>(w[i], s2, o2),
-                                        two_values<DT, 3>(w[i], s2, o2)));
+      if constexpr (HD == 128) {
+        const uint4 y = *reinterpret_cast<const uint4*>(from + B::pair(r, 0));
+        pr[0] = y.x, pr[1] = y.y, pr[2] = y.z, pr[3] = y.w;
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(from + B::pair(r, 0));
+        pr[0] = y.x, pr[1] = y.y;
       }
-    };
-    // A node's row: the thread's half, zeros behind the last node; of values the ones that are not finite set aside.
-    auto copy_row = [&](const Segment& s, int x, uint32_t to, bool values) {
-      const int j = kUnit * (x - s.cached) + key;
-      const char* from = (values ? p.v + (int64_t)(s.s0 + j) * p.v_n + s.kvh * p.v_h : p.k + (int64_t)(s.s0 + j) * p.k_n + s.kvh * p.k_h) + half * HD;
-      bool sick = false;
-#pragma unroll
-      for (int i = 0; i < C::kWords; ++i) {
-        const int at = HD == 128 ? i ^ (half ? 4 : 0) : i;
-        uint4 v = j < s.n ? *reinterpret_cast<const uint4*>(from + 16 * at) : make_uint4(0, 0, 0, 0);
-        if (values) {
-          uint32_t* w = &v.x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool lo = not_finite<DT>(w[e]), hi = not_finite<DT>(w[e] >> 16);
-            sick |= lo || hi;
-            w[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-          }
-        }
-        write(to + piece(i), v);
-      }
-      return sick;
     };
     bool ok = true;
     int seg = 0, j = 0;
-    Segment next;
-    ok = planned(0, s);
-    bool more = ok;
-    C c;
-    int page = more ? page_at(s, s.x0) : -1;
-    if (more) fetch(s, s.x0, page, c);
-    int seg_next = 0, x_next = s.x0;  // the tile that comes after: its segment's number, its unit
-    next = s;
-    auto advance = [&]() {
-      if (x_next + 1 < next.x1) {
-        ++x_next;
-        return true;
-      }
-      if (!planned(++seg_next, next)) return false;
-      x_next = next.x0;
-      return true;
-    };
-    ok = true;
+    bool more = planned(0, s);
     int x = s.x0;
+    if (more) fetch(s, x, page_at(s, x));
 #pragma unroll 1
-    while (more && ok) {
-      const bool follows = advance();
-      const int next_page = follows ? page_at(next, x_next) : -1;
+    while (more) {
+      // The tile after this one: the segment's next, or the first of the next segment.
+      const bool ends = x + 1 == s.x1;
+      Segment next;
+      const bool follows = !ends || planned(seg + 1, next);
+      if (!ends) next = s;
+      const int x_next = ends ? next.x0 : x + 1, page = follows ? page_at(next, x_next) : 0;
       const int stage = j % kStages;
-      const bool cached = x < s.cached, masked = is_masked(p, s, x);
-      const uint32_t at_k = base + S::kOffK + stage * S::kTile, at_v = base + S::kOffV + stage * S::kTile;
-      if (j >= kStages) ok = agreed(wait_for(k_empty + 8 * stage, (j / kStages - 1) & 1, failed));
-      if (!ok) break;
-      if (cached) turn(at_k, c.k, c.kp);
-      else copy_row(s, x, at_k, false);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_full + 8 * stage);
+      const uint32_t tile = tiles_at + stage * S::kTile;
+      const bool cached = x < s.cached;
       bool sick = false;
-      if (cached && masked) {
+      if (values && cached && is_masked(p, s, x)) {
         // What no row sees is 0; NaN that only some rows see is set aside.
         const int at = place_of(s, x) + key;
         const bool hidden = at >= s.len || (p.window && at < s.len - (p.window - 1) && at >= p.sinks);
 #pragma unroll
-        for (int i = 0; i < C::kPairs; ++i) {
-          if (hidden) c.vp[i] = 0;
-          if (not_finite<DT>(c.vp[i]) || not_finite<DT>(c.vp[i] >> 16)) {
+        for (int i = 0; i < kPairs; ++i) {
+          if (hidden) pr[i] = 0;
+          if (not_finite<DT>(pr[i]) || not_finite<DT>(pr[i] >> 16)) {
             sick = true;
-            c.vp[i] = 0;
+            pr[i] = 0;
           }
         }
       }
-      if (j >= kStages) ok = agreed(wait_for(v_empty + 8 * stage, (j / kStages - 1) & 1, failed));
+      if (j >= kStages) ok = agreed(wait_for(empty + 8 * stage, (j / kStages - 1) & 1, failed));
       if (!ok) break;
-      if (cached) turn(at_v, c.v, c.vp);
-      else sick = copy_row(s, x, at_v, true);
+      if (cached) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          const uint32_t s2 = __byte_perm(pr[i / 4], 0, 0x1010), o2 = __byte_perm(pr[i / 4], 0, 0x3232);
+          write(tile, i, make_uint4(two_values<DT, 0>(w[i], s2, o2), two_values<DT, 1>(w[i], s2, o2), two_values<DT, 2>(w[i], s2, o2),
+                                    two_values<DT, 3>(w[i], s2, o2)));
+        }
+      } else {
+        // A node's row, zeros behind the last node; of values the ones that are not finite are set aside.
+        const int node = kUnit * (x - s.cached) + key;
+        const char* from = values ? p.v + (int64_t)(s.s0 + node) * p.v_n + s.kvh * p.v_h : p.k + (int64_t)(s.s0 + node) * p.k_n + s.kvh * p.k_h;
+#pragma unroll 4
+        for (int i = 0; i < kWords; ++i) {
+          uint4 v = node < s.n ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+          if (values) {
+            uint32_t* y = &v.x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool lo = not_finite<DT>(y[e]), hi = not_finite<DT>(y[e] >> 16);
+              sick |= lo || hi;
+              y[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+            }
+          }
+          write(tile, i, v);
+        }
+      }
       if (sick) atomicOr(&found[seg % kPlans], 1u << ((x - s.x0) >> found_shift(s.x1 - s.x0)));
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(v_full + 8 * stage);
+      if (lane == 0) mbar_arrive(full + 8 * stage);
+      if (follows) fetch(next, x_next, page);  // (on its way while the next stage is waited for)
       ++j;
-      if (x + 1 == s.x1) read(seg);
-      more = follows;
-      if (more) {
-        if (seg != seg_next) s = next;
-        seg = seg_next;
-        x = x_next;
-        fetch(s, x, next_page, c);
+      if (ends) {
+        read(seg++);
+        s = next;
       }
+      more = follows;
+      x = x_next;
     }
     if (!ok) give_up();
-  } else {
+  } else if (warp < kSoft) {
+    registers_up<kRegsSoft>();
     // ---------------- softmax of row r of the pipe's tiles ----------------
     const int quad = warp & 3, pipe = warp >> 2, r = 32 * quad + lane;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quad) << 16);
@@ -559,24 +551,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
               else vis[c] = r < rows && k < s.n ? seen_nodes(p, s.s0, s.n, node, k) : 0u;
             }
           }
-          // Scores; hidden ones -inf.
-          auto load = [&](int c, uint32_t* y) {
-            tmem_load32(at_s + 64 * half + 32 * c, y);
-            if (masked) {
+          constexpr int C = kUnit / 2;
+          uint32_t y[C];
+          tmem_load64(at_s + C * half, y);
+          if (masked) {  // hidden scores are -inf
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (!((vis[c] >> i) & 1u)) y[i] = 0xff800000u;
-            }
-          };
-          uint32_t y[32];
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                if (!((vis[c] >> i) & 1u)) y[32 * c + i] = 0xff800000u;
+          }
+          float top[4];
 #pragma unroll
-          for (int c = 1; c >= 0; --c) {  // (the first 32 last: they stay in the registers)
-            load(c, y);
+          for (int c = 0; c < 4; ++c) {
+            top[c] = __uint_as_float(y[16 * c]);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(y[i + 2 * e]), __uint_as_float(y[i + 2 * e + 1])));
+            for (int i = 1; i < 15; i += 2) top[c] = fmaxf(top[c], fmaxf(__uint_as_float(y[16 * c + i]), __uint_as_float(y[16 * c + i + 1])));
+            top[c] = fmaxf(top[c], __uint_as_float(y[16 * c + 15]));
           }
           const float t_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
           const bool raise = m == kUnset ? t_max > kUnset : t_max > m + (kLead<DT> + kRaise);
@@ -600,22 +591,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
             }
           }
           const uint64_t sc2 = pair(sc, sc), nm2 = pair(-m, -m);
+          uint32_t e[C / 2];
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            if (c) load(1, y);
-            uint32_t e[16];
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float2 a = unpair(fma2(pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), sc2, nm2));
-              const float2 b = unpair(fma2(pair(__uint_as_float(y[2 * i + 2]), __uint_as_float(y[2 * i + 3])), sc2, nm2));
-              const float a0 = ex2(a.x), a1 = ex2(a.y), b0 = ex2(b.x), b1 = ex2(b.y);
-              l0 = add2(l0, pair(a0, a1));
-              l1 = add2(l1, pair(b0, b1));
-              e[i] = pack2<DT>(a0, a1);
-              e[i + 1] = pack2<DT>(b0, b1);
-            }
-            tmem_store16(at_s + 64 * half + 16 * c, e);
+          for (int i = 0; i < C / 2; i += 2) {
+            const float2 a = unpair(fma2(pair(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), sc2, nm2));
+            const float2 b = unpair(fma2(pair(__uint_as_float(y[2 * i + 2]), __uint_as_float(y[2 * i + 3])), sc2, nm2));
+            const float a0 = ex2(a.x), a1 = ex2(a.y), b0 = ex2(b.x), b1 = ex2(b.y);
+            l0 = add2(l0, pair(a0, a1));
+            l1 = add2(l1, pair(b0, b1));
+            e[i] = pack2<DT>(a0, a1);
+            e[i + 1] = pack2<DT>(b0, b1);
           }
+          tmem_store32(at_s + C * half, e);
           tmem_wait_store();
         }
         tc_fence_before();
