@@ -9,15 +9,15 @@
 // With more than 128 rows they are two row tiles over the same keys; with
 // fewer, one row tile over the even and the odd key tiles, joined at the end.
 // Four warps turn a tile's keys into values and write them where the tensor cores take them (a thread has a key; 16-byte
-// pieces, 128-byte swizzle), with the next tile's codes on their way to registers, and four its values, on their own: with
-// one after the other in eight warps the keys of a tile waited for the products with the values two tiles before
-// (8 trees of 20 to 64 nodes, 32 heads: 114 us). 64 KB a tile go through shared memory twice, some 1000 cycles of its
-// 128 bytes, next to 512 cycles of products per pipe. A softmax thread owns a row, so no scores are exchanged; 64 of
-// them at a time in registers, of which these warps get 152 each, and the others 64 and 48. The reference maximum of a row is
-// raised only when a score passes it by 2^8.
+// pieces, 128-byte swizzle), with their next tile's codes on the way to registers; two such groups take turns with
+// the tiles, and as many do the same for the values. (8 trees of 20 to 64 nodes, 32 heads: keys and values one after the other
+// in eight warps 114 us, the keys of a tile waited for the products with the values two tiles before; four warps each
+// 105 us, at 6000 cycles a tile, 2000 of them for the turning and as many for latencies.) 64 KB a tile go through shared memory
+// twice, some 1000 cycles of its 128 bytes, next to 512 cycles of products per pipe. A softmax thread owns a row, so no
+// scores are exchanged. The reference maximum of a row is raised only when a score passes it by 2^8.
 //
-// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-11: keys; 12-15: values;
-// warp 16 issues S, warp 17 O, warp 18 plans.
+// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-15: keys; 16-23: values;
+// warp 24 issues S, warp 25 O, warp 26 plans.
 #include "int4_attention.cuh"
 
 namespace af {
@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kUnit = kWideUnit;           // keys of a tile
 constexpr int kRows = 128;                 // rows of a pipe
-constexpr int kSoft = 8, kTurn = 8;        // warps (of the latter half for keys, half for values)
+constexpr int kSoft = 8, kGroups = 1, kTurn = 8 * kGroups;  // warps; groups of four that take turns with the tiles (of the latter half for keys, half for values)
 constexpr int kMmaS = kSoft + kTurn, kMmaO = kMmaS + 1, kPlan = kMmaS + 2;
 constexpr int kThreads = 32 * (kPlan + 2);  // (whole groups of four warps share out registers)
 constexpr int kReaders = kSoft + kTurn + 2;  // of a plan
@@ -84,24 +84,40 @@ __device__ __forceinline__ void tmem_load8(uint32_t taddr, uint32_t* r) {
                : "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void tmem_load16x2(uint32_t a, uint32_t b, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(a), "r"(b)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+                 "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+                 "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr)
+               : "memory");
+}
 // 64 consecutive columns of the thread's TMEM lane.
 __device__ __forceinline__ void tmem_load64(uint32_t taddr, uint32_t* r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]),
-        "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]),
-        "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]),
-        "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
-        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
-      : "r"(taddr)
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr), "r"(taddr + 32)
       : "memory");
 }
 
@@ -206,7 +222,7 @@ __device__ __forceinline__ void registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 constexpr int kRegsSoft = 152, kRegsTurn = 64, kRegsRest = 48;  // of a thread; at launch all have 96
-static_assert(8 * kRegsSoft + 8 * kRegsTurn + 4 * kRegsRest <= 20 * 96, "no more than the launch has");
+static_assert(kThreads == 20 * 32 && 8 * kRegsSoft + 8 * kRegsTurn + 4 * kRegsRest <= 20 * 96, "no more than the launch has");
 
 template <int DT, int HD>
 __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __grid_constant__ Params p) {
@@ -226,9 +242,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
 
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(k_full + 8 * i, kTurn / 2);
+      mbar_init(k_full + 8 * i, 4);
       mbar_init(k_empty + 8 * i, 1);
-      mbar_init(v_full + 8 * i, kTurn / 2);
+      mbar_init(v_full + 8 * i, 4);
       mbar_init(v_empty + 8 * i, 1);
     }
     for (int i = 0; i < 4; ++i) {  // [pipe][half]
@@ -294,14 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     if (!ok) give_up();
   } else if (warp == kMmaS) {
     // ---------------- S: two row tiles of a key tile, or one of every other key tile ----------------
-    constexpr uint32_t id_s = idesc_bf16(kRows, kUnit) ^ kind;
+    // With two, 64 keys at a time: a half's S goes where P of the half before it has been multiplied, while the softmax works on
+    // the other half (4 requests of 64 nodes x 7 heads over up to 65 K keys 268 -> 255 us). With one the other pipe fills the gaps,
+    // and products of 64 columns cost three quarters of those of 128 (8 trees of 20 to 64 nodes, 32 heads 96 -> 99 us).
+    constexpr uint32_t id_half = idesc_bf16(kRows, kUnit / 2) ^ kind, id_all = idesc_bf16(kRows, kUnit) ^ kind;
     const uint64_t d_k = sw128_desc(base + S::kOffK), d_q = sw128_desc(base + S::kOffQ);
     bool ok = true;
     int seg = 0, j = 0, used0 = 0, used1 = 0;  // tiles; tiles of S of the pipes
 #pragma unroll 1
     while (ok && planned(seg, s)) {
       const bool two = s.n * p.group - s.row0 > kRows && p.rows > kRows;
-      const int tiles = s.x1 - s.x0, steps = two ? 2 : 1;  // of a key tile
+      const int tiles = s.x1 - s.x0, steps = two ? 4 : 1;  // of a key tile
       ok = agreed(wait_for(q_full, seg & 1, failed));
 #pragma unroll 1
       for (int t = 0; ok && t < tiles; ++t, ++j) {
@@ -309,22 +328,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         ok = agreed(wait_for(k_full + 8 * stage, (j / kStages) & 1, failed));
 #pragma unroll 1
         for (int x = 0; ok && x < steps; ++x) {
-          const int pipe = two ? x : t & 1, used = pipe ? used1 : used0;
-          if (used) ok = agreed(wait_for(done + 8 * (2 * pipe + 1), (used - 1) & 1, failed));  // P V of the pipe's last keys
+          const int half = two ? x >> 1 : 0, pipe = two ? x & 1 : t & 1, bar = 2 * pipe + half, used = pipe ? used1 : used0;
+          if (used) ok = agreed(wait_for(done + 8 * (two ? bar : bar + 1), (used - 1) & 1, failed));  // P V of the last keys there
           if (!ok) break;
           tc_fence_after();
-          const uint64_t a = d_q + (two && pipe ? (uint32_t)S::kTile >> 4 : 0u), b = d_k + (uint32_t)stage * (S::kTile >> 4);
+          const uint64_t a = d_q + ((p.rows > kRows ? two && pipe : seg & 1) ? (uint32_t)S::kTile >> 4 : 0u), b = d_k + (uint32_t)stage * (S::kTile >> 4) + half * (kPanel >> 5);
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk)
-              mma_from_smem(tmem + 128 * pipe, a + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3), b + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3), id_s, kk ? 1u : 0u);
-            tc_commit(s_full + 8 * pipe);
+              mma_from_smem(tmem + 128 * pipe + 64 * half, a + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3), b + (kk >> 2) * (kPanel >> 4) + 2 * (kk & 3),
+                            two ? id_half : id_all, kk ? 1u : 0u);
+            tc_commit(s_full + 8 * bar);
+            if (!two) tc_commit(s_full + 8 * (bar + 1));
             if (x == steps - 1) tc_commit(k_empty + 8 * stage);
           }
           __syncwarp();
-          if (pipe) ++used1;
-          else ++used0;
         }
+        used0 += two || !(t & 1);
+        used1 += two || (t & 1);
       }
       read(seg++);
     }
@@ -373,36 +394,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     if (!ok) give_up();
   } else if (warp >= kSoft && warp < kMmaS) {
     registers_down<kRegsTurn>();
-    // ---------------- keys or values into 16 bits: thread = a key of every tile ----------------
+    // ---------------- keys or values into 16 bits: thread = a key of the group's tiles ----------------
     constexpr int kWords = HD / 8, kPairs = HD / 32;
     const bool values = warp >= kSoft + kTurn / 2;
-    const int key = tid & 127, part = values ? B::kPart : 0;
-    const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty, tiles_at = base + (values ? S::kOffV : S::kOffK) + key * 128;
+    const int key = tid & 127, group = (warp >> 2) % kGroups;
+    const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
+    const uint32_t tiles_at = base + (values ? S::kOffV : S::kOffK) + key * 128;
     auto write = [&](uint32_t tile, int i, uint4 v) {  // dims 8 i .. 8 i + 7
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(tile + (i >> 3) * kPanel + 16 * ((i & 7) ^ (key & 7))), "r"(v.x), "r"(v.y), "r"(v.z),
                    "r"(v.w)
                    : "memory");
     };
-    // The page of the thread's key of unit x (nothing where it is no cached key).
-    auto page_at = [&](const Segment& s, int x) -> int {
-      const int at = x < s.cached ? place_of(s, x) + key : s.len;
-      return at < s.len ? p.tables[(int64_t)s.b * p.tables_ld + entry_of(p, at)] : 0;
+    // The group's next tile: unit x of segment seg, its place of the thread's key (-1: none that is cached) and that one's page.
+    int seg = 0, x = 0, at = -1, page = 0;
+    auto look_up = [&]() {
+      const Segment& f = plans[seg % kPlans];
+      at = x < f.cached ? place_of(f, x) + key : f.len;
+      if (at >= f.len) at = -1;
+      page = at < 0 ? 0 : p.tables[(int64_t)f.b * p.tables_ld + entry_of(p, at)];
+    };
+    auto first_of = [&]() {  // from unit 0 of segment seg on
+#pragma unroll 1
+      for (;; ++seg) {
+        if (!agreed(wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed))) {
+          *failed = 1;
+          return false;
+        }
+        const Segment& f = plans[seg % kPlans];
+        if (f.x1 <= 0) return false;
+        x = f.x0 + (group - f.j0 % kGroups + kGroups) % kGroups;
+        if (x < f.x1) return true;
+      }
     };
     uint32_t w[kWords], pr[kPairs];
-    // The thread's codes and pairs of unit x; zeros where there is no cached key, and of a page out of range.
-    auto fetch = [&](const Segment& s, int x, int page) {
-      const int at = x < s.cached ? place_of(s, x) + key : s.len;
+    // The thread's codes and pairs; zeros where there is no cached key, and of a page out of range.
+    auto fetch = [&]() {
 #pragma unroll
       for (int i = 0; i < kWords; ++i) w[i] = 0;
 #pragma unroll
       for (int i = 0; i < kPairs; ++i) pr[i] = 0;
-      if (at >= s.len) return;
+      if (at < 0) return;
       if (page < 0 || page >= p.pages) {
         if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
         return;
       }
       const int off = at - entry_of(p, at) * p.page, r = off % kBlockTokens;
-      const char* from = p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes + part;
+      const char* from = p.data + page * p.d_page + plans[seg % kPlans].kvh * p.d_head + (off / kBlockTokens) * B::kBytes + (values ? B::kPart : 0);
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
         const uint4 y = *reinterpret_cast<const uint4*>(from + B::word(r, 4 * i));
@@ -416,27 +453,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         pr[0] = y.x, pr[1] = y.y;
       }
     };
-    bool ok = true;
-    int seg = 0, j = 0;
-    bool more = planned(0, s);
-    int x = s.x0;
-    if (more) fetch(s, x, page_at(s, x));
+    bool ok = true, more = first_of();
+    if (more) {
+      look_up();
+      fetch();
+    }
+    int done_with = 0;  // segments that this warp no longer reads
+    for (; done_with < seg; ++done_with) read(done_with);
 #pragma unroll 1
     while (more) {
-      // The tile after this one: the segment's next, or the first of the next segment.
-      const bool ends = x + 1 == s.x1;
-      Segment next;
-      const bool follows = !ends || planned(seg + 1, next);
-      if (!ends) next = s;
-      const int x_next = ends ? next.x0 : x + 1, page = follows ? page_at(next, x_next) : 0;
-      const int stage = j % kStages;
+      const Segment& f = plans[seg % kPlans];
+      const int now = seg, x_now = x, at_now = at, j = f.j0 + x - f.x0, stage = j % kStages;
       const uint32_t tile = tiles_at + stage * S::kTile;
-      const bool cached = x < s.cached;
+      const bool cached = x < f.cached;
+      // The next tile's page is looked up meanwhile. (Each segment has a tile, and every kGroups-th is the group's: the next lies at
+      // most two segments on, which are planned while this one is still held.)
+      x += kGroups;
+      more = x < f.x1;
+      if (!more) {
+        ++seg;
+        more = first_of();
+      }
+      if (more) look_up();
       bool sick = false;
-      if (values && cached && is_masked(p, s, x)) {
-        // What no row sees is 0; NaN that only some rows see is set aside.
-        const int at = place_of(s, x) + key;
-        const bool hidden = at >= s.len || (p.window && at < s.len - (p.window - 1) && at >= p.sinks);
+      if (values && cached && is_masked(p, f, x_now)) {
+        // What no row sees is 0 (as what there is no key for); NaN that only some rows see is set aside.
+        const bool hidden = at_now < 0 || (p.window && at_now < f.len - (p.window - 1) && at_now >= p.sinks);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
           if (hidden) pr[i] = 0;
@@ -457,11 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         }
       } else {
         // A node's row, zeros behind the last node; of values the ones that are not finite are set aside.
-        const int node = kUnit * (x - s.cached) + key;
-        const char* from = values ? p.v + (int64_t)(s.s0 + node) * p.v_n + s.kvh * p.v_h : p.k + (int64_t)(s.s0 + node) * p.k_n + s.kvh * p.k_h;
+        const int node = kUnit * (x_now - f.cached) + key;
+        const char* from = values ? p.v + (int64_t)(f.s0 + node) * p.v_n + f.kvh * p.v_h : p.k + (int64_t)(f.s0 + node) * p.k_n + f.kvh * p.k_h;
+        const bool there = node < f.n;
 #pragma unroll 4
         for (int i = 0; i < kWords; ++i) {
-          uint4 v = node < s.n ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+          uint4 v = there ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
           if (values) {
             uint32_t* y = &v.x;
 #pragma unroll
@@ -474,18 +517,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
           write(tile, i, v);
         }
       }
-      if (sick) atomicOr(&found[seg % kPlans], 1u << ((x - s.x0) >> found_shift(s.x1 - s.x0)));
+      if (sick) atomicOr(&found[now % kPlans], 1u << ((x_now - f.x0) >> found_shift(f.x1 - f.x0)));
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(full + 8 * stage);
-      if (follows) fetch(next, x_next, page);  // (on its way while the next stage is waited for)
-      ++j;
-      if (ends) {
-        read(seg++);
-        s = next;
-      }
-      more = follows;
-      x = x_next;
+      if (more) fetch();  // (on its way while the stage is waited for)
+      for (; done_with < seg; ++done_with) read(done_with);
     }
     if (!ok) give_up();
   } else if (warp < kSoft) {
@@ -501,6 +538,47 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     };
     int seg = 0, taken = 0;  // halves of S of this pipe so far
     bool wrote_start = false;
+    // Q of a segment: the thread's row, 16-byte pieces swizzled over 128 bytes; zeros where there is no row. Two row tiles have a
+    // buffer each and come when the segment begins, one has both by turns and comes while the one before it is worked on.
+    auto q_tile = [&](int number, int pipe) { return p.rows > kRows ? pipe : number & 1; };
+    auto bring_q = [&](int number) {
+      if (!agreed(wait_for(plan_full + 8 * (number % kPlans), (number / kPlans) & 1, failed))) return;
+      const Segment& f = plans[number % kPlans];
+      if (f.x1 <= 0) return;
+      const int all = min(p.rows, f.n * p.group - f.row0), row = p.rows > kRows ? kRows * pipe + r : r;
+      if (p.rows <= kRows ? pipe > 0 : all <= kRows * pipe) return;
+      const int flat = f.row0 + min(row, all - 1);
+      const char* from = p.q + (int64_t)(f.s0 + flat / p.group) * p.q_n + (f.kvh * p.group + flat % p.group) * p.q_h;
+      const uint32_t to = base + S::kOffQ + q_tile(number, pipe) * S::kTile + r * 128;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + (i >> 3) * kPanel + 16 * ((i & 7) ^ (r & 7))), "l"(from + 16 * i),
+                     "r"(row < all ? 16 : 0)
+                     : "memory");
+    };
+    // Q of a segment has landed: S may read it.
+    auto landed = [&](int number) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (p.q_flip | ~p.q_keep) {  // (a scale that is not positive)
+        const uint32_t mine = base + S::kOffQ + q_tile(number, pipe) * S::kTile + r * 128;
+#pragma unroll 1
+        for (int i = 0; i < HD / 8 && (p.rows > kRows || pipe == 0); ++i) {
+          uint4 v;
+          const uint32_t at = mine + (i >> 3) * kPanel + 16 * (i & 7);
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"((v.x ^ p.q_flip) & p.q_keep), "r"((v.y ^ p.q_flip) & p.q_keep),
+                       "r"((v.z ^ p.q_flip) & p.q_keep), "r"((v.w ^ p.q_flip) & p.q_keep)
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    };
+    if (p.rows <= kRows) {
+      bring_q(0);
+      landed(0);
+    }
     // Into the next segment go all softmax warps or none, whatever each has seen of a plan or of a wait that ran out: the
     // barriers inside have no limit of their own.
     auto enter = [&]() {
@@ -516,21 +594,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       const int rows = min(kRows, two && pipe ? all - kRows : all);
       const int flat = s.row0 + min(row, all - 1), node = flat / p.group, head = s.kvh * p.group + flat % p.group;
       const bool busy = 32 * quad < rows;                     // any of the warp's rows is one
-      // Q: its row, 16-byte pieces swizzled over 128 bytes; zeros where there is no row. (S of the segment before is complete: all pipes have read it.)
-      if (two || pipe == 0) {
-        const char* from = p.q + (int64_t)(s.s0 + node) * p.q_n + head * p.q_h;
-        const uint32_t to = base + S::kOffQ + pipe * S::kTile + r * 128;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          const uint4 v = r < rows ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + (i >> 3) * kPanel + 16 * ((i & 7) ^ (r & 7))), "r"((v.x ^ p.q_flip) & p.q_keep),
-                       "r"((v.y ^ p.q_flip) & p.q_keep), "r"((v.z ^ p.q_flip) & p.q_keep), "r"((v.w ^ p.q_flip) & p.q_keep)
-                       : "memory");
-        }
-        fence_proxy_async_smem();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      if (p.rows > kRows) bring_q(seg);  // (S of the segment before is complete: all pipes have read it)
+      if (p.rows > kRows) landed(seg);
+      if (p.rows <= kRows) bring_q(seg + 1);
       const int first = first_place(p, s.s0, s.n, s.len, node);
       float m = kUnset;
       uint64_t l0 = 0ull, l1 = 0ull;
@@ -539,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         const int x = s.x0 + (x2 >> 1), half = x2 & 1, bar = 2 * pipe + half;  // a half of a tile at a time
         const bool cached = x < s.cached, masked = is_masked(p, s, x);
         const int key0 = (cached ? place_of(s, x) : kUnit * (x - s.cached)) + 64 * half;
-        if (half == 0) wait(s_full + 8 * pipe, (taken >> 1) & 1);
+        wait(s_full + 8 * bar, (taken >> 1) & 1);
         tc_fence_after();
         if (busy) {
           uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
@@ -609,6 +675,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * bar);
       }
+      if (p.rows <= kRows) landed(seg + 1);  // (its first S are made while this segment's rows are written)
       // ---- the segment's rows ----
       const float2 la = unpair(add2(l0, l1));
       const float mine = la.x + la.y;
@@ -640,29 +707,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         char* out = p.out + (int64_t)(s.s0 + node) * p.out_n + head * p.out_h;
         float* part = scratch.sums(blockIdx.x, which) + (int64_t)row * HD;
 #pragma unroll 1
-        for (int d = d0; d < d1; d += 8) {
-          uint32_t o[8];
-          float y[8];
-          tmem_load8(from + d, o);
+        for (int d = d0; d < d1; d += 16) {
+          uint32_t o[32];
+          float y[16];
+          tmem_load16x2(from + d, from + d + (single ? 0 : 128), o);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(o[i]) * f0;
-          if (!single) {
-            tmem_load8(from + 128 + d, o);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = fmaf(__uint_as_float(o[i]), f1, y[i]);
+          for (int i = 0; i < 16; ++i) {
+            y[i] = __uint_as_float(o[i]) * f0;
+            if (!single) y[i] = fmaf(__uint_as_float(o[16 + i]), f1, y[i]);
           }
           if (r < rows) {
             if (aside) {
-              float more[8];
-              set_aside<DT, HD>(p, plans + seg % kPlans, aside, node, first, d, more);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[i] += more[i];
+              for (int x = 0; x < 16; x += 8) {
+                float more[8];
+                set_aside<DT, HD>(p, plans + seg % kPlans, aside, node, first, d + x, more);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[x + i] += more[i];
+              }
             }
-            if (whole) {
-              *reinterpret_cast<uint4*>(out + 2 * d) = make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
-            } else {
-              *reinterpret_cast<float4*>(part + d) = make_float4(y[0], y[1], y[2], y[3]);
-              *reinterpret_cast<float4*>(part + d + 4) = make_float4(y[4], y[5], y[6], y[7]);
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+              if (whole) {
+                *reinterpret_cast<uint4*>(out + 2 * (d + i)) =
+                    make_uint4(pack2<DT>(y[i], y[i + 1]), pack2<DT>(y[i + 2], y[i + 3]), pack2<DT>(y[i + 4], y[i + 5]), pack2<DT>(y[i + 6], y[i + 7]));
+              } else {
+                *reinterpret_cast<float4*>(part + d + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+                *reinterpret_cast<float4*>(part + d + i + 4) = make_float4(y[i + 4], y[i + 5], y[i + 6], y[i + 7]);
+              }
             }
           }
         }
