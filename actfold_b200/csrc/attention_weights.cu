@@ -5,9 +5,9 @@
 // over the places p that row i sees. The rows' sums are known (lse), so keys
 // are independent: a warp takes 32 of them, all rows of the request against
 // 16 at a time in registers (m16n8k16, the keys as the M side: few rows waste little), and adds to their
-// weights without atomics. The rows of a request and head, 64 at a time, lie in shared memory with their sums. With few rows
-// HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and 8 of its weight; with many the products
-// do. See int4_attention.cu for the fragments' order.
+// weights without atomics. The rows of a request and head, 64 at a time, lie in shared memory with their sums. 4-bit
+// keys come by bulk copies, a unit ahead. With few rows HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and 8
+// of its weight; with many the products do. See int4_attention.cu for the fragments' order.
 #include <string>
 
 #include "int4_attention.cuh"
@@ -16,7 +16,7 @@ namespace af {
 namespace kv4 {
 namespace {
 
-constexpr int kUnit = 32, kThreads = 256, kCtas = 3, kRows = 64;  // keys of a unit; CTAs per SM; rows in shared memory at once
+constexpr int kUnit = 32, kThreads = 256, kCtas = 2, kRows = 64;  // keys of a unit; CTAs per SM; rows in shared memory at once
 
 struct WeightArgs {
   Params p;                     // q, tables, lengths, starts, window, sinks, scale; data: the cache
@@ -46,6 +46,10 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, ui
   }
 }
 
+// Dynamic shared memory: two units' 4-bit keys per warp.
+template <int HD>
+constexpr int kRing = kThreads / 32 * 2 * (kUnit / kBlockTokens) * Block<HD>::kPart;
+
 template <int DT, int HD, bool INT4>
 __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_constant__ WeightArgs a) {
   using B = Block<HD>;
@@ -54,9 +58,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
   __shared__ __align__(16) uint4 s_q[kRows * (HD / 8)];
   __shared__ float s_sum[kRows];  // -lse in log2 units; -inf where there is no row
   __shared__ int s_first[kRows];  // first place of the row's window
+  __shared__ __align__(8) uint64_t s_full[2 * W];
+  extern __shared__ __align__(128) uint8_t ring[];
+  constexpr int kUnitBytes = kUnit / kBlockTokens * B::kPart;
   const Params& p = a.p;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   Request<kUnit> r;
+  if (tid < 2 * W) {
+    mbar_init(smem_u32(s_full + tid), 1);
+    fence_barrier_init();
+  }
   if (warp == 0) {
     bool disorder = false;
     int all = 0;
@@ -97,6 +108,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
   if (u0 >= end) return;
   int of = units_of(a, b, r);
   const int kap = !INT4 ? g : g & 1 ? 4 + ((g >> 1) ^ 1) : g >> 1;
+  uint8_t* slots = ring + warp * 2 * kUnitBytes;
+  const uint32_t full = smem_u32(s_full + 2 * warp);
+  int brought = 0, taken = 0;  // units of this warp
+  bool lost = false;           // a wait has run out
 #pragma unroll 1
   while (u0 < end) {
 #pragma unroll 1
@@ -129,105 +144,152 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
         s_first[tid] = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
       }
       __syncthreads();
+      // A unit's keys: lane y brings block y, if its page is one; what there is no key for reads as zeros.
+      auto bring = [&](int x) {
+        if (x >= x1 || lost) return;
+        const int at = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from) + kBlockTokens * lane, slot = brought & 1;
+        const bool mine = lane < kUnit / kBlockTokens, needed = mine && at < r.len;
+        const int entry = needed ? entry_of(p, at) : 0, page = needed ? table[entry] : 0;
+        const bool there = needed && page >= 0 && page < p.pages;
+        if (needed && !there && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+        if (mine && !there) {
+          for (int y = 0; y < B::kPart / 16; ++y) reinterpret_cast<uint4*>(slots + slot * kUnitBytes + lane * B::kPart)[y] = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        const uint32_t blocks = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, __popc(blocks) * B::kPart);
+        __syncwarp();
+        if (there) {
+          const char* from = p.data + page * p.d_page + h * p.d_head + (int64_t)((at - entry * p.page) / kBlockTokens) * B::kBytes;
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           smem_u32(slots) + slot * kUnitBytes + lane * B::kPart),
+                       "l"(from), "r"(B::kPart), "r"(full + 8 * slot)
+                       : "memory");
+        }
+        ++brought;
+      };
+      if constexpr (INT4) bring(x0 + warp);
 #pragma unroll 1
-      for (int x = x0 + warp; x < x1; x += W) {
+      for (int x = x0 + warp; x < x1 && !lost; x += W) {
+        if constexpr (INT4) {
+          bring(x + W);
+          int tries = 0;
+          while (!lost && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1)) lost = ++tries > kPatience;
+          lost = __any_sync(0xffffffffu, lost);
+          if (lost) {
+            if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
+            break;
+          }
+        }
         const int place = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from);
         // The lane adds up the weight of one key: row kap of block t.
         const int mine = place + 8 * t + kap;
         float* at_weight = a.weights + b * a.w_request + h * a.w_head + mine;
         const float old = mine < r.len ? *at_weight : 0.f;
-        float given = 0.f;
         const bool masked = place + kUnit > r.len || (p.window && place < first_all && place + kUnit > p.sinks);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          if (place + 16 * half >= r.len) break;
-          uint32_t k[KS][4];  // the operand: keys kap of two blocks, the 32 (16) dims that the lane takes
-          bool bad = false;
+        uint32_t k[2][KS][4];  // the operand, 16 keys each: keys kap of two blocks, the 32 (16) dims that the lane takes
+        bool bad = false;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int at = place + 16 * half + 8 * y, entry = entry_of(p, at), off = at - entry * p.page;
-            const int page = at < r.len ? table[entry] : 0;
-            const bool there = page >= 0 && page < p.pages && at < r.len;
-            bad |= page < 0 || page >= p.pages;
-            const char* from = p.data + (there ? page : 0) * p.d_page + h * p.d_head;
             if constexpr (INT4) {
-              from += (int64_t)(off / kBlockTokens) * B::kBytes;
-              uint32_t w[HD / 32], pr = 0;
-#pragma unroll
-              for (int i = 0; i < HD / 32; ++i) w[i] = 0;
-              if (there) {
-                const char* words = from + B::word(kap, HD / 32 * t);
-                if constexpr (HD == 128) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(words);
-                  w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                } else {
-                  const uint2 v = *reinterpret_cast<const uint2*>(words);
-                  w[0] = v.x, w[1] = v.y;
-                }
-                pr = *reinterpret_cast<const uint32_t*>(from + B::pair(kap, (HD / 4) * t / kGroup));
+              const uint8_t* block = slots + (taken & 1) * kUnitBytes + (2 * half + y) * B::kPart;
+              uint32_t w[HD / 32];
+              if constexpr (HD == 128) {
+                const uint4 v = *reinterpret_cast<const uint4*>(block + B::word(kap, 4 * t));
+                w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+              } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(block + B::word(kap, 2 * t));
+                w[0] = v.x, w[1] = v.y;
               }
+              const uint32_t pr = *reinterpret_cast<const uint32_t*>(block + B::pair(kap, (HD / 4) * t / kGroup));
               const uint32_t s2 = __byte_perm(pr, 0, 0x1010), o2 = __byte_perm(pr, 0, 0x3232);
 #pragma unroll
               for (int i = 0; i < HD / 32; ++i) {
-                k[2 * i][y] = two_values<DT, 0>(w[i], s2, o2);
-                k[2 * i][2 + y] = two_values<DT, 1>(w[i], s2, o2);
-                k[2 * i + 1][y] = two_values<DT, 2>(w[i], s2, o2);
-                k[2 * i + 1][2 + y] = two_values<DT, 3>(w[i], s2, o2);
+                k[half][2 * i][y] = two_values<DT, 0>(w[i], s2, o2);
+                k[half][2 * i][2 + y] = two_values<DT, 1>(w[i], s2, o2);
+                k[half][2 * i + 1][y] = two_values<DT, 2>(w[i], s2, o2);
+                k[half][2 * i + 1][2 + y] = two_values<DT, 3>(w[i], s2, o2);
               }
             } else {
-              from += (int64_t)(off + kap) * a.d_token + t * (HD / 2);
-              const bool row = there && at + kap < r.len;
+              const int at = place + 16 * half + 8 * y, entry = entry_of(p, at), page = at < r.len ? table[entry] : 0;
+              bad |= page < 0 || page >= p.pages;
+              const bool row = page >= 0 && page < p.pages && at + kap < r.len;
+              const char* from = p.data + (row ? page : 0) * p.d_page + h * p.d_head + (int64_t)(at - entry * p.page + kap) * a.d_token + t * (HD / 2);
 #pragma unroll
               for (int i = 0; i < KS / 2; ++i) {
                 const uint4 v = row ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
-                k[2 * i][y] = v.x, k[2 * i][2 + y] = v.y, k[2 * i + 1][y] = v.z, k[2 * i + 1][2 + y] = v.w;
+                k[half][2 * i][y] = v.x, k[half][2 * i][2 + y] = v.y, k[half][2 * i + 1][y] = v.z, k[half][2 * i + 1][2 + y] = v.w;
               }
             }
           }
-          if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-          float sum[2] = {0.f, 0.f};
+        if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
+        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [half][block]
+        const uint4* q_even = s_q + g * (HD / 8) + t + 4 * (g & 1);  // pieces 4 i + t, those of odd rows exchanged
+        const uint4* q_odd = s_q + g * (HD / 8) + t + 4 - 4 * (g & 1);
 #pragma unroll 1
-          for (int tile = 0; tile < tiles; ++tile) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int tile = 0; tile < tiles; ++tile) {
+          float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-            for (int i = 0; i < KS / 2; ++i) {
-              const uint4 v = s_q[(8 * tile + g) * (HD / 8) + ((4 * i + t) ^ (4 * (g & 1)))];
-              mma<DT>(c, k[2 * i], v.x, v.y);
-              mma<DT>(c, k[2 * i + 1], v.z, v.w);
+          for (int i = 0; i < KS / 2; ++i) {
+            const uint4 v = (i & 1 ? q_odd : q_even)[tile * HD + 4 * (i & 2)];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              mma<DT>(c[half], k[half][2 * i], v.x, v.y);
+              mma<DT>(c[half], k[half][2 * i + 1], v.z, v.w);
             }
-            const float2 less = *reinterpret_cast<const float2*>(s_sum + 8 * tile + 2 * t);
-            if (masked) {
-              const int2 first = *reinterpret_cast<const int2*>(s_first + 8 * tile + 2 * t);
+          }
+          const float2 less = *reinterpret_cast<const float2*>(s_sum + 8 * tile + 2 * t);
+          if (masked) {
+            const int2 first = *reinterpret_cast<const int2*>(s_first + 8 * tile + 2 * t);
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
                 const int at = place + 16 * half + 8 * y + kap;
                 const bool in = at < r.len, sink = at < p.sinks;
-                if (in && (sink || at >= first.x)) sum[y] += ex2(fmaf(c[2 * y], p.scale, less.x));
-                if (in && (sink || at >= first.y)) sum[y] += ex2(fmaf(c[2 * y + 1], p.scale, less.y));
+                if (in && (sink || at >= first.x)) sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x));
+                if (in && (sink || at >= first.y)) sum[half][y] += ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
               }
-            } else {
+          } else {
 #pragma unroll
-              for (int y = 0; y < 2; ++y) sum[y] += ex2(fmaf(c[2 * y], p.scale, less.x)) + ex2(fmaf(c[2 * y + 1], p.scale, less.y));
-            }
-          }
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
-            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
-            if (t == 2 * half + y) given = sum[y];
+              for (int y = 0; y < 2; ++y)
+                sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x)) + ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
           }
         }
+        float given = 0.f;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          float x = sum[y >> 1][y & 1];
+          x += __shfl_xor_sync(0xffffffffu, x, 1);
+          x += __shfl_xor_sync(0xffffffffu, x, 2);
+          if (t == y) given = x;
+        }
         if (mine < r.len) *at_weight = old + given;
+        ++taken;
+        __syncwarp();
       }
     }
   }
+  // Copies in flight (there is one only when a wait ran out) land before the CTA's shared memory is given up (bounded).
+  for (; INT4 && taken < brought; ++taken)
+    for (int tries = 0; tries < kPatience && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1); ++tries) {
+    }
 }
 
 template <int DT, int HD>
-void launch(const WeightArgs& a, bool int4, cudaStream_t s) {
+int launch(const WeightArgs& a, bool int4, cudaStream_t s) {
   const int ctas = sm_count() * kCtas;
-  if (int4) k_weights<DT, HD, true><<<ctas, kThreads, 0, s>>>(a);
-  else k_weights<DT, HD, false><<<ctas, kThreads, 0, s>>>(a);
+  if (int4) {
+    if (int st = allow_smem<k_weights<DT, HD, true>>(kRing<HD>)) return st;
+    k_weights<DT, HD, true><<<ctas, kThreads, kRing<HD>, s>>>(a);
+  } else {
+    k_weights<DT, HD, false><<<ctas, kThreads, 0, s>>>(a);
+  }
+  return check_launch("af_attention_weights");
 }
 
 }  // namespace
@@ -284,7 +346,6 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   a.places = w.places;
   cudaStream_t s = as_stream(stream);
   const bool int4 = w.token_stride == 0;
-  if (c.dtype == AF_DTYPE_BF16) c.head_dim == 128 ? kv4::launch<AF_DTYPE_BF16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_BF16, 64>(a, int4, s);
-  else c.head_dim == 128 ? kv4::launch<AF_DTYPE_F16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_F16, 64>(a, int4, s);
-  return check_launch("af_attention_weights");
+  if (c.dtype == AF_DTYPE_BF16) return c.head_dim == 128 ? kv4::launch<AF_DTYPE_BF16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_BF16, 64>(a, int4, s);
+  return c.head_dim == 128 ? kv4::launch<AF_DTYPE_F16, 128>(a, int4, s) : kv4::launch<AF_DTYPE_F16, 64>(a, int4, s);
 }

@@ -1,8 +1,11 @@
 // Rows into and out of the 4-bit paged cache (sm_100a).
 //
-// Both kernels are bound by HBM: per token and head of 128 dims 512 bytes of
-// 16-bit rows against 160 of the cache. A lane takes 8 dims (16 bytes) of a row, a
-// code word; the four lanes of a group of 32 dims share its extremes by two exchanges.
+// Per token and head of 128 dims 512 bytes of 16-bit rows against 160 of the
+// cache, so HBM bounds both kernels once the arithmetic is cheap enough: an SM has
+// 27 cycles for the 256 values of that token and head. Writing: a lane takes
+// the 32 dims of a pair (64 bytes), so that extremes, scale and reciprocal are
+// found once for them. Reading: a lane takes 8 dims, a code word and 16 bytes out, of one
+// head after the other.
 #include <string>
 
 #include "int4_cache.cuh"
@@ -61,126 +64,161 @@ __device__ __noinline__ uint32_t careful_code(float x, float offset, float d, fl
   return (uint32_t)fminf(k + (up ? 1.f : 0.f), 15.f);
 }
 
-// One lane's code word of 8 values, and its group's pair (the same in the group's four lanes).
+// Eight codes next to one another, as exact arithmetic rounds them.
 template <int DT>
-__device__ __forceinline__ void encode(const uint4& x, uint32_t& word, uint32_t& pair) {
+__device__ __noinline__ uint32_t careful_word(uint4 x, float offset, float scale) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t word = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const float y = from16<DT>((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+    word |= careful_code(y, offset, y - offset, scale) << (4 * (i >> 1) + 16 * (i & 1));
+  }
+  return word;
+}
+
+// The 32 values of a pair into four code words.
+template <int DT>
+__device__ __forceinline__ uint4 encode(const uint4* x, uint32_t& pair) {
   using P = Pair16<DT>;
-  auto lo2 = __hmin2_nan(__hmin2_nan(P::make(x.x), P::make(x.y)), __hmin2_nan(P::make(x.z), P::make(x.w)));
-  auto hi2 = __hmax2_nan(__hmax2_nan(P::make(x.x), P::make(x.y)), __hmax2_nan(P::make(x.z), P::make(x.w)));
+  auto lo2 = P::make(x[0].x), hi2 = lo2;
 #pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo2 = __hmin2_nan(lo2, P::make(__shfl_xor_sync(0xffffffffu, bits_of(lo2), o)));
-    hi2 = __hmax2_nan(hi2, P::make(__shfl_xor_sync(0xffffffffu, bits_of(hi2), o)));
+  for (int i = 0; i < 4; ++i) {
+    lo2 = __hmin2_nan(lo2, __hmin2_nan(__hmin2_nan(P::make(x[i].x), P::make(x[i].y)), __hmin2_nan(P::make(x[i].z), P::make(x[i].w))));
+    hi2 = __hmax2_nan(hi2, __hmax2_nan(__hmax2_nan(P::make(x[i].x), P::make(x[i].y)), __hmax2_nan(P::make(x[i].z), P::make(x[i].w))));
   }
   const float l0 = from16<DT>(bits_of(lo2) & 0xffffu), l1 = from16<DT>(bits_of(lo2) >> 16);
   const float h0 = from16<DT>(bits_of(hi2) & 0xffffu), h1 = from16<DT>(bits_of(hi2) >> 16);
   const float low = fminf(l0, l1), range = fmaxf(h0, h1) - low;
   const bool sound = !(isnan(l0) || isnan(l1)) && fabsf(range) <= 3.402823466e38f;
   if (!sound) {  // the group stands for NaN
-    word = 0;
     pair = (DT == AF_DTYPE_BF16 ? 0x7fc0u : 0x7e00u) << 16;
-    return;
+    return make_uint4(0, 0, 0, 0);
   }
   uint32_t s16 = to16<DT>(range / 15.f);
   if (!finite16<DT>(to16<DT>(fmaf(15.f, from16<DT>(s16), low)))) --s16;
   pair = s16 | to16<DT>(low) << 16;
-  const float scale = from16<DT>(s16);
-  word = 0;
-  if (scale == 0.f) return;
-  constexpr float magic = 12582912.f;  // 1.5 * 2^23: a number below 2^22 added to it is rounded to a whole one
-  // (Where the reciprocal overflows every code takes the careful way.)
-  const float inv = scale < 1e-37f ? 0.f : 1.f / scale, half = 0.5f * scale;
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  const float scale = from16<DT>(s16), half = 0.5f * scale;
+  if (scale == 0.f) return make_uint4(0, 0, 0, 0);
+  // A number below 2^22 added to 1.5 * 2^23 is rounded to a whole one, here to one of the two codes that x - offset lies between:
+  // the reciprocal is not exact. What is left, r = x - offset - code * scale, is, and says which one: the other where |r| is more than
+  // half a step, or is half a step and the code odd. (As whole numbers the magnitudes of floats are in their order.)
+  constexpr float magic = 12582912.f;
+  constexpr uint32_t magic_bits = 0x4b400000u;
+  const float inv = 1.f / scale;
+  const int half_bits = __float_as_int(half);
+  const bool usual = inv <= 3.402823466e38f && range <= 15.25f * scale;  // else the scale has lost its precision, and codes may pass 15
+  uint32_t out[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    uint32_t word = 0;
+    int off = 0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float y = from16<DT>(h ? w[i] >> 16 : w[i] & 0xffffu), d = y - low;
-      const float t = fminf(fmaf(d, inv, magic), magic + 15.f);
-      // Next to a border between two codes, or past the last: |d - code * scale| is no less than half a step.
-      uint32_t c = __float_as_uint(t) & 15u;
-      if (fabsf(fmaf(-(t - magic), scale, d)) >= half) c = careful_code(y, low, d, scale);
-      word |= c << (4 * i + 16 * h);
+    for (int c = 0; c < 8; ++c) {
+      const float d = from16<DT>(c & 1 ? w[c >> 1] >> 16 : w[c >> 1] & 0xffffu) - low;
+      const float t = fmaf(d, inv, magic), r = fmaf(magic - t, scale, d);
+      const int left = __float_as_int(fabsf(r)), odd = __float_as_int(t) & 1;
+      off = max(off, left);
+      const uint32_t step = left + odd > half_bits ? 1u | (__float_as_int(r) >> 31) : 0u;
+      word += (__float_as_uint(t) - magic_bits + step) << (4 * (c >> 1) + 16 * (c & 1));
     }
+    bool sure = usual;
+    if (off >= half_bits) {
+      // A tie is none where the difference x - offset has lost something in fp32.
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float y = from16<DT>(c & 1 ? w[c >> 1] >> 16 : w[c >> 1] & 0xffffu);
+        sure &= low + (y - low) == y;
+      }
+    }
+    out[i] = sure ? word : careful_word<DT>(x[i], low, scale);
   }
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
-// A warp takes 32 U code words (keys, then values, of one head after the other) of one row.
-template <int DT, int HD, int U, bool WRITE>
-__global__ void __launch_bounds__(kThreads) k_rows(const RowArgs a, int chunks) {
+// A thread takes the 32 dims of a pair, of a key or value of one head.
+template <int DT, int HD>
+__global__ void __launch_bounds__(kThreads) k_write(const RowArgs a) {
   using B = Block<HD>;
-  constexpr int W = HD / 8;  // words of a row
+  constexpr int G = HD / kGroup;  // pairs of a row
+  const uint32_t item = blockIdx.x * kThreads + threadIdx.x, per_row = 2 * G * a.heads;  // (below 2^31: checked by the host)
+  const int m = (int)(item / per_row), x = (int)(item - m * per_row), l = blockIdx.y;
+  if (m >= a.count) return;
+  const int64_t slot = a.slots[m];
+  const int64_t row = a.rows ? a.rows[m] : m;
+  if (slot < 0 || row < 0) return;
+  if (slot >= a.n_slots || row >= a.n_rows) {
+    if (x == 0 && a.status) atomicOr(a.status, AF_STATUS_BOUNDS);
+    return;
+  }
+  const int h = x / (2 * G), val = x / G % 2, g = x % G;
+  const uint4* from = reinterpret_cast<const uint4*>((val ? a.v + l * a.vl + row * a.vn + h * a.vh : a.k + l * a.kl + row * a.kn + h * a.kh) + 64 * g);
+  uint4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = from[i];
+  const int64_t pg = slot < 0x7fffffff ? (int)slot / a.page : slot / a.page;
+  const int t = (int)(slot - pg * a.page), r = t % kBlockTokens;
+  char* part = a.data + l * a.dl + pg * a.dp + h * a.dh + (int64_t)(t / kBlockTokens) * B::kBytes + val * B::kPart;
+  uint32_t pair;
+  *reinterpret_cast<uint4*>(part + B::word(r, 4 * g)) = encode<DT>(v, pair);
+  *reinterpret_cast<uint32_t*>(part + B::pair(r, g)) = pair;
+}
+
+// A warp takes U passes over one slot's heads: with 128 dims the 32 code words of a head's key and value, with 64 those of two heads.
+template <int DT, int HD, int U>
+__global__ void __launch_bounds__(kThreads) k_read(const RowArgs a, int chunks) {
+  using B = Block<HD>;
+  constexpr int W = HD / 8, H = 32 / (2 * W);  // words of a row; heads of a pass
   const int lane = threadIdx.x & 31;
-  const int item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);  // (row, chunk)
-  const int m = item / chunks, chunk = item - m * chunks, l = blockIdx.y;
+  const int item = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);  // (row, chunk of heads)
+  const int m = chunks == 1 ? item : item / chunks, chunk = item - m * chunks, l = blockIdx.y;
   if (m >= a.count) return;
   int64_t slot = a.slots[m];
-  int64_t row = WRITE && a.rows ? a.rows[m] : m;
-  if (WRITE && (slot < 0 || row < 0)) return;
-  if (slot >= a.n_slots || (WRITE && row >= a.n_rows)) {
+  if (slot >= a.n_slots) {
     if (lane == 0 && a.status) atomicOr(a.status, AF_STATUS_BOUNDS);
-    if (WRITE) return;
     slot = -1;
   }
   const int64_t pg = slot < 0x7fffffff ? (int)slot / a.page : slot / a.page;
   const int t = (int)(slot - pg * a.page), r = t % kBlockTokens;
-  char* block = a.data + l * a.dl + pg * a.dp + (int64_t)(t / kBlockTokens) * B::kBytes;
-  const int words = 2 * W * a.heads, x0 = chunk * 32 * U + lane;
-  if constexpr (WRITE) {
-    const char* k = a.k + l * a.kl + row * a.kn;
-    const char* v = a.v + l * a.vl + row * a.vn;
-    uint4 buf[U];
+  const int h0 = chunk * U * H + lane / (2 * W), val = lane / W % 2, w = lane % W;
+  const char* word_at = a.data + l * a.dl + pg * a.dp + h0 * a.dh + (int64_t)(t / kBlockTokens) * B::kBytes + val * B::kPart;
+  const char* pair_at = word_at + B::pair(r, w / 4);
+  word_at += B::word(r, w);
+  const int64_t step = H * a.dh, oh = val ? a.vh : a.kh;
+  char* to = (val ? a.v_out + l * a.vl + m * a.vn : a.k_out + l * a.kl + m * a.kn) + h0 * oh + 16 * w;
+  uint32_t word[U], pair[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int x = x0 + 32 * u, h = x / (2 * W), val = x / W % 2, w = x % W;
-      buf[u] = x < words ? *reinterpret_cast<const uint4*>((val ? v + h * a.vh : k + h * a.kh) + 16 * w) : make_uint4(0, 0, 0, 0);
-    }
+  for (int u = 0; u < U; ++u) {
+    const bool there = slot >= 0 && h0 + u * H < a.heads;
+    word[u] = there ? *reinterpret_cast<const uint32_t*>(word_at + u * step) : 0;
+    pair[u] = there ? *reinterpret_cast<const uint32_t*>(pair_at + u * step) : 0;
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int x = x0 + 32 * u, h = x / (2 * W), val = x / W % 2, w = x % W;
-      uint32_t word, pair;
-      encode<DT>(buf[u], word, pair);
-      if (x < words) {
-        char* part = block + h * a.dh + val * B::kPart;
-        *reinterpret_cast<uint32_t*>(part + B::word(r, w)) = word;
-        if (w % 4 == 0) *reinterpret_cast<uint32_t*>(part + B::pair(r, w / 4)) = pair;
-      }
-    }
-  } else {
-    char* k = a.k_out + l * a.kl + m * a.kn;
-    char* v = a.v_out + l * a.vl + m * a.vn;
-    uint32_t word[U], pair[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int x = x0 + 32 * u, h = x / (2 * W), val = x / W % 2, w = x % W;
-      const bool there = slot >= 0 && x < words;
-      const char* part = block + h * a.dh + val * B::kPart;
-      word[u] = there ? *reinterpret_cast<const uint32_t*>(part + B::word(r, w)) : 0;
-      pair[u] = there ? *reinterpret_cast<const uint32_t*>(part + B::pair(r, w / 4)) : 0;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int x = x0 + 32 * u, h = x / (2 * W), val = x / W % 2, w = x % W;
-      if (x >= words) continue;
-      // Word and pair are 0 where there is no slot, and so are the values.
-      const uint32_t s2 = __byte_perm(pair[u], 0, 0x1010), o2 = __byte_perm(pair[u], 0, 0x3232);
-      const uint4 y = make_uint4(two_values<DT, 0>(word[u], s2, o2), two_values<DT, 1>(word[u], s2, o2), two_values<DT, 2>(word[u], s2, o2),
-                                 two_values<DT, 3>(word[u], s2, o2));
-      *reinterpret_cast<uint4*>((val ? v + h * a.vh : k + h * a.kh) + 16 * w) = y;
-    }
+  for (int u = 0; u < U; ++u) {
+    // Word and pair are 0 where there is no slot, and so are the values.
+    const uint32_t s2 = __byte_perm(pair[u], 0, 0x1010), o2 = __byte_perm(pair[u], 0, 0x3232);
+    const uint4 y = make_uint4(two_values<DT, 0>(word[u], s2, o2), two_values<DT, 1>(word[u], s2, o2), two_values<DT, 2>(word[u], s2, o2),
+                               two_values<DT, 3>(word[u], s2, o2));
+    if (h0 + u * H < a.heads) *reinterpret_cast<uint4*>(to + u * (H * oh)) = y;
   }
 }
 
 template <int DT, int HD, bool WRITE>
 void launch(const RowArgs& a, cudaStream_t s) {
-  // Four words of a lane in flight where a row has them: rows of 4 heads x 128 dims fill a warp's 128.
-  const int words = HD / 4 * a.heads;
-  const int u = words > 64 ? 4 : words > 32 ? 2 : 1;
-  const int chunks = (int)ceil_div(words, 32 * u);
-  const dim3 grid((unsigned)ceil_div((int64_t)chunks * a.count, kThreads / 32), (unsigned)a.layers);
-  if (u == 4) k_rows<DT, HD, 4, WRITE><<<grid, kThreads, 0, s>>>(a, chunks);
-  else if (u == 2) k_rows<DT, HD, 2, WRITE><<<grid, kThreads, 0, s>>>(a, chunks);
-  else k_rows<DT, HD, 1, WRITE><<<grid, kThreads, 0, s>>>(a, chunks);
+  if constexpr (WRITE) {
+    const dim3 grid((unsigned)ceil_div(a.count * 2 * (HD / kGroup) * a.heads, kThreads), (unsigned)a.layers);
+    k_write<DT, HD><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    // As many passes in flight as a row has, up to eight.
+    const int passes = (int)ceil_div(a.heads, 128 / HD), u = passes > 4 ? 8 : passes > 2 ? 4 : passes > 1 ? 2 : 1;
+    const int chunks = (int)ceil_div(passes, u);
+    const dim3 grid((unsigned)ceil_div((int64_t)chunks * a.count, kThreads / 32), (unsigned)a.layers);
+    if (u == 8) k_read<DT, HD, 8><<<grid, kThreads, 0, s>>>(a, chunks);
+    else if (u == 4) k_read<DT, HD, 4><<<grid, kThreads, 0, s>>>(a, chunks);
+    else if (u == 2) k_read<DT, HD, 2><<<grid, kThreads, 0, s>>>(a, chunks);
+    else k_read<DT, HD, 1><<<grid, kThreads, 0, s>>>(a, chunks);
+  }
 }
 
 template <bool WRITE>
@@ -214,7 +252,7 @@ int rows_call(const af_int4_rows* w, uint32_t* status, void* stream, const char*
   a.page = (int)c.page_size;
   a.heads = (int)c.heads;
   a.status = status;
-  AF_REQUIRE(a.count <= 0x7fffffff && a.count * ceil_div(c.head_dim / 4 * a.heads, 32) <= 0x7fffffff, what + "too many rows");
+  AF_REQUIRE(a.count <= (1 << 28) && a.count * (2 * (c.head_dim / kGroup) * a.heads + 32) <= 0x7fffff00, what + "too many rows");
   cudaStream_t s = as_stream(stream);
   const bool bf16 = c.dtype == AF_DTYPE_BF16;
   if (c.head_dim == 128) bf16 ? launch<AF_DTYPE_BF16, 128, WRITE>(a, s) : launch<AF_DTYPE_F16, 128, WRITE>(a, s);
