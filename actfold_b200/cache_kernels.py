@@ -51,29 +51,40 @@ class Int4Cache:
     __slots__ = ("data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
 
     def __init__(self, data: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> None:
-        if data.dtype is not torch.uint8 or data.dim() not in (4, 5) or data.shape[-1] not in (640, 1280):
-            raise ValueError(f"Int4Cache: data must be uint8 [(layers,) pages, kv_heads, page_size / 8, 640 or 1280], got {data.dtype} {tuple(data.shape)}")
+        shape = data.shape
+        if data.dtype is not torch.uint8 or len(shape) not in (4, 5) or shape[-1] not in (640, 1280):
+            raise ValueError(f"Int4Cache: data must be uint8 [(layers,) pages, kv_heads, page_size / 8, 640 or 1280], got {data.dtype} {tuple(shape)}")
         if dtype is not torch.bfloat16 and dtype is not torch.float16:
             raise ValueError(f"Int4Cache: dtype must be fp16 or bf16, got {dtype}")
-        *outer, blocks, size = data.shape
+        if len(shape) == 4:
+            (pages, heads, blocks, size), layers = shape, None
+            (sp, sh, sb, inner), sl = data.stride(), 0
+        else:
+            layers, pages, heads, blocks, size = shape
+            sl, sp, sh, sb, inner = data.stride()
         if blocks == 0:
             raise ValueError("Int4Cache: page_size must be positive")
-        strides = list(data.stride())
-        if strides[-1] != 1 or (blocks > 1 and strides[-2] != size):
+        if inner != 1 or (sb != size and blocks > 1):
             raise ValueError("Int4Cache: the blocks of a page's head must be contiguous")
-        outer_strides = [0 if n <= 1 else s for n, s in zip(outer, strides)]
-        if any(s <= 0 and n > 1 for n, s in zip(outer, outer_strides)):
+        if heads <= 1:
+            sh = 0
+        elif sh <= 0:
             raise ValueError("Int4Cache: data has entries that share memory")
-        if any(s & 15 for s in outer_strides) or data.data_ptr() & 15:
+        if pages <= 1:
+            sp = 0
+        elif sp <= 0:
+            raise ValueError("Int4Cache: data has entries that share memory")
+        if layers is not None and layers > 1:
+            if sl <= 0:
+                raise ValueError("Int4Cache: data has entries that share memory")
+        else:
+            sl = 0
+        at = data.data_ptr()
+        if (sl | sp | sh | at) & 15:
             raise ValueError("Int4Cache: data's address and strides must be multiples of 16 bytes")
-        self.data, self.dtype, self.dim = data, dtype, size // 10
-        self.layers = outer[0] if len(outer) == 3 else None
-        self.pages, self.kv_heads = outer[-2], outer[-1]
-        self.page_size = 8 * blocks
-        if self.layers is None:
-            outer_strides = [0, *outer_strides]
-        self._packed = (data.data_ptr(), *outer_strides, 1 if self.layers is None else self.layers, self.pages, self.page_size, self.kv_heads, self.dim,
-                        _lib.DTYPE[dtype])
+        self.data, self.dtype, self.dim, self.layers, self.pages, self.kv_heads = data, dtype, size // 10, layers, pages, heads
+        self.page_size = page = 8 * blocks
+        self._packed = (at, sl, sp, sh, 1 if layers is None else layers, pages, page, heads, size // 10, _lib.DTYPE[dtype])
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, dtype: torch.dtype = torch.bfloat16, layers: int | None = None,
@@ -100,12 +111,10 @@ class EvictedCache(NamedTuple):
 
 def _row_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
     """Strides in bytes of 16-bit rows [layers, n, heads, dim], or None where they or the address are not multiples of 16."""
-    e = t.element_size()
     a, b, c, d = t.stride()
-    if (d != 1 and t.shape[3] > 1) or t.data_ptr() & 15:
-        return None
-    out = tuple(0 if n <= 1 else s * e for n, s in zip(t.shape, (a, b, c)))
-    return None if any(s & 15 for s in out) else out
+    layers, n, heads, _ = t.shape
+    a, b, c = 0 if layers <= 1 else 2 * a, 0 if n <= 1 else 2 * b, 0 if heads <= 1 else 2 * c
+    return None if d != 1 or (a | b | c | t.data_ptr()) & 15 else (a, b, c)
 
 
 def write_cache_int4(
@@ -161,8 +170,9 @@ def read_cache_int4(
         raise ValueError(f"read_cache_int4: slots must be int64, got {slots.dtype}")
     index = _same_device("read_cache_int4", cache.data, slots, word := _word(status))
     slots = slots.contiguous()
-    outer = () if cache.layers is None else (cache.layers,)
-    k, v = (torch.empty((*outer, *slots.shape, cache.kv_heads, cache.dim), dtype=cache.dtype, device=slots.device) for _ in range(2))
+    shape = (*slots.shape, cache.kv_heads, cache.dim) if cache.layers is None else (cache.layers, *slots.shape, cache.kv_heads, cache.dim)
+    k = torch.empty(shape, dtype=cache.dtype, device=slots.device)
+    v = torch.empty_like(k)
     count, row = slots.numel(), 2 * cache.kv_heads * cache.dim
     st = (count * row, row, 2 * cache.dim)
     args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *st, *st, slots.data_ptr(), 0, count, count, *cache._packed)
@@ -266,11 +276,9 @@ def _check_window(what: str, window: int | None, sinks: int) -> int:
 
 
 def _rows16(t: torch.Tensor) -> tuple[torch.Tensor, tuple | list]:
-    """16-bit rows [n, heads, dim] and their strides in bytes, copied where these or the address are not multiples of 16."""
-    if (grid := _row_grid(t)) is None:
-        t = t.clone(memory_format=torch.contiguous_format)
-        grid = _row_grid(t)
-    return t, grid
+    """A copy of 16-bit rows [n, heads, dim] whose address and strides are multiples of 16 bytes, and these."""
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _row_grid(t)
 
 
 def tree_attention_int4(
@@ -338,7 +346,12 @@ def tree_attention_int4(
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts = lengths.contiguous(), starts.contiguous()
-    (q, q_grid), (k, k_grid), (v, v_grid) = _rows16(q), _rows16(k), _rows16(v)
+    if (q_grid := _row_grid(q)) is None:
+        q, q_grid = _rows16(q)
+    if (k_grid := _row_grid(k)) is None:
+        k, k_grid = _rows16(k)
+    if (v_grid := _row_grid(v)) is None:
+        v, v_grid = _rows16(v)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
         out_grid = (2 * heads * dim, 2 * dim)
@@ -390,9 +403,10 @@ def attention_weights(
             raise ValueError("attention_weights: the cache's innermost dimension must be contiguous, its other strides multiples of 16 bytes")
         keys, dtype = cache, cache.dtype
         parts, token = (cache.data_ptr(), 0, grid[0], grid[2], 1, pages, page, kv, dim, _lib.DTYPE[dtype]), grid[1]
-    total, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-    if q.dim() != 3 or q.dtype is not dtype or q.shape[2] != dim or heads == 0 or heads % kv:
-        raise ValueError(f"attention_weights: q {q.dtype} {tuple(q.shape)} and cache {dtype} {tuple(keys.shape)} do not match")
+    qs = q.shape
+    total, heads = (qs[0], qs[1]) if len(qs) == 3 else (0, 0)
+    if heads == 0 or q.dtype is not dtype or qs[2] != dim or heads % kv:
+        raise ValueError(f"attention_weights: q {q.dtype} {tuple(qs)} and cache {dtype} {tuple(keys.shape)} do not match")
     batch, most = _check_tables("attention_weights", tables, lengths)
     if starts.dtype is not _I32 or starts.dim() != 1:
         _not_vectors("attention_weights", _I32, starts=starts)
@@ -403,17 +417,19 @@ def attention_weights(
     if weights.dtype is not torch.float32 or weights.dim() != 3 or weights.shape[:2] != (batch, kv):
         raise ValueError(f"attention_weights: weights must be float32 [{batch}, {kv}, places], got {weights.dtype} {tuple(weights.shape)}")
     places = weights.shape[2]
-    if (places > 1 and weights.stride(2) != 1) or any(s == 0 and n > 1 for s, n in zip(weights.stride(), weights.shape)):
+    w_request, w_head, inner = weights.stride()
+    if (places > 1 and inner != 1) or (w_request == 0 and batch > 1) or (w_head == 0 and kv > 1):
         raise ValueError("attention_weights: the innermost dimension of weights must be contiguous, and its entries must not share memory")
     window = _check_window("attention_weights", window, sinks)
     index = _same_device("attention_weights", q, keys, tables, lengths, starts, lse, weights, word := _word(status))
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts, lse = lengths.contiguous(), starts.contiguous(), lse.contiguous()
-    q, q_grid = _rows16(q)
+    if (q_grid := _row_grid(q)) is None:
+        q, q_grid = _rows16(q)
     args = _WEIGHTS.pack(q.data_ptr(), *q_grid, *parts, token, tables.data_ptr(), tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(),
                          starts.data_ptr(), batch, total, heads, window, sinks, dim ** -0.5 if scale is None else scale, lse.data_ptr(),
-                         weights.data_ptr(), weights.stride(0), weights.stride(1), places)
+                         weights.data_ptr(), w_request, w_head, places)
     _launch("attention_weights", index, _lib.load().af_attention_weights, args, _lib.ptr(word))
     return weights
 

@@ -145,11 +145,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
       }
       __syncthreads();
       // A unit's keys: lane y brings block y, if its page is one; what there is no key for reads as zeros.
-      auto bring = [&](int x) {
+      auto place_of = [&](int x) { return kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from) + kBlockTokens * lane; };
+      auto look_up = [&](int x) { return x < x1 && lane < kUnit / kBlockTokens && place_of(x) < r.len ? table[entry_of(p, place_of(x))] : 0; };
+      auto bring = [&](int x, int page) {
         if (x >= x1 || lost) return;
-        const int at = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from) + kBlockTokens * lane, slot = brought & 1;
+        const int at = place_of(x), slot = brought & 1;
         const bool mine = lane < kUnit / kBlockTokens, needed = mine && at < r.len;
-        const int entry = needed ? entry_of(p, at) : 0, page = needed ? table[entry] : 0;
         const bool there = needed && page >= 0 && page < p.pages;
         if (needed && !there && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
         if (mine && !there) {
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
         if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, __popc(blocks) * B::kPart);
         __syncwarp();
         if (there) {
-          const char* from = p.data + page * p.d_page + h * p.d_head + (int64_t)((at - entry * p.page) / kBlockTokens) * B::kBytes;
+          const char* from = p.data + page * p.d_page + h * p.d_head + (int64_t)((at - entry_of(p, at) * p.page) / kBlockTokens) * B::kBytes;
           asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                            smem_u32(slots) + slot * kUnitBytes + lane * B::kPart),
                        "l"(from), "r"(B::kPart), "r"(full + 8 * slot)
@@ -168,11 +169,16 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
         }
         ++brought;
       };
-      if constexpr (INT4) bring(x0 + warp);
+      int page = 0;  // of the lane's block of the unit after next
+      if constexpr (INT4) {
+        bring(x0 + warp, look_up(x0 + warp));
+        page = look_up(x0 + warp + W);
+      }
 #pragma unroll 1
       for (int x = x0 + warp; x < x1 && !lost; x += W) {
         if constexpr (INT4) {
-          bring(x + W);
+          bring(x + W, page);
+          page = look_up(x + 2 * W);
           int tries = 0;
           while (!lost && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1)) lost = ++tries > kPatience;
           lost = __any_sync(0xffffffffu, lost);
