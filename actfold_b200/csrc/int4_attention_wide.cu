@@ -168,14 +168,15 @@ __device__ __forceinline__ bool is_masked(const Params& p, const Segment& s, int
 // 2^shift of them, from the segment's first.
 __device__ __forceinline__ int found_shift(int units) { return max(0, 27 - __clz(units - 1 | 1)); }
 
-// Such values of dims d .. d + 7, added up for a row of node i, whose window begins at `first`.
+// Such values of dims d .. d + 15, added up for a row of node i, whose window begins at `first`. (Four keys' loads at a time: of a
+// long chain with such values in every unit a row's end looks through all nodes.)
 template <int DT, int HD>
 __device__ __noinline__ void set_aside(const Params& p, const Segment* plan, uint32_t found, int i, int first, int d, float* sum) {
   using B = Block<HD>;
   const Segment& s = *plan;
   const int units = s.x1 - s.x0, shift = found_shift(units);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum[e] = 0.f;
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
 #pragma unroll 1
   for (; found; found &= found - 1) {
     const int u0 = (__ffs(found) - 1) << shift;
@@ -183,30 +184,41 @@ __device__ __noinline__ void set_aside(const Params& p, const Segment* plan, uin
     for (int x = s.x0 + u0; x < s.x0 + min(units, u0 + (1 << shift)); ++x) {
       if (!is_masked(p, s, x)) continue;
       if (x < s.cached) {
-        const int place0 = place_of(s, x);
-#pragma unroll 1
-        for (int at = place0; at < min(s.len, place0 + kUnit); ++at) {
-          if (at < first && at >= p.sinks) continue;
-          const int page = p.tables[(int64_t)s.b * p.tables_ld + at / p.page], off = at % p.page;
-          if (page < 0 || page >= p.pages) continue;
-          const uint32_t pr = *reinterpret_cast<const uint32_t*>(p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes +
-                                                                B::kPart + B::pair(off % kBlockTokens, d / kGroup));
-          if (not_finite<DT>(pr) || not_finite<DT>(pr >> 16))
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] = NAN;
+        const int place0 = place_of(s, x), end = min(s.len, place0 + kUnit);
+        bool bad = false;
+#pragma unroll 4
+        for (int at = place0; at < end; ++at) {
+          const int entry = entry_of(p, at), off = at - entry * p.page, page = p.tables[(int64_t)s.b * p.tables_ld + entry];
+          uint32_t pr = 0;
+          if ((at >= first || at < p.sinks) && page >= 0 && page < p.pages)
+            pr = *reinterpret_cast<const uint32_t*>(p.data + page * p.d_page + s.kvh * p.d_head + (int64_t)(off / kBlockTokens) * B::kBytes + B::kPart +
+                                                    B::pair(off % kBlockTokens, d / kGroup));
+          bad |= not_finite<DT>(pr) || not_finite<DT>(pr >> 16);
         }
-      } else {
-        const int n0 = kUnit * (x - s.cached);
-#pragma unroll 1
-        for (int j = n0; j < min(s.n, n0 + kUnit); ++j) {
-          if (!((seen_nodes(p, s.s0, s.n, i, j & ~31) >> (j & 31)) & 1u)) continue;
-          const uint4 v = *reinterpret_cast<const uint4*>(p.v + (int64_t)(s.s0 + j) * p.v_n + s.kvh * p.v_h + 2 * d);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (bad)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const uint32_t b = (w[e / 2] >> (16 * (e & 1))) & 0xffffu;
-            if (not_finite<DT>(b)) sum[e] += from_bits<DT>(b);
-          }
+          for (int e = 0; e < 16; ++e) sum[e] = NAN;
+      } else {
+        const int n0 = kUnit * (x - s.cached), end = min(s.n, n0 + kUnit);
+        const char* from = p.v + (int64_t)s.s0 * p.v_n + s.kvh * p.v_h + 2 * d;
+#pragma unroll 1
+        for (int j = n0; j < end; j += 4) {
+          uint4 v[4][2];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              v[u][h] = j + u < end ? *reinterpret_cast<const uint4*>(from + (int64_t)(j + u) * p.v_n + 16 * h) : make_uint4(0, 0, 0, 0);
+          const uint32_t seen = seen_nodes(p, s.s0, s.n, i, j & ~31) >> (j & 31);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if ((seen >> u) & 1u) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint32_t w = reinterpret_cast<const uint32_t*>(&v[u][e / 8])[e % 8 / 2], b = (w >> (16 * (e & 1))) & 0xffffu;
+                if (not_finite<DT>(b)) sum[e] += from_bits<DT>(b);
+              }
+            }
         }
       }
     }
@@ -718,13 +730,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
           }
           if (r < rows) {
             if (aside) {
+              float more[16];
+              set_aside<DT, HD>(p, plans + seg % kPlans, aside, node, first, d, more);
 #pragma unroll
-              for (int x = 0; x < 16; x += 8) {
-                float more[8];
-                set_aside<DT, HD>(p, plans + seg % kPlans, aside, node, first, d + x, more);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[x + i] += more[i];
-              }
+              for (int i = 0; i < 16; ++i) y[i] += more[i];
             }
 #pragma unroll
             for (int i = 0; i < 16; i += 8) {
@@ -753,6 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       read(seg);
       ++seg;  // (the next segment's maxima go where these ones are: enter() is a barrier)
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (copies of Q are in flight only after a wait that ran out)
     if (!wrote_start && tid == 0) scratch.started(blockIdx.x)->last = 0;
   }
 

@@ -139,13 +139,14 @@ def attention(q, k, v, data, dtype, tables, lengths, starts, bits, window=0, sin
                 top = torch.where(torch.isfinite(top), top, 0.0)
                 e = torch.where(see, torch.exp(s - top), 0.0)
                 l = e.sum(-1, keepdim=True)
-                w = torch.where(l > 0, e / l, torch.zeros_like(e))
+                some = see.any(-1, keepdim=True)  # (a row that sees a key that is not finite is NaN, one that sees nothing 0)
+                w = torch.where(some, e / l, torch.zeros_like(e))
                 if bool(torch.isfinite(vv).all()):
                     o, a, f = w @ vv, w @ vv.abs(), see.double() @ vv.abs()
                 else:  # a hidden value has no influence, not even as 0 * NaN
                     o, a, f = (torch.stack([y[i][see[i]] @ z[see[i]] for i in range(n)]) for y, z in ((w, vv), (w, vv.abs()), (see.double(), vv.abs())))
                 out[lo:hi, h] = o
-                lse[lo:hi, h] = torch.where(l > 0, top + torch.log(l), -math.inf)[:, 0]
+                lse[lo:hi, h] = torch.where(some, top + torch.log(l), -math.inf)[:, 0]
                 big = torch.where(see, (x.abs() @ kk.abs().nan_to_num(0, 0, 0).T) * abs(scale), 0.0).amax(-1, keepdim=True).nan_to_num(0, 0, 0)
                 d = 2.0 ** -23 * dim * big + 2.0 ** -24 * 4 * (2 * big + 1) + 2.0 ** -22
                 sub = 2.0 ** -32 * f / l.clamp(min=1e-300) + 2.0 ** -25 if q.dtype == torch.float16 else 0.0
@@ -185,3 +186,4 @@ def weights(q, keys, slots, lengths, starts, lse, old, window=0, sinks=0, scale=
             tol[b, g, :t] += torch.where(p > 0, p * d.exp() * d, 0.0).sum(0)
     rows = (max((hi - lo for lo, hi in zip(starts, starts[1:])), default=0)) * heads // kv
     return out, tol + (rows + 2) * 2.0 ** -24 * out.abs()
+

@@ -24,7 +24,7 @@ def _i64(x):
 
 
 def _bits(x):
-    return x.contiguous().view(torch.int16) if x.dtype in (BF, HF) else x
+    return x.contiguous().view(torch.int16 if x.dtype in (BF, HF) else torch.int32) if x.is_floating_point() else x
 
 
 def _same(a, b):
@@ -387,3 +387,384 @@ def test_weights_are_those_of_the_attention():
     own = torch.einsum("bhd,bhd->bh", a["q"].double(), a["k"].double().repeat_interleave(heads // kv, 1)) * 128 ** -0.5
     left = (1 - torch.exp(own - lse.double())).view(3, kv, -1).sum(-1)
     assert bool(((w.double().sum(-1) - left).abs() <= 2.0 ** -14).all())  # 700 keys, scores below 32: 2^-23 * 128 * 32 * 4 terms
+
+
+# Shapes that reach every kernel: 1 to 8 rows a head, 9 to 16, 17 to 128 (one row tile), more (two).
+KINDS = {"8": dict(ns=[1, 3, 1], heads=4, kv=2), "16": dict(ns=[5, 9, 3], heads=4, kv=2), "128": dict(ns=[30, 40, 7], heads=4, kv=2),
+         "256": dict(ns=[90, 20, 100], heads=4, kv=2)}
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, BF), (128, HF), (128, BF)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (60, 3)])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_with_values_that_are_not_finite(kind, tree, window, sinks, dim, dtype):
+    """NaN and infinities in keys and values, cached and drafted, reach the rows that see them and no others."""
+    from actfold_b200.speculative import write_cache_int4
+
+    ls = [200, 65, 130]
+    a, starts, bits = _attention_case(ls=ls, dim=dim, page=16, dtype=dtype, tree=tree, seed=len(kind) + dim, **KINDS[kind])
+    kv = KINDS[kind]["kv"]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    # Cached: a value of request 0 that only some windows hold, one among the sinks, a key of request 1.
+    for r, place, part, d, x in ((0, 200 - 45, 1, 40, math.nan), (0, 1, 1, 3, math.inf), (1, 30, 0, 9, math.nan), (2, 129, 1, 20, -math.inf)):
+        k, v = torch.randn(1, kv, dim, device="cuda", generator=g).to(dtype), torch.randn(1, kv, dim, device="cuda", generator=g).to(dtype)
+        (k, v)[part][0, 1, d] = x
+        write_cache_int4(k, v, a["cache"], a["tables"][r].long()[place // 16] * 16 + place % 16 + _i64([0]))
+    # Drafted: values and a key of nodes that not all see.
+    for r, node, part, d, x in ((0, -1, 1, 5, math.nan), (1, KINDS[kind]["ns"][1] // 2, 1, 50, math.inf), (1, KINDS[kind]["ns"][1] // 2 + 1, 1, 50, -math.inf),
+                                (2, -1, 0, 7, math.nan)):
+        lo, hi = starts[r], starts[r + 1]
+        (a["k"], a["v"])[part][hi - 1 if node < 0 else lo + node, 1, d] = x
+    out = _check_attention(a, ls, starts, bits, window, sinks)
+    assert out.isnan().any() and torch.isfinite(out[:, : KINDS[kind]["heads"] // 2]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_strided_tensors(kind):
+    """Rows, tables, lengths and results that are parts of larger tensors, and rows that are not 16-byte aligned."""
+    ls = [70, 300, 33]
+    for shift in (0, 1):
+        a, starts, bits = _attention_case(ls=ls, dim=64, page=24, dtype=HF, tree=True, seed=3, extra_rows=2, **KINDS[kind])
+        total, heads = a["q"].shape[:2]
+        wide = torch.zeros(total, 3, heads + 2, 72, dtype=HF, device="cuda")
+        q, k, v = (wide[:, i, : x.shape[1], shift:64 + shift].copy_(x) for i, x in enumerate((a["q"], a["k"], a["v"])))
+        tables = torch.full((3, 2 * a["tables"].shape[1]), 10 ** 6, dtype=torch.int32, device="cuda")[:, ::2].copy_(a["tables"])
+        lengths = torch.zeros(6, dtype=torch.int32, device="cuda")[::2].copy_(a["lengths"])
+        mask = torch.full((total, 2 * a["mask"].shape[1]), -1, dtype=torch.int32, device="cuda")[:, : a["mask"].shape[1]].copy_(a["mask"])
+        big = torch.full((total, heads, 2, 64), 5.0, dtype=HF, device="cuda")
+        b = dict(a, q=q, k=k, v=v, tables=tables, lengths=lengths, mask=mask)
+        out = _check_attention(b, ls, starts, bits, 50, 2, out=big[:, :, 1])
+        assert out.data_ptr() == big[:, :, 1].data_ptr()
+        assert bool((big[:, :, 0] == 5.0).all()) and bool((big[starts[-1]:] == 5.0).all())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.5, 1e-4])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_scales(kind, scale):
+    ls = [70, 300, 33]
+    a, starts, bits = _attention_case(ls=ls, dim=128, page=16, dtype=HF if scale > 1 else BF, tree=True, seed=4, **KINDS[kind])
+    _check_attention(a, ls, starts, bits, 100, 1, scale=scale)
+
+
+def test_attention_with_rows_that_see_nothing():
+    """Masks without a bit over an empty prefix, bits behind the tree's end, a mask of ones."""
+    from actfold_b200.speculative import tree_attention_int4
+
+    for kind in KINDS:
+        a, starts, _ = _attention_case(ls=[0, 40, 5], dim=64, page=8, dtype=BF, tree=False, seed=5, **KINDS[kind])
+        words = 4
+        a["mask"] = torch.full((starts[-1], words), -1, dtype=torch.int32, device="cuda")  # ones, behind the end too
+        n = KINDS[kind]["ns"]
+        bits = [torch.ones(x, x, dtype=torch.bool) for x in n]
+        _check_attention(a, [0, 40, 5], starts, bits)
+        a["mask"][0] = 0
+        bits[0][0] = False
+        a["mask"][starts[1]] = 0
+        bits[1][0] = False
+        out = _check_attention(a, [0, 40, 5], starts, bits)
+        assert not out[0].any()
+        lse = torch.zeros(starts[-1], a["q"].shape[1], device="cuda")
+        tree_attention_int4(**a, lse=lse)
+        assert bool((lse[0] == -math.inf).all()) and torch.isfinite(lse[1:]).all()
+
+
+@pytest.mark.parametrize("ns,ls,heads,kv,window", [([1], [30000], 7, 1, None), ([2] * 300, [90 + i for i in range(300)], 4, 2, None), ([1] * 50, [5000] * 50, 2, 2, 900),
+                                                   ([20], [20000], 4, 1, None), ([60, 64], [9000, 7000], 8, 2, None), ([64] * 40, [300] * 40, 2, 2, 128)])
+def test_attention_of_long_rows_and_many_requests(ns, ls, heads, kv, window):
+    """Rows that many CTAs share, CTAs with many rows; the same bits in every run."""
+    from actfold_b200.speculative import tree_attention_int4
+
+    a, starts, bits = _attention_case(ns, ls, heads, kv, 128, 16, BF, False, 6)
+    out = _check_attention(a, ls, starts, bits, window)
+    for _ in range(3):
+        assert torch.equal(_bits(tree_attention_int4(**a, window=window)), _bits(out))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_reports_bad_values(kind):
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention_int4
+
+    ls = [70, 300, 33]
+    a, starts, bits = _attention_case(ls=ls, dim=64, page=16, dtype=BF, tree=False, seed=7, **KINDS[kind])
+    good = tree_attention_int4(**a)
+    st = DeviceStatus()
+    for r, x in ((0, -1), (2, 10 ** 7)):  # lengths that are none: the request is left out
+        lengths = a["lengths"].clone()
+        lengths[r] = x
+        out = torch.full_like(good, 3.0)
+        tree_attention_int4(**{**a, "lengths": lengths}, out=out, status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+        mine = torch.zeros(starts[-1], dtype=torch.bool, device="cuda")
+        mine[starts[r]:starts[r + 1]] = True
+        assert bool((out[mine] == 3.0).all()) and torch.allclose(out[~mine].float(), good[~mine].float(), rtol=2 ** -6, atol=2 ** -6)
+    for bad in ([0, starts[2], starts[1], starts[3]], [0, starts[1], starts[2], starts[3] + 1], [-1, *starts[1:]]):
+        tree_attention_int4(**{**a, "starts": _i32(bad)}, status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+    for page in (-1, 10 ** 6):  # read as zeros
+        tables = a["tables"].clone()
+        tables[1, 3] = page
+        out = tree_attention_int4(**{**a, "tables": tables}, status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+        assert torch.equal(_bits(out[: starts[1]]), _bits(good[: starts[1]])) and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("kind", [*KINDS, "long"])
+def test_attention_ends_when_a_wait_runs_out(kind):
+    """No attempt but the first for every wait: the call ends and says so, or no wait was long (an attempt sleeps some microseconds); the
+    next call is right. Values that are not finite in all of a long chain make row ends, and so some waits, long for certain."""
+    from actfold_b200 import _lib
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import tree_attention_int4
+
+    ls = [3000, 900, 1400]
+    shape = dict(ns=[1500, 3, 900], heads=4, kv=2) if kind == "long" else KINDS[kind]
+    a, starts, bits = _attention_case(ls=ls, dim=128, page=16, dtype=BF, tree=False, seed=8, **shape)
+    st = DeviceStatus()
+    v = a["v"].clone()
+    if kind == "long":
+        v[::64] = math.inf
+    _lib.check(_lib.load().af_tree_attention_wait_limit(0))
+    try:
+        out = tree_attention_int4(**{**a, "v": v}, status=st)
+        ran_out = bool(int(st.status) & 1)
+        if kind == "long":
+            assert ran_out
+        if ran_out:
+            with pytest.raises(TimeoutError):
+                st.check_status()
+    finally:
+        _lib.check(_lib.load().af_tree_attention_wait_limit(-1))
+    if kind != "long":
+        good = _check_attention(a, ls, starts, bits)
+        assert ran_out or torch.equal(_bits(out), _bits(good))
+    else:
+        assert torch.isfinite(tree_attention_int4(**a, status=st)).all()
+    st.check_status()
+
+
+def test_weights_of_every_kind_of_row():
+    """Keys that are not finite, rows without weight, more rows than are held at once; the same bits in every run."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import attention_weights, read_cache_int4, write_cache_int4
+
+    ns, ls, heads, kv = [3, 40], [90, 200], 8, 2
+    a, starts, _ = _attention_case(ns, ls, heads, kv, 64, 16, HF, False, 11)
+    k = torch.zeros(1, kv, 64, dtype=HF, device="cuda")
+    k[0, 1, 5] = math.nan
+    write_cache_int4(k, k, a["cache"], a["tables"][0, 1].long() * 16 + _i64([3]))  # place 19 of request 0
+    lse = torch.full((43, heads), 2.5, device="cuda")
+    lse[1] = -math.inf
+    lse[7] = math.inf
+    runs = []
+    for held in (4, 16):
+        keys = read_cache_int4(a["cache"], torch.arange(a["cache"].pages * 16, device="cuda"))[0]
+        cache = a["cache"] if held == 4 else keys.view(-1, 16, kv, 64)
+        for window, sinks in ((None, 0), (30, 2)):
+            slots = [a["tables"][b].long()[torch.arange(t, device="cuda") // 16] * 16 + torch.arange(t, device="cuda") % 16 for b, t in enumerate(ls)]
+            want, tol = U.weights(a["q"], keys, slots, ls, starts, lse, torch.zeros(2, kv, 200, device="cuda"), window or 0, sinks)
+            got = [attention_weights(a["q"], cache, a["tables"], a["lengths"], a["starts"], lse, torch.zeros(2, kv, 200, device="cuda"), window=window, sinks=sinks)
+                   for _ in range(2)]
+            assert torch.equal(got[0].nan_to_num(7.0), got[1].nan_to_num(7.0))
+            if window is None:
+                assert got[0][0, 1, 19].isnan() and torch.isfinite(got[0][0, 0]).all()
+                want[0, 1, 19] = math.nan
+            assert U.close(got[0], want, tol)
+    st = DeviceStatus()
+    w = torch.zeros(2, kv, 150, device="cuda")
+    attention_weights(a["q"], a["cache"], a["tables"], a["lengths"], a["starts"], lse, w, status=st)  # 200 places do not fit into 150
+    with pytest.raises(RuntimeError):
+        st.check_status()
+    assert not w[1].any() and w[0, 0, :90].all()
+    for bad in ([0, 40, 3], [0, 3, 44]):
+        attention_weights(a["q"], a["cache"], a["tables"], a["lengths"], _i32(bad), lse, torch.zeros(2, kv, 200, device="cuda"), status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+    for cache in (a["cache"], keys.view(-1, 16, kv, 64)):
+        tables = a["tables"].clone()
+        tables[1, 2] = 10 ** 6
+        attention_weights(a["q"], cache, tables, a["lengths"], a["starts"], lse, torch.zeros(2, kv, 200, device="cuda"), status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ together
+def test_steps_of_a_batch_over_its_budget():
+    """Prompts in, then steps of one token: attention, weights, rows written, eviction, pages back. A plain loop keeps lists of rows."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import Int4Cache, attention_weights, block_tables, evict_cache, tree_attention_int4, write_cache_int4
+
+    layers, kv, heads, dim, page, keep, sinks, recent, pool = 3, 2, 4, 64, 8, 24, 2, 6, 40
+    prompts = [30, 9, 17, 24]
+    n = len(prompts)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF)
+    st = DeviceStatus()
+    cache = Int4Cache.empty(pool, page, kv, dim, BF, layers)
+    tables = torch.full((n, 8), -1, dtype=torch.int32, device="cuda")
+    free, span = torch.arange(pool, dtype=torch.int32, device="cuda"), _i64([0, pool])
+    weights = torch.zeros(layers, n, kv, 64, device="cuda")
+    k, v = rand(layers, sum(prompts), kv, dim), rand(layers, sum(prompts), kv, dim)
+    new = block_tables(tables, _i32([0] * n), _i32(prompts), free, span, page, sum(prompts), status=st)
+    write_cache_int4(k, v, cache, new.slots, status=st)
+    span, lengths = new.free_range, new.totals
+    vk, vv = (U.values(*U.encode(x)) for x in (k, v))
+    at = [0, *np.cumsum(prompts).tolist()]
+    kept = [[[[(vk[l, i, h], vv[l, i, h]) for i in range(at[r], at[r + 1])] for h in range(kv)] for r in range(n)] for l in range(layers)]
+    given = [[[[0.0] * p for _ in range(kv)] for p in prompts] for _ in range(layers)]
+    for step in range(4):
+        old = lengths
+        q, k, v = rand(layers, n, heads, dim), rand(layers, n, kv, dim), rand(layers, n, kv, dim)
+        starts = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+        for l in range(layers):
+            lse = torch.empty(n, heads, device="cuda")
+            out = tree_attention_int4(q[l], k[l], v[l], cache[l], tables, lengths, starts, lse=lse, status=st)
+            attention_weights(q[l], cache[l], tables, lengths, starts, lse, weights[l], status=st)
+            for r in range(n):
+                for h in range(heads):
+                    gk = h * kv // heads
+                    kk = torch.stack([x for x, _ in kept[l][r][gk]] + [k[l, r, gk]]).double()
+                    ww = torch.stack([x for _, x in kept[l][r][gk]] + [v[l, r, gk]]).double()
+                    p = torch.softmax(kk @ q[l, r, h].double() * dim ** -0.5, 0)
+                    assert torch.allclose(out[r, h].double(), p @ ww, rtol=2 ** -7, atol=2 ** -6)
+                    for i, x in enumerate(p[:-1].tolist()):
+                        given[l][r][gk][i] += x
+        grown = block_tables(tables, lengths, torch.ones_like(lengths), free, span, page, n, status=st)
+        write_cache_int4(k, v, cache, grown.slots, status=st)
+        vk, vv = (U.values(*U.encode(x)) for x in (k, v))
+        for l in range(layers):
+            for r in range(n):
+                for h in range(kv):
+                    kept[l][r][h].append((vk[l, r, h], vv[l, r, h]))
+                    given[l][r][h].append(0.0)
+        span = grown.free_range
+        e = evict_cache(cache, tables, grown.totals, weights, keep, sinks=sinks, recent=recent, status=st)
+        for l in range(layers):
+            for r in range(n):
+                for h in range(kv):
+                    t = len(kept[l][r][h])
+                    places = e.kept[l, r, h].tolist()
+                    mine = U.evict(weights[l, r, h, :t].tolist(), keep, sinks, recent)
+                    assert places == mine + [-1] * (keep - len(mine))
+                    assert torch.allclose(weights[l, r, h, :t].double().cpu(), torch.tensor(given[l][r][h], dtype=torch.float64), rtol=1e-3, atol=1e-5)
+                    kept[l][r][h] = [kept[l][r][h][i] for i in mine]
+                    given[l][r][h] = [given[l][r][h][i] for i in mine]
+        weights = e.weights.clone()
+        back = block_tables(tables, e.lengths, torch.zeros_like(lengths), free, span, page, 0, held=grown.totals, status=st)
+        span, lengths = back.free_range, e.lengths
+        st.check_status()
+        assert lengths.tolist() == [min(keep, t + 1) for t in old.tolist()]
+        used = sum(-(-t // page) for t in lengths.tolist())
+        assert (span[1] - span[0]).item() == pool - used
+
+
+def test_captured_steps_on_another_stream():
+    """Every operator in graphs of one pool that are replayed with other lengths, one of them past what was written: the eager results, bit by bit."""
+    from actfold_b200.speculative import Int4Cache, attention_weights, evict_cache, read_cache_int4, tree_attention_int4, write_cache_int4
+
+    def case(kind, seed):
+        a, starts, _ = _attention_case(ls=[300, 1200, 40], dim=128, page=16, dtype=BF, tree=False, seed=seed, **KINDS[kind])
+        total, heads = a["q"].shape[:2]
+        kv = KINDS[kind]["kv"]
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        a["weights"] = torch.rand(3, kv, 1300, device="cuda", generator=g)
+        a["slots"] = a["tables"][1, 5].long() * 16 + torch.arange(4, device="cuda")
+        a["rows"] = torch.randn(4, kv, 128, device="cuda", generator=g).to(BF)
+        return a
+
+    def step(a, cache, weights):
+        args = {x: a[x] for x in ("q", "k", "v", "tables", "lengths", "starts", "mask")}
+        lse = torch.empty(a["q"].shape[0], a["q"].shape[1], device="cuda")
+        write_cache_int4(a["rows"], a["rows"], cache, a["slots"])
+        out = tree_attention_int4(**args, cache=cache, lse=lse)
+        attention_weights(a["q"], cache, a["tables"], a["lengths"], a["starts"], lse, weights)
+        e = evict_cache(cache, a["tables"], a["lengths"], weights, 200, sinks=2, recent=20)
+        return out, lse, *e, *read_cache_int4(cache, a["slots"])
+
+    cases = [case(kind, 20 + i) for i, kind in enumerate(KINDS)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs, results, caches, sums = [], [], [], []
+    pool = torch.cuda.graph_pool_handle()
+    with torch.cuda.stream(side):
+        for a in cases:
+            caches.append(Int4Cache(a["cache"].data.clone(), BF))
+            sums.append(a["weights"].clone())
+            step(a, caches[-1], sums[-1])
+        side.synchronize()
+        for a, c, w in zip(cases, caches, sums):
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, pool=pool, stream=side):
+                results.append(step(a, c, w))
+            graphs.append(gr)
+    for ls in ([300, 1200, 40], [1, 900, 201], [0, 0, 640]):
+        for a, gr, r, c, w in zip(cases, graphs, results, caches, sums):
+            a["lengths"].copy_(_i32(ls))
+            c.data.copy_(a["cache"].data)
+            w.copy_(a["weights"])
+            c2, w2 = Int4Cache(a["cache"].data.clone(), BF), a["weights"].clone()
+            want = step(a, c2, w2)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                gr.replay()
+            side.synchronize()
+            for x, y in zip((*r, c.data, w), (*want, c2.data, w2)):
+                assert torch.equal(_bits(x), _bits(y))
+    torch.cuda.synchronize()
+
+
+def test_calls_at_once_on_two_streams():
+    """Two attentions and two evictions on streams of their own, each with its own scratch."""
+    from actfold_b200.speculative import Int4Cache, evict_cache, tree_attention_int4
+
+    cases = [_attention_case(ls=[3000, 2000, 900], dim=128, page=16, dtype=BF, tree=False, seed=30 + i, **KINDS[kind])[0] for i, kind in enumerate(("8", "128"))]
+    want = [tree_attention_int4(**a) for a in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i, (a, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(tree_attention_int4(**a))
+    evicted = []
+    for a, s in zip(cases, streams):
+        with torch.cuda.stream(s):
+            c = Int4Cache(a["cache"].data.clone(), BF)
+            w = torch.arange(3000, device="cuda", dtype=torch.float32).flip(0).expand(3, 2, 3000)
+            evicted.append((c, evict_cache(c, a["tables"], a["lengths"], w, 1000)))
+    for s in streams:
+        s.synchronize()
+    for x, y in zip(want, got):
+        assert all(torch.equal(_bits(x), _bits(z)) for z in y)
+    for c, e in evicted:
+        assert e.lengths.tolist() == [1000, 1000, 900] and torch.equal(e.kept[0, 0], torch.arange(1000, device="cuda", dtype=torch.int32))
+
+
+def test_empty_calls():
+    from actfold_b200.speculative import Int4Cache, attention_weights, evict_cache, read_cache_int4, tree_attention_int4, write_cache_int4
+
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+    cache = Int4Cache.empty(2, 8, 2, 64, BF)
+    none = Int4Cache.empty(0, 8, 2, 64, BF)
+    q, k = (torch.ones(3, h, 64, dtype=BF, device="cuda") for h in (4, 2))
+    assert tree_attention_int4(q[:0], k[:0], k[:0], cache, i32(2, 1), i32(2), i32(3)).shape == (0, 4, 64)
+    assert tree_attention_int4(q, k, k, cache, i32(0, 1), i32(0), i32(1)).shape == (3, 4, 64)
+    for c, t in ((cache, i32(1, 0)), (none, i32(1, 2)), (cache, i32(1, 1))):  # no table entries, no pages, no cached token
+        out = tree_attention_int4(q, k, k, c, t, i32(1), _i32([0, 3]))
+        assert torch.equal(out, q)
+    w = torch.ones(1, 2, 8, device="cuda")
+    for c, t in ((cache, i32(1, 0)), (none, i32(1, 2)), (cache, i32(1, 1))):
+        assert bool((attention_weights(q, c, t, i32(1), _i32([0, 3]), torch.zeros(3, 4, device="cuda"), w) == 1).all())
+        e = evict_cache(c, t, i32(1), w, 4)
+        assert e.lengths.tolist() == [0] and bool((e.kept == -1).all()) and not e.weights.any()
+    assert evict_cache(cache, i32(0, 1), i32(0), w[:0], 4).kept.shape == (0, 2, 4)
+    empty = torch.zeros(0, 2, 8, 2, 64, dtype=BF, device="cuda")
+    e = evict_cache((empty, empty), i32(1, 1), _i32([9]), torch.zeros(0, 1, 2, 8, device="cuda"), 4)
+    assert e.lengths.tolist() == [4] and e.kept.shape == (0, 1, 2, 4)
+    write_cache_int4(k, k, none, torch.full((3,), -1, dtype=torch.int64, device="cuda"))
+    assert not read_cache_int4(none, torch.full((3,), -1, dtype=torch.int64, device="cuda"))[0].any()
