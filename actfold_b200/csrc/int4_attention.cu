@@ -590,7 +590,7 @@ int launch(const Params& p, cudaStream_t s) {
   const int ctas = CTAS * sm_count();
   cudaError_t e = launch_ex(k_int4_attention<DT, HD, NT, W, CTAS>, dim3(ctas), dim3(S::kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
   if (e == cudaSuccess && p.joins)
-    e = launch_ex(k_join<DT, S::kRows, HD>, dim3(ctas, S::kRows / 8 * 4), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+    e = launch_ex(k_join<DT, S::kRows, HD>, dim3(ctas, S::kRows), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: launch: ") + cudaGetErrorString(e));
   return check_launch("af_tree_attention_int4");
 }
@@ -680,9 +680,9 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   const int64_t rows = ceil_div(a.total, a.batch) * p.group;  // of the average request and head
   const bool wide = rows > 16;
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
-  p.row_cost = wide ? 3 : 10;
-  p.whole = wide ? 8 : 32;
-  p.whole_long = 8;
+  p.row_cost = p.rows > 128 ? 5 : wide ? 3 : 10;
+  p.whole = wide ? 2 : 32;
+  p.whole_long = wide ? 2 : 8;
   p.least = wide ? 2 : 14;
   // Units are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
   const int64_t most = (a.max_pages * c.page_size + a.total) / (wide ? kv4::kWideUnit : kv4::kUnit) + 3;  // of a row tile

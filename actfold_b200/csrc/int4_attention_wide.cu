@@ -792,7 +792,7 @@ int launch(const Params& p, cudaStream_t s) {
   const int ctas = sm_count();
   cudaError_t e = launch_ex(k_int4_attention_wide<DT, HD>, dim3(ctas), dim3(kThreads), (size_t)Wide<HD>::kBytes, s, false, dim3(1), p);
   if (e == cudaSuccess && p.joins)
-    e = launch_ex(k_join<DT, 2 * kRows, HD>, dim3(ctas, 16), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
+    e = launch_ex(k_join<DT, 2 * kRows, HD>, dim3(ctas, 32), dim3(kJoinThreads), 0, s, true, dim3(1), p, ctas);
   if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: launch: ") + cudaGetErrorString(e));
   return check_launch("af_tree_attention_int4");
 }
