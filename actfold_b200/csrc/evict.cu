@@ -146,13 +146,12 @@ struct MoveArgs {
   int64_t tables_ld, capacity;
   int batch, heads, pages, page, places, keep;
   int columns, pieces;                              // CTAs side by side of a row; pieces of 16 (of 4 bits and 64 dims: 8) bytes of each
-  int rows;                                         // of a warp's step: at most 32, and kWarpPieces pieces
+  int rows;                                         // of a warp's step: at most 32, and Move::kPieces pieces
   uint32_t by_pieces;                               // p / pieces = p * by_pieces >> 20 for p < 2048, pieces <= 256
   unsigned* status;
 };
 
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32, kStages = 3;  // steps in flight
-constexpr int kWarpPieces = 256, kPer = kWarpPieces / 32;  // of a step
 
 // Where a row lies: its first piece, and its row of a 4-bit block.
 struct Place {
@@ -160,11 +159,14 @@ struct Place {
   int r;
 };
 
-template <int BYTES>
-struct MoveShared {
-  static constexpr int kData = kStages * kMoveWarps * kWarpPieces * BYTES;
+// HD = 0: rows of 16 bits (or any other) type; 64 or 128: 4-bit blocks of that many dims.
+template <int HD>
+struct Move {
+  static constexpr int kBytes = HD == 64 ? 8 : 16;             // of a piece
+  static constexpr int kPieces = HD == 0 ? 256 : 5 * 32;       // of a warp's step
+  static constexpr int kData = kStages * kMoveWarps * kPieces * kBytes;
   static constexpr int kPlaces = kMoveWarps * 32 * (int)sizeof(Place);  // of a step's rows: where from, and per stage where to
-  static constexpr int kBytes = kData + (1 + kStages) * kPlaces;
+  static constexpr int kShared = kData + (1 + kStages) * kPlaces;
 };
 
 template <int BYTES>
@@ -173,13 +175,12 @@ __device__ __forceinline__ void copy_in(uint32_t dst, const char* src) {
   else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// HD = 0: rows of 16 bits (or any other) type; 64 or 128: 4-bit blocks of that many dims. CLUSTER CTAs share each step's rows.
-// A warp's step: its lanes look up a row each (page and place, where from and where to), then move the rows' pieces together.
+// CLUSTER CTAs share each step's rows. A warp's step: its lanes look up a row each (page and place, where from and where to), then move the rows' pieces together.
 template <int HD, int CLUSTER>
 __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
-  constexpr int kBytes = HD == 64 ? 8 : 16;
   using B = kv4::Block<HD == 0 ? 64 : HD>;
-  using M = MoveShared<kBytes>;
+  using M = Move<HD>;
+  constexpr int kBytes = M::kBytes, kWarpPieces = M::kPieces, kPer = kWarpPieces / 32;
   extern __shared__ __align__(16) uint8_t buf[];
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -288,16 +289,20 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
 
 template <int HD, int CLUSTER>
 cudaError_t launch_move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
-  constexpr int bytes = MoveShared<HD == 64 ? 8 : 16>::kBytes;
+  constexpr int bytes = Move<HD>::kShared;
   // The same for every call: set each time, which costs less than keeping track of the devices.
   const cudaError_t e = cudaFuncSetAttribute(k_move<HD, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
   return launch_ex(k_move<HD, CLUSTER>, dim3((unsigned)(segments * a.columns * CLUSTER)), dim3(kMoveThreads), (size_t)bytes, s, true, dim3(CLUSTER), a);
 }
 
+// A CTA holds some 60 to 100 KB: two or three fit an SM. Clusters as long as all of their CTAs do at once.
 template <int HD>
 cudaError_t move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
-  return segments * a.columns < 148 ? launch_move<HD, 8>(a, segments, s) : launch_move<HD, 1>(a, segments, s);
+  const int64_t ctas = segments * a.columns, room = 3 * sm_count();
+  if (8 * ctas <= room) return launch_move<HD, 8>(a, segments, s);
+  if (4 * ctas <= room) return launch_move<HD, 4>(a, segments, s);
+  return 2 * ctas <= room ? launch_move<HD, 2>(a, segments, s) : launch_move<HD, 1>(a, segments, s);
 }
 
 }  // namespace
@@ -361,13 +366,13 @@ extern "C" int af_evict_cache(const af_evict_args* args, uint32_t* status, void*
     al = reinterpret_cast<uintptr_t>(m.k) | reinterpret_cast<uintptr_t>(m.v) | (uint64_t)w.head_bytes;
     for (int i = 0; i < 4; ++i) al |= (uint64_t)w.k_cache_strides[i] | (uint64_t)w.v_cache_strides[i];
     const int whole = (int)(w.head_bytes / 16);
-    // Whole rows a CTA where there are enough segments for all SMs, else 64 bytes.
-    m.pieces = 2 * segments < 296 && whole % 4 == 0 ? 4 : whole > 0 ? whole : 1;
+    // Whole rows a CTA where there are many segments for each SM, else 128 or 64 bytes: few long CTAs leave the last ones waiting.
+    m.pieces = 2 * segments < 2 * sm_count() && whole % 4 == 0 ? 4 : 2 * segments < 16 * sm_count() && whole % 8 == 0 ? 8 : whole > 0 ? whole : 1;
     m.columns = whole > 0 ? 2 * (whole / m.pieces) : 2;
   }
   AF_REQUIRE(!moves || (al & 15) == 0, "af_evict_cache: addresses and strides must be multiples of 16 bytes");
   m.by_pieces = (uint32_t)(((1 << 20) + m.pieces - 1) / m.pieces);
-  m.rows = kv_evict::kWarpPieces / m.pieces < 32 ? kv_evict::kWarpPieces / m.pieces : 32;
+  m.rows = packed || 256 / m.pieces > 32 ? 32 : 256 / m.pieces;  // (Move::kPieces)
   m.tables = w.tables;
   m.tables_ld = w.tables_stride;
   m.lengths = w.lengths;
