@@ -32,7 +32,7 @@ struct SelectArgs {
   unsigned* status;
 };
 
-constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32, kBins = 2048;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32, kBins = 2048, kOwn = kBins / kSelThreads;
 
 // Ascending whole numbers for ascending weights; -0 equals 0, and NaN is above all numbers.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, above = pass == 0 ? 32 : shift + (pass == 1 ? 11 : 10);
       const uint32_t mask = pass == 2 ? 1023u : 2047u;
-      s_hist[tid] = s_hist[tid + kSelThreads] = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) s_hist[tid + i * kSelThreads] = 0;
       __syncthreads();
 #pragma unroll 4
       for (int i = lo + tid; i < hi; i += kSelThreads) {
@@ -82,9 +83,11 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
         if (pass == 0 || k >> above == prefix >> above) atomicAdd(&s_hist[(k >> shift) & mask], 1);
       }
       __syncthreads();
-      // Thread x has the bins 2047 - 2 x and 2046 - 2 x; from the top down, the one in which the need-th token lies.
-      const int c0 = s_hist[kBins - 1 - 2 * tid], c1 = s_hist[kBins - 2 - 2 * tid];
-      int upto = c0 + c1;
+      // Thread x has kOwn bins, from 2047 - kOwn x on downwards; from the top down, the one in which the need-th token lies.
+      int c[kOwn], upto = 0;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) upto += c[i] = s_hist[kBins - 1 - kOwn * tid - i];
+      const int mine = upto;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
@@ -92,14 +95,15 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
       }
       if (lane == 31) s_sum[0][warp] = upto;
       __syncthreads();
-      int before = lane < warp ? s_sum[0][lane] : 0;
+      const int before = __reduce_add_sync(0xffffffffu, lane < warp ? s_sum[0][lane] : 0);
+      int begin = before + upto - mine;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      const int end = before + upto, begin = end - c0 - c1;
-      if (begin < need && need <= end) {
-        const bool first = need <= begin + c0;
-        s_bin = kBins - 1 - 2 * tid - (first ? 0 : 1);
-        s_need = need - begin - (first ? 0 : c0);
+      for (int i = 0; i < kOwn; ++i) {
+        if (begin < need && need <= begin + c[i]) {
+          s_bin = kBins - 1 - kOwn * tid - i;
+          s_need = need - begin;
+        }
+        begin += c[i];
       }
       __syncthreads();
       prefix |= (uint32_t)s_bin << shift;
@@ -107,7 +111,7 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
     }
   }
   // Tokens above `prefix` stay, and the first `need` of those that equal it. In order: the number of certain ones and of equal
-  // ones before each, both in one word (a chunk has 1024 places).
+  // ones before each, both in one word (a chunk has fewer than 2^16 places).
   int certain = 0, equal = 0;
 #pragma unroll 1
   for (int i0 = 0, turn = 0; i0 < t; i0 += kSelThreads, turn ^= 1) {
@@ -119,13 +123,8 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
     const uint32_t sures = __ballot_sync(0xffffffffu, sure), ties = __ballot_sync(0xffffffffu, tie);
     if (lane == 0) s_sum[turn][warp] = __popc(sures) | __popc(ties) << 16;
     __syncthreads();
-    const int all = s_sum[turn][lane];
-    int before = lane < warp ? all : 0, total = all;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
+    const int all = lane < kSelWarps ? s_sum[turn][lane] : 0;
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? all : 0), total = __reduce_add_sync(0xffffffffu, all);
     const uint32_t below = (1u << lane) - 1u;
     const int sure_at = certain + (before & 0xffff) + __popc(sures & below), tie_at = equal + (before >> 16) + __popc(ties & below);
     if (sure || (tie && tie_at < need)) {
