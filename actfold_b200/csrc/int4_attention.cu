@@ -331,36 +331,45 @@ __global__ void __launch_bounds__(32 * (W + 1), CTAS) k_int4_attention(const __g
           const uint32_t unit = base + slot * S::kUnitBytes;
           auto sees = [&](int at, int nt, int e) { return at < s.len && (at >= first[nt][e] || at < p.sinks); };
           bool sick = false;
-#pragma unroll 1
+          // S of both halves first: its chain of products is over by the time that the softmax looks at it.
+          float both[2][NT][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t blocks = unit + 2 * h * B::kBytes;
+            auto& sc = both[h];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sc[nt][c] = 0.f;
+            uint32_t w[2][KW], pr[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              lds<4 * KW>(blocks + r * B::kBytes + k_at, w[r]);
+              lds<4>(blocks + r * B::kBytes + kp_at, &pr[r]);
+            }
+            const uint32_t s0 = __byte_perm(pr[0], 0, 0x1010), o0 = __byte_perm(pr[0], 0, 0x3232);
+            const uint32_t s1 = __byte_perm(pr[1], 0, 0x1010), o1 = __byte_perm(pr[1], 0, 0x3232);
+#pragma unroll
+            for (int i = 0; i < KW; ++i) {
+              const uint32_t a0 = two_values<DT, 0>(w[0][i], s0, o0), a1 = two_values<DT, 0>(w[1][i], s1, o1);
+              const uint32_t a2 = two_values<DT, 1>(w[0][i], s0, o0), a3 = two_values<DT, 1>(w[1][i], s1, o1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], a0, a1, a2, a3, q[nt][4 * i], q[nt][4 * i + 1]);
+              const uint32_t b0 = two_values<DT, 2>(w[0][i], s0, o0), b1 = two_values<DT, 2>(w[1][i], s1, o1);
+              const uint32_t b2 = two_values<DT, 3>(w[0][i], s0, o0), b3 = two_values<DT, 3>(w[1][i], s1, o1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], b0, b1, b2, b3, q[nt][4 * i + 2], q[nt][4 * i + 3]);
+            }
+          }
+#pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t blocks = unit + 2 * h * B::kBytes;
             float sc[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) sc[nt][c] = 0.f;
+              for (int c = 0; c < 4; ++c) sc[nt][c] = h ? both[1][nt][c] : both[0][nt][c];
             uint32_t pf[NT][2];
-            {
-              uint32_t w[2][KW], pr[2];
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                lds<4 * KW>(blocks + r * B::kBytes + k_at, w[r]);
-                lds<4>(blocks + r * B::kBytes + kp_at, &pr[r]);
-              }
-              const uint32_t s0 = __byte_perm(pr[0], 0, 0x1010), o0 = __byte_perm(pr[0], 0, 0x3232);
-              const uint32_t s1 = __byte_perm(pr[1], 0, 0x1010), o1 = __byte_perm(pr[1], 0, 0x3232);
-#pragma unroll
-              for (int i = 0; i < KW; ++i) {
-                const uint32_t a0 = two_values<DT, 0>(w[0][i], s0, o0), a1 = two_values<DT, 0>(w[1][i], s1, o1);
-                const uint32_t a2 = two_values<DT, 1>(w[0][i], s0, o0), a3 = two_values<DT, 1>(w[1][i], s1, o1);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], a0, a1, a2, a3, q[nt][4 * i], q[nt][4 * i + 1]);
-                const uint32_t b0 = two_values<DT, 2>(w[0][i], s0, o0), b1 = two_values<DT, 2>(w[1][i], s1, o1);
-                const uint32_t b2 = two_values<DT, 3>(w[0][i], s0, o0), b3 = two_values<DT, 3>(w[1][i], s1, o1);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma<DT>(sc[nt], b0, b1, b2, b3, q[nt][4 * i + 2], q[nt][4 * i + 3]);
-              }
-            }
             uint32_t w[2][2][VW], pr[2][2];  // [block][key of the lane's two]
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
