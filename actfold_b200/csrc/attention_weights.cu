@@ -124,8 +124,45 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
     u0 += x1 - x0;
     const int* table = p.tables + (int64_t)b * p.tables_ld;
     const int rows = r.n * p.group, first_all = p.window ? max(0, r.len - max(0, p.window - r.n)) : 0;
+    // The warp's units of the segment, eight at a time: lane 4 y + z knows where block z of the y-th of them lies (null: there is no
+    // such key, or its page is none: reads as zeros).
+    int known = x0 + warp - 8 * W, next = x0 + warp;
+    const char* from = nullptr;
+    auto bring = [&]() {
+      if (next >= x1 || lost) return;
+      if (next - known >= 8 * W) {
+        known = next;
+        const int x = known + W * (lane >> 2), at = kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from) + kBlockTokens * (lane & 3);
+        from = nullptr;
+        if (x < x1 && at < r.len) {
+          const int entry = entry_of(p, at), page = table[entry];
+          if (page >= 0 && page < p.pages)
+            from = p.data + page * p.d_page + h * p.d_head + (int64_t)((at - entry * p.page) / kBlockTokens) * B::kBytes;
+          else if (p.status)
+            atomicOr(p.status, AF_STATUS_BOUNDS);
+        }
+      }
+      const int slot = brought & 1;
+      const bool mine = (lane >> 2) * W == next - known;
+      uint8_t* to = slots + slot * kUnitBytes + (lane & 3) * B::kPart;
+      if (mine && !from) {
+        for (int y = 0; y < B::kPart / 16; ++y) reinterpret_cast<uint4*>(to)[y] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+      }
+      const uint32_t blocks = __ballot_sync(0xffffffffu, mine && from);
+      if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, __popc(blocks) * B::kPart);
+      __syncwarp();
+      if (mine && from)
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(B::kPart),
+                     "r"(full + 8 * slot)
+                     : "memory");
+      ++brought;
+      next += W;
+    };
 #pragma unroll 1
     for (int row0 = 0; row0 < rows; row0 += kRows) {
+      if (INT4 && row0 > 0) known = x0 + warp - 8 * W, next = x0 + warp;
+      if constexpr (INT4) bring();  // (on its way while the rows are laid out)
       // A row's 16-byte pieces in the order in which the lanes of a quad take them, exchanged by halves of 128 bytes in odd rows:
       // eight lanes read different banks.
       const int count = min(kRows, rows - row0), tiles = (count + 7) / 8;
@@ -144,41 +181,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
         s_first[tid] = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
       }
       __syncthreads();
-      // A unit's keys: lane y brings block y, if its page is one; what there is no key for reads as zeros.
-      auto place_of = [&](int x) { return kUnit * (x < r.sink_units ? x : x - r.sink_units + r.from) + kBlockTokens * lane; };
-      auto look_up = [&](int x) { return x < x1 && lane < kUnit / kBlockTokens && place_of(x) < r.len ? table[entry_of(p, place_of(x))] : 0; };
-      auto bring = [&](int x, int page) {
-        if (x >= x1 || lost) return;
-        const int at = place_of(x), slot = brought & 1;
-        const bool mine = lane < kUnit / kBlockTokens, needed = mine && at < r.len;
-        const bool there = needed && page >= 0 && page < p.pages;
-        if (needed && !there && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-        if (mine && !there) {
-          for (int y = 0; y < B::kPart / 16; ++y) reinterpret_cast<uint4*>(slots + slot * kUnitBytes + lane * B::kPart)[y] = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();
-        }
-        const uint32_t blocks = __ballot_sync(0xffffffffu, there);
-        if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, __popc(blocks) * B::kPart);
-        __syncwarp();
-        if (there) {
-          const char* from = p.data + page * p.d_page + h * p.d_head + (int64_t)((at - entry_of(p, at) * p.page) / kBlockTokens) * B::kBytes;
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                           smem_u32(slots) + slot * kUnitBytes + lane * B::kPart),
-                       "l"(from), "r"(B::kPart), "r"(full + 8 * slot)
-                       : "memory");
-        }
-        ++brought;
-      };
-      int page = 0;  // of the lane's block of the unit after next
-      if constexpr (INT4) {
-        bring(x0 + warp, look_up(x0 + warp));
-        page = look_up(x0 + warp + W);
-      }
 #pragma unroll 1
       for (int x = x0 + warp; x < x1 && !lost; x += W) {
         if constexpr (INT4) {
-          bring(x + W, page);
-          page = look_up(x + 2 * W);
+          bring();
           int tries = 0;
           while (!lost && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1)) lost = ++tries > kPatience;
           lost = __any_sync(0xffffffffu, lost);
