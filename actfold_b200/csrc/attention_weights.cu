@@ -348,6 +348,7 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   p.capacity = w.max_pages * c.page_size;
   p.window = (int)w.window;
   p.sinks = (int)w.sinks;
+  p.reach = p.window - 1;
   p.scale = (float)(w.scale * 1.4426950408889634);
   p.rows = 8;
   p.status = status;

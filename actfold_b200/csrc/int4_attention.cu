@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(32 * (W + 1), CTAS) k_int4_attention(const __g
           first[nt][e] = first_place(p, s.s0, s.n, s.len, node[nt][e]);
         }
       // No row sees places from the sinks up to first_any; all see those from first_all on.
-      const int first_any = p.window ? max(0, s.len - (p.window - 1)) : 0, first_all = p.window ? max(0, s.len - max(0, p.window - s.n)) : 0;
+      const int first_any = p.window ? max(0, s.len - p.reach) : 0, first_all = p.window ? max(0, s.len - max(0, p.window - s.n)) : 0;
       float o[VT][NT][4];  // [dims 2 VT' .. of the lane's 16][row]
       float m[NT][2], l[NT][2];
 #pragma unroll
@@ -678,6 +678,7 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.capacity = c.pages ? a.max_pages * c.page_size : 0;
   p.window = (int)a.window;
   p.sinks = (int)a.sinks;
+  p.reach = p.window - (a.mask ? 0 : 1);
   p.scale = a.scale == 0. ? 1.f : (float)(fabs(a.scale) * 1.4426950408889634);
   p.q_flip = a.scale < 0. ? 0x80008000u : 0u;
   p.q_keep = a.scale == 0. ? 0u : 0xffffffffu;

@@ -34,6 +34,7 @@ struct Params {
   int runs;                                     // that 32 tokens of a cache lie in: of 32, 16 or 8 tokens, so that none leaves a page
   int64_t capacity;                             // tokens that a table row can hold
   int window, sinks;                            // window 0: all of the prefix is visible
+  int reach;                                    // tokens of the prefix that a window can hold: all, of a chain, whose nodes see themselves, one less
   float scale;                                  // times log2(e); of the attention kernels positive: q is flipped, or made 0, instead
   uint32_t q_flip, q_keep;                      // q = (q ^ flip) & keep, in pairs
   char* out;
@@ -83,9 +84,8 @@ __device__ __forceinline__ Request<UNIT> request(const Params& p, int b) {
   const int all = (r.len + UNIT - 1) / UNIT;
   r.sink_units = r.from = 0;
   if (p.window) {
-    // A node sees itself, so of the prefix at most the last window - 1 tokens.
     r.sink_units = (min(p.sinks, r.len) + UNIT - 1) / UNIT;
-    r.from = max(r.sink_units, max(0, r.len - (p.window - 1)) / UNIT);
+    r.from = max(r.sink_units, max(0, r.len - p.reach) / UNIT);
   }
   r.cached = r.sink_units + max(0, all - r.from);
   r.units = r.cached + (r.n + UNIT - 1) / UNIT;

@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       bool sick = false;
       if (values && cached && is_masked(p, f, x_now)) {
         // What no row sees is 0 (as what there is no key for); NaN that only some rows see is set aside.
-        const bool hidden = at_now < 0 || (p.window && at_now < f.len - (p.window - 1) && at_now >= p.sinks);
+        const bool hidden = at_now < 0 || (p.window && at_now < f.len - p.reach && at_now >= p.sinks);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
           if (hidden) pr[i] = 0;

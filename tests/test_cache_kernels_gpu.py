@@ -469,6 +469,66 @@ def test_attention_with_rows_that_see_nothing():
         assert bool((lse[0] == -math.inf).all()) and torch.isfinite(lse[1:]).all()
 
 
+@pytest.mark.parametrize("window,sinks", [(1, 0), (31, 2), (64, 0), (257, 5)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_windows_with_any_bits(kind, window, sinks):
+    """Nodes that see others but not themselves, or none: their windows reach to the last `window` tokens."""
+    lengths = [window + 128, 384 + window, window + 31]  # the window's first token is the first, or last, of a unit
+    a, starts, _ = _attention_case(ls=lengths, dim=128, page=16, dtype=BF, tree=False, seed=window, **KINDS[kind])
+    n = KINDS[kind]["ns"]
+    g = torch.Generator().manual_seed(window)
+    bits = [torch.rand(x, x, generator=g) < torch.rand(x, 1, generator=g) for x in n]
+    words = -(-max(n) // 32)
+    a["mask"] = torch.zeros(starts[-1], words, dtype=torch.int32, device="cuda")
+    for b, m in enumerate(bits):
+        m[0] = False
+        full = torch.zeros(n[b], 32 * words, dtype=torch.int64)
+        full[:, :n[b]] = m
+        packed = (full.view(n[b], words, 32) << torch.arange(32)).sum(2)
+        a["mask"][starts[b]:starts[b + 1]] = torch.where(packed >= 1 << 31, packed - (1 << 32), packed).to(torch.int32).cuda()
+    _check_attention(a, lengths, starts, bits, window, sinks)
+
+
+def test_offsets_past_32_bits():
+    """Pages, heads and layers that lie gigabytes apart give what a compact cache gives."""
+    from actfold_b200.speculative import Int4Cache, attention_weights, evict_cache, read_cache_int4, tree_attention_int4, write_cache_int4
+
+    layers, pages, page, kv, dim = 2, 3, 24, 2, 128
+    blocks = page // 8
+    far = torch.empty(5 << 31, dtype=torch.uint8, device="cuda")
+    strides = ((1 << 32) + (1 << 31) + 16, (1 << 30) + 32, (1 << 29) + 48, 10 * dim, 1)
+    assert sum((x - 1) * s for x, s in zip((layers, pages, kv, blocks, 10 * dim), strides)) < far.numel()
+    caches = [Int4Cache(far.as_strided((layers, pages, kv, blocks, 10 * dim), strides), BF), Int4Cache.empty(pages, page, kv, dim, BF, layers=layers)]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(layers, pages * page, kv, dim, device="cuda", generator=g).to(BF) for _ in range(2))
+    slots = torch.randperm(pages * page, device="cuda", generator=g)
+    tables, lengths = _i32([[2, 0, 1]]), _i32([70])
+    results = []
+    for cache in caches:
+        write_cache_int4(k, v, cache, slots)
+        got = [*read_cache_int4(cache, slots)]
+        for n, heads in ((1, 4), (20, 8)):
+            starts, q = _i32([0, n]), k[0, :n].repeat(1, heads // kv, 1)
+            lse, w = torch.zeros(n, heads, device="cuda"), torch.zeros(layers, 1, kv, 72, device="cuda")
+            for l in range(layers):
+                got.append(tree_attention_int4(q, k[1, :n], v[1, :n], cache[l], tables, lengths, starts, lse=lse))
+                attention_weights(q, cache[l], tables, lengths, starts, lse, w[l])
+            got += [lse, w]
+        got += [*evict_cache(cache, tables, lengths, w, 40, 1, 8), *read_cache_int4(cache, slots)]
+        results.append(got)
+    assert all(torch.equal(_bits(x), _bits(y)) for x, y in zip(*results))
+    # The same of 16-bit keys.
+    strides = ((1 << 31) + (1 << 30) + 8, (1 << 29) + 16, kv * dim, dim, 1)
+    results = []
+    for keys in (far.view(BF).as_strided((layers, pages, page, kv, dim), strides), torch.empty(layers, pages, page, kv, dim, dtype=BF, device="cuda")):
+        keys.copy_(k.view(keys.shape))
+        w = torch.zeros(layers, 1, kv, 72, device="cuda")
+        for l in range(layers):
+            attention_weights(q, keys[l], tables, lengths, starts, lse, w[l])
+        results.append([w, *evict_cache((keys, v.view(keys.shape).clone()), tables, lengths, w, 40, 1, 8), keys])
+    assert all(torch.equal(_bits(x), _bits(y)) for x, y in zip(*results))
+
+
 @pytest.mark.parametrize("ns,ls,heads,kv,window", [([1], [30000], 7, 1, None), ([2] * 300, [90 + i for i in range(300)], 4, 2, None), ([1] * 50, [5000] * 50, 2, 2, 900),
                                                    ([20], [20000], 4, 1, None), ([60, 64], [9000, 7000], 8, 2, None), ([64] * 40, [300] * 40, 2, 2, 128)])
 def test_attention_of_long_rows_and_many_requests(ns, ls, heads, kv, window):
