@@ -439,19 +439,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       }
     };
     uint32_t w[kWords], pr[kPairs];
-    // The thread's codes and pairs; zeros where there is no cached key, and of a page out of range.
-    auto fetch = [&]() {
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) w[i] = 0;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) pr[i] = 0;
+    // Where the thread's codes and pairs lie: they are brought into the L2 while the tile before is worked on. Null where there is no
+    // cached key, and of a page out of range.
+    const int r = key % kBlockTokens;  // (units begin with a block)
+    const char* from = nullptr;
+    auto locate = [&]() {
+      from = nullptr;
       if (at < 0) return;
       if (page < 0 || page >= p.pages) {
         if (p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
         return;
       }
-      const int off = at - entry_of(p, at) * p.page, r = off % kBlockTokens;
-      const char* from = p.data + page * p.d_page + plans[seg % kPlans].kvh * p.d_head + (off / kBlockTokens) * B::kBytes + (values ? B::kPart : 0);
+      const int off = at - entry_of(p, at) * p.page;
+      from = p.data + page * p.d_page + plans[seg % kPlans].kvh * p.d_head + (off / kBlockTokens) * B::kBytes + (values ? B::kPart : 0);
+      prefetch_l2(from + B::word(r, 0));
+      prefetch_l2(from + B::pair(r, 0));
+    };
+    // They; zeros where there are none.
+    auto fetch = [&]() {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = 0;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) pr[i] = 0;
+      if (!from) return;
 #pragma unroll
       for (int i = 0; i < kWords / 4; ++i) {
         const uint4 y = *reinterpret_cast<const uint4*>(from + B::word(r, 4 * i));
@@ -468,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     bool ok = true, more = first_of();
     if (more) {
       look_up();
+      locate();
       fetch();
     }
     int done_with = 0;  // segments that this warp no longer reads
@@ -502,6 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       }
       if (j >= kStages) ok = agreed(wait_for(empty + 8 * stage, (j / kStages - 1) & 1, failed));
       if (!ok) break;
+      if (more) locate();
       if (cached) {
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
@@ -512,11 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       } else {
         // A node's row, zeros behind the last node; of values the ones that are not finite are set aside.
         const int node = kUnit * (x_now - f.cached) + key;
-        const char* from = values ? p.v + (int64_t)(f.s0 + node) * p.v_n + f.kvh * p.v_h : p.k + (int64_t)(f.s0 + node) * p.k_n + f.kvh * p.k_h;
+        const char* row = values ? p.v + (int64_t)(f.s0 + node) * p.v_n + f.kvh * p.v_h : p.k + (int64_t)(f.s0 + node) * p.k_n + f.kvh * p.k_h;
         const bool there = node < f.n;
 #pragma unroll 4
         for (int i = 0; i < kWords; ++i) {
-          uint4 v = there ? *reinterpret_cast<const uint4*>(from + 16 * i) : make_uint4(0, 0, 0, 0);
+          uint4 v = there ? *reinterpret_cast<const uint4*>(row + 16 * i) : make_uint4(0, 0, 0, 0);
           if (values) {
             uint32_t* y = &v.x;
 #pragma unroll
