@@ -210,7 +210,7 @@ def evict_cache(
     same for all layers and heads. Other requests stay as they are. The tables are not changed: a
     :func:`~actfold_b200.tree_kernels.block_tables` call with ``lengths`` the result's and ``held`` the old ones returns the pages.
     Keys are moved as they are, so they have to hold their positions (as rotated keys do); a window of
-    :func:`tree_attention_int4` counts places.
+    :func:`tree_attention_int4` counts places. No page may lie in the tables of two requests, or twice in one.
     """
     packed = isinstance(cache, Int4Cache)
     if not packed:

@@ -6,8 +6,13 @@
 // are independent: a warp takes 32 of them, all rows of the request against
 // 16 at a time in registers (m16n8k16, the keys as the M side: few rows waste little), and adds to their
 // weights without atomics. The rows of a request and head, 64 at a time, lie in shared memory with their sums. 4-bit
-// keys come by bulk copies, a unit ahead. With few rows HBM bounds it, 80 bytes a key and head in 4 bits (256 in 16) and 8
-// of its weight; with many the products do. See int4_attention.cu for the fragments' order.
+// keys come by bulk copies, a unit ahead of each warp. The bytes are 80 a key and head in 4 bits (256 in 16) and 8
+// of its weight; what bounds it is the chain of a warp's unit (operands, products, exponentials), with four warps a scheduler
+// (issue 52 %, tensor pipe 28 %, HBM 22 %). See int4_attention.cu for the fragments' order.
+//   64 requests of 1 to 4 tokens, 90 to 8000 keys, 28 heads over 4: 50 us in 4 bits; the bytes need 14.
+//   One token over 523 keys: 5.5 us.
+// Tried: rows from global memory for each unit (137 us), keys looked up and loaded unit by unit (70); four chains of products
+// (53), 16 keys at a time with two or three CTAs an SM (54, 56), shares by rows as well as units (53 to 59): slower.
 #include <string>
 
 #include "int4_attention.cuh"

@@ -14,10 +14,19 @@
 // together before the codes are taken out. P^T gets from the accumulators' layout to the operand's by
 // two 8 x 8 transposes.
 //
-// A CTA per SM. A producer warp plans (see int4_attention.cuh) and brings units of 32 keys, a bulk
-// copy per page run, into a ring of 32 slots; consumer warps take units in turn, each with maxima,
-// sums and an O of its own, joined through shared memory at the end of a row tile. The step's own nodes are
-// units too, read from their 16-bit rows. Every wait is bounded; a timeout sets AF_STATUS_TIMEOUT.
+// A producer warp plans (see int4_attention.cuh) and brings units of 32 keys, a bulk
+// copy per page run, into a ring of slots; seven consumer warps take units in turn, each with maxima,
+// sums and an O of its own, joined through shared memory at the end of a row tile. Up to 8 rows: two CTAs of 16 slots on an SM, whose
+// ends of row tiles overlap (windows of 4100 tokens 160 -> 140 us); up to 16 rows: one CTA of 32 slots, for the registers. The step's own
+// nodes are units too, read from their 16-bit rows. Every wait is bounded; a timeout sets AF_STATUS_TIMEOUT.
+//
+// What bounds it is issue: some 860 instructions a unit and 8 rows, of which the values take 512, at 0.59 a cycle and scheduler
+// (ALU pipe 46 % busy, HBM 40 %).
+//   64 requests of one token, 90 to 8000 keys, 28 heads over 4: 60 us; the bytes need 25.5.
+//   24 requests of one token in windows of 4096 and 4 first tokens, 500 to 30000 keys, 32 heads over 32: 134 us; the bytes need 73.
+//   One token over 523 keys: 10.4 us, of which a launch, the plan, a table, a unit and two joins are the chain.
+// Tried: no producer, each warp brings its own units (spills); units by turns of 15 over two CTAs' warps (135 -> 150 us); Q of the
+// next row tile ahead; 15 consumer warps in one CTA: slower or the same.
 #include <math.h>
 
 #include "int4_attention.cuh"
@@ -687,12 +696,24 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.ws = static_cast<char*>(a.workspace);
   p.status = status;
   p.patience = attention_patience();
-  const int64_t rows = ceil_div(a.total, a.batch) * p.group;  // of the average request and head
+  // Rows of the average request and head choose the kernel and its row tile. 16 requests of 300 to 4100 keys, 4 heads of keys:
+  //   12 and 16 rows: 28.4 and 29.3 us in one tile of 16, 29.6 and 30.2 in two of 8, 32.7 and 32.8 as 128 (tensor cores);
+  //   20 and 28 rows: 35.4 and 36.4 us in two tiles of 16, 33.5 and 33.8 as 128;
+  //   140 and 224 rows: 50.5 and 57.0 us as 256, 56.0 and 61.3 in two tiles of 128.
+  const int64_t rows = ceil_div(a.total, a.batch) * p.group;
   const bool wide = rows > 16;
   p.rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+  // What a row tile costs besides its units (of 32 keys; wide 128), in units: the joins of the warps, the output. Few rows: 64 tokens
+  // 63.6 us with 4, 60.5 with 10, 59.4 with 20, but where few rows are cut into more (8 requests of up to 1500 keys, 32 heads) 31.8, 27.5, 30.6. Wide:
+  // 8 trees 111 us with 1, 94 with 3, 96 with 8; 2 of 64 nodes over 30000 keys, two row tiles, 120 with 1, 110 with 5 and 8.
   p.row_cost = p.rows > 128 ? 5 : wide ? 3 : 10;
+  // Units up to which a row tile is not cut: a second CTA's part costs a trip through memory and the join. One token over 523 keys
+  // 10.4 us with 32, 13.0 with 8; where shares are long such rows would make them uneven: 64 tokens 60.5 us with 8, 67.7 with 32.
+  // Wide: 16 requests of 21 to 42 rows 34 us with 2, 46 with 8.
   p.whole = wide ? 2 : 32;
   p.whole_long = wide ? 2 : 8;
+  // Units of a share, at least. Few rows: one token over 2000 and up to 8000 keys 13.7 and 14.9 us with 14, 17.2 and 18.5 with 28, 13.1
+  // and 15.8 with 4. Wide: one tree of 26 nodes over 900 keys 25.7 us with 2, 30.5 with 1, 34.7 with 6.
   p.least = wide ? 2 : 14;
   // Units are counted in 32 bits: no more than this can come of any device-side values (starts out of order are refused there).
   const int64_t most = (a.max_pages * c.page_size + a.total) / (wide ? kv4::kWideUnit : kv4::kUnit) + 3;  // of a row tile

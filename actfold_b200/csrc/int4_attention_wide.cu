@@ -8,16 +8,22 @@
 // which P is written in place (16 bits, TMEM operand of the second product).
 // With more than 128 rows they are two row tiles over the same keys; with
 // fewer, one row tile over the even and the odd key tiles, joined at the end.
-// Four warps turn a tile's keys into values and write them where the tensor cores take them (a thread has a key; 16-byte
-// pieces, 128-byte swizzle), with their next tile's codes on the way to registers; two such groups take turns with
-// the tiles, and as many do the same for the values. (8 trees of 20 to 64 nodes, 32 heads: keys and values one after the other
-// in eight warps 114 us, the keys of a tile waited for the products with the values two tiles before; four warps each
-// 105 us, at 6000 cycles a tile, 2000 of them for the turning and as many for latencies.) 64 KB a tile go through shared memory
-// twice, some 1000 cycles of its 128 bytes, next to 512 cycles of products per pipe. A softmax thread owns a row, so no
-// scores are exchanged. The reference maximum of a row is raised only when a score passes it by 2^8.
+// Four warps turn a tile's keys into values and write them where the tensor cores take
+// them (a thread has a key; 16-byte pieces, 128-byte swizzle), four others the values; the next tile's codes are brought into the L2
+// meanwhile. A softmax thread owns a row, so no scores are exchanged. The reference maximum of a row is raised only when a
+// score passes it by 2^8.
 //
-// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; warps 8-15: keys; 16-23: values;
-// warp 24 issues S, warp 25 O, warp 26 plans.
+// The work of a tile: 64 KB that go through shared memory twice (some 1000 cycles of its 128 bytes), 512 cycles of products per
+// pipe, 128 exponentials a row. No unit is busy all the time: it is the chain of turning, product, softmax and product, through
+// two buffers, that bounds it (per tile some 5500 cycles with one row tile, of which the turning warps take some 4300 with what they wait for; the softmax
+// 1500 to 1900 for half a tile of 128 rows).
+//   8 trees of 20 to 64 nodes, 32 heads over 32, 300 to 4100 keys: 246 us with the kernel of few rows, 94 now; its bytes need 17.
+//   4 trees of 48 to 64 nodes, 28 heads over 4, 30 to 65 K keys: 2204 us with that kernel, 259 now; its products need 107.
+// Tried: keys and values one after the other in eight warps (114 us instead of 105 at that time: a tile's keys waited for the
+// products with the values two tiles before); 16 turning warps with 72 registers, more registers for the issue warps or the turning
+// ones, the codes a tile ahead in shared memory (the long trees 259 -> 274 us), halves of S with one row tile too (96 -> 99): slower.
+//
+// Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; 8-11: keys; 12-15: values; 16 issues S, 17 O, 18 plans, 19 is idle.
 #include "int4_attention.cuh"
 
 namespace af {
@@ -27,7 +33,7 @@ namespace {
 
 constexpr int kUnit = kWideUnit;           // keys of a tile
 constexpr int kRows = 128;                 // rows of a pipe
-constexpr int kSoft = 8, kGroups = 1, kTurn = 8 * kGroups;  // warps; groups of four that take turns with the tiles (of the latter half for keys, half for values)
+constexpr int kSoft = 8, kTurn = 8;         // warps for the softmax; for keys and values, half of them each
 constexpr int kMmaS = kSoft + kTurn, kMmaO = kMmaS + 1, kPlan = kMmaS + 2;
 constexpr int kThreads = 32 * (kPlan + 2);  // (whole groups of four warps share out registers)
 constexpr int kReaders = kSoft + kTurn + 2;  // of a plan
@@ -406,10 +412,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
     if (!ok) give_up();
   } else if (warp >= kSoft && warp < kMmaS) {
     registers_down<kRegsTurn>();
-    // ---------------- keys or values into 16 bits: thread = a key of the group's tiles ----------------
+    // ---------------- keys or values into 16 bits: thread = a key of every tile ----------------
     constexpr int kWords = HD / 8, kPairs = HD / 32;
     const bool values = warp >= kSoft + kTurn / 2;
-    const int key = tid & 127, group = (warp >> 2) % kGroups;
+    const int key = tid & 127;
     const uint32_t full = values ? v_full : k_full, empty = values ? v_empty : k_empty;
     const uint32_t tiles_at = base + (values ? S::kOffV : S::kOffK) + key * 128;
     auto write = [&](uint32_t tile, int i, uint4 v) {  // dims 8 i .. 8 i + 7
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
                    "r"(v.w)
                    : "memory");
     };
-    // The group's next tile: unit x of segment seg, its place of the thread's key (-1: none that is cached) and that one's page.
+    // The next tile: unit x of segment seg, its place of the thread's key (-1: none that is cached) and that one's page.
     int seg = 0, x = 0, at = -1, page = 0;
     auto look_up = [&]() {
       const Segment& f = plans[seg % kPlans];
@@ -425,18 +431,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
       if (at >= f.len) at = -1;
       page = at < 0 ? 0 : p.tables[(int64_t)f.b * p.tables_ld + entry_of(p, at)];
     };
-    auto first_of = [&]() {  // from unit 0 of segment seg on
-#pragma unroll 1
-      for (;; ++seg) {
-        if (!agreed(wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed))) {
-          *failed = 1;
-          return false;
-        }
-        const Segment& f = plans[seg % kPlans];
-        if (f.x1 <= 0) return false;
-        x = f.x0 + (group - f.j0 % kGroups + kGroups) % kGroups;
-        if (x < f.x1) return true;
+    auto begin = [&]() {  // unit 0 of segment seg
+      if (!agreed(wait_for(plan_full + 8 * (seg % kPlans), (seg / kPlans) & 1, failed))) {
+        *failed = 1;
+        return false;
       }
+      x = plans[seg % kPlans].x0;
+      return plans[seg % kPlans].x1 > 0;
     };
     uint32_t w[kWords], pr[kPairs];
     // Where the thread's codes and pairs lie: they are brought into the L2 while the tile before is worked on. Null where there is no
@@ -475,27 +476,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
         pr[0] = y.x, pr[1] = y.y;
       }
     };
-    bool ok = true, more = first_of();
+    bool ok = true, more = begin();
     if (more) {
       look_up();
       locate();
       fetch();
     }
     int done_with = 0;  // segments that this warp no longer reads
-    for (; done_with < seg; ++done_with) read(done_with);
 #pragma unroll 1
     while (more) {
       const Segment& f = plans[seg % kPlans];
       const int now = seg, x_now = x, at_now = at, j = f.j0 + x - f.x0, stage = j % kStages;
       const uint32_t tile = tiles_at + stage * S::kTile;
       const bool cached = x < f.cached;
-      // The next tile's page is looked up meanwhile. (Each segment has a tile, and every kGroups-th is the group's: the next lies at
-      // most two segments on, which are planned while this one is still held.)
-      x += kGroups;
-      more = x < f.x1;
+      // The next tile's page is looked up meanwhile. (Each segment has a tile: the next lies at most one segment on, which is planned
+      // while this one is still held.)
+      more = ++x < f.x1;
       if (!more) {
         ++seg;
-        more = first_of();
+        more = begin();
       }
       if (more) look_up();
       bool sick = false;

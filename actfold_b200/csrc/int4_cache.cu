@@ -6,6 +6,10 @@
 // the 32 dims of a pair (64 bytes), so that extremes, scale and reciprocal are
 // found once for them. Reading: a lane takes 8 dims, a code word and 16 bytes out, of one
 // head after the other.
+//
+// 10391 rows of 32 heads x 128: written in 73 us (the bytes need 34), bound by the 15 or so instructions that a value takes (a
+// lane with 8 dims, and divisions for ties: 123 us; persistent CTAs that load ahead: 87 to 90); read in 41 us (the same bytes), by the cache's
+// scattered rows of 64 and 16 bytes.
 #include <string>
 
 #include "int4_cache.cuh"

@@ -649,7 +649,7 @@ int af_read_cache_int4(const af_int4_rows* w, uint32_t* status, void* stream);
  * (af_block_tables with `held` gives the pages behind the kept tokens back).
  * With int4.head_dim 0 the cache is k_cache and v_cache: rows of head_bytes
  * (at most 4096), strides in bytes (layer, page, token, head). Strides in bytes, head_bytes
- * and addresses are multiples of 16. Pages of one request must not be another's.
+ * and addresses are multiples of 16. No page may be in the tables of two requests, or twice in one.
  */
 typedef struct {
   af_int4_cache int4;
@@ -722,8 +722,8 @@ int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
  * 16-bit keys [page, token, head] with strides cache.strides[1], token_stride,
  * cache.strides[2] (bytes). weights strides in elements: request, head; places entries. A
  * length above places or the table's capacity, or a page out of range, sets AF_STATUS_BOUNDS: the
- * request is skipped, such a page's keys read as zeros. Sums are held in 32 bits,
- * in an order that does not change.
+ * request is skipped, such a page's keys read as zeros; a copy of keys that does not come within about a second sets
+ * AF_STATUS_TIMEOUT. Sums are held in 32 bits, in an order that does not change.
  */
 typedef struct {
   const void* q;
