@@ -11,10 +11,10 @@
 // values, and with few segments 64 or 128 bytes of them, are CTAs of their own, and
 // with fewer still a cluster shares each step's rows.
 //
-// k_move is bound by HBM: every moved byte is read and written once. k_select is bound by latency: three passes over weights that
-// the L1 and L2 hold, and one in order, with a barrier for each 512 places.
-//   One request of 4100 tokens down to 2048, 28 layers of 4 heads x 128 in 4 bits: 37 us; the bytes need 35.
-//   16 requests of 900 to 4100 down to 1500, 6 layers of 4 heads x 128 in 16 bits: 122 us; the bytes need 74.
+// k_move is bound by HBM: every moved byte is read and written once. k_select is bound by latency: three passes over weights, of
+// which a thread holds the first eight in registers, and one in order, with a barrier for each 512 places (122 -> 113 us for the second).
+//   One request of 4100 tokens down to 2048, 28 layers of 4 heads x 128 in 4 bits: 36 us; the bytes need 12.
+//   16 requests of 900 to 4100 down to 1500, 6 layers of 4 heads x 128 in 16 bits: 113 us; the bytes need 74.
 // (Rows one by one instead of a warp's rows together 338 us for the second, a binary search for the threshold instead of
 // histograms 11 us more for the first and 25 for the second.)
 #include <string>
@@ -39,6 +39,7 @@ struct SelectArgs {
 };
 
 constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32, kBins = 2048, kOwn = kBins / kSelThreads;
+constexpr int kHeld = 8;  // places of a thread whose weights stay in registers
 
 // Ascending whole numbers for ascending weights; -0 equals 0, and NaN is above all numbers.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -73,6 +74,17 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
   }
   // The weights of places [lo, hi) decide; need of them stay (keep >= sinks + recent, t > keep: hi - lo > need).
   const int lo = a.sinks, hi = t - a.recent, need0 = a.keep - a.sinks - a.recent;
+  uint32_t held[kHeld];
+#pragma unroll
+  for (int c = 0; c < kHeld; ++c) held[c] = c * kSelThreads + tid < t ? order_of(w[c * kSelThreads + tid]) : 0;
+  // f(place, order of its weight) for the thread's places, and some behind the last token.
+  auto for_places = [&](auto f) {
+#pragma unroll
+    for (int c = 0; c < kHeld; ++c)
+      if (c * kSelThreads < t) f(c * kSelThreads + tid, held[c]);
+#pragma unroll 4
+    for (int i0 = kHeld * kSelThreads; i0 < t; i0 += kSelThreads) f(i0 + tid, i0 + tid < t ? order_of(w[i0 + tid]) : 0u);
+  };
   uint32_t prefix = 0;
   int need = need0;
   if (need0 > 0) {
@@ -83,11 +95,9 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
 #pragma unroll
       for (int i = 0; i < kOwn; ++i) s_hist[tid + i * kSelThreads] = 0;
       __syncthreads();
-#pragma unroll 4
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t k = order_of(w[i]);
-        if (pass == 0 || k >> above == prefix >> above) atomicAdd(&s_hist[(k >> shift) & mask], 1);
-      }
+      for_places([&](int i, uint32_t k) {
+        if (i >= lo && i < hi && (pass == 0 || k >> above == prefix >> above)) atomicAdd(&s_hist[(k >> shift) & mask], 1);
+      });
       __syncthreads();
       // Thread x has kOwn bins, from 2047 - kOwn x on downwards; from the top down, the one in which the need-th token lies.
       int c[kOwn], upto = 0;
@@ -118,13 +128,9 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
   }
   // Tokens above `prefix` stay, and the first `need` of those that equal it. In order: the number of certain ones and of equal
   // ones before each, both in one word (a chunk has fewer than 2^16 places).
-  int certain = 0, equal = 0;
-#pragma unroll 1
-  for (int i0 = 0, turn = 0; i0 < t; i0 += kSelThreads, turn ^= 1) {
-    const int i = i0 + tid;
-    const float x = i < t ? w[i] : 0.f;
+  int certain = 0, equal = 0, turn = 0;
+  for_places([&](int i, uint32_t k) {
     const bool middle = i >= lo && i < hi;
-    const uint32_t k = order_of(x);
     const bool sure = i < t && (!middle || (need0 > 0 && k > prefix)), tie = middle && need0 > 0 && k == prefix;
     const uint32_t sures = __ballot_sync(0xffffffffu, sure), ties = __ballot_sync(0xffffffffu, tie);
     if (lane == 0) s_sum[turn][warp] = __popc(sures) | __popc(ties) << 16;
@@ -136,11 +142,12 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
     if (sure || (tie && tie_at < need)) {
       const int at = sure_at + min(tie_at, need);
       kept[at] = i;
-      out[at] = x;
+      out[at] = w[i];
     }
     certain += total & 0xffff;
     equal += total >> 16;
-  }
+    turn ^= 1;
+  });
   for (int i = a.keep + tid; i < a.places; i += kSelThreads) out[i] = 0.f;
 }
 
@@ -202,13 +209,10 @@ __global__ void __launch_bounds__(kMoveThreads) k_move(const MoveArgs a) {
   // Rows before the first gap stay where they are: kept[r] - r never falls.
   int first = 0;
   for (int n = a.keep; n > 0;) {
-    const int half = n / 2;
-    if (kept[first + half] == first + half) {
-      first += half + 1;
-      n -= half + 1;
-    } else {
-      n = half;
-    }
+    const int step = (n + 31) / 32, at = lane * step;
+    const int stay = __popc(__ballot_sync(0xffffffffu, at < n && kept[first + min(at, n - 1)] == first + at));
+    first += stay ? (stay - 1) * step + 1 : 0;
+    n = stay ? min(step - 1, n - (stay - 1) * step - 1) : 0;
   }
   const int step_rows = CLUSTER * kMoveWarps * a.rows;
   const int steps = (a.keep - first + step_rows - 1) / step_rows;
