@@ -45,10 +45,11 @@ class Int4Cache:
     ``data`` is uint8 [pages, kv_heads, page_size / 8, 10 * dim], or with a leading dimension of layers, dim 64 or 128; ``dtype``
     (fp16 or bf16) is that of the rows that go in and come out, and of the scales and offsets. Its last two dimensions are
     contiguous, its other strides multiples of 16 bytes. :meth:`empty` makes one; ``cache[l]`` is layer l. The pages hold what
-    :func:`write_cache_int4` wrote; places that were never written are never used.
+    :func:`write_cache_int4` wrote; places that were never written are never used. A cache stays with the memory that it
+    was made with: for another tensor make another one.
     """
 
-    __slots__ = ("_data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
+    __slots__ = ("data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
 
     def __init__(self, data: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> None:
         shape = data.shape
@@ -82,14 +83,9 @@ class Int4Cache:
         at = data.data_ptr()
         if (sl | sp | sh | at) & 15:
             raise ValueError("Int4Cache: data's address and strides must be multiples of 16 bytes")
-        self._data, self.dtype, self.dim, self.layers, self.pages, self.kv_heads = data, dtype, size // 10, layers, pages, heads
+        self.data, self.dtype, self.dim, self.layers, self.pages, self.kv_heads = data, dtype, size // 10, layers, pages, heads
         self.page_size = page = 8 * blocks
         self._packed = (at, sl, sp, sh, 1 if layers is None else layers, pages, page, heads, size // 10, _lib.DTYPE[dtype])
-
-    @property
-    def data(self) -> torch.Tensor:
-        """The cache's memory. (A cache in other memory is another one.)"""
-        return self._data
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, dtype: torch.dtype = torch.bfloat16, layers: int | None = None,
@@ -103,7 +99,7 @@ class Int4Cache:
     def __getitem__(self, layer: int) -> "Int4Cache":
         if self.layers is None:
             raise ValueError("Int4Cache: the cache has no layers")
-        return Int4Cache(self._data[layer], self.dtype)
+        return Int4Cache(self.data[layer], self.dtype)
 
 
 class EvictedCache(NamedTuple):
@@ -141,7 +137,7 @@ def write_cache_int4(
     """
     layered = cache.layers is not None
     if v.shape != k.shape or k.dim() != (4 if layered else 3) or k.shape[-2:] != (cache.kv_heads, cache.dim) or (layered and k.shape[0] != cache.layers):
-        raise ValueError(f"write_cache_int4: k, v {tuple(k.shape)}, {tuple(v.shape)} do not match a cache {tuple(cache._data.shape)}")
+        raise ValueError(f"write_cache_int4: k, v {tuple(k.shape)}, {tuple(v.shape)} do not match a cache {tuple(cache.data.shape)}")
     if k.dtype is not cache.dtype or v.dtype is not cache.dtype:
         raise ValueError(f"write_cache_int4: rows {k.dtype}, {v.dtype} differ from the cache's {cache.dtype}")
     if slots.dtype is not _I64 or (rows is not None and (rows.dtype is not _I32 or rows.shape != slots.shape)):
@@ -151,7 +147,7 @@ def write_cache_int4(
     n, count = k.shape[1], slots.numel()
     if rows is None and count > n:
         raise ValueError(f"write_cache_int4: {count} slots for {n} rows")
-    index = _same_device("write_cache_int4", k, v, cache._data, slots, rows, word := _word(status))
+    index = _same_device("write_cache_int4", k, v, cache.data, slots, rows, word := _word(status))
     if (ks := _row_strides(k)) is None:
         k = k.clone(memory_format=torch.contiguous_format)
         ks = _row_strides(k)
@@ -173,7 +169,7 @@ def read_cache_int4(
     """Keys and values [(layers,) *slots.shape, kv_heads, dim] of the cache's dtype that lie in ``slots`` (int64; negative ones read as 0)."""
     if slots.dtype is not _I64:
         raise ValueError(f"read_cache_int4: slots must be int64, got {slots.dtype}")
-    index = _same_device("read_cache_int4", cache._data, slots, word := _word(status))
+    index = _same_device("read_cache_int4", cache.data, slots, word := _word(status))
     slots = slots.contiguous()
     shape = (*slots.shape, cache.kv_heads, cache.dim) if cache.layers is None else (cache.layers, *slots.shape, cache.kv_heads, cache.dim)
     k = torch.empty(shape, dtype=cache.dtype, device=slots.device)
@@ -240,10 +236,10 @@ def evict_cache(
                 raise ValueError("evict_cache: the caches' rows and strides must be multiples of 16 bytes")
             strides += st
         held = (k_cache, v_cache)
-        parts = (*_NO_CACHE, k_cache._data_ptr(), v_cache._data_ptr(), *strides, layers, pages, page, heads, dim * e)
+        parts = (*_NO_CACHE, k_cache.data_ptr(), v_cache.data_ptr(), *strides, layers, pages, page, heads, dim * e)
     else:
         layered, layers, heads = cache.layers is not None, 1 if cache.layers is None else cache.layers, cache.kv_heads
-        held = (cache._data, None)
+        held = (cache.data, None)
         parts = (*cache._packed, *((0,) * 15))
     n, most = _check_tables("evict_cache", tables, lengths)
     if weights.dtype is not torch.float32 or weights.dim() != (4 if layered else 3) or weights.shape[-3:-1] != (n, heads) \
@@ -321,7 +317,7 @@ def tree_attention_int4(
         raise ValueError("tree_attention_int4: cache must be one layer (cache[l])")
     qs, ks = q.shape, k.shape
     if len(qs) != 3 or len(ks) != 3 or v.shape != ks or ks[0] != qs[0] or ks[1] != cache.kv_heads or ks[2] != cache.dim or qs[2] != cache.dim:
-        raise ValueError(f"tree_attention_int4: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} and cache {tuple(cache._data.shape)} do not match")
+        raise ValueError(f"tree_attention_int4: q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)} and cache {tuple(cache.data.shape)} do not match")
     total, heads, dim = qs
     dtype = cache.dtype
     if q.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype:
@@ -347,7 +343,7 @@ def tree_attention_int4(
         raise ValueError("tree_attention_int4: out must have q's shape and dtype, a contiguous innermost dimension and 16-byte strides")
     if lse is not None and (lse.shape != (total, heads) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
         raise ValueError(f"tree_attention_int4: lse must be contiguous float32 [{total}, {heads}]")
-    index = _same_device("tree_attention_int4", q, k, v, cache._data, tables, lengths, starts, mask, out, lse, word := _word(status))
+    index = _same_device("tree_attention_int4", q, k, v, cache.data, tables, lengths, starts, mask, out, lse, word := _word(status))
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts = lengths.contiguous(), starts.contiguous()
@@ -397,7 +393,7 @@ def attention_weights(
     if packed:
         if cache.layers is not None:
             raise ValueError("attention_weights: cache must be one layer (cache[l])")
-        keys, dtype, kv, dim, parts, token = cache._data, cache.dtype, cache.kv_heads, cache.dim, cache._packed, 0
+        keys, dtype, kv, dim, parts, token = cache.data, cache.dtype, cache.kv_heads, cache.dim, cache._packed, 0
     else:
         if cache.dim() != 4 or cache.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"attention_weights: cache must be an Int4Cache or 16-bit [pages, page_size, kv_heads, dim], got {cache.dtype} {tuple(cache.shape)}")
@@ -407,7 +403,7 @@ def attention_weights(
         if (grid := _grid(cache)) is None:
             raise ValueError("attention_weights: the cache's innermost dimension must be contiguous, its other strides multiples of 16 bytes")
         keys, dtype = cache, cache.dtype
-        parts, token = (cache._data_ptr(), 0, grid[0], grid[2], 1, pages, page, kv, dim, _lib.DTYPE[dtype]), grid[1]
+        parts, token = (cache.data_ptr(), 0, grid[0], grid[2], 1, pages, page, kv, dim, _lib.DTYPE[dtype]), grid[1]
     qs = q.shape
     total, heads = (qs[0], qs[1]) if len(qs) == 3 else (0, 0)
     if heads == 0 or q.dtype is not dtype or qs[2] != dim or heads % kv:

@@ -305,8 +305,9 @@ cudaError_t launch_move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
   return launch_ex(k_move<HD, CLUSTER>, dim3((unsigned)(segments * a.columns * CLUSTER)), dim3(kMoveThreads), (size_t)bytes, s, true, dim3(CLUSTER), a);
 }
 
-// A CTA holds some 60 to 115 KB: two or three fit an SM. Clusters as long as all of their CTAs do at once. (One request over 28
-// layers, 224 columns: 37 us in pairs, 38 without.)
+// A CTA holds some 40 to 115 KB: two or three fit an SM. Clusters as long as all of their CTAs do at once. One request of 4100 tokens
+// down to 2048, 4 heads x 128 in 4 bits, by clusters of 1, 2, 4 and 8: one layer 28, 23, 19 and 16 us, 14 layers 32, 29, 31 and 35,
+// 28 layers 36, 46, 48 and 55.
 template <int HD>
 cudaError_t move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
   const int64_t ctas = segments * a.columns, room = 3 * sm_count();

@@ -78,8 +78,6 @@ def test_cache_refusals():
     c = S.Int4Cache.empty(4, 24, 3, 128, HF, layers=2, device="cpu")
     assert (c.layers, c.pages, c.page_size, c.kv_heads, c.dim, c.dtype) == (2, 4, 24, 3, 128, HF) and c[1].layers is None
     assert c[1].data.data_ptr() == c.data.data_ptr() + 4 * 3 * 3 * 1280
-    with pytest.raises(AttributeError):
-        c.data = c.data.clone()  # the calls would go on using the memory that it was made with
 
 
 def test_row_refusals():
