@@ -21,7 +21,8 @@
 //   4 trees of 48 to 64 nodes, 28 heads over 4, 30 to 65 K keys: 2204 us with that kernel, 259 now; its products need 107.
 // Tried: keys and values one after the other in eight warps (114 us instead of 105 at that time: a tile's keys waited for the
 // products with the values two tiles before); 16 turning warps with 72 registers, more registers for the issue warps or the turning
-// ones, the codes a tile ahead in shared memory (the long trees 259 -> 274 us), halves of S with one row tile too (96 -> 99): slower.
+// ones, the codes a tile ahead in shared memory (the long trees 259 -> 274 us) or half a tile ahead in registers (the first 93 -> 105), halves of S
+// with one row tile too (96 -> 99): slower.
 //
 // Warps 0-3 and 4-7: softmax of pipe 0 and 1, and Q; 8-11: keys; 12-15: values; 16 issues S, 17 O, 18 plans, 19 is idle.
 #include "int4_attention.cuh"
