@@ -113,6 +113,9 @@ __device__ __forceinline__ uint4 encode(const uint4* x, uint32_t& pair) {
   constexpr uint32_t magic_bits = 0x4b400000u;
   const float inv = 1.f / scale;
   const bool usual = inv <= 3.402823466e38f && range <= 15.25f * scale;  // else the scale has lost its precision, and codes may pass 15
+  // Differences lose nothing of an offset that is 0 or not far below them: its last bit is worth 2^-10 of it or more, that of x - offset 2^-23
+  // of the range at most.
+  const bool near = low == 0.f || fabsf(low) >= range * (1.f / 8192.f);
   auto shift = [](int c) { return 4 * (c >> 1) + 16 * (c & 1); };
   uint32_t out[4];
 #pragma unroll
@@ -130,12 +133,12 @@ __device__ __forceinline__ uint4 encode(const uint4* x, uint32_t& pair) {
     if (!usual) {
       word = careful_word<DT>(x[i], low, scale);
     } else if (off >= half) {
-      bool sure = true;
+      bool sure = near;
       word = 0;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const float y = value(c), d = y - low, t = fmaf(d, inv, magic), r = fmaf(magic - t, scale, d);
-        sure &= low + d == y;  // (a tie is none where the difference has lost something in fp32)
+        sure &= low + d == y;  // (a tie is none where the difference has lost something in fp32: here of y)
         const uint32_t step = __float_as_int(fabsf(r)) + (__float_as_int(t) & 1) > __float_as_int(half) ? 1u | (__float_as_int(r) >> 31) : 0u;
         word += (__float_as_uint(t) - magic_bits + step) << shift(c);
       }
