@@ -306,7 +306,9 @@ def tree_attention_int4(
     sees the nodes whose bits are set in ``mask[i]`` ([nodes, words] int32), without a mask the nodes of its chain up to itself.
 
     With a ``window`` a node that sees c nodes (itself among them) sees the last ``window - c`` tokens of the prefix (none where
-    that is negative) and the prefix's first ``sinks`` tokens; in a chain, which has no mask, it sees the last ``window`` nodes.
+    that is negative) and the prefix's first ``sinks`` tokens. A chain, which has no mask, goes on where the prefix ends: a node sees
+    the last ``window`` tokens of prefix and chain, itself among them, and the request's first ``sinks`` tokens, of which the chain holds
+    those that the prefix does not; so a prompt may be cut anywhere.
     Nodes that a mask shows stay visible whatever the window. Only pages with visible tokens are read.
 
     ``scale`` defaults to dim ** -0.5. A row that sees nothing is 0. ``lse`` [nodes, heads] float32 receives the natural log of

@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(32 * (W + 1), CTAS) k_int4_attention(const __g
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              bits[nt][e] = seen_nodes(p, s.s0, s.n, node[nt][e], j0);
+              bits[nt][e] = seen_nodes(p, s.s0, s.n, s.len, node[nt][e], j0);
               any |= bits[nt][e];
             }
           if (__any_sync(0xffffffffu, any != 0)) {  // (most units of a long chain are seen by no row of the tile)

@@ -256,11 +256,12 @@ __device__ __forceinline__ float from_bits(uint32_t bits) {
   return load_scalar<DT>(reinterpret_cast<const char*>(&b), 0);
 }
 
-// Nodes j0 .. j0 + 31 of the tree (n nodes from s0 on) that node i sees, as bits. j0 is a multiple of 32.
-__device__ __forceinline__ uint32_t seen_nodes(const Params& p, int s0, int n, int i, int j0) {
+// Nodes j0 .. j0 + 31 of the tree (n nodes from s0 on, behind len cached tokens) that node i sees, as bits. j0 is a multiple of 32.
+// A chain goes on where the cache ends: the first `sinks` tokens stay visible wherever they lie.
+__device__ __forceinline__ uint32_t seen_nodes(const Params& p, int s0, int n, int len, int i, int j0) {
   auto below = [](int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; };
   if (p.mask) return p.mask[(int64_t)(s0 + i) * p.mask_ld + (j0 >> 5)] & below(n - j0);
-  return below(i + 1 - j0) & (p.window ? ~below(i + 1 - p.window - j0) : 0xffffffffu);
+  return below(i + 1 - j0) & (p.window ? ~below(i + 1 - p.window - j0) | below(p.sinks - len - j0) : 0xffffffffu);
 }
 
 // The first place behind the sinks that node i sees: its window holds the nodes that it sees, and then the last tokens of the prefix.
@@ -270,7 +271,7 @@ __device__ __forceinline__ int first_place(const Params& p, int s0, int n, int l
   if (p.mask) {
     count = 0;
 #pragma unroll 1
-    for (int j = 0; j < n && count < p.window; j += 32) count += __popc(seen_nodes(p, s0, n, i, j));
+    for (int j = 0; j < n && count < p.window; j += 32) count += __popc(seen_nodes(p, s0, n, len, i, j));
   }
   return max(0, len - max(0, p.window - count));
 }

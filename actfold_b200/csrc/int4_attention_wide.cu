@@ -216,7 +216,7 @@ __device__ __noinline__ void set_aside(const Params& p, const Segment* plan, uin
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               v[u][h] = j + u < end ? *reinterpret_cast<const uint4*>(from + (int64_t)(j + u) * p.v_n + 16 * h) : make_uint4(0, 0, 0, 0);
-          const uint32_t seen = seen_nodes(p, s.s0, s.n, i, j & ~31) >> (j & 31);
+          const uint32_t seen = seen_nodes(p, s.s0, s.n, s.len, i, j & ~31) >> (j & 31);
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             if ((seen >> u) & 1u) {
@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_int4_attention_wide(const __gri
             for (int c = 0; c < 2; ++c) {
               const int k = key0 + 32 * c;
               if (cached) vis[c] = below(s.len - k) & (~below(first - k) | below(p.sinks - k));
-              else vis[c] = r < rows && k < s.n ? seen_nodes(p, s.s0, s.n, node, k) : 0u;
+              else vis[c] = r < rows && k < s.n ? seen_nodes(p, s.s0, s.n, s.len, node, k) : 0u;
             }
           }
           constexpr int C = kUnit / 2;

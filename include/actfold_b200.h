@@ -680,7 +680,9 @@ int af_evict_cache(const af_evict_args* a, uint32_t* status, void* stream);
  * n_heads / cache.heads. window 0: a node sees all of the prefix. Else it
  * sees the last max(0, window - c) tokens of the prefix, where c counts the
  * nodes that it sees (itself among them), and the prefix's first `sinks`
- * tokens; without a mask only the last `window` nodes of its chain. Nodes
+ * tokens. Without a mask a node is the request's token lengths[b] + i, and sees
+ * the last `window` nodes of its chain (c of them) and the nodes among the request's
+ * first `sinks` tokens, so that a prompt may be cut anywhere. Nodes
  * that a mask shows stay visible whatever the window. Values that a row
  * does not see have no influence on it. workspace:
  * af_tree_attention_int4_workspace_bytes() bytes, not shared by calls that

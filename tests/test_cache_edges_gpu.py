@@ -2,12 +2,14 @@
 
 from __future__ import annotations
 
+import math
 from fractions import Fraction
 
 import pytest
 import torch
 
 import cache_util as U
+from test_cache_kernels_gpu import KINDS, _attention_case, _check_attention, _i32
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +54,69 @@ def test_codes_of_ties_beside_a_tiny_minimum(dtype, dim):
         for i in range(n):
             U.put(want, i, part, codes[i], scales[i], offsets[i])
     assert torch.equal(cache.data, want), (cache.data != want).nonzero()[:8]
+
+
+# ------------------------------------------------------------------------------------------------ chains behind a window
+def _seen_in_chain(n, t, bits, window, sinks):
+    """[n, t + n]: a chain goes on where the cache ends, so the token at place t + i sees its last `window` places and the first `sinks`."""
+    if bits is not None:
+        return PREFIX_ONLY(n, t, bits, window, sinks)
+    place, at = torch.arange(t + n)[None], t + torch.arange(n)[:, None]
+    return (place <= at) & ((place > at - window) | (place < sinks) if window else True)
+
+
+PREFIX_ONLY = U.visible
+
+
+@pytest.mark.parametrize("window,sinks", [(4, 2), (1, 1), (16, 40), (33, 5), (20, 300)])
+@pytest.mark.parametrize("dim,dtype", [(64, HF), (128, BF)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_first_tokens_of_a_chain_stay_visible(monkeypatch, kind, dim, dtype, window, sinks):
+    """An empty prefix, one shorter than the first tokens, one longer: all of the request's first tokens stay, wherever they lie."""
+    monkeypatch.setattr(U, "visible", _seen_in_chain)
+    for ls in ([0, 3, 130], [1, 0, 0], [35, 260, 2]):
+        a, starts, bits = _attention_case(ls=ls, dim=dim, page=16, dtype=dtype, tree=False, seed=window + sinks, **KINDS[kind])
+        _check_attention(a, ls, starts, bits, window, sinks)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_first_tokens_of_a_long_chain(monkeypatch, kind):
+    """Rows far behind the first tokens, and values that are not finite among those and among tokens that only some windows hold."""
+    monkeypatch.setattr(U, "visible", _seen_in_chain)
+    shape = dict(KINDS[kind], ns=[{"8": 4, "16": 8, "128": 64, "256": 200}[kind]] * 8 + [300])
+    ls = [0, 1, 5, 64, 300, 0, 0, 2, 0]
+    a, starts, bits = _attention_case(ls=ls, dim=128, page=8, dtype=BF, tree=False, seed=9, **shape)
+    _check_attention(a, ls, starts, bits, 70, 6)
+    for node, x in ((2, math.inf), (100, math.nan), (150, -math.inf)):
+        a["v"][starts[-2] + node, 1, 17 + node % 3] = x
+    a["k"][starts[-2] + 4, 1, 3] = math.nan
+    out = _check_attention(a, ls, starts, bits, 70, 3)
+    assert out[starts[-2]:].isnan().any() and torch.isfinite(out[:, : shape["heads"] // 2]).all()
+
+
+def test_a_prompt_may_be_cut_anywhere():
+    """A chain in one call gives what it gives in pieces, each behind the rows that the cache holds of the pieces before."""
+    from actfold_b200.speculative import Int4Cache, read_cache_int4, tree_attention_int4, write_cache_int4
+
+    n, heads, kv, dim, window, sinks = 60, 4, 2, 64, 9, 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g).to(BF)
+    cache = Int4Cache.empty(9, 8, kv, dim, BF)
+    slots = torch.arange(n, device="cuda")
+    write_cache_int4(rand(n, kv, dim), rand(n, kv, dim), cache, slots)
+    k, v = read_cache_int4(cache, slots)  # rows that 4 bits hold exactly: the same keys, cached or not
+    q, tables = rand(n, heads, dim), _i32([list(range(9))])
+    at = 0
+    whole = tree_attention_int4(q, k, v, cache, tables, _i32([0]), _i32([0, n]), window=window, sinks=sinks)
+    see = _seen_in_chain(n, 0, None, window, sinks).cuda()
+    for h in range(heads):
+        s = torch.where(see, q[:, h].double() @ k[:, h // 2].double().T * dim ** -0.5, -math.inf)
+        w = torch.softmax(s, 1)
+        # Probabilities and results rounded to 8 bits: half a step each, and a hair for fp32 (see U.attention).
+        tol = 2.0 ** -8 * (w @ v[:, h // 2].double().abs()) * 1.01 + 2.0 ** -8 * (w @ v[:, h // 2].double()).abs()
+        assert bool(((whole[:, h].double() - w @ v[:, h // 2].double()).abs() <= tol).all())
+    for end in (3, 4, 11, 40, n):
+        part = tree_attention_int4(q[at:end], k[at:end], v[at:end], cache, tables, _i32([at]), _i32([0, end - at]), window=window, sinks=sinks)
+        # Both lie within 2^-7 of the largest value, by the same bound.
+        assert bool(((part.double() - whole[at:end].double()).abs() <= 2.0 ** -6 * v.double().abs().max()).all())
+        at = end
