@@ -301,7 +301,10 @@ def _own(s):
         return {"k": k, "v": v}
     if s["op"] == "attention":
         cache = spec.Int4Cache(s["data"], s["dtype"])
-        return {"out": spec.tree_attention_int4(s["q"], s["k"], s["v"], cache, s["tables"], s["lengths"], s["starts"], s["mask"],
+        mask = s["mask"]
+        if mask is None and s["sinks"] and s["window"] < s["most_nodes"]:
+            mask = _last_nodes(s)  # the first tokens that stay are the prefix's here; without bits a chain's own first ones would stay too
+        return {"out": spec.tree_attention_int4(s["q"], s["k"], s["v"], cache, s["tables"], s["lengths"], s["starts"], mask,
                                                 window=s["window"], sinks=s["sinks"])}
     if s["op"] == "weights":
         cache = spec.Int4Cache(s["data"], s["dtype"]) if s["held"] == 4 else s["k_cache"]
@@ -313,6 +316,16 @@ def _own(s):
         return {"kept": r.kept, "lengths": r.lengths, "weights": r.weights, "k": s["k_cache"], "v": s["v_cache"]}
     k, v = spec.read_cache_int4(cache, _kept_slots(s))
     return {"kept": r.kept, "lengths": r.lengths, "weights": r.weights, "k": k, "v": v}
+
+
+def _last_nodes(s):
+    """Bits of the last `window` nodes of its chain for every node."""
+    starts, total = s["starts"].long(), s["q"].shape[0]
+    i = torch.arange(total, device=DEV) - starts[:-1].repeat_interleave(starts[1:] - starts[:-1], output_size=total)
+    j = torch.arange(32 * _pages(s["most_nodes"], 32), device=DEV)
+    sees = (j <= i[:, None]) & (j > i[:, None] - s["window"])
+    bits = (sees.view(total, -1, 32).long() << torch.arange(32, device=DEV)).sum(-1)
+    return torch.where(bits >= 2 ** 31, bits - 2 ** 32, bits).to(torch.int32)
 
 
 def _kept_slots(s):
