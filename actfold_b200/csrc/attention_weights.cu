@@ -14,6 +14,7 @@
 // Tried: rows from global memory for each unit (137 us), keys looked up and loaded unit by unit (70); four chains of products
 // (53), 16 keys at a time with two or three CTAs an SM (54, 56), shares by rows as well as units (53 to 59): slower.
 #include <string>
+#include <type_traits>
 
 #include "int4_attention.cuh"
 
@@ -21,6 +22,10 @@ namespace af {
 namespace kv4 {
 namespace {
 
+// -lse of a row that gives nothing: one behind the last, or whose lse is -inf. It is added as 2^-kNothing = 0, but what
+// a key that is not finite makes of that is not: units whose sums are not finite are added up once more without such rows (to leave
+// them out at once takes 53 us instead of 51 for the 64 requests).
+constexpr float kNothing = -3.402823466e38f;
 constexpr int kUnit = 32, kThreads = 256, kCtas = 2, kRows = 64;  // keys of a unit; CTAs per SM; rows in shared memory at once
 
 struct WeightArgs {
@@ -61,7 +66,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
   constexpr int W = kThreads / 32, KS = HD / 16;
   __shared__ int s_share[4];  // first unit, the one behind the last; the request that the share begins with, and the units before it
   __shared__ __align__(16) uint4 s_q[kRows * (HD / 8)];
-  __shared__ float s_sum[kRows];  // -lse in log2 units; -inf where there is no row
+  __shared__ float s_sum[kRows];  // -lse in log2 units, or kNothing
   __shared__ int s_first[kRows];  // first place of the row's window
   __shared__ __align__(8) uint64_t s_full[2 * W];
   extern __shared__ __align__(128) uint8_t ring[];
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
       if (tid < tiles * 8) {
         const int flat = row0 + tid, node = flat / p.group;
         const float lse = tid < count ? a.lse[(int64_t)(r.s0 + node) * p.heads + h * p.group + flat % p.group] : -INFINITY;
-        s_sum[tid] = lse == -INFINITY ? -INFINITY : lse * -1.4426950408889634f;
+        s_sum[tid] = lse == -INFINITY ? kNothing : lse * -1.4426950408889634f;
         s_first[tid] = p.window ? max(0, r.len - max(0, p.window - (node + 1))) : 0;
       }
       __syncthreads();
@@ -242,41 +247,51 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
             }
           }
         if (bad && p.status) atomicOr(p.status, AF_STATUS_BOUNDS);
-        float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // [half][block]
+        float sum[2][2];  // [half][block]
         const uint4* q_even = s_q + g * (HD / 8) + t + 4 * (g & 1);  // pieces 4 i + t, those of odd rows exchanged
         const uint4* q_odd = s_q + g * (HD / 8) + t + 4 - 4 * (g & 1);
+        // careful: row by row, which rows see a key, and which give anything.
+        auto add_up = [&](auto careful) {
+          sum[0][0] = sum[0][1] = sum[1][0] = sum[1][1] = 0.f;
 #pragma unroll 1
-        for (int tile = 0; tile < tiles; ++tile) {
-          float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          for (int tile = 0; tile < tiles; ++tile) {
+            float c[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-          for (int i = 0; i < KS / 2; ++i) {
-            const uint4 v = (i & 1 ? q_odd : q_even)[tile * HD + 4 * (i & 2)];
+            for (int i = 0; i < KS / 2; ++i) {
+              const uint4 v = (i & 1 ? q_odd : q_even)[tile * HD + 4 * (i & 2)];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              mma<DT>(c[half], k[half][2 * i], v.x, v.y);
-              mma<DT>(c[half], k[half][2 * i + 1], v.z, v.w);
+              for (int half = 0; half < 2; ++half) {
+                mma<DT>(c[half], k[half][2 * i], v.x, v.y);
+                mma<DT>(c[half], k[half][2 * i + 1], v.z, v.w);
+              }
+            }
+            const float2 less = *reinterpret_cast<const float2*>(s_sum + 8 * tile + 2 * t);
+            if constexpr (decltype(careful)::value) {
+              const int2 first = *reinterpret_cast<const int2*>(s_first + 8 * tile + 2 * t);
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  const int at = place + 16 * half + 8 * y + kap;
+                  const bool in = at < r.len, sink = at < p.sinks;
+                  if (in && less.x != kNothing && (sink || at >= first.x)) sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x));
+                  if (in && less.y != kNothing && (sink || at >= first.y)) sum[half][y] += ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
+                }
+            } else {
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+                  sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x)) + ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
             }
           }
-          const float2 less = *reinterpret_cast<const float2*>(s_sum + 8 * tile + 2 * t);
-          if (masked) {
-            const int2 first = *reinterpret_cast<const int2*>(s_first + 8 * tile + 2 * t);
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const int at = place + 16 * half + 8 * y + kap;
-                const bool in = at < r.len, sink = at < p.sinks;
-                if (in && (sink || at >= first.x)) sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x));
-                if (in && (sink || at >= first.y)) sum[half][y] += ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
-              }
-          } else {
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-                sum[half][y] += ex2(fmaf(c[half][2 * y], p.scale, less.x)) + ex2(fmaf(c[half][2 * y + 1], p.scale, less.y));
-          }
+        };
+        bool again = masked;
+        if (!masked) {
+          add_up(std::false_type{});
+          again = !__all_sync(0xffffffffu, sum[0][0] + sum[0][1] + sum[1][0] + sum[1][1] < INFINITY);
         }
+        if (again) add_up(std::true_type{});
         float given = 0.f;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {

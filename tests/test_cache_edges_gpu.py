@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import cache_util as U
-from test_cache_kernels_gpu import KINDS, _attention_case, _check_attention, _i32
+from test_cache_kernels_gpu import KINDS, _attention_case, _check_attention, _i32, _i64
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +120,58 @@ def test_a_prompt_may_be_cut_anywhere():
         # Both lie within 2^-7 of the largest value, by the same bound.
         assert bool(((part.double() - whole[at:end].double()).abs() <= 2.0 ** -6 * v.double().abs().max()).all())
         at = end
+
+
+# ------------------------------------------------------------------------------------------------ weights
+def _given(q, keys, lse, window, sinks):
+    """Sums over rows and heads of the group, of one request, in 64 bits; rows whose lse is -inf give nothing."""
+    n, heads, dim = q.shape
+    t, kv = keys.shape[:2]
+    out = torch.zeros(kv, t, dtype=torch.float64, device=q.device)
+    see = U.visible(n, t, None, window, sinks)[:, :t].to(q.device)
+    for h in range(heads):
+        x = (q[:, h, None].double() * keys[None, :, h * kv // heads].double()).sum(-1) * dim ** -0.5 - lse[:, h, None].double()
+        out[h * kv // heads] += torch.where(see & (lse[:, h, None] != -math.inf), torch.exp(x), 0.0).sum(0)
+    return out
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (30, 2)])
+@pytest.mark.parametrize("n,heads,kv", [(1, 7, 1), (1, 8, 1), (3, 4, 2), (13, 10, 2), (16, 8, 2)])
+@pytest.mark.parametrize("dim,dtype", [(64, HF), (128, BF)])
+def test_weights_of_keys_that_are_infinite(dim, dtype, n, heads, kv, window, sinks):
+    """An infinite key gives what its scores say (0, an infinity or NaN), however many rows there are; rows without weight give nothing to any."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import Int4Cache, attention_weights, read_cache_int4, write_cache_int4
+
+    t, page = 75, 16
+    g = torch.Generator(device="cuda").manual_seed(n * heads)
+    q = torch.randn(n, heads, dim, device="cuda", generator=g).abs().to(dtype)  # all positive: an infinite key's score is its infinity
+    cache = Int4Cache.empty(6, page, kv, dim, dtype)
+    keys = torch.randn(96, kv, dim, device="cuda", generator=g).to(dtype)
+    write_cache_int4(keys, keys, cache, torch.arange(96, device="cuda"))
+    keys = read_cache_int4(cache, torch.arange(96, device="cuda"))[0]
+    nan = keys[:1].clone()
+    nan[0, 0, 5] = math.nan
+    write_cache_int4(nan, nan, cache, _i64([50]))
+    held = read_cache_int4(cache, torch.arange(96, device="cuda"))[0]
+    keys[1, 0, 3] = -math.inf
+    keys[20, 0, 9] = math.inf
+    keys[50, 0, 5] = math.nan
+    keys[60, kv - 1, 0] = -math.inf
+    keys[74, 0, 1], keys[74, 0, 2] = math.inf, -math.inf
+    lse = torch.full((n, heads), 3.0, device="cuda") + torch.rand(n, heads, device="cuda", generator=g)
+    st = DeviceStatus()
+    for none in (False, True):
+        if none:  # every other row, then all rows of a group
+            lse[::2] = -math.inf
+            lse[:, : heads // kv] = -math.inf
+        for c, k in ((keys.view(6, page, kv, dim), keys), (cache, held)):
+            w = attention_weights(q, c, _i32([list(range(6))]), _i32([t]), _i32([0, n]), lse, torch.zeros(1, kv, t, device="cuda"), window=window,
+                                  sinks=sinks, status=st)
+            st.check_status()
+            want = _given(q, k[:t], lse, window or 0, sinks)
+            # dim products in fp32 and an exponential of up to 2^6: 2^-23 (dim + 2^4) 2^6 relative, times e for the shift.
+            near = (w[0].double() - want).abs() <= 2.0 ** -12 * want.abs()
+            assert bool((near | (w[0] == want) | (w[0].isnan() & want.isnan())).all()), (w[0], want)
+            if none:
+                assert not w[0, 0].any()
