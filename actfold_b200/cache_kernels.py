@@ -45,11 +45,11 @@ class Int4Cache:
     ``data`` is uint8 [pages, kv_heads, page_size / 8, 10 * dim], or with a leading dimension of layers, dim 64 or 128; ``dtype``
     (fp16 or bf16) is that of the rows that go in and come out, and of the scales and offsets. Its last two dimensions are
     contiguous, its other strides multiples of 16 bytes. :meth:`empty` makes one; ``cache[l]`` is layer l. The pages hold what
-    :func:`write_cache_int4` wrote; places that were never written are never used. A cache stays with the memory that it
-    was made with: for another tensor make another one.
+    :func:`write_cache_int4` wrote; places that were never written are never used. ``data`` may be set
+    to another tensor of the same layout, which all calls after that use; for any other make another cache.
     """
 
-    __slots__ = ("data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
+    __slots__ = ("_data", "dtype", "dim", "kv_heads", "pages", "page_size", "layers", "_packed")
 
     def __init__(self, data: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> None:
         shape = data.shape
@@ -83,9 +83,29 @@ class Int4Cache:
         at = data.data_ptr()
         if (sl | sp | sh | at) & 15:
             raise ValueError("Int4Cache: data's address and strides must be multiples of 16 bytes")
-        self.data, self.dtype, self.dim, self.layers, self.pages, self.kv_heads = data, dtype, size // 10, layers, pages, heads
+        self._data, self.dtype, self.dim, self.layers, self.pages, self.kv_heads = data, dtype, size // 10, layers, pages, heads
         self.page_size = page = 8 * blocks
         self._packed = (at, sl, sp, sh, 1 if layers is None else layers, pages, page, heads, size // 10, _lib.DTYPE[dtype])
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @data.setter
+    def data(self, data: torch.Tensor) -> None:
+        old = self._data
+        if data.dtype is not old.dtype or data.shape != old.shape or data.stride() != old.stride():
+            raise ValueError(f"Int4Cache: data {data.dtype} {tuple(data.shape)} {data.stride()} has another layout than {tuple(old.shape)} {old.stride()}")
+        self._data = data
+        self._packed = (None, *self._packed[1:])
+
+    def _at(self) -> tuple[int, ...]:
+        """The cache as the C entry points take it, once ``data`` has been set to another tensor: its address is asked for when a call needs it."""
+        if self._packed[0] is None:
+            if (at := self._data.data_ptr()) & 15:
+                raise ValueError("Int4Cache: data's address must be a multiple of 16 bytes")
+            self._packed = (at, *self._packed[1:])
+        return self._packed
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, dim: int, dtype: torch.dtype = torch.bfloat16, layers: int | None = None,
@@ -157,7 +177,7 @@ def write_cache_int4(
     slots = slots.contiguous()
     if rows is not None:
         rows = rows.contiguous()
-    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *ks, *vs, slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n, count, *cache._packed)
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *ks, *vs, slots.data_ptr(), 0 if rows is None else rows.data_ptr(), n, count, *cache._at())
     _launch("write_cache_int4", index, _lib.load().af_write_cache_int4, args, _lib.ptr(word))
 
 
@@ -176,7 +196,7 @@ def read_cache_int4(
     v = torch.empty_like(k)
     count, row = slots.numel(), 2 * cache.kv_heads * cache.dim
     st = (count * row, row, 2 * cache.dim)
-    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *st, *st, slots.data_ptr(), 0, count, count, *cache._packed)
+    args = _ROWS.pack(k.data_ptr(), v.data_ptr(), *st, *st, slots.data_ptr(), 0, count, count, *cache._at())
     _launch("read_cache_int4", index, _lib.load().af_read_cache_int4, args, _lib.ptr(word))
     return k, v
 
@@ -240,7 +260,6 @@ def evict_cache(
     else:
         layered, layers, heads = cache.layers is not None, 1 if cache.layers is None else cache.layers, cache.kv_heads
         held = (cache.data, None)
-        parts = (*cache._packed, *((0,) * 15))
     n, most = _check_tables("evict_cache", tables, lengths)
     if weights.dtype is not torch.float32 or weights.dim() != (4 if layered else 3) or weights.shape[-3:-1] != (n, heads) \
             or (layered and weights.shape[0] != layers):
@@ -248,6 +267,8 @@ def evict_cache(
     if keep < 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
         raise ValueError(f"evict_cache: sinks {sinks} and recent {recent} must not be negative, and together not more than keep {keep}")
     index = _same_device("evict_cache", *held, tables, lengths, weights, word := _word(status))
+    if packed:
+        parts = (*cache._at(), *((0,) * 15))
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths = lengths.contiguous()
@@ -361,7 +382,7 @@ def tree_attention_int4(
     size = _scratch.get(index) or _workspace_bytes(index)
     workspace = lengths.new_empty(size >> 2)
     args = _ATTENTION.pack(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q_grid, *k_grid, *v_grid, *cache._packed, tables.data_ptr(),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *q_grid, *k_grid, *v_grid, *cache._at(), tables.data_ptr(),
         tables.stride(0) if batch > 1 else most, most, lengths.data_ptr(), starts.data_ptr(), mask_at, mask_row if total > 1 else words, words, batch, total,
         heads, window, sinks, dim ** -0.5 if scale is None else scale, out.data_ptr(), *out_grid, 0 if lse is None else lse.data_ptr(),
         workspace.data_ptr(), size)
@@ -395,7 +416,7 @@ def attention_weights(
     if packed:
         if cache.layers is not None:
             raise ValueError("attention_weights: cache must be one layer (cache[l])")
-        keys, dtype, kv, dim, parts, token = cache.data, cache.dtype, cache.kv_heads, cache.dim, cache._packed, 0
+        keys, dtype, kv, dim, token = cache.data, cache.dtype, cache.kv_heads, cache.dim, 0
     else:
         if cache.dim() != 4 or cache.dtype not in (torch.float16, torch.bfloat16):
             raise ValueError(f"attention_weights: cache must be an Int4Cache or 16-bit [pages, page_size, kv_heads, dim], got {cache.dtype} {tuple(cache.shape)}")
@@ -425,6 +446,8 @@ def attention_weights(
         raise ValueError("attention_weights: the innermost dimension of weights must be contiguous, and its entries must not share memory")
     window = _check_window("attention_weights", window, sinks)
     index = _same_device("attention_weights", q, keys, tables, lengths, starts, lse, weights, word := _word(status))
+    if packed:
+        parts = cache._at()
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths, starts, lse = lengths.contiguous(), starts.contiguous(), lse.contiguous()

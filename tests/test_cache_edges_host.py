@@ -1,0 +1,63 @@
+"""What the 4-bit cache's operators hand to the library, at the edges of what their inputs may be (CPU only)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from actfold_b200 import _lib
+from actfold_b200 import cache_kernels as K
+from actfold_b200 import speculative as S
+from test_cache_kernels_host import _attention, _cache, _evict, _weights, _z, lib  # noqa: F401 (lib: a fixture)
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture
+def launched(monkeypatch, lib):  # noqa: F811
+    """The packed arguments of the calls, which go no further."""
+    calls = []
+    monkeypatch.setattr(K, "_same_device", lambda *a: 0)
+    monkeypatch.setattr(K, "_launch", lambda what, index, fn, args, status: calls.append(args))
+    monkeypatch.setattr(K, "_scratch", {0: 64})
+    return calls
+
+
+def _calls(cache):
+    """Every operator that takes the cache, and where in its arguments the cache's numbers begin."""
+    k, slots = _z(3, 2, 64, dtype=BF), _z(3, dtype=torch.int64)
+    return ((lambda: S.write_cache_int4(k, k, cache, slots), K._ROWS, 12), (lambda: S.read_cache_int4(cache, slots), K._ROWS, 12),
+            (lambda: S.tree_attention_int4(**_attention(cache=cache)), K._ATTENTION, 9), (lambda: S.attention_weights(**_weights(cache=cache)), K._WEIGHTS, 3),
+            (lambda: S.evict_cache(**_evict(cache=cache)), K._EVICT, 0))
+
+
+def test_calls_use_the_tensor_that_data_is_now(launched):
+    """No call reads or writes memory that the cache had before: it may have been freed."""
+    cache = _cache()
+    old = cache.data
+    for call, _, _ in _calls(cache):
+        call()
+    cache.data = new = _z(3, 2, 2, 640, dtype=torch.uint8)
+    for call, _, _ in _calls(cache):
+        call()
+    for i, (_, struct, at) in enumerate(_calls(cache)):
+        assert struct.unpack(launched[i])[at] == old.data_ptr()
+        fields = struct.unpack(launched[i + 5])[at:at + 10]
+        assert fields == (new.data_ptr(), 0, 2560, 1280, 1, 3, 16, 2, 64, _lib.DTYPE[BF])
+    assert cache.data is new
+
+
+def test_data_keeps_its_layout(launched):
+    cache = _cache()
+    held = cache.data
+    u8 = torch.uint8
+    for bad in (_z(3, 2, 2, 640), _z(5, 2, 2, 640, dtype=u8), _z(1, 3, 2, 2, 640, dtype=u8), _z(3, 2, 2, 1280, dtype=u8), _z(3, 2, 4, 640, dtype=u8)[:, :, ::2],
+                _z(2, 3, 2, 640, dtype=u8).transpose(0, 1), _z(1, 2, 2, 640, dtype=u8).expand(3, 2, 2, 640)):
+        with pytest.raises(ValueError, match="Int4Cache"):
+            cache.data = bad
+    assert cache.data is held
+    cache.data = _z(3 * 2 * 2 * 640 + 16, dtype=u8)[8:-8].view(3, 2, 2, 640)  # not on a 16-byte border
+    for call, _, _ in _calls(cache):
+        with pytest.raises(ValueError, match="16 bytes"):
+            call()
+    assert not launched
