@@ -228,7 +228,8 @@ def evict_cache(
     :func:`attention_weights` adds them up. For each layer, request and head by itself the first ``sinks`` tokens, the last
     ``recent`` and, of those between, the ones with the largest weights stay (equal weights: the earlier tokens; NaN counts as the
     largest), ``keep`` in all. They move, in their order, to the request's first ``keep`` places, in place, so lengths stay the
-    same for all layers and heads. Other requests stay as they are. The tables are not changed: a
+    same for all layers and heads. Other requests stay as they are, also those of a length that is none (it sets ``status``, and
+    the result holds it, and all weights, as they were). The tables are not changed: a
     :func:`~actfold_b200.tree_kernels.block_tables` call with ``lengths`` the result's and ``held`` the old ones returns the pages.
     Keys are moved as they are, so they have to hold their positions (as rotated keys do); a window of
     :func:`tree_attention_int4` counts places. No page may lie in the tables of two requests, or twice in one.

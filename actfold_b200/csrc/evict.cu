@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kSelThreads) k_select(const SelectArgs a) {
   }
   if (t <= a.keep) {  // all stay
     for (int i = tid; i < a.keep; i += kSelThreads) kept[i] = i < t ? i : -1;
-    for (int i = tid; i < a.places; i += kSelThreads) out[i] = i < t ? w[i] : 0.f;
+    // (all of them where the length is none: whoever takes the result's weights over loses nothing)
+    for (int i = tid; i < a.places; i += kSelThreads) out[i] = i < t || bad ? w[i] : 0.f;
     return;
   }
   // The weights of places [lo, hi) decide; need of them stay (keep >= sinks + recent, t > keep: hi - lo > need).

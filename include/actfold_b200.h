@@ -644,7 +644,7 @@ int af_read_cache_int4(const af_int4_rows* w, uint32_t* status, void* stream);
  * last; lengths_out[b] = min(lengths[b], keep). weights [layers, batch, heads,
  * places] (strides in elements: layer, request, head). A length that is
  * negative or above places or the table's capacity, or a page out of range, sets
- * AF_STATUS_BOUNDS: such a request keeps its length and its rows, kept is
+ * AF_STATUS_BOUNDS: a request of such a length keeps it, its rows and all its weights, kept is
  * -1; rows of such a page are not moved. The tables are not changed
  * (af_block_tables with `held` gives the pages behind the kept tokens back).
  * With int4.head_dim 0 the cache is k_cache and v_cache: rows of head_bytes

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import cache_util as U
-from test_cache_kernels_gpu import KINDS, _attention_case, _check_attention, _i32, _i64
+from test_cache_kernels_gpu import KINDS, _attention_case, _check_attention, _evict_case, _i32, _i64
 
 pytestmark = pytest.mark.gpu
 
@@ -175,3 +175,20 @@ def test_weights_of_keys_that_are_infinite(dim, dtype, n, heads, kv, window, sin
             assert bool((near | (w[0] == want) | (w[0].isnan() & want.isnan())).all()), (w[0], want)
             if none:
                 assert not w[0, 0].any()
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+@pytest.mark.parametrize("held", [4, 16])
+def test_evict_keeps_the_weights_of_requests_with_bad_lengths(held):
+    """As their rows and their lengths, so that a caller who takes the result's weights over loses nothing."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import evict_cache
+
+    for length in (-1, 10 ** 6, 34):  # negative, past the table, past the weights
+        cache, _, tables, w = _evict_case(2, [32, 30], 2, 64, 8, BF, held, 2, extra=1)
+        st = DeviceStatus()
+        r = evict_cache(cache, tables, _i32([length, 30]), w, 20, status=st)
+        with pytest.raises(RuntimeError):
+            st.check_status()
+        assert torch.equal(r.weights[:, 0], w[:, 0]) and r.lengths.tolist() == [length, 20]
+        assert bool((r.kept[:, 0] == -1).all()) and not r.weights[:, 1, :, 20:].any()
