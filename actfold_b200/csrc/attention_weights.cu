@@ -195,8 +195,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) k_weights(const __grid_consta
       for (int x = x0 + warp; x < x1 && !lost; x += W) {
         if constexpr (INT4) {
           bring();
-          int tries = 0;
-          while (!lost && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1)) lost = ++tries > kPatience;
+          // (no attempts, no wait: the copy counts as lost)
+          if (p.patience == 0 || !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1)) {
+            int left = p.patience;
+            do lost = --left < 0;
+            while (!lost && !mbar_try_wait(full + 8 * (taken & 1), (taken >> 1) & 1));
+          }
           lost = __any_sync(0xffffffffu, lost);
           if (lost) {
             if (lane == 0 && p.status) atomicOr(p.status, AF_STATUS_TIMEOUT);
@@ -372,6 +376,7 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   p.scale = (float)(w.scale * 1.4426950408889634);
   p.rows = 8;
   p.status = status;
+  p.patience = attention_patience();
   a.d_token = w.token_stride;
   a.lse = w.lse;
   a.weights = w.weights;

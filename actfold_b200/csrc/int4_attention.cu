@@ -33,8 +33,6 @@
 
 namespace af {
 
-int attention_patience();  // tree_attention.cu: af_tree_attention_wait_limit sets it for all tree attention
-
 namespace kv4 {
 
 namespace {

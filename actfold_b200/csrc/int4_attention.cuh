@@ -10,6 +10,9 @@
 #include "tree.cuh"
 
 namespace af {
+
+int attention_patience();  // tree_attention.cu: af_tree_attention_wait_limit sets it for all tree attention, and for the attention weights
+
 namespace kv4 {
 
 constexpr int kPlans = 4;           // segments planned ahead in shared memory

@@ -578,8 +578,8 @@ int af_tree_attention_workspace_bytes(int64_t* bytes);
 
 /*
  * Attempts (of a few microseconds each) after which a wait inside later
- * af_tree_attention and af_tree_attention_int4 calls of this process gives up: the call then ends with
- * AF_STATUS_TIMEOUT in *status and rows of out that mean nothing. -1: the
+ * af_tree_attention, af_tree_attention_int4 and af_attention_weights calls of this process gives up: the call
+ * then ends with AF_STATUS_TIMEOUT in *status and rows of out, or weights, that mean nothing. -1: the
  * default, 2^18 attempts or about a second, which is also the most.
  */
 int af_tree_attention_wait_limit(int64_t attempts);
@@ -724,8 +724,8 @@ int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
  * 16-bit keys [page, token, head] with strides cache.strides[1], token_stride,
  * cache.strides[2] (bytes). weights strides in elements: request, head; places entries. A
  * length above places or the table's capacity, or a page out of range, sets AF_STATUS_BOUNDS: the
- * request is skipped, such a page's keys read as zeros; a copy of keys that does not come within about a second sets
- * AF_STATUS_TIMEOUT. Sums are held in 32 bits, in an order that does not change.
+ * request is skipped, such a page's keys read as zeros; a copy of keys that does not come in time (about a second,
+ * or what af_tree_attention_wait_limit says) sets AF_STATUS_TIMEOUT. Sums are held in 32 bits, in an order that does not change.
  */
 typedef struct {
   const void* q;

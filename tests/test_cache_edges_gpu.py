@@ -177,6 +177,37 @@ def test_weights_of_keys_that_are_infinite(dim, dtype, n, heads, kv, window, sin
                 assert not w[0, 0].any()
 
 
+def test_weights_end_when_a_wait_runs_out():
+    """No attempts: every copy of keys counts as one that did not come. The call ends and says so, with copies in flight, and the next one is right."""
+    from actfold_b200 import _lib
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import attention_weights, read_cache_int4
+
+    ls = [9000, 9000, 3000, 1]
+    a, starts, _ = _attention_case([4, 1, 30, 2], ls, 8, 2, 128, 16, BF, False, 5)  # (120 rows a head: more than are held at once)
+    lse = torch.full((starts[-1], 8), 9.0, device="cuda")
+    rows = read_cache_int4(a["cache"], torch.arange(a["cache"].pages * 16, device="cuda"))[0].view(-1, 16, 2, 128)
+    st = DeviceStatus()
+
+    def call(cache):
+        return attention_weights(a["q"], cache, a["tables"], a["lengths"], a["starts"], lse, torch.zeros(4, 2, 9000, device="cuda"), status=st)
+
+    good, good16 = call(a["cache"]), call(rows)
+    st.check_status()
+    _lib.check(_lib.load().af_tree_attention_wait_limit(0))
+    try:
+        for _ in range(20):
+            call(a["cache"])
+            with pytest.raises(TimeoutError):
+                st.check_status()
+        assert torch.equal(call(rows), good16)  # (rows of 16 bits come without a wait)
+        st.check_status()
+    finally:
+        _lib.check(_lib.load().af_tree_attention_wait_limit(-1))
+    assert torch.equal(call(a["cache"]), good)
+    st.check_status()
+
+
 # ------------------------------------------------------------------------------------------------ eviction
 @pytest.mark.parametrize("held", [4, 16])
 def test_evict_keeps_the_weights_of_requests_with_bad_lengths(held):
