@@ -347,8 +347,10 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   AF_REQUIRE(w.total <= (1 << 28) && c.pages <= 0x7fffffff && w.n_heads <= (1 << 16) && w.max_pages <= (1 << 30) && w.max_pages * c.page_size <= (1 << 30) &&
                  w.total * (w.n_heads / c.heads) <= (1 << 30) && w.batch <= (1 << 20),
              "af_attention_weights: size too large");
-  if (w.batch == 0 || w.total == 0 || w.max_pages == 0 || c.pages == 0) return AF_OK;
-  AF_REQUIRE(w.q && c.data && w.tables && w.lengths && w.starts && w.lse && (w.places == 0 || w.weights), "af_attention_weights: null pointer");
+  // Without pages there is nothing to add, but lengths that say otherwise are reported.
+  const bool none = w.max_pages == 0 || c.pages == 0;
+  if (w.batch == 0 || w.total == 0 || (none && !status)) return AF_OK;
+  AF_REQUIRE(w.q && (none || (c.data && w.tables)) && w.lengths && w.starts && w.lse && (w.places == 0 || w.weights), "af_attention_weights: null pointer");
   AF_REQUIRE((double)c.heads * w.batch * (w.max_pages * c.page_size / kv4::kUnit + 2) < 2147483000.0, "af_attention_weights: more than 2^31 units of 32 keys");
   uint64_t al = reinterpret_cast<uintptr_t>(w.q) | reinterpret_cast<uintptr_t>(c.data) | (uint64_t)w.q_strides[0] | (uint64_t)w.q_strides[1] |
                 (uint64_t)c.strides[1] | (uint64_t)c.strides[2] | (uint64_t)w.token_stride;
@@ -369,7 +371,7 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   p.group = (int)(w.n_heads / c.heads);
   p.pages = (int)c.pages;
   kv4::set_page(p, c.page_size);
-  p.capacity = w.max_pages * c.page_size;
+  p.capacity = none ? 0 : w.max_pages * c.page_size;
   p.window = (int)w.window;
   p.sinks = (int)w.sinks;
   p.reach = p.window - 1;

@@ -177,6 +177,21 @@ def test_weights_of_keys_that_are_infinite(dim, dtype, n, heads, kv, window, sin
                 assert not w[0, 0].any()
 
 
+def test_weights_report_lengths_without_pages():
+    """Lengths that no page and no table can hold are reported, and nothing is added."""
+    from actfold_b200.kernels import DeviceStatus
+    from actfold_b200.speculative import Int4Cache, attention_weights
+
+    q, lse = torch.ones(3, 4, 64, dtype=BF, device="cuda"), torch.zeros(3, 4, device="cuda")
+    none, cache = Int4Cache.empty(0, 8, 2, 64, BF), Int4Cache.empty(2, 8, 2, 64, BF)
+    rows = torch.zeros(0, 8, 2, 64, dtype=BF, device="cuda")
+    for c, tables in ((none, _i32([[0, 0]])), (rows, _i32([[0, 0]])), (cache, torch.zeros(1, 0, dtype=torch.int32, device="cuda"))):
+        for length in (0, 5, -1):
+            st, w = DeviceStatus(), torch.ones(1, 2, 8, device="cuda")
+            attention_weights(q, c, tables, _i32([length]), _i32([0, 3]), lse, w, status=st)
+            assert int(st.status) == (4 if length else 0) and bool((w == 1).all())
+
+
 def test_weights_end_when_a_wait_runs_out():
     """No attempts: every copy of keys counts as one that did not come. The call ends and says so, with copies in flight, and the next one is right."""
     from actfold_b200 import _lib
