@@ -67,16 +67,17 @@ class Int4Cache:
             raise ValueError("Int4Cache: page_size must be positive")
         if inner != 1 or (sb != size and blocks > 1):
             raise ValueError("Int4Cache: the blocks of a page's head must be contiguous")
+        run = blocks * size
         if heads <= 1:
             sh = 0
-        elif sh <= 0:
+        elif sh < run:
             raise ValueError("Int4Cache: data has entries that share memory")
         if pages <= 1:
             sp = 0
-        elif sp <= 0:
+        elif sp < run:
             raise ValueError("Int4Cache: data has entries that share memory")
         if layers is not None and layers > 1:
-            if sl <= 0:
+            if sl < run:
                 raise ValueError("Int4Cache: data has entries that share memory")
         else:
             sl = 0

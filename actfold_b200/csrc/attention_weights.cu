@@ -352,6 +352,8 @@ extern "C" int af_attention_weights(const af_attention_weights_args* args, uint3
   if (w.batch == 0 || w.total == 0 || (none && !status)) return AF_OK;
   AF_REQUIRE(w.q && (none || (c.data && w.tables)) && w.lengths && w.starts && w.lse && (w.places == 0 || w.weights), "af_attention_weights: null pointer");
   AF_REQUIRE((double)c.heads * w.batch * (w.max_pages * c.page_size / kv4::kUnit + 2) < 2147483000.0, "af_attention_weights: more than 2^31 units of 32 keys");
+  AF_REQUIRE(w.token_stride > 0 || (w.token_stride == 0 && kv4::runs_apart(c, false)),
+             "af_attention_weights: token_stride must be 0 (blocks of 4 bits, whose page and head strides let no entries share memory) or positive");
   uint64_t al = reinterpret_cast<uintptr_t>(w.q) | reinterpret_cast<uintptr_t>(c.data) | (uint64_t)w.q_strides[0] | (uint64_t)w.q_strides[1] |
                 (uint64_t)c.strides[1] | (uint64_t)c.strides[2] | (uint64_t)w.token_stride;
   AF_REQUIRE((al & 15) == 0, "af_attention_weights: addresses and strides must be multiples of 16 bytes");

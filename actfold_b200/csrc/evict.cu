@@ -346,6 +346,7 @@ extern "C" int af_evict_cache(const af_evict_args* args, uint32_t* status, void*
              "af_evict_cache: size too large");
   const bool moves = pages > 0 && w.max_pages > 0 && w.keep > 0 && (packed || w.head_bytes > 0);
   AF_REQUIRE(w.lengths && w.lengths_out && (w.places == 0 || (w.weights && w.weights_out)) && (w.keep == 0 || w.kept), "af_evict_cache: null pointer");
+  AF_REQUIRE(!packed || kv4::runs_apart(w.int4, true), "af_evict_cache: the cache's strides let its entries share memory");
   AF_REQUIRE(!moves || (w.tables && (packed ? w.int4.data != nullptr : w.k_cache && w.v_cache)), "af_evict_cache: null pointer");
   kv_evict::SelectArgs a;
   a.lengths = w.lengths;

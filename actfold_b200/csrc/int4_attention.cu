@@ -632,6 +632,7 @@ int check_args(const af_tree_attention_int4_args& a) {
   AF_REQUIRE(a.window >= 0 && a.sinks >= 0 && a.window <= (1 << 30) && a.sinks <= (1 << 30), "af_tree_attention_int4: window and sinks must not be negative");
   AF_REQUIRE(!a.mask || (a.words > 0 && a.words <= AF_TREE_MAX_NODES / 32 && a.mask_stride >= a.words), "af_tree_attention_int4: bad mask");
   if (a.batch == 0 || a.total == 0) return AF_OK;
+  AF_REQUIRE(runs_apart(c, false), "af_tree_attention_int4: the cache's strides let its entries share memory");
   AF_REQUIRE(a.q && a.k && a.v && a.out && a.lengths && a.starts && a.workspace, "af_tree_attention_int4: null pointer");
   AF_REQUIRE(a.max_pages == 0 || c.pages == 0 || (c.data && a.tables), "af_tree_attention_int4: null pointer");
   uint64_t al = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |

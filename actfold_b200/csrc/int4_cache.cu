@@ -245,6 +245,7 @@ int rows_call(const af_int4_rows* w, uint32_t* status, void* stream, const char*
   if (c.layers == 0 || c.heads == 0 || w->count == 0) return AF_OK;
   AF_REQUIRE(w->slots && ((WRITE && w->n_rows == 0) || (w->k && w->v)) && (c.pages == 0 || c.data), what + "null pointer");
   AF_REQUIRE(c.heads <= (1 << 16) && c.page_size <= (1 << 20) && c.layers <= 65535 && c.pages <= 0x7fffffff, what + "size too large");
+  AF_REQUIRE(runs_apart(c, true), what + "the cache's strides let its entries share memory");
   uint64_t al = reinterpret_cast<uintptr_t>(w->k) | reinterpret_cast<uintptr_t>(w->v) | reinterpret_cast<uintptr_t>(c.data);
   for (int i = 0; i < 3; ++i) al |= (uint64_t)w->k_strides[i] | (uint64_t)w->v_strides[i] | (uint64_t)c.strides[i];
   AF_REQUIRE((al & 15) == 0, what + "addresses and strides must be multiples of 16 bytes");

@@ -33,6 +33,12 @@ struct Block {
   __host__ __device__ static constexpr int pair(int r, int group) { return kPairsAt + r * kPairs + 4 * group; }
 };
 
+// A page's head is one run of blocks, so entries that share no memory lie at least that far apart.
+inline bool runs_apart(const af_int4_cache& c, bool layers) {
+  const int64_t run = c.page_size / kBlockTokens * 10 * c.head_dim;
+  return (!layers || c.layers <= 1 || c.strides[0] >= run) && (c.pages <= 1 || c.strides[1] >= run) && (c.heads <= 1 || c.strides[2] >= run);
+}
+
 template <int DT>
 struct Pair16;
 template <>

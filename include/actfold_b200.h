@@ -600,7 +600,7 @@ int af_tree_attention_wait_limit(int64_t attempts);
  * ---------------------------------------------------------------------- */
 typedef struct {
   void* data;
-  int64_t strides[3]; /* layer, page, head: bytes, multiples of 16 */
+  int64_t strides[3]; /* layer, page, head: bytes, multiples of 16, where there are several no less than a page's head takes */
   int64_t layers, pages, page_size, heads, head_dim, dtype;
 } af_int4_cache;
 
@@ -720,7 +720,7 @@ int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
  * lse_i), for the places p < lengths[b] that row i sees (window and sinks as
  * in af_tree_attention_int4 without a mask). lse [total, n_heads]: natural log
  * of each row's sum of exponentials, as the attention leaves it; a row of
- * -inf gives nothing. The cache is one layer: 4-bit blocks where token_stride is 0, else
+ * -inf gives nothing. The cache is one layer: 4-bit blocks where token_stride is 0, else (it is positive)
  * 16-bit keys [page, token, head] with strides cache.strides[1], token_stride,
  * cache.strides[2] (bytes). weights strides in elements: request, head; places entries. A
  * length above places or the table's capacity, or a page out of range, sets AF_STATUS_BOUNDS: the

@@ -61,3 +61,28 @@ def test_data_keeps_its_layout(launched):
         with pytest.raises(ValueError, match="16 bytes"):
             call()
     assert not launched
+
+
+def test_entries_that_share_memory_are_refused(launched, lib):  # noqa: F811
+    """A page's head is one run of blocks: entries nearer to one another than that overlap, and may run past the tensor's end as read."""
+    u8 = _z(4 * 3 * 2 * 4 * 640, dtype=torch.uint8)
+    for shape, strides in (((3, 2, 4, 640), (2 * 2560, 1280, 640, 1)), ((3, 2, 4, 640), (640, 3 * 2560, 640, 1)), ((4, 3, 2, 4, 640), (2544, 5120, 2560, 640, 1))):
+        with pytest.raises(ValueError, match="share memory"):
+            S.Int4Cache(u8.as_strided(shape, strides))
+    for shape, strides in (((3, 2, 4, 640), (2560, 3 * 2560, 640, 1)), ((1, 1, 4, 640), (16, 16, 640, 1)), ((1, 3, 2, 4, 640), (16, 5120, 2560, 640, 1))):
+        S.Int4Cache(u8.as_strided(shape, strides))
+    good = (u8.data_ptr() + 15 & ~15, 1 << 20, 5120, 2560, 2, 3, 32, 2, 64, _lib.DTYPE[BF])
+    p = good[0]
+    rows = lambda c: K._ROWS.pack(p, p, *(0, 256, 128) * 2, p, 0, 1, 1, *c)
+    evict = lambda c: K._EVICT.pack(*c, *(0,) * 15, p, 2, 2, p, 1, p, 0, 64, 32, 32, 20, 0, 0, p, p, p)
+    attention = lambda c: K._ATTENTION.pack(p, p, p, 256, 128, 128, 64, 128, 64, *c, p, 2, 2, p, p, 0, 0, 0, 1, 1, 2, 0, 0, 0.1, p, 256, 128, 0, p, 1 << 40)
+    weights = lambda c, token=0: K._WEIGHTS.pack(p, 256, 128, *c, token, p, 2, 2, p, p, 1, 1, 2, 0, 0, 0.1, p, p, 64, 32, 32)
+    for i in (1, 2, 3):
+        near = (*good[:i], 2544, *good[i + 1:])
+        calls = [(lib.af_write_cache_int4, rows), (lib.af_read_cache_int4, rows), (lib.af_evict_cache, evict)]
+        for fn, pack in calls + ([] if i == 1 else [(lib.af_tree_attention_int4, attention), (lib.af_attention_weights, weights)]):
+            assert fn(pack(near), None, None) == _lib.AF_ERR_ARG, (fn, i)
+            assert b"share" in lib.af_last_error_string()
+    # Rows of 16 bits whose tokens share one: no blocks of 4 bits, and no such rows either.
+    for token in (0, -256):
+        assert lib.af_attention_weights(weights((p, 0, 4096, 128, 1, 3, 32, 2, 64, good[9]), token), None, None) == _lib.AF_ERR_ARG
