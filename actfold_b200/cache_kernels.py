@@ -431,7 +431,7 @@ def attention_weights(
         parts, token = (cache.data_ptr(), 0, grid[0], grid[2], 1, pages, page, kv, dim, _lib.DTYPE[dtype]), grid[1]
     qs = q.shape
     total, heads = (qs[0], qs[1]) if len(qs) == 3 else (0, 0)
-    if heads == 0 or q.dtype is not dtype or qs[2] != dim or heads % kv:
+    if heads == 0 or kv == 0 or q.dtype is not dtype or qs[2] != dim or heads % kv:
         raise ValueError(f"attention_weights: q {q.dtype} {tuple(qs)} and cache {dtype} {tuple(keys.shape)} do not match")
     batch, most = _check_tables("attention_weights", tables, lengths)
     if starts.dtype is not _I32 or starts.dim() != 1:

@@ -86,3 +86,10 @@ def test_entries_that_share_memory_are_refused(launched, lib):  # noqa: F811
     # Rows of 16 bits whose tokens share one: no blocks of 4 bits, and no such rows either.
     for token in (0, -256):
         assert lib.af_attention_weights(weights((p, 0, 4096, 128, 1, 3, 32, 2, 64, good[9]), token), None, None) == _lib.AF_ERR_ARG
+
+
+def test_a_cache_without_heads():
+    """Calls that need query heads for it are refused."""
+    cache = S.Int4Cache(_z(3, 0, 2, 640, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="attention_weights"):
+        S.attention_weights(**_weights(cache=cache, weights=_z(2, 0, 40, dtype=torch.float32)))
