@@ -687,9 +687,10 @@ extern "C" int af_tree_attention_int4(const af_tree_attention_int4_args* args, u
   p.window = (int)a.window;
   p.sinks = (int)a.sinks;
   p.reach = p.window - (a.mask ? 0 : 1);
-  p.scale = a.scale == 0. ? 1.f : (float)(fabs(a.scale) * 1.4426950408889634);
+  p.scale = (float)(fabs(a.scale) * 1.4426950408889634);
   p.q_flip = a.scale < 0. ? 0x80008000u : 0u;
-  p.q_keep = a.scale == 0. ? 0u : 0xffffffffu;
+  p.q_keep = p.scale == 0.f ? 0u : 0xffffffffu;
+  if (p.scale == 0.f) p.scale = 1.f;  // (0, and what is 0 in fp32: hidden scores of -inf times 0 would be NaN)
   p.out = static_cast<char*>(a.out), p.out_n = a.out_strides[0], p.out_h = a.out_strides[1];
   p.lse = a.lse;
   p.ws = static_cast<char*>(a.workspace);

@@ -122,6 +122,17 @@ def test_a_prompt_may_be_cut_anywhere():
         at = end
 
 
+def test_attention_with_a_scale_below_fp32():
+    """A scale that is no fp32 number but 0 is 0, not NaN where something is hidden."""
+    from actfold_b200.speculative import tree_attention_int4
+
+    for kind in KINDS:
+        a, starts, bits = _attention_case(ls=[70, 300, 33], dim=64, page=16, dtype=BF, tree=True, seed=4, **KINDS[kind])
+        zero = tree_attention_int4(**a, scale=0.0)
+        for scale in (1e-50, -1e-50):
+            assert torch.equal(tree_attention_int4(**a, scale=scale), zero)
+
+
 # ------------------------------------------------------------------------------------------------ weights
 def _given(q, keys, lse, window, sinks):
     """Sums over rows and heads of the group, of one request, in 64 bits; rows whose lse is -inf give nothing."""
