@@ -306,12 +306,13 @@ cudaError_t launch_move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
   return launch_ex(k_move<HD, CLUSTER>, dim3((unsigned)(segments * a.columns * CLUSTER)), dim3(kMoveThreads), (size_t)bytes, s, true, dim3(CLUSTER), a);
 }
 
-// A CTA holds some 40 to 115 KB: two or three fit an SM. Clusters as long as all of their CTAs do at once. One request of 4100 tokens
+// Of a CTA of 46 to 112 KB two or four fit an SM. Clusters as long as all of their CTAs do at once. One request of 4100 tokens
 // down to 2048, 4 heads x 128 in 4 bits, by clusters of 1, 2, 4 and 8: one layer 28, 23, 19 and 16 us, 14 layers 32, 29, 31 and 35,
-// 28 layers 36, 46, 48 and 55.
+// 28 layers 36, 46, 48 and 55. (Clusters that need a second wave, from a replayed graph: 20 layers 47 us with two CTAs, 39 with one.)
 template <int HD>
 cudaError_t move(const MoveArgs& a, int64_t segments, cudaStream_t s) {
-  const int64_t ctas = segments * a.columns, room = 3 * sm_count();
+  constexpr int fit = 233472 / (Move<HD>::kShared + 1024);  // of an SM's shared memory
+  const int64_t ctas = segments * a.columns, room = fit * sm_count();
   if (8 * ctas <= room) return launch_move<HD, 8>(a, segments, s);
   if (4 * ctas <= room) return launch_move<HD, 4>(a, segments, s);
   return 2 * ctas <= room ? launch_move<HD, 2>(a, segments, s) : launch_move<HD, 1>(a, segments, s);
