@@ -320,7 +320,7 @@ template <int DT, int HD>
 int launch(const WeightArgs& a, bool int4, cudaStream_t s) {
   const int ctas = sm_count() * kCtas;
   if (int4) {
-    if (int st = allow_smem<k_weights<DT, HD, true>>(kRing<HD>)) return st;
+    if (int st = allow_smem<k_weights<DT, HD, true>>(kRing<HD>, "af_attention_weights")) return st;
     k_weights<DT, HD, true><<<ctas, kThreads, kRing<HD>, s>>>(a);
   } else {
     k_weights<DT, HD, false><<<ctas, kThreads, 0, s>>>(a);

@@ -602,7 +602,7 @@ template <int DT, int HD, int NT, int W, int CTAS>
 int launch(const Params& p, cudaStream_t s) {
   using S = Shape<HD, NT, W, CTAS>;
   static_assert(CTAS * (S::kBytes + 1024) <= 233472, "shared memory");
-  if (int st = allow_smem<k_int4_attention<DT, HD, NT, W, CTAS>>(S::kBytes)) return st;
+  if (int st = allow_smem<k_int4_attention<DT, HD, NT, W, CTAS>>(S::kBytes, "af_tree_attention_int4")) return st;
   const int ctas = CTAS * sm_count();
   cudaError_t e = launch_ex(k_int4_attention<DT, HD, NT, W, CTAS>, dim3(ctas), dim3(S::kThreads), (size_t)S::kBytes, s, false, dim3(1), p);
   if (e == cudaSuccess && p.joins)

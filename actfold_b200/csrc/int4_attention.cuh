@@ -34,7 +34,6 @@ struct Params {
   int words, batch, total, heads, kv_heads, group, pages, page;
   uint32_t page_mul;                            // see entry_of
   int page_shift;
-  int runs;                                     // that 32 tokens of a cache lie in: of 32, 16 or 8 tokens, so that none leaves a page
   int64_t capacity;                             // tokens that a table row can hold
   int window, sinks;                            // window 0: all of the prefix is visible
   int reach;                                    // tokens of the prefix that a window can hold: all, of a chain, whose nodes see themselves, one less
@@ -300,14 +299,14 @@ constexpr int kWideUnit = 128;
 int wide_launch(const Params& p, bool bf16, int head_dim, cudaStream_t s);
 
 template <auto Kernel>
-int allow_smem(int bytes) {
+int allow_smem(int bytes, const char* what) {
   static std::atomic<uint64_t> allowed{0};  // a bit per device
   int device = 0;
   cudaGetDevice(&device);
   const uint64_t bit = 1ull << (device & 63);
   if (allowed.load(std::memory_order_relaxed) & bit) return AF_OK;
   const cudaError_t e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string("af_tree_attention_int4: ") + cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail(AF_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
   allowed.fetch_or(bit, std::memory_order_relaxed);
   return AF_OK;
 }
