@@ -271,6 +271,8 @@ def evict_cache(
     index = _same_device("evict_cache", *held, tables, lengths, weights, word := _word(status))
     if packed:
         parts = (*cache._at(), *((0,) * 15))
+    elif k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("evict_cache: k_cache and v_cache share memory, whose rows would move twice")
     if most > 1 and tables.stride(1) != 1:
         tables = tables.contiguous()
     lengths = lengths.contiguous()

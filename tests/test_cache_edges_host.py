@@ -93,3 +93,14 @@ def test_a_cache_without_heads():
     cache = S.Int4Cache(_z(3, 0, 2, 640, dtype=torch.uint8))
     with pytest.raises(ValueError, match="attention_weights"):
         S.attention_weights(**_weights(cache=cache, weights=_z(2, 0, 40, dtype=torch.float32)))
+
+
+def test_one_cache_for_keys_and_values_is_not_moved_twice(launched):
+    """Keys and values are moved by CTAs that do not wait for one another."""
+    rows = _z(3, 2, 16, 2, 64, dtype=BF)
+    S.evict_cache(**_evict(cache=(rows[:, 0], rows[:, 1])))
+    assert len(launched) == 1
+    for one in (rows[:, 0], rows[None, :, 0]):
+        with pytest.raises(ValueError, match="share memory"):
+            S.evict_cache(**_evict(cache=(one, one), weights=_z(*one.shape[:-4], 2, 2, 40, dtype=torch.float32)))
+    assert len(launched) == 1
