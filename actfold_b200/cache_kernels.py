@@ -412,9 +412,12 @@ def attention_weights(
     ``weights`` float32 [requests, kv_heads, places]: entry (b, h, p) grows by the sum, over request b's rows and the query heads
     of group h, of ``exp(scale * q . k_p - lse)`` for the places p < ``lengths[b]`` that the row sees. ``q`` [nodes, heads, dim]
     and ``lse`` float32 [nodes, heads], as :func:`~actfold_b200.tree_kernels.tree_attention` or :func:`tree_attention_int4` left
-    them for these rows; request b's rows ``starts[b] .. starts[b + 1]`` follow one another (a prompt, one token, or the accepted path
-    of a tree), and ``window``, ``sinks`` and ``scale`` are that call's. ``cache`` is one layer: an :class:`Int4Cache` or a 16-bit
-    k_cache [pages, page_size, kv_heads, dim]. :func:`evict_cache` takes the weights.
+    them for these rows; request b's rows ``starts[b] .. starts[b + 1]`` follow one another (one token, the accepted path of a tree,
+    a prompt's next piece), and ``lengths``, ``window``, ``sinks`` and ``scale`` are that call's: of the tokens cached before the rows.
+    What rows give to one another is not counted. A prompt over an empty cache adds nothing; in pieces, every piece adds to
+    those before it. ``cache`` is one layer: an :class:`Int4Cache` or a 16-bit k_cache [pages, page_size, kv_heads, dim], page_size a
+    multiple of 8, dim 64 or 128 (``window`` and ``sinks`` are there for rows whose attention had them; ``tree_attention`` has none).
+    :func:`evict_cache` takes the weights.
     """
     packed = isinstance(cache, Int4Cache)
     if packed:

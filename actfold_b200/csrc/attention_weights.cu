@@ -10,7 +10,8 @@
 // of its weight; what bounds it is the chain of a warp's unit (operands, products, exponentials), with four warps a scheduler
 // (issue 52 %, tensor pipe 28 %, HBM 22 %). See int4_attention.cu for the fragments' order.
 //   64 requests of 1 to 4 tokens, 90 to 8000 keys, 28 heads over 4: 50 us in 4 bits; the bytes need 14.
-//   One token over 523 keys: 5.5 us.
+//   The same over keys in 16 bits, which are loaded as they are needed: 65 us; the bytes need 42.
+//   One token over 1500 keys: 5.6 us.
 // Tried: rows from global memory for each unit (137 us), keys looked up and loaded unit by unit (70); four chains of products
 // (53), 16 keys at a time with two or three CTAs an SM (54, 56), shares by rows as well as units (53 to 59): slower.
 #include <string>

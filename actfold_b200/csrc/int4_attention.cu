@@ -20,11 +20,15 @@
 // ends of row tiles overlap (windows of 4100 tokens 160 -> 140 us); up to 16 rows: one CTA of 32 slots, for the registers. The step's own
 // nodes are units too, read from their 16-bit rows. Every wait is bounded; a timeout sets AF_STATUS_TIMEOUT.
 //
-// What bounds it is issue: some 860 instructions a unit and 8 rows, of which the values take 512, at 0.59 a cycle and scheduler
-// (ALU pipe 46 % busy, HBM 40 %).
+// No unit is near full: 0.52 to 0.59 instructions a cycle and scheduler, ALU pipe 45 %, HBM 35 to 40 %. What bounds it is a warp's chain
+// through a unit (codes, values, products, softmax, products), some 860 instructions for 8 rows, of which the values take 512; the
+// registers leave an SM 16 warps, too few to cover it. (A value is rounded once, as it is read back, which costs a subtraction and a
+// multiply-add for each pair; scale and offset applied to sums of codes would need fewer, and give other scores. Not tried.)
+// Probabilities are rounded to the values' type, which the products take (half a step of each; sums and outputs stay in 32 bits until
+// the one rounding of the result): 0.0022 instead of 0.0017 over whole outputs in bf16, 0.00029 instead of 0.00021 in fp16.
 //   64 requests of one token, 90 to 8000 keys, 28 heads over 4: 60 us; the bytes need 25.5.
 //   24 requests of one token in windows of 4096 and 4 first tokens, 500 to 30000 keys, 32 heads over 32: 134 us; the bytes need 73.
-//   One token over 523 keys: 10.4 us, of which a launch, the plan, a table, a unit and two joins are the chain.
+//   One token over 523 keys: 10.9 us, of which a launch, the plan, a table, a unit and two joins are the chain.
 // Tried: no producer, each warp brings its own units (spills); units by turns of 15 over two CTAs' warps (135 -> 150 us); Q of the
 // next row tile ahead; 15 consumer warps in one CTA: slower or the same.
 #include <math.h>

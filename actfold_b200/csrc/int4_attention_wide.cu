@@ -13,12 +13,15 @@
 // meanwhile. A softmax thread owns a row, so no scores are exchanged. The reference maximum of a row is raised only when a
 // score passes it by 2^8.
 //
+// Probabilities are rounded to the values' type as in int4_attention.cu: half a step of each, in the place of S.
+//
 // The work of a tile: 64 KB that go through shared memory twice (some 1000 cycles of its 128 bytes), 512 cycles of products per
 // pipe, 128 exponentials a row. No unit is busy all the time: it is the chain of turning, product, softmax and product, through
 // two buffers, that bounds it (per tile some 5500 cycles with one row tile, of which the turning warps take some 4300 with what they wait for; the softmax
 // 1500 to 1900 for half a tile of 128 rows).
 //   8 trees of 20 to 64 nodes, 32 heads over 32, 300 to 4100 keys: 246 us with the kernel of few rows, 94 now; its bytes need 17.
 //   4 trees of 48 to 64 nodes, 28 heads over 4, 30 to 65 K keys: 2204 us with that kernel, 259 now; its products need 107.
+// (The 16-bit cache's attention takes 79 and 252 to 257 us for them: the codes' turning costs what their fewer bytes gain.)
 // Tried: keys and values one after the other in eight warps (114 us instead of 105 at that time: a tile's keys waited for the
 // products with the values two tiles before); 16 turning warps with 72 registers, more registers for the issue warps or the turning
 // ones, the codes a tile ahead in shared memory (the long trees 259 -> 274 us) or half a tile ahead in registers (the first 93 -> 105), halves of S

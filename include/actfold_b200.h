@@ -610,7 +610,7 @@ typedef struct {
  *
  * As af_write_cache: for every layer and i < count with slots[i] >= 0 (and
  * rows[i] >= 0, rows null: row i). Per row and group of 32 dims: offset = the
- * smallest value, scale = (largest - smallest) / 15 rounded to dtype (one step
+ * smallest value, scale = (largest - smallest) / 15, in fp32, rounded to dtype (one step
  * less where 15 * scale + offset would overflow), code = (x - offset) / scale
  * rounded half to even, in 0 .. 15 (0 where scale is 0). A group with a value
  * that is not finite, or with a range past fp32's, stands for NaN throughout.
@@ -716,7 +716,7 @@ int af_tree_attention_int4_workspace_bytes(int64_t* bytes);
  * af_attention_weights -- the attention that cached tokens are given.
  *
  * weights[b, h, p] += sum over the request's rows i (a chain: [starts[b],
- * starts[b + 1])) and the query heads of group h of exp(scale * q_i . k_p -
+ * starts[b + 1]), behind the lengths[b] cached tokens; what rows give to one another is not counted) and the query heads of group h of exp(scale * q_i . k_p -
  * lse_i), for the places p < lengths[b] that row i sees (window and sinks as
  * in af_tree_attention_int4 without a mask). lse [total, n_heads]: natural log
  * of each row's sum of exponentials, as the attention leaves it; a row of
